@@ -1,0 +1,63 @@
+// attn_kernels.h -- arguments and host launchers of the attention kernels
+// (internal): the position rotation with the append to the paged key-value
+// cache, and attention of new tokens over that cache.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace gxmoe {
+
+// A paged cache: element (page, kv head, slot, dim) of K and of V lies at
+// page * sb + head * sh + slot * st + dim.  Pages hold 1 << bs_shift slots.
+struct KvPages {
+  void* k;
+  void* v;
+  const float* k_scale;  // [kv_heads], e4m3 only; null = 1
+  const float* v_scale;
+  int64_t sb, sh, st;
+  int num_blocks, bs_shift, kv_heads, head_dim;
+  bool e4m3;
+};
+
+struct AppendArgs {
+  const uint16_t* qkv;  // [T][(heads + 2 kv_heads) head_dim]
+  int64_t qkv_stride;
+  const int32_t* positions;  // [T]
+  const int32_t* slots;      // [T], outside the cache: not stored
+  const float* table;        // [max_positions][2][rotary / 2]
+  int max_positions, rotary, interleaved;
+  int T, heads;
+  uint16_t* q_out;
+  int64_t q_stride;
+  KvPages kv;
+};
+
+struct AttendArgs {
+  const uint16_t* q;  // [rows][heads head_dim]
+  int64_t q_stride;
+  uint16_t* out;
+  int64_t out_stride;
+  KvPages kv;
+  const int32_t* tables;  // [B][table_stride], max_blocks entries used
+  int64_t table_stride;
+  int max_blocks;
+  const int32_t* lens;     // [B], tokens of the sequence, the new ones included
+  const int32_t* offsets;  // [B + 1] first row of each sequence; null: one row each
+  int B, rows, heads;
+  float scale_log2;  // scale * log2(e): softmax runs on powers of two
+  int window, first;
+  const uint16_t* sinks;  // [heads] or null
+};
+
+struct RopeTableArgs {
+  float* table;
+  int rotary, max_positions;
+  double theta, factor, original, beta_fast, beta_slow, concentration;
+};
+
+hipError_t launch_rope_table(const RopeTableArgs& a, hipStream_t s);
+hipError_t launch_rope_append(const AppendArgs& a, hipStream_t s);
+hipError_t launch_attend_rows(const AttendArgs& a, hipStream_t s);
+
+}  // namespace gxmoe

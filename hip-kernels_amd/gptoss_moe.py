@@ -85,6 +85,22 @@ class ProfRecord(ctypes.Structure):
                 ("start_ms", _F * 4), ("dur_ms", _F * 4)]
 
 
+class KvCacheDesc(ctypes.Structure):
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P),
+                ("block_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64),
+                ("dtype", _I), ("num_blocks", _I), ("block_size", _I), ("num_kv_heads", _I), ("head_dim", _I)]
+
+
+class RopeConfig(ctypes.Structure):
+    _fields_ = [("rotary_dim", _I), ("max_positions", _I), ("theta", ctypes.c_double),
+                ("scaling_factor", ctypes.c_double), ("original_positions", ctypes.c_double),
+                ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double)]
+
+
+class AttentionConfig(ctypes.Structure):
+    _fields_ = [("scale", _F), ("window", _I), ("first_tokens", _I), ("sinks", _P)]
+
+
 def _sig(name, args, res=_I):
     f = getattr(_lib, name)
     f.argtypes = args
@@ -142,6 +158,13 @@ _sig("gptoss_fused_residual_rmsnorm_forward", [_P, _P, _P, _P, _P, _I, _I, _F, _
 _sig("gptoss_moe_combine_forward", [_P, _P, _P, _P, _P, _I, _I, _I, _P])
 _sig("gptoss_mxfp4_dequant", [_P, _P, _I, _I, _P, _P])
 _sig("gptoss_moe_grouped_mxfp4_gemm", [_P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _F, _F, _P, _P, _P])
+_L = ctypes.c_int64
+_sig("gptoss_rope_config_default", [ctypes.POINTER(RopeConfig)])
+_sig("gptoss_rope_table", [ctypes.POINTER(RopeConfig), _P, _P])
+_sig("gptoss_rope_kv_append", [_P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _P, _L, _P, _P])
+_sig("gptoss_paged_attention_workspace_bytes", [_I, _I, _I, _I, _I], _SZ)
+_sig("gptoss_paged_attention_decode", [_P, _L, _P, _P, _L, _I, _P, _I, _I, _P, _P, _L, _P, _SZ, _P])
+_sig("gptoss_paged_attention_prefill", [_P, _L, _P, _I, _P, _P, _L, _I, _P, _I, _I, _P, _P, _L, _P, _SZ, _P])
 
 lib = _lib
 
@@ -833,3 +856,253 @@ def grouped_mxfp4_gemm(x, offsets, tiled_nib, tiled_sc, N: int, K: int, rows: in
                                              _ptr(tiled_sc), _ptr(bias), N, K, 1 if swiglu else 0, alpha, limit,
                                              _ptr(out), _ptr(gate_up), _stream(stream)))
     return out
+
+
+# ---------------------------------------------------------------------------
+# attention over a paged key-value cache
+# ---------------------------------------------------------------------------
+GPTOSS_KV_BF16 = 0
+GPTOSS_KV_E4M3 = 1
+
+
+def default_rope_config() -> RopeConfig:
+    """GPT-OSS's rotary positions (config.h:29-36)."""
+    cfg = RopeConfig()
+    check(_lib.gptoss_rope_config_default(ctypes.byref(cfg)))
+    return cfg
+
+
+def rope_table(cfg: RopeConfig | None = None, device="cuda", stream=None) -> torch.Tensor:
+    """fp32 [max_positions][2][rotary_dim / 2]: the cosines of each position, then its sines."""
+    cfg = cfg or default_rope_config()
+    if cfg.rotary_dim < 2 or cfg.max_positions < 1:
+        _bad(f"rotary_dim={cfg.rotary_dim} and max_positions={cfg.max_positions} must be positive")
+    device = torch.device(device)
+    with _alloc_on(stream, device):
+        table = torch.empty((cfg.max_positions, 2, cfg.rotary_dim // 2), dtype=torch.float32, device=device)
+    with _on(table):
+        check(_lib.gptoss_rope_table(ctypes.byref(cfg), _ptr(table), _stream(stream)))
+    return table
+
+
+class _on:
+    """The device of `t` as the current one within the block."""
+
+    def __init__(self, t):
+        self._to = t.device.index if t.device.type == "cuda" else None
+
+    def __enter__(self):
+        self._was = None
+        if self._to is not None and torch.cuda.current_device() != self._to:
+            self._was = torch.cuda.current_device()
+            torch.cuda.set_device(self._to)
+
+    def __exit__(self, *exc):
+        if self._was is not None:
+            torch.cuda.set_device(self._was)
+
+
+def _on_device(name: str, t, device, dtype=None, dim: int | None = None) -> None:
+    if not isinstance(t, torch.Tensor):
+        _bad(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if dtype is not None and t.dtype != dtype:
+        _bad(f"{name} has dtype {t.dtype}, expected {dtype}")
+    if dim is not None and t.dim() != dim:
+        _bad(f"{name} must be {dim}-D, got shape {tuple(t.shape)}")
+    if t.device != device:
+        _bad(f"{name} is on {t.device}, the cache is on {device}")
+
+
+def _row_tensor(name: str, t, device, cols: int) -> None:
+    """bf16 [rows, cols] on `device`, rows any distance apart."""
+    _on_device(name, t, device, torch.bfloat16, 2)
+    if t.shape[1] != cols:
+        _bad(f"{name} has shape {tuple(t.shape)}, expected [rows, {cols}]")
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < cols):
+        _bad(f"{name} must have contiguous rows, strides are {t.stride()}")
+
+
+def _vector(name: str, t, device, n: int, dtype) -> None:
+    _on_device(name, t, device, dtype, 1)
+    if t.shape[0] != n:
+        _bad(f"{name} has {t.shape[0]} entries, expected {n}")
+    if not t.is_contiguous():
+        _bad(f"{name} must be contiguous")
+
+
+def _needs_gpu(device) -> None:
+    if device.type != "cuda":
+        _bad(f"the cache is on {device}, a GPU is needed")
+
+
+class _alloc_on:
+    """Allocations within the block belong to `stream` (None: the current one), where the kernels that use
+    them run: torch hands a freed block out again in the order of its own stream only."""
+
+    def __init__(self, stream, device):
+        self._with = None
+        if stream is not None and device.type == "cuda":
+            if isinstance(stream, int):
+                stream = torch.cuda.default_stream(device) if stream == 0 else \
+                    torch.cuda.ExternalStream(stream, device=device)
+            self._with = torch.cuda.stream(stream)
+
+    def __enter__(self):
+        if self._with is not None:
+            self._with.__enter__()
+
+    def __exit__(self, *exc):
+        if self._with is not None:
+            self._with.__exit__(*exc)
+
+
+def _row_stride(t) -> int:
+    # torch gives a single row any stride
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
+
+
+class KVCache:
+    """A paged key-value cache over the caller's tensors (borrowed): k and v of
+    [num_blocks, kv_heads, block_size, head_dim], bfloat16 or float8_e4m3fn with
+    the last dim contiguous and the same strides, so a permuted view covers
+    token-major pages and k = slab[:, 0], v = slab[:, 1] an interleaved slab.
+    8-bit caches stand for code * scale, scales float32 [kv_heads] (None: 1)."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
+                 v_scale: torch.Tensor | None = None):
+        for name, t in (("k", k), ("v", v)):
+            if not isinstance(t, torch.Tensor) or t.dim() != 4:
+                _bad(f"{name} must be a 4-D tensor [num_blocks, kv_heads, block_size, head_dim]")
+            if t.dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+                _bad(f"{name} has dtype {t.dtype}, expected torch.bfloat16 or torch.float8_e4m3fn")
+        if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
+            _bad("k and v differ in shape, dtype, device or strides")
+        if k.numel() == 0:
+            _bad(f"empty cache of shape {tuple(k.shape)}")
+        if k.stride(3) != 1:
+            _bad("k and v must be contiguous along head_dim")
+        blocks, heads, size, dim = k.shape
+        # strides of dims of size 1 are never used, and torch gives them any value
+        stride = [st if n > 1 else dim for n, st in zip(k.shape[:3], k.stride()[:3])]
+        # slots must not share memory: each stride covers what lies within it
+        reach = dim
+        for n, st in sorted((m for m in zip(k.shape[:3], stride) if m[0] > 1), key=lambda m: m[1]):
+            if st < reach:
+                _bad(f"k and v overlap themselves: strides {k.stride()} of shape {tuple(k.shape)}")
+            reach = st * (n - 1) + reach
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t is None:
+                continue
+            if k.dtype == torch.bfloat16:
+                _bad(f"{name}: a bfloat16 cache has no scales")
+            _vector(name, t, k.device, heads, torch.float32)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device, self.num_blocks, self.kv_heads, self.block_size, self.head_dim = k.device, blocks, heads, size, dim
+        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), _ptr(k_scale), _ptr(v_scale), stride[0], stride[1], stride[2],
+                                GPTOSS_KV_BF16 if k.dtype == torch.bfloat16 else GPTOSS_KV_E4M3, blocks, size, heads, dim)
+        self._desc = ctypes.addressof(self.desc)
+
+
+def rope_kv_append(qkv, positions, slots, table, cache: KVCache, num_heads: int, interleaved: bool = False, q_out=None,
+                   stream=None):
+    """Turns the queries and keys of qkv [T, (num_heads + 2 kv_heads) * head_dim] by their positions (int32
+    [T]) and stores keys and values in the cache's slots (int32 [T], page * block_size + place; -1: not stored).
+    Rows whose position is outside the table (rope_table()) write nothing.  Returns the queries
+    [T, num_heads * head_dim]; q_out may be qkv[:, :num_heads * head_dim]."""
+    dev, D = cache.device, cache.head_dim
+    _row_tensor("qkv", qkv, dev, (num_heads + 2 * cache.kv_heads) * D)
+    T = qkv.shape[0]
+    _vector("positions", positions, dev, T, torch.int32)
+    _vector("slots", slots, dev, T, torch.int32)
+    _on_device("table", table, dev, torch.float32, 3)
+    if table.shape[1] != 2 or not table.is_contiguous():
+        _bad(f"table must be contiguous [max_positions, 2, rotary_dim / 2], got {tuple(table.shape)}")
+    if q_out is None:
+        with _alloc_on(stream, dev):
+            q_out = torch.empty((T, num_heads * D), dtype=torch.bfloat16, device=dev)
+    else:
+        _row_tensor("q_out", q_out, dev, num_heads * D)
+        if q_out.shape[0] != T:
+            _bad(f"q_out has {q_out.shape[0]} rows, expected {T}")
+    _needs_gpu(dev)
+    q_stride = _row_stride(q_out)
+    if T == 1 and q_out.data_ptr() == qkv.data_ptr():
+        q_stride = _row_stride(qkv)
+    with _on(qkv):
+        check(_lib.gptoss_rope_kv_append(qkv.data_ptr(), _row_stride(qkv), positions.data_ptr(), slots.data_ptr(),
+                                         table.data_ptr(), 2 * table.shape[2], table.shape[0], 1 if interleaved else 0,
+                                         T, num_heads, q_out.data_ptr(), q_stride, cache._desc, _stream(stream)))
+    return q_out
+
+
+def paged_attention_workspace_bytes(num_tokens: int, num_seqs: int, num_heads: int, cache: KVCache) -> int:
+    """Bytes of workspace that suffice for a call on num_tokens rows of num_seqs sequences."""
+    return _lib.gptoss_paged_attention_workspace_bytes(num_tokens, num_seqs, num_heads, cache.kv_heads, cache.head_dim)
+
+
+def _attend(q, offsets, cache, block_tables, seq_lens, scale, window, first_tokens, sinks, out, workspace, stream):
+    dev, D = cache.device, cache.head_dim
+    if not isinstance(q, torch.Tensor) or q.dim() != 2 or q.shape[1] % D != 0 or q.shape[1] == 0:
+        _bad(f"q must be [rows, num_heads * {D}]")
+    _row_tensor("q", q, dev, q.shape[1])
+    rows, H = q.shape[0], q.shape[1] // D
+    _on_device("block_tables", block_tables, dev, torch.int32, 2)
+    B, blocks = block_tables.shape
+    if blocks > 1 and block_tables.stride(1) != 1:
+        _bad("block_tables must have contiguous rows")
+    _vector("seq_lens", seq_lens, dev, B, torch.int32)
+    if sinks is not None:
+        _vector("sinks", sinks, dev, H, torch.bfloat16)
+    if offsets is None:
+        if rows != B:
+            _bad(f"q has {rows} rows for {B} sequences")
+    else:
+        _vector("query_offsets", offsets, dev, B + 1, torch.int32)
+    if out is None:
+        with _alloc_on(stream, dev):
+            out = torch.empty((rows, H * D), dtype=torch.bfloat16, device=dev)
+    else:
+        _row_tensor("out", out, dev, H * D)
+        if out.shape[0] != rows:
+            _bad(f"out has {out.shape[0]} rows, expected {rows}")
+    _needs_gpu(dev)
+    need = _lib.gptoss_paged_attention_workspace_bytes(rows, B, H, cache.kv_heads, D)
+    if workspace is None:
+        with _alloc_on(stream, dev):
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    else:
+        _on_device("workspace", workspace, dev)
+        if not workspace.is_contiguous():
+            _bad("workspace must be contiguous")
+    cfg = AttentionConfig(D ** -0.5 if scale is None else scale, window, first_tokens, _ptr(sinks))
+    tail = (cache._desc, block_tables.data_ptr(), block_tables.stride(0) if B > 1 else blocks, blocks, seq_lens.data_ptr(),
+            B, H, ctypes.addressof(cfg), out.data_ptr(), _row_stride(out), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size())
+    with _on(q):
+        if offsets is None:
+            check(_lib.gptoss_paged_attention_decode(q.data_ptr(), _row_stride(q), *tail, _stream(stream)))
+        else:
+            check(_lib.gptoss_paged_attention_prefill(q.data_ptr(), _row_stride(q), offsets.data_ptr(), rows, *tail,
+                                                      _stream(stream)))
+    return out
+
+
+def paged_attention_decode(q, cache: KVCache, block_tables, seq_lens, scale: float | None = None, window: int = 0,
+                           first_tokens: int = 0, sinks=None, out=None, workspace=None, stream=None):
+    """Attention of one new token per sequence (already appended): q [B, num_heads * head_dim] over the pages
+    block_tables (int32 [B, max_blocks], -1: none) of seq_lens (int32 [B]) tokens.  scale: head_dim ** -0.5 when
+    None.  window: 0, or how many of the last tokens are seen, besides the first first_tokens.  sinks: bf16
+    [num_heads], a logit that joins the softmax's sum.  workspace: of paged_attention_workspace_bytes(); when None it
+    is allocated, like out."""
+    return _attend(q, None, cache, block_tables, seq_lens, scale, window, first_tokens, sinks, out, workspace, stream)
+
+
+def paged_attention_prefill(q, query_offsets, cache: KVCache, block_tables, seq_lens, scale: float | None = None,
+                            window: int = 0, first_tokens: int = 0, sinks=None, out=None, workspace=None, stream=None):
+    """Causal attention of prompt chunks: rows query_offsets[b] (int32 [B + 1]) to query_offsets[b + 1] - 1 of
+    q are the last tokens of sequence b, already appended.  Rows of no sequence are left as they were in `out`
+    (unset when it is allocated here).  Otherwise as paged_attention_decode."""
+    if query_offsets is None:
+        _bad("query_offsets must be a tensor")
+    return _attend(q, query_offsets, cache, block_tables, seq_lens, scale, window, first_tokens, sinks, out, workspace,
+                   stream)

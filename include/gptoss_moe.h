@@ -442,6 +442,127 @@ int gptoss_moe_grouped_mxfp4_gemm(const uint16_t* x, const int32_t* row_index,
 int gptoss_mxfp4_dequant(const uint8_t* tiled_nibbles, const uint8_t* tiled_scales, int N, int K,
                          uint16_t* out, void* stream);
 
+/* ---- Attention over a paged key-value cache ------------------------------
+ * The attention half of a layer (src/model/attention.cu:635-959) between its
+ * two projections.  A decode step calls, on the rows of the QKV projection, gptoss_rope_kv_append and then
+ * gptoss_paged_attention_decode; a prompt chunk the same with
+ * gptoss_paged_attention_prefill.  None of these calls synchronises the host or
+ * allocates, so a layer hook (gptoss_moe_stack_decode_step) may capture them;
+ * lengths, positions, slots and page tables are read on the device, so a
+ * replayed graph follows the values that those buffers hold then.
+ * These entry points are additions: the ABI version stays. */
+
+enum { GPTOSS_KV_BF16 = 0, GPTOSS_KV_E4M3 = 1 };
+
+/* Where the cache lies.  Element (page, kv head, slot, dim) of K is at
+ * page * block_stride + head * head_stride + slot * token_stride + dim
+ * elements from k, and of V from v.  All three strides 0: the reference's
+ * [num_blocks][kv_heads][block_size][head_dim] without gaps.  Strides are
+ * multiples of 16 bytes and at least head_dim, k and v are 16-byte aligned, so
+ * token-major pages and K / V interleaved by page are covered.  head_dim is 64
+ * or 128, block_size a power of two from 16 to 256.  E4M3 (OCP, gfx950's own)
+ * elements stand for code * scale[kv head]; a null scale is 1, and bf16 caches
+ * have none. */
+typedef struct gptoss_kv_cache {
+  void* k;
+  void* v;
+  const float* k_scale;  /* device [num_kv_heads] or NULL */
+  const float* v_scale;
+  int64_t block_stride, head_stride, token_stride; /* elements */
+  int dtype;             /* GPTOSS_KV_BF16 or GPTOSS_KV_E4M3 */
+  int num_blocks, block_size, num_kv_heads, head_dim;
+} gptoss_kv_cache;
+
+/* YaRN rotary positions (rope.cu:42-512): rotary_dim dims of a head turn, dim
+ * pair i at frequency theta^(-2i/rotary_dim), or that over scaling_factor
+ * where it turns less than beta_slow times within original_positions, with a
+ * linear ramp from the dims that turn beta_fast times.  cos and sin carry the
+ * concentration 0.1 ln(scaling_factor) + 1.  scaling_factor 1: plain rotary
+ * positions. */
+typedef struct gptoss_rope_config {
+  int rotary_dim;      /* a positive multiple of 16 */
+  int max_positions;
+  double theta;        /* > 1 */
+  double scaling_factor; /* >= 1 */
+  double original_positions, beta_fast, beta_slow; /* > 0; unused at factor 1 */
+} gptoss_rope_config;
+
+/* GPT-OSS: rotary_dim 64, 131072 positions, theta 150000, factor 32 over 4096,
+ * beta 32 / 1 (include/config.h:29-36). */
+int gptoss_rope_config_default(gptoss_rope_config* cfg);
+
+/* table: [max_positions][2][rotary_dim / 2] fp32, the cosines of a position and
+ * then its sines; angles are formed in 64 bits. */
+int gptoss_rope_table(const gptoss_rope_config* cfg, float* table, void* stream);
+
+/* Position rotation, and the append to the cache (the reference's pieces of it:
+ * attention.cu:105-380, kv_cache_manager.cu:32).  Row t of qkv holds the
+ * num_heads queries, the kv heads' keys and their values, head_dim each, rows
+ * qkv_stride elements apart (a multiple of 8).  Queries and keys are turned by
+ * positions[t] (pair i is dims i and i + rotary_dim / 2, or 2i and 2i + 1 if
+ * interleaved != 0; dims from rotary_dim on are kept): products and their sum
+ * are fp32 operations, rounded once.  Queries go to q_out as bf16 (rows q_stride
+ * apart, a multiple of 8); keys and values to slot slots[t] = page *
+ * block_size + place of the cache, as bf16 or as e4m3 of value / scale, those
+ * past +-448 as +-448.  A row whose slot is not in the cache (as -1) stores no
+ * key or value; one whose position is not in the table [0, max_positions)
+ * writes nothing at all.  Slots of one call are distinct: of rows that share
+ * one, any may be found there, in pieces.  q_out may be the queries' place in
+ * qkv (same pointer and stride) and otherwise lies apart from qkv.
+ * qkv, q_out and rope_table are 16-byte aligned; rotary_dim <= head_dim. */
+int gptoss_rope_kv_append(const uint16_t* qkv, int64_t qkv_stride, const int32_t* positions,
+                          const int32_t* slots, const float* rope_table, int rotary_dim, int max_positions,
+                          int interleaved, int num_tokens, int num_heads, uint16_t* q_out, int64_t q_stride,
+                          const gptoss_kv_cache* cache, void* stream);
+
+/* What a query at position p sees: the tokens t <= p, and with window > 0 of
+ * those only the last `window` (its own among them) and the first
+ * first_tokens of the sequence.  sinks (device bf16 [num_heads], may be NULL)
+ * adds exp(sinks[head]) to the softmax's sum, as a token without a value.  A
+ * query that sees nothing gives zeros. */
+typedef struct gptoss_attention_config {
+  float scale;       /* of the scores; > 0 */
+  int window;        /* 0: no window */
+  int first_tokens;
+  const uint16_t* sinks;
+} gptoss_attention_config;
+
+/* Sequence b's token t lies in page block_tables[b * table_stride +
+ * t / block_size] at place t % block_size.  Tokens of a page number outside
+ * [0, num_blocks) (as -1 for a page given back once it left the window) are not
+ * seen.  seq_lens[b] counts the tokens in the cache, the new ones included;
+ * negative ones are 0, and those past max_blocks pages are cut to that.  What
+ * pages hold past a sequence's end, or outside of what is seen, has no effect,
+ * NaN included.
+ *
+ * Decode (the reference's: paged_attention.cu:112-717): one new token per
+ * sequence, at position seq_lens[b] - 1; q and out are [num_seqs][num_heads *
+ * head_dim] bf16, rows q_stride and out_stride elements apart (multiples of
+ * 8), apart from each other, 16-byte aligned.  num_heads is a multiple of the
+ * kv heads, at most 128 per kv head.  The scores and sums are fp32, the
+ * weights bf16 against bf16 values.
+ * workspace: gptoss_paged_attention_workspace_bytes bytes, 16-byte aligned,
+ * that no call running at the same time uses (two graphs that may overlap need
+ * two); nothing is kept in it between calls. */
+size_t gptoss_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads,
+                                              int head_dim);
+int gptoss_paged_attention_decode(const uint16_t* q, int64_t q_stride, const gptoss_kv_cache* cache,
+                                  const int32_t* block_tables, int64_t table_stride, int max_blocks,
+                                  const int32_t* seq_lens, int num_seqs, int num_heads,
+                                  const gptoss_attention_config* cfg, uint16_t* out, int64_t out_stride,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+/* Prompt chunks (the reference's: flash_attention.cu:100-447, there without a
+ * cache): rows query_offsets[b] to query_offsets[b + 1] - 1 of q and out (num_tokens
+ * rows) are the last tokens of sequence b, already appended, so row i of n is
+ * at position seq_lens[b] - n + i; rows at negative positions give zeros.
+ * query_offsets is [num_seqs + 1], nondecreasing; rows outside
+ * [query_offsets[0], query_offsets[num_seqs]) are left as they were. */
+int gptoss_paged_attention_prefill(const uint16_t* q, int64_t q_stride, const int32_t* query_offsets,
+                                   int num_tokens, const gptoss_kv_cache* cache, const int32_t* block_tables,
+                                   int64_t table_stride, int max_blocks, const int32_t* seq_lens, int num_seqs,
+                                   int num_heads, const gptoss_attention_config* cfg, uint16_t* out,
+                                   int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
