@@ -71,6 +71,8 @@ int check_cache(const gptoss_kv_cache* c, KvPages* kv) {
       return set_error(GPTOSS_ERR_INVALID, "cache strides %lld, %lld, %lld must be multiples of %d and at least head_dim",
                        static_cast<long long>(kv->sb), static_cast<long long>(kv->sh), static_cast<long long>(kv->st),
                        static_cast<int>(unit));
+  if (kv->st > (1 << 24))
+    return set_error(GPTOSS_ERR_UNSUPPORTED, "token_stride=%lld above 2^24", static_cast<long long>(kv->st));
   kv->num_blocks = c->num_blocks;
   kv->bs_shift = __builtin_ctz(static_cast<unsigned>(c->block_size));
   kv->kv_heads = c->num_kv_heads;
@@ -126,8 +128,11 @@ int check_attend(AttendArgs* a, const gptoss_kv_cache* cache, const gptoss_atten
                        need);
     if (!aligned16(workspace)) return set_error(GPTOSS_ERR_INVALID, "workspace must be 16-byte aligned");
   }
-  if (static_cast<int64_t>(rows) * a->heads > 0x7fffffff)
+  if (static_cast<int64_t>(rows) * a->heads > 0x7fffffff || a->heads > 65535)
     return set_error(GPTOSS_ERR_UNSUPPORTED, "%d rows of %d heads in one call", rows, a->heads);
+  // all sequences' tokens, in units of 16, are counted in 32 bits
+  if (static_cast<int64_t>(a->max_blocks) * (1 << a->kv.bs_shift) / 16 + 1 > 0x7fffffff / B)
+    return set_error(GPTOSS_ERR_UNSUPPORTED, "tables of %d pages for %d sequences", a->max_blocks, B);
   a->B = B;
   a->rows = rows;
   a->scale_log2 = cfg->scale * 1.44269504088896340736f;
@@ -215,8 +220,8 @@ int gptoss_rope_kv_append(const uint16_t* qkv, int64_t qkv_stride, const int32_t
 
 size_t gptoss_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads,
                                               int head_dim) {
-  (void)num_tokens, (void)num_seqs, (void)num_heads, (void)num_kv_heads, (void)head_dim;
-  return 0;
+  if (num_tokens < 1 || num_seqs < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1) return 0;
+  return decode_workspace_bytes(num_seqs, num_heads, num_kv_heads, head_dim);
 }
 
 int gptoss_paged_attention_decode(const uint16_t* q, int64_t q_stride, const gptoss_kv_cache* cache,
@@ -238,7 +243,7 @@ int gptoss_paged_attention_decode(const uint16_t* q, int64_t q_stride, const gpt
   const int rc = check_attend(&a, cache, cfg, num_seqs, num_seqs, workspace, workspace_bytes);
   if (rc != GPTOSS_OK) return rc;
   if (num_seqs == 0) return ok();
-  HIP_TRY(launch_attend_rows(a, static_cast<hipStream_t>(stream)), "paged attention decode launch");
+  HIP_TRY(launch_decode(a, workspace, static_cast<hipStream_t>(stream)), "paged attention decode launch");
   return ok();
 }
 

@@ -1,0 +1,488 @@
+// attn_decode.hip -- attention of one new token per sequence over the paged
+// cache (gfx950).
+//
+// Mathematics.  With base-2 scores s = (q . k) scale log2(e), a wave keeps for
+// each head a reference m, the sum l of 2^(s - m) and the weighted sum O of
+// the values; two such triples over disjoint tokens join as
+//   M = max(m1, m2), l = l1 2^(m1 - M) + l2 2^(m2 - M), O likewise,
+// so tokens are split over tiles, waves and work-groups in any way.
+//
+// Bound by reading K and V once: 8 heads on a kv head take 16 flops per byte.
+// Everything else is laid out so that nothing but the loads is slow: K and V go
+// from memory to registers, whole 128-byte rows, and from there into the
+// matrix cores without passing through LDS.
+//   S^T = K Q^T   (16 tokens x 16 heads a product): a lane holds one token's
+//                 quarter of the dims, the same quarter of its head's query.
+//   O^T = V^T P^T (16 dims x 16 heads): the lane that S^T leaves with head
+//                 l % 16 and tokens 4 (l / 16) + i is the one that holds these as
+//                 the second operand, so the weights stay where they are; V's
+//                 rows are read 16 lanes to a row and interleaved by byte
+//                 permutes (the order of dims and tokens inside a product is free
+//                 as long as both operands agree).
+// The reference m of a head moves only when a score exceeds it by 2^8: until
+// then weights up to 256 lose nothing in bf16 or fp32, and the tile needs no
+// exchange between lanes.
+#include "attn_device.h"
+
+namespace gxmoe {
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTile = 32;      // tokens per step of a wave
+constexpr float kSlack = 8.0f;  // how far a score may exceed the reference, in powers of two
+
+// The tiles of a sequence that its new token sees: the first nf tiles (first
+// tokens of a windowed sequence), then all from tile `main` on.
+struct Seen {
+  int len, low;  // tokens from `low` on are inside the window
+  int nf, main, tiles;
+};
+
+__device__ __forceinline__ Seen seen_tiles(const AttendArgs& a, int len) {
+  Seen s;
+  s.len = len;
+  s.low = a.window > 0 && len > a.window ? len - a.window : 0;
+  s.main = s.low / kTile;
+  s.nf = min((min(a.first, s.low) + kTile - 1) / kTile, s.main);
+  s.tiles = s.nf + (len + kTile - 1) / kTile - s.main;
+  return s;
+}
+
+struct SplitArgs {
+  int slots, min_tiles;  // pieces aimed at (0: one per sequence), smallest piece
+  float* part_o;         // [piece][heads][D] sums of the cut sequences' pieces
+  float* part_ml;        // [piece][heads][4] reference, sum, whether any token was seen
+  int* plan;             // [B][2] first piece and number of pieces
+};
+
+// What a work-group does: tiles [t0, t1) of sequence b, piece `slot` of all.
+struct Piece {
+  int b, t0, t1, chunks, first_slot;
+  Seen seen;
+};
+
+__device__ __forceinline__ int wave_sum(int v) {
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) v += __shfl_xor(v, x);
+  return v;
+}
+
+// Sequences are cut into pieces of `size` tiles, the size chosen from all
+// lengths so that the pieces of one kv head are about a.slots in number; every
+// wave works it out from the lengths, which only the device knows.
+__device__ __forceinline__ bool find_piece(const AttendArgs& a, const SplitArgs& sp, int slot, Piece* p) {
+  const int lane = threadIdx.x & 63;
+  int total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64)
+    total += b0 + lane < a.B ? seen_tiles(a, seq_len(a, min(b0 + lane, a.B - 1))).tiles : 0;
+  total = __builtin_amdgcn_readfirstlane(wave_sum(total));
+  const int size = max(sp.min_tiles, (total + sp.slots - 1) / sp.slots);
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const bool in = b0 + lane < a.B;
+    const int tiles = in ? seen_tiles(a, seq_len(a, b0 + lane)).tiles : 0;
+    const int mine = in ? max(1, (tiles + size - 1) / size) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+      const int y = __shfl_up(upto, x);
+      if (lane >= x) upto += y;
+    }
+    const int all = __builtin_amdgcn_readlane(upto, 63);
+    if (slot < before + all) {
+      const int at = slot - before;
+      const int who = __builtin_ctzll(__ballot(at < upto));
+      p->b = b0 + who;
+      p->chunks = __builtin_amdgcn_readlane(mine, who);
+      const int first = __builtin_amdgcn_readlane(upto, who) - p->chunks;
+      p->first_slot = before + first;
+      p->seen = seen_tiles(a, __builtin_amdgcn_readfirstlane(seq_len(a, p->b)));
+      p->t0 = (at - first) * size;
+      p->t1 = min(p->t0 + size, p->seen.tiles);
+      return true;
+    }
+    before += all;
+  }
+  return false;
+}
+
+// One tile's K and V as a lane holds them.  Half j: tokens 16 j + l % 16, dims
+// (l / 16) D/4 on.  Row i: token 16 (i / 4) + 4 (l / 16) + i % 4, dims
+// (l % 16) D/16 on.
+template <int D, bool kE4m3>
+struct TileRegs {
+  static constexpr int kKd = D / 16 * (kE4m3 ? 1 : 2);  // dwords of K per half
+  static constexpr int kVd = D / 64 * (kE4m3 ? 1 : 2);  // dwords of a row of V
+  uint32_t k[2][kKd];
+  uint32_t v[8][kVd];
+};
+
+template <int N>
+__device__ __forceinline__ void load_dwords(const uint8_t* p, uint32_t (&d)[N]) {
+  if constexpr (N == 1) {
+    d[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+  } else if constexpr (N == 2) {
+    const attn_u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const attn_u32x2*>(p));
+    d[0] = x[0], d[1] = x[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const attn_u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const attn_u32x4*>(p) + i);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) d[4 * i + c] = x[c];
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t bits(bf16x2 v) { return __builtin_bit_cast(uint32_t, v); }
+
+// The four e4m3 codes of a dword as bf16 (exact).
+__device__ __forceinline__ void widen(uint32_t codes, uint32_t* out) {
+  out[0] = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false));
+  out[1] = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true));
+}
+
+template <int D, bool kE4m3, int W>
+__global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitArgs sp) {
+  typedef TileRegs<D, kE4m3> Regs;
+  constexpr int kSteps = D / 32;             // products of 32 dims per half
+  constexpr int kDt = D / 16;                // tiles of 16 dims of the output
+  constexpr int kSize = kE4m3 ? 1 : 2;       // bytes per element
+  constexpr int kRow = D + 4;                // floats of a head's partial result in LDS
+  __shared__ float s_o[W][16][kRow];
+  __shared__ float s_m[W][16], s_l[W][16];
+  __shared__ int s_any[W];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int group = a.heads / a.kv.kv_heads;
+  const int parts = (group + 15) / 16;  // tiles of 16 heads per kv head
+  const int kvh = blockIdx.y / parts, h0 = kvh * group + (blockIdx.y % parts) * 16;
+  const int nh = min(16, (kvh + 1) * group - h0);
+
+  Piece p;
+  if (sp.slots > 0) {
+    if (!find_piece(a, sp, blockIdx.x, &p)) return;
+  } else {
+    p.b = blockIdx.x;
+    p.chunks = 1;
+    p.first_slot = 0;
+    p.seen = seen_tiles(a, __builtin_amdgcn_readfirstlane(seq_len(a, p.b)));
+    p.t0 = 0;
+    p.t1 = p.seen.tiles;
+  }
+  if (sp.slots > 0 && p.t0 == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+    sp.plan[2 * p.b] = p.first_slot;
+    sp.plan[2 * p.b + 1] = p.chunks;
+  }
+
+  // queries: head h0 + n, dims g D/4 + 8 s on for step s
+  bf16x8 q[kSteps];
+  {
+    const uint16_t* row = a.q + p.b * a.q_stride + static_cast<int64_t>(h0 + min(n, nh - 1)) * D + g * (D / 4);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      attn_u32x4 x = reinterpret_cast<const attn_u32x4*>(row)[s];
+      if (n >= nh) x = attn_u32x4{0, 0, 0, 0};
+      q[s] = __builtin_bit_cast(bf16x8, x);
+    }
+  }
+  const float scale = a.scale_log2 * (kE4m3 && a.kv.k_scale ? a.kv.k_scale[kvh] : 1.0f);
+
+  // Pages of 32 of this wave's tiles at a time: lane 2 i + j has half j of
+  // the i-th (tile t0 + wave + W i).
+  const int mine = max(0, (p.t1 - p.t0 - wave + W - 1) / W);
+  auto tile_of = [&](int i) {  // where the wave's i-th tile begins
+    const int t = p.t0 + wave + W * i;
+    return (t < p.seen.nf ? t : p.seen.main + t - p.seen.nf) * kTile;
+  };
+  auto load_pages = [&](int i0) {
+    const int i = i0 + (lane >> 1);
+    int page = -1;
+    if (i < mine) {
+      const int t = tile_of(i) + 16 * (lane & 1);
+      if (t < p.seen.len) page = a.tables[p.b * a.table_stride + (t >> a.kv.bs_shift)];
+      if (page >= a.kv.num_blocks) page = -1;
+    }
+    return page;
+  };
+  const uint8_t* kb = static_cast<const uint8_t*>(a.kv.k) + kvh * a.kv.sh * kSize;
+  const uint8_t* vb = static_cast<const uint8_t*>(a.kv.v) + kvh * a.kv.sh * kSize;
+  const int st = static_cast<int>(a.kv.st) * kSize;
+  const uint32_t koff = n * st + g * (D / 4) * kSize, voff = 4 * g * st + n * (D / 16) * kSize;
+  const int mask = (1 << a.kv.bs_shift) - 1;
+
+  int pages = load_pages(0), next_pages = -1;
+  auto load = [&](int i, Regs& r) {
+    const int t = tile_of(i);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int page = max(0, __builtin_amdgcn_readlane(pages, 2 * (i & 31) + j));
+      const int64_t at = page * a.kv.sb * kSize + static_cast<int64_t>((t + 16 * j) & mask) * st;
+      load_dwords(kb + at + koff, r.k[j]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) load_dwords(vb + at + voff + static_cast<uint32_t>(c * st), r.v[4 * j + c]);
+    }
+  };
+
+  float m = kNegInf, l = 0.0f;
+  bool any = false;  // whether the wave saw a token (its scores may all be -inf)
+  f32x4 o[kDt];
+#pragma unroll
+  for (int d = 0; d < kDt; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  auto compute = [&](int i, int have0, int have1, Regs& r) {
+    const int t = tile_of(i);
+    f32x4 s[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t kd[D / 8];
+      if constexpr (kE4m3) {
+#pragma unroll
+        for (int c = 0; c < Regs::kKd; ++c) widen(r.k[j][c], kd + 2 * c);
+      } else {
+#pragma unroll
+        for (int c = 0; c < Regs::kKd; ++c) kd[c] = r.k[j][c];
+      }
+      s[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c)
+        s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(bf16x8, attn_u32x4{kd[4 * c], kd[4 * c + 1], kd[4 * c + 2], kd[4 * c + 3]}), q[c], s[j], 0,
+            0, 0);
+    }
+    uint32_t vd[8][D / 32];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      if constexpr (kE4m3) {
+#pragma unroll
+        for (int x = 0; x < Regs::kVd; ++x) widen(r.v[c][x], vd[c] + 2 * x);
+      } else {
+#pragma unroll
+        for (int x = 0; x < Regs::kVd; ++x) vd[c][x] = r.v[c][x];
+      }
+    }
+    const bool whole = have0 && have1 && t + kTile <= p.seen.len && (t >= p.seen.low || t + kTile <= a.first);
+    if (whole) {
+      any = true;
+    } else {
+      // hidden tokens: no score, and a value of zero, whatever the page holds
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const int at = t + 16 * (c >> 2) + 4 * g + (c & 3);
+        const bool in = (c < 4 ? have0 : have1) && at < p.seen.len && (at >= p.seen.low || at < a.first);
+        any |= __ballot(in) != 0;
+        s[c >> 2][c & 3] = in ? s[c >> 2][c & 3] : kNegInf;
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) vd[c][x] = in ? vd[c][x] : 0u;
+      }
+    }
+    float top = __builtin_fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int c = 1; c < 4; ++c) top = __builtin_fmaxf(top, __builtin_fmaxf(s[0][c], s[1][c]));
+    top *= scale;
+    if (__ballot(top > m + kSlack) != 0) {
+      top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+      const float mn = __builtin_fmaxf(m, top);
+      const float keep = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
+      m = mn;
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < kDt; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[d][c] *= keep;
+    }
+    const float base = m == kNegInf ? 0.0f : m;
+    float w[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) w[c] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c >> 2][c & 3], scale, -base));
+    l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    const bf16x8 wb = __builtin_bit_cast(
+        bf16x8, attn_u32x4{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]), pack_bf16x2(w[4], w[5]), pack_bf16x2(w[6], w[7])});
+#pragma unroll
+    for (int d = 0; d < kDt; ++d) {
+      const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;  // the high or the low halves of two dwords
+      attn_u32x4 x;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] = __builtin_amdgcn_perm(vd[2 * c + 1][d >> 1], vd[2 * c][d >> 1], sel);
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), wb, o[d], 0, 0, 0);
+    }
+  };
+
+  Regs ra, rb;
+  if (mine > 0) load(0, ra);
+  for (int i = 0; i < mine; i += 2) {
+    const int a0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31)) >= 0, a1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1) >= 0;
+    const int b0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 2) >= 0, b1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 3) >= 0;
+    if ((i & 31) == 0 && i + 32 < mine) next_pages = load_pages(i + 32);
+    if (i + 1 < mine) load(i + 1, rb);
+    compute(i, a0, a1, ra);
+    if ((i & 31) == 30) pages = next_pages;
+    if (i + 2 < mine) load(i + 2, ra);
+    if (i + 1 < mine) compute(i + 1, b0, b1, rb);
+  }
+
+  // the wave's sum, then the waves'
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (lane == 0) s_any[wave] = any;
+  if (n < nh) {
+    if (g == 0) s_m[wave][n] = m, s_l[wave][n] = l;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int d = 0; d < kDt; d += 4)  // row 4 g + c of tile d is dim (4 g + c) D/16 + d
+        *reinterpret_cast<f32x4*>(&s_o[wave][n][(4 * g + c) * kDt + d]) = f32x4{o[d][c], o[d + 1][c], o[d + 2][c], o[d + 3][c]};
+  }
+  __syncthreads();
+  const float vs = kE4m3 && a.kv.v_scale ? a.kv.v_scale[kvh] : 1.0f;
+  any = false;
+#pragma unroll
+  for (int w = 0; w < W; ++w) any |= s_any[w] != 0;
+  for (int e = threadIdx.x; e < nh * (D / 4); e += 64 * W) {
+    const int h = e / (D / 4), d = e % (D / 4) * 4, head = h0 + h;
+    const bool last = p.chunks == 1;
+    float top = last && a.sinks ? bf16_to_f32(a.sinks[head]) * kLog2e : kNegInf;
+    const float sink = top;
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = __builtin_fmaxf(top, s_m[w][h]);
+    const float base = top == kNegInf ? 0.0f : top;
+    float sum = last && a.sinks ? __builtin_amdgcn_exp2f(sink - base) : 0.0f;
+    f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = __builtin_amdgcn_exp2f(s_m[w][h] - base);
+      sum += s_l[w][h] * f;
+      const f32x4 x = *reinterpret_cast<const f32x4*>(&s_o[w][h][d]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(x[c], f, acc[c]);
+    }
+    if (last) {
+      const float f = any ? vs / sum : 0.0f;
+      uint32_t* to = reinterpret_cast<uint32_t*>(a.out + p.b * a.out_stride + static_cast<int64_t>(head) * D + d);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[c] = any ? acc[c] * f : 0.0f;
+      *reinterpret_cast<attn_u32x2*>(to) = attn_u32x2{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+    } else {
+      const int64_t at = static_cast<int64_t>(blockIdx.x) * a.heads + head;
+      *reinterpret_cast<f32x4*>(sp.part_o + at * D + d) = acc;
+      if (d == 0) reinterpret_cast<f32x4*>(sp.part_ml)[at] = f32x4{top, sum, any ? 1.0f : 0.0f, 0.0f};
+    }
+  }
+}
+
+// Joins the pieces of a sequence, one work-group per (sequence, head): wave w
+// takes pieces w, w + 4, ...; a lane takes D / 64 dims.
+template <int D>
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs a, SplitArgs sp, bool e4m3) {
+  constexpr int W = 4, kDl = D / 64;
+  __shared__ float s_o[W][D];
+  __shared__ float s_l[W];
+  __shared__ int s_any[W];
+  const int b = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+  const int first = sp.plan[2 * b], chunks = sp.plan[2 * b + 1];
+  if (chunks <= 1) return;  // written by its only work-group
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const f32x4* ml = reinterpret_cast<const f32x4*>(sp.part_ml) + static_cast<int64_t>(first) * a.heads + head;
+  const float sink = a.sinks ? bf16_to_f32(a.sinks[head]) * kLog2e : kNegInf;
+  float top = sink;
+  for (int c = lane; c < chunks; c += 64) top = __builtin_fmaxf(top, ml[static_cast<int64_t>(c) * a.heads][0]);
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x));
+  const float base = top == kNegInf ? 0.0f : top;
+  float l = 0.0f, o[kDl];
+  int any = 0;
+#pragma unroll
+  for (int d = 0; d < kDl; ++d) o[d] = 0.0f;
+  const float* po = sp.part_o + (static_cast<int64_t>(first) * a.heads + head) * D;
+#pragma unroll 4
+  for (int c = wave; c < chunks; c += W) {
+    const f32x4 x = ml[static_cast<int64_t>(c) * a.heads];
+    const float f = __builtin_amdgcn_exp2f(x[0] - base);
+    l = __builtin_fmaf(x[1], f, l);
+    any |= x[2] != 0.0f;
+#pragma unroll
+    for (int d = 0; d < kDl; ++d)
+      o[d] = __builtin_fmaf(po[static_cast<int64_t>(c) * a.heads * D + d * 64 + lane], f, o[d]);
+  }
+#pragma unroll
+  for (int d = 0; d < kDl; ++d) s_o[wave][d * 64 + lane] = o[d];
+  if (lane == 0) s_l[wave] = l, s_any[wave] = any;
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  float acc = 0.0f, sum = a.sinks ? __builtin_amdgcn_exp2f(sink - base) : 0.0f;
+  any = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) acc += s_o[w][threadIdx.x], sum += s_l[w], any |= s_any[w];
+  const float vs = e4m3 && a.kv.v_scale ? a.kv.v_scale[head / (a.heads / a.kv.kv_heads)] : 1.0f;
+  a.out[b * a.out_stride + static_cast<int64_t>(head) * D + threadIdx.x] = f32_to_bf16(any ? acc * vs / sum : 0.0f);
+}
+
+// Work-groups of W waves.  With one piece to each sequence (a context or a
+// window that short) the call is one launch.
+constexpr int kWaves = 4;
+constexpr int kMinTiles = 4;      // tiles of the smallest piece of a cut sequence
+constexpr int kWorkGroups = 1024;  // aimed at
+
+struct Cut {
+  int slots;      // pieces aimed at for each tile of 16 heads; 0: none is cut
+  int max_slots;  // and their largest number
+};
+
+Cut cut_of(int B, int64_t most_tiles, int tiles_of_heads) {
+  if (most_tiles <= kMinTiles) return Cut{0, B};
+  const int slots = (kWorkGroups + tiles_of_heads - 1) / tiles_of_heads;
+  // sum of ceil(tiles / size) <= B + slots
+  return Cut{slots, B + slots};
+}
+
+int tiles_of_heads(int heads, int kv_heads) { return kv_heads * ((heads / kv_heads + 15) / 16); }
+
+}  // namespace
+
+size_t decode_workspace_bytes(int B, int heads, int kv_heads, int head_dim) {
+  const Cut c = cut_of(B, 1 << 30, tiles_of_heads(heads, kv_heads));
+  const size_t pieces = static_cast<size_t>(c.max_slots) * heads;
+  return pieces * (head_dim + 4) * sizeof(float) + ((static_cast<size_t>(B) * 2 * sizeof(int) + 15) & ~size_t{15});
+}
+
+hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
+  const int64_t cap = static_cast<int64_t>(a.max_blocks) << a.kv.bs_shift;
+  int64_t most = (cap + kTile - 1) / kTile;
+  if (a.window > 0) most = min(most, (static_cast<int64_t>(a.window) + kTile - 2) / kTile + 1 +
+                                         (static_cast<int64_t>(a.first) + kTile - 1) / kTile);
+  const int th = tiles_of_heads(a.heads, a.kv.kv_heads);
+  const Cut c = cut_of(a.B, most, th);
+  SplitArgs sp{};
+  sp.slots = c.slots;
+  sp.min_tiles = kMinTiles;
+  const size_t pieces = static_cast<size_t>(c.max_slots) * a.heads;
+  sp.part_o = static_cast<float*>(workspace);
+  sp.part_ml = sp.part_o + pieces * a.kv.head_dim;
+  sp.plan = reinterpret_cast<int*>(sp.part_ml + pieces * 4);
+  const dim3 grid(c.max_slots, th);
+#define GX_DECODE(D_, E_) hipLaunchKernelGGL((decode_kernel<D_, E_, kWaves>), grid, dim3(64 * kWaves), 0, s, a, sp)
+  if (a.kv.head_dim == 64) {
+    if (a.kv.e4m3) GX_DECODE(64, true);
+    else GX_DECODE(64, false);
+  } else {
+    if (a.kv.e4m3) GX_DECODE(128, true);
+    else GX_DECODE(128, false);
+  }
+#undef GX_DECODE
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || c.slots == 0) return e;
+  const dim3 joins(static_cast<unsigned>(a.B) * a.heads);
+  if (a.kv.head_dim == 64)
+    hipLaunchKernelGGL(join_kernel<64>, joins, dim3(256), 0, s, a, sp, a.kv.e4m3);
+  else
+    hipLaunchKernelGGL(join_kernel<128>, joins, dim3(256), 0, s, a, sp, a.kv.e4m3);
+  return hipGetLastError();
+}
+
+}  // namespace gxmoe
