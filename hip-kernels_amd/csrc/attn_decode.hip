@@ -65,33 +65,34 @@ struct Piece {
   Seen seen;
 };
 
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) v += __shfl_xor(v, x);
+// The sum over this lane and those before it.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes before in the row of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row 0's sum to row 1, row 2's to row 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // the lower half's to the upper
   return v;
 }
 
 // Sequences are cut into pieces of `size` tiles, the size chosen from all
-// lengths so that the pieces of one kv head are about a.slots in number; every
-// wave works it out from the lengths, which only the device knows.
+// lengths so that the pieces of one kv head are about sp.slots in number; every
+// wave works it out from the lengths, which only the device knows (64 at a
+// time, with scans over the lanes' registers).
 __device__ __forceinline__ bool find_piece(const AttendArgs& a, const SplitArgs& sp, int slot, Piece* p) {
   const int lane = threadIdx.x & 63;
-  int total = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64)
-    total += b0 + lane < a.B ? seen_tiles(a, seq_len(a, min(b0 + lane, a.B - 1))).tiles : 0;
-  total = __builtin_amdgcn_readfirstlane(wave_sum(total));
+  const int len0 = lane < a.B ? seq_len(a, lane) : 0;
+  int total = lane < a.B ? seen_tiles(a, len0).tiles : 0;
+  for (int b0 = 64; b0 < a.B; b0 += 64) total += b0 + lane < a.B ? seen_tiles(a, seq_len(a, b0 + lane)).tiles : 0;
+  total = __builtin_amdgcn_readlane(wave_scan(total), 63);
   const int size = max(sp.min_tiles, (total + sp.slots - 1) / sp.slots);
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const bool in = b0 + lane < a.B;
-    const int tiles = in ? seen_tiles(a, seq_len(a, b0 + lane)).tiles : 0;
-    const int mine = in ? max(1, (tiles + size - 1) / size) : 0;
-    int upto = mine;
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-      const int y = __shfl_up(upto, x);
-      if (lane >= x) upto += y;
-    }
+    const int len = b0 == 0 ? len0 : in ? seq_len(a, b0 + lane) : 0;
+    const int mine = in ? max(1, (seen_tiles(a, len).tiles + size - 1) / size) : 0;
+    const int upto = wave_scan(mine);
     const int all = __builtin_amdgcn_readlane(upto, 63);
     if (slot < before + all) {
       const int at = slot - before;
@@ -100,7 +101,7 @@ __device__ __forceinline__ bool find_piece(const AttendArgs& a, const SplitArgs&
       p->chunks = __builtin_amdgcn_readlane(mine, who);
       const int first = __builtin_amdgcn_readlane(upto, who) - p->chunks;
       p->first_slot = before + first;
-      p->seen = seen_tiles(a, __builtin_amdgcn_readfirstlane(seq_len(a, p->b)));
+      p->seen = seen_tiles(a, __builtin_amdgcn_readlane(len, who));
       p->t0 = (at - first) * size;
       p->t1 = min(p->t0 + size, p->seen.tiles);
       return true;
@@ -110,8 +111,9 @@ __device__ __forceinline__ bool find_piece(const AttendArgs& a, const SplitArgs&
   return false;
 }
 
-// One tile's K and V as a lane holds them.  Half j: tokens 16 j + l % 16, dims
-// (l / 16) D/4 on.  Row i: token 16 (i / 4) + 4 (l / 16) + i % 4, dims
+// One tile's K and V as a lane holds them.  Half j: of token 16 j + l % 16 the
+// 16 bytes from 64 c + 16 (l / 16) on, for every c, so that a load takes 64
+// bytes of a row.  Row i: token 16 (i / 4) + 4 (l / 16) + i % 4, dims
 // (l % 16) D/16 on.
 template <int D, bool kE4m3>
 struct TileRegs {
@@ -121,17 +123,33 @@ struct TileRegs {
   uint32_t v[8][kVd];
 };
 
+typedef const __attribute__((address_space(1))) uint8_t* GlobalBytes;
+
+// A lane's offset as the block at hand sees it: 32 bits on a pointer in scalar
+// registers.  (Hoisted out of the loop it would be a 64-bit sum per load.)
+__device__ __forceinline__ uint32_t here(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// A pointer that is the same in all lanes, kept apart from their offsets.
+__device__ __forceinline__ GlobalBytes scalar(GlobalBytes p) {
+  asm("" : "+s"(p));
+  return p;
+}
+
+// N dwords, 16 bytes at a time `step` bytes apart.
 template <int N>
-__device__ __forceinline__ void load_dwords(const uint8_t* p, uint32_t (&d)[N]) {
+__device__ __forceinline__ void load_dwords(GlobalBytes p, uint32_t (&d)[N], int step = 16) {
   if constexpr (N == 1) {
-    d[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+    d[0] = __builtin_nontemporal_load(reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(p));
   } else if constexpr (N == 2) {
-    const attn_u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const attn_u32x2*>(p));
+    const attn_u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const __attribute__((address_space(1))) attn_u32x2*>(p));
     d[0] = x[0], d[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const attn_u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const attn_u32x4*>(p) + i);
+      const attn_u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const __attribute__((address_space(1))) attn_u32x4*>(p + i * step));
 #pragma unroll
       for (int c = 0; c < 4; ++c) d[4 * i + c] = x[c];
     }
@@ -161,32 +179,42 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
   const int n = lane & 15, g = lane >> 4;
   const int group = a.heads / a.kv.kv_heads;
   const int parts = (group + 15) / 16;  // tiles of 16 heads per kv head
-  const int kvh = blockIdx.y / parts, h0 = kvh * group + (blockIdx.y % parts) * 16;
+  // the tiles of heads of a piece side by side: the pieces that there are come
+  // first in the grid and lie on all CUs (piece-minor, 128 of 1032 work-groups
+  // shared a few CUs: one sequence of 4000, 17.9 us)
+  const int th = a.kv.kv_heads * parts;
+  const int piece = blockIdx.x / th, tile_of_heads = blockIdx.x % th;
+  const int kvh = tile_of_heads / parts, h0 = kvh * group + (tile_of_heads % parts) * 16;
   const int nh = min(16, (kvh + 1) * group - h0);
 
   Piece p;
   if (sp.slots > 0) {
-    if (!find_piece(a, sp, blockIdx.x, &p)) return;
+    if (!find_piece(a, sp, piece, &p)) return;
+    for (int* x : {&p.b, &p.t0, &p.t1, &p.chunks, &p.first_slot, &p.seen.len, &p.seen.low, &p.seen.nf, &p.seen.main,
+                   &p.seen.tiles})
+      *x = __builtin_amdgcn_readfirstlane(*x);  // the same in all lanes: addresses in scalar registers
   } else {
-    p.b = blockIdx.x;
+    p.b = piece;
     p.chunks = 1;
     p.first_slot = 0;
     p.seen = seen_tiles(a, __builtin_amdgcn_readfirstlane(seq_len(a, p.b)));
     p.t0 = 0;
     p.t1 = p.seen.tiles;
   }
-  if (sp.slots > 0 && p.t0 == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+  if (sp.slots > 0 && p.t0 == 0 && tile_of_heads == 0 && threadIdx.x == 0) {
     sp.plan[2 * p.b] = p.first_slot;
     sp.plan[2 * p.b + 1] = p.chunks;
   }
 
-  // queries: head h0 + n, dims g D/4 + 8 s on for step s
+  // queries: head h0 + n, the dims that K's loads bring for step s (a load of
+  // 16 bytes is one step of bf16 and two of e4m3)
   bf16x8 q[kSteps];
   {
-    const uint16_t* row = a.q + p.b * a.q_stride + static_cast<int64_t>(h0 + min(n, nh - 1)) * D + g * (D / 4);
+    const uint16_t* row = a.q + p.b * a.q_stride + static_cast<int64_t>(h0 + min(n, nh - 1)) * D;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      attn_u32x4 x = reinterpret_cast<const attn_u32x4*>(row)[s];
+      const int d = kE4m3 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
+      attn_u32x4 x = *reinterpret_cast<const attn_u32x4*>(row + d);
       if (n >= nh) x = attn_u32x4{0, 0, 0, 0};
       q[s] = __builtin_bit_cast(bf16x8, x);
     }
@@ -206,26 +234,42 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
     if (i < mine) {
       const int t = tile_of(i) + 16 * (lane & 1);
       if (t < p.seen.len) page = a.tables[p.b * a.table_stride + (t >> a.kv.bs_shift)];
-      if (page >= a.kv.num_blocks) page = -1;
     }
     return page;
   };
-  const uint8_t* kb = static_cast<const uint8_t*>(a.kv.k) + kvh * a.kv.sh * kSize;
-  const uint8_t* vb = static_cast<const uint8_t*>(a.kv.v) + kvh * a.kv.sh * kSize;
+  GlobalBytes kb = (GlobalBytes)(static_cast<const uint8_t*>(a.kv.k) + kvh * a.kv.sh * kSize);
+  GlobalBytes vb = (GlobalBytes)(static_cast<const uint8_t*>(a.kv.v) + kvh * a.kv.sh * kSize);
   const int st = static_cast<int>(a.kv.st) * kSize;
-  const uint32_t koff = n * st + g * (D / 4) * kSize, voff = 4 * g * st + n * (D / 16) * kSize;
+  const uint32_t koff = n * st + g * 16, voff = 4 * g * st + n * (D / 16) * kSize;
   const int mask = (1 << a.kv.bs_shift) - 1;
 
-  int pages = load_pages(0), next_pages = -1;
+  // where their halves lie in K and V (the cache's first page where there is
+  // none: what is read there is hidden), and which have a page
+  int64_t off;
+  uint64_t paged;
+  auto locate = [&](int i0, int page) {
+    const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.num_blocks);
+    const int t = tile_of(i0 + (lane >> 1)) + 16 * (lane & 1);
+    off = (ok ? page : 0) * a.kv.sb * kSize + static_cast<int64_t>(t & mask) * st;
+    paged = __ballot(ok);
+  };
+  locate(0, load_pages(0));
+  int next_pages = -1;
   auto load = [&](int i, Regs& r) {
-    const int t = tile_of(i);
+    const uint32_t ko = here(koff), vo = here(voff);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int page = max(0, __builtin_amdgcn_readlane(pages, 2 * (i & 31) + j));
-      const int64_t at = page * a.kv.sb * kSize + static_cast<int64_t>((t + 16 * j) & mask) * st;
-      load_dwords(kb + at + koff, r.k[j]);
+      const int from = 2 * (i & 31) + j;
+      const int64_t at =
+          static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(
+                                   __builtin_amdgcn_readlane(static_cast<int>(off >> 32), from)))
+                               << 32) |
+          static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(off), from));
+      GlobalBytes ks = scalar(kb + at);
+      GlobalBytes vs = vb + at;
+      load_dwords(ks + ko, r.k[j], 64);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) load_dwords(vb + at + voff + static_cast<uint32_t>(c * st), r.v[4 * j + c]);
+      for (int c = 0; c < 4; ++c) load_dwords(scalar(vs + c * st) + vo, r.v[4 * j + c]);
     }
   };
 
@@ -235,7 +279,7 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
 #pragma unroll
   for (int d = 0; d < kDt; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  auto compute = [&](int i, int have0, int have1, Regs& r) {
+  auto compute = [&](int i, bool have0, bool have1, Regs& r) {
     const int t = tile_of(i);
     f32x4 s[2];
 #pragma unroll
@@ -314,17 +358,25 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
     }
   };
 
-  Regs ra, rb;
-  if (mine > 0) load(0, ra);
-  for (int i = 0; i < mine; i += 2) {
-    const int a0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31)) >= 0, a1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1) >= 0;
-    const int b0 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 2) >= 0, b1 = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 3) >= 0;
-    if ((i & 31) == 0 && i + 32 < mine) next_pages = load_pages(i + 32);
-    if (i + 1 < mine) load(i + 1, rb);
-    compute(i, a0, a1, ra);
-    if ((i & 31) == 30) pages = next_pages;
-    if (i + 2 < mine) load(i + 2, ra);
-    if (i + 1 < mine) compute(i + 1, b0, b1, rb);
+  // Two tiles in turn: the next one is on its way while one is worked on.  The
+  // loads stand outside of any branch, since a wait counts the loads behind it
+  // and a branch would make that number the smaller one (a wave's last load is
+  // its last tile again).
+  auto have = [&](int i, int j) { return (paged >> (2 * (i & 31) + j) & 1) != 0; };
+  if (mine > 0) {
+    Regs ra, rb;
+    load(0, ra);
+    int i = 0;
+    for (; i + 1 < mine; i += 2) {
+      const bool a0 = have(i, 0), a1 = have(i, 1), b0 = have(i + 1, 0), b1 = have(i + 1, 1);
+      if ((i & 31) == 0) next_pages = load_pages(i + 32);
+      load(i + 1, rb);
+      compute(i, a0, a1, ra);
+      if ((i & 31) == 30 && i + 2 < mine) locate(i + 2, next_pages);
+      load(min(i + 2, mine - 1), ra);
+      compute(i + 1, b0, b1, rb);
+    }
+    if (i < mine) compute(i, have(i, 0), have(i, 1), ra);
   }
 
   // the wave's sum, then the waves'
@@ -369,84 +421,134 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
       for (int c = 0; c < 4; ++c) acc[c] = any ? acc[c] * f : 0.0f;
       *reinterpret_cast<attn_u32x2*>(to) = attn_u32x2{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
     } else {
-      const int64_t at = static_cast<int64_t>(blockIdx.x) * a.heads + head;
+      const int64_t at = static_cast<int64_t>(piece) * a.heads + head;
       *reinterpret_cast<f32x4*>(sp.part_o + at * D + d) = acc;
       if (d == 0) reinterpret_cast<f32x4*>(sp.part_ml)[at] = f32x4{top, sum, any ? 1.0f : 0.0f, 0.0f};
     }
   }
 }
 
-// Joins the pieces of a sequence, one work-group per (sequence, head): wave w
-// takes pieces w, w + 4, ...; a lane takes D / 64 dims.
-template <int D>
+// Joins the pieces of a sequence: T threads for each (sequence, head), 256 / T
+// of these to a work-group.  A lane takes four dims of the pieces row, row + R,
+// ..., with a reference of its own, so that nothing but the plan is waited for
+// before they are read.
+template <int D, int T>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, SplitArgs sp, bool e4m3) {
-  constexpr int W = 4, kDl = D / 64;
-  __shared__ float s_o[W][D];
-  __shared__ float s_l[W];
-  __shared__ int s_any[W];
-  const int b = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
-  const int first = sp.plan[2 * b], chunks = sp.plan[2 * b + 1];
-  if (chunks <= 1) return;  // written by its only work-group
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const f32x4* ml = reinterpret_cast<const f32x4*>(sp.part_ml) + static_cast<int64_t>(first) * a.heads + head;
+  constexpr int kLanes = D / 4, R = T / kLanes;
+  __shared__ f32x4 s_o[256 / kLanes][kLanes];
+  __shared__ float s_m[256 / kLanes], s_l[256 / kLanes];
+  __shared__ int s_any[256 / kLanes];
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (256 / T) + threadIdx.x / T;
+  const int d = threadIdx.x % kLanes, row = threadIdx.x / kLanes, r0 = row / R * R;
+  const bool in = at < static_cast<int64_t>(a.B) * a.heads;
+  const int b = in ? static_cast<int>(at / a.heads) : 0, head = in ? static_cast<int>(at % a.heads) : 0;
+  const int first = sp.plan[2 * b], chunks = in ? sp.plan[2 * b + 1] : 0;
   const float sink = a.sinks ? bf16_to_f32(a.sinks[head]) * kLog2e : kNegInf;
-  float top = sink;
-  for (int c = lane; c < chunks; c += 64) top = __builtin_fmaxf(top, ml[static_cast<int64_t>(c) * a.heads][0]);
+  const float vs = e4m3 && a.kv.v_scale ? a.kv.v_scale[head / (a.heads / a.kv.kv_heads)] : 1.0f;
+  if (chunks > 1) {  // otherwise written by its only work-group
+    const f32x4* ml = reinterpret_cast<const f32x4*>(sp.part_ml) + static_cast<int64_t>(first) * a.heads + head;
+    const f32x4* po = reinterpret_cast<const f32x4*>(sp.part_o + (static_cast<int64_t>(first) * a.heads + head) * D) + d;
+    float m = kNegInf, l = 0.0f;
+    f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    int any = 0;
+    constexpr int U = 8;
+    for (int c0 = row - r0; c0 < chunks; c0 += U * R) {
+      f32x4 x[U], y[U];
+      float top = m;
 #pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x));
+      for (int u = 0; u < U; ++u) {
+        const int64_t c = min(c0 + u * R, chunks - 1);
+        x[u] = ml[c * a.heads];
+        y[u] = po[c * a.heads * kLanes];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (c0 + u * R >= chunks) x[u] = f32x4{kNegInf, 0.0f, 0.0f, 0.0f};
+        top = __builtin_fmaxf(top, x[u][0]);
+      }
+      const float base = top == kNegInf ? 0.0f : top;
+      const float keep = __builtin_amdgcn_exp2f(m - base);
+      m = top;
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= keep;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (c0 + u * R >= chunks) continue;
+        const float f = __builtin_amdgcn_exp2f(x[u][0] - base);
+        l = __builtin_fmaf(x[u][1], f, l);
+        any |= x[u][2] != 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(y[u][e], f, o[e]);
+      }
+    }
+    s_o[row][d] = o;
+    if (d == 0) s_m[row] = m, s_l[row] = l, s_any[row] = any;
+  }
+  __syncthreads();
+  if (chunks <= 1 || row != r0) return;
+  float top = sink;
+#pragma unroll
+  for (int r = 0; r < R; ++r) top = __builtin_fmaxf(top, s_m[r0 + r]);
   const float base = top == kNegInf ? 0.0f : top;
-  float l = 0.0f, o[kDl];
+  float sum = a.sinks ? __builtin_amdgcn_exp2f(sink - base) : 0.0f;
+  f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   int any = 0;
 #pragma unroll
-  for (int d = 0; d < kDl; ++d) o[d] = 0.0f;
-  const float* po = sp.part_o + (static_cast<int64_t>(first) * a.heads + head) * D;
-#pragma unroll 4
-  for (int c = wave; c < chunks; c += W) {
-    const f32x4 x = ml[static_cast<int64_t>(c) * a.heads];
-    const float f = __builtin_amdgcn_exp2f(x[0] - base);
-    l = __builtin_fmaf(x[1], f, l);
-    any |= x[2] != 0.0f;
+  for (int r = 0; r < R; ++r) {
+    const float f = __builtin_amdgcn_exp2f(s_m[r0 + r] - base);
+    sum = __builtin_fmaf(s_l[r0 + r], f, sum);
+    any |= s_any[r0 + r];
 #pragma unroll
-    for (int d = 0; d < kDl; ++d)
-      o[d] = __builtin_fmaf(po[static_cast<int64_t>(c) * a.heads * D + d * 64 + lane], f, o[d]);
+    for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(s_o[r0 + r][d][e], f, acc[e]);
   }
+  const float f = vs / sum;
 #pragma unroll
-  for (int d = 0; d < kDl; ++d) s_o[wave][d * 64 + lane] = o[d];
-  if (lane == 0) s_l[wave] = l, s_any[wave] = any;
-  __syncthreads();
-  if (threadIdx.x >= D) return;
-  float acc = 0.0f, sum = a.sinks ? __builtin_amdgcn_exp2f(sink - base) : 0.0f;
-  any = 0;
-#pragma unroll
-  for (int w = 0; w < W; ++w) acc += s_o[w][threadIdx.x], sum += s_l[w], any |= s_any[w];
-  const float vs = e4m3 && a.kv.v_scale ? a.kv.v_scale[head / (a.heads / a.kv.kv_heads)] : 1.0f;
-  a.out[b * a.out_stride + static_cast<int64_t>(head) * D + threadIdx.x] = f32_to_bf16(any ? acc * vs / sum : 0.0f);
+  for (int e = 0; e < 4; ++e) acc[e] = any ? acc[e] * f : 0.0f;
+  *reinterpret_cast<attn_u32x2*>(a.out + b * a.out_stride + static_cast<int64_t>(head) * D + 4 * d) =
+      attn_u32x2{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
 }
 
 // Work-groups of W waves.  With one piece to each sequence (a context or a
 // window that short) the call is one launch.
 constexpr int kWaves = 4;
-constexpr int kMinTiles = 4;      // tiles of the smallest piece of a cut sequence
-constexpr int kWorkGroups = 1024;  // aimed at
+constexpr int kMinTiles = 8;       // tiles of the smallest piece of a cut sequence
+constexpr int kWideJoins = 1024;   // (sequence, head) pairs up to which a join is a whole work-group
 
 struct Cut {
   int slots;      // pieces aimed at for each tile of 16 heads; 0: none is cut
   int max_slots;  // and their largest number
 };
 
-Cut cut_of(int B, int64_t most_tiles, int tiles_of_heads) {
+// Work-groups aimed at: three for each CU with heads of 64 dims, two with 128,
+// which is what the registers leave there.  Four with 64 dims are possible and
+// slower (one sequence of 131072, bf16: 55.7 against 52.7 us; 32 of 2000: 33.3
+// against 29.7; fewer partial sums, and a CU's loads are enough in flight).
+Cut cut_of(int B, int64_t most_tiles, int tiles_of_heads, int head_dim) {
   if (most_tiles <= kMinTiles) return Cut{0, B};
-  const int slots = (kWorkGroups + tiles_of_heads - 1) / tiles_of_heads;
+  const int work_groups = head_dim == 64 ? 768 : 512;
+  const int slots = (work_groups + tiles_of_heads - 1) / tiles_of_heads;
   // sum of ceil(tiles / size) <= B + slots
-  return Cut{slots, B + slots};
+  const int64_t pieces = static_cast<int64_t>(B) * ((most_tiles + kMinTiles - 1) / kMinTiles);
+  return Cut{slots, static_cast<int>(pieces < B + slots ? pieces : B + slots)};
 }
 
 int tiles_of_heads(int heads, int kv_heads) { return kv_heads * ((heads / kv_heads + 15) / 16); }
 
+template <int D>
+void launch_join(const AttendArgs& a, const SplitArgs& sp, hipStream_t s) {
+  const int64_t pairs = static_cast<int64_t>(a.B) * a.heads;
+  if (pairs <= kWideJoins)
+    hipLaunchKernelGGL((join_kernel<D, 256>), dim3(static_cast<unsigned>(pairs)), dim3(256), 0, s, a, sp, a.kv.e4m3);
+  else
+    hipLaunchKernelGGL((join_kernel<D, 64>), dim3(static_cast<unsigned>((pairs + 3) / 4)), dim3(256), 0, s, a, sp,
+                       a.kv.e4m3);
+}
+
 }  // namespace
 
 size_t decode_workspace_bytes(int B, int heads, int kv_heads, int head_dim) {
-  const Cut c = cut_of(B, 1 << 30, tiles_of_heads(heads, kv_heads));
+  const Cut c = cut_of(B, 1 << 30, tiles_of_heads(heads, kv_heads), head_dim);
   const size_t pieces = static_cast<size_t>(c.max_slots) * heads;
   return pieces * (head_dim + 4) * sizeof(float) + ((static_cast<size_t>(B) * 2 * sizeof(int) + 15) & ~size_t{15});
 }
@@ -457,7 +559,7 @@ hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
   if (a.window > 0) most = min(most, (static_cast<int64_t>(a.window) + kTile - 2) / kTile + 1 +
                                          (static_cast<int64_t>(a.first) + kTile - 1) / kTile);
   const int th = tiles_of_heads(a.heads, a.kv.kv_heads);
-  const Cut c = cut_of(a.B, most, th);
+  const Cut c = cut_of(a.B, most, th, a.kv.head_dim);
   SplitArgs sp{};
   sp.slots = c.slots;
   sp.min_tiles = kMinTiles;
@@ -465,7 +567,7 @@ hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
   sp.part_o = static_cast<float*>(workspace);
   sp.part_ml = sp.part_o + pieces * a.kv.head_dim;
   sp.plan = reinterpret_cast<int*>(sp.part_ml + pieces * 4);
-  const dim3 grid(c.max_slots, th);
+  const dim3 grid(static_cast<unsigned>(c.max_slots) * th);
 #define GX_DECODE(D_, E_) hipLaunchKernelGGL((decode_kernel<D_, E_, kWaves>), grid, dim3(64 * kWaves), 0, s, a, sp)
   if (a.kv.head_dim == 64) {
     if (a.kv.e4m3) GX_DECODE(64, true);
@@ -475,13 +577,10 @@ hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
     else GX_DECODE(128, false);
   }
 #undef GX_DECODE
-  hipError_t e = hipGetLastError();
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess || c.slots == 0) return e;
-  const dim3 joins(static_cast<unsigned>(a.B) * a.heads);
-  if (a.kv.head_dim == 64)
-    hipLaunchKernelGGL(join_kernel<64>, joins, dim3(256), 0, s, a, sp, a.kv.e4m3);
-  else
-    hipLaunchKernelGGL(join_kernel<128>, joins, dim3(256), 0, s, a, sp, a.kv.e4m3);
+  if (a.kv.head_dim == 64) launch_join<64>(a, sp, s);
+  else launch_join<128>(a, sp, s);
   return hipGetLastError();
 }
 
