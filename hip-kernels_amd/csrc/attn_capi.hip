@@ -128,7 +128,7 @@ int check_attend(AttendArgs* a, const gptoss_kv_cache* cache, const gptoss_atten
                        need);
     if (!aligned16(workspace)) return set_error(GPTOSS_ERR_INVALID, "workspace must be 16-byte aligned");
   }
-  if (static_cast<int64_t>(rows) * a->heads > 0x7fffffff || a->heads > 65535)
+  if (static_cast<int64_t>(rows > B ? rows : B) * a->heads > 0x7fffffff - 65536 || a->heads > 65535)
     return set_error(GPTOSS_ERR_UNSUPPORTED, "%d rows of %d heads in one call", rows, a->heads);
   // all sequences' tokens, in units of 16, are counted in 32 bits
   if (static_cast<int64_t>(a->max_blocks) * (1 << a->kv.bs_shift) / 16 + 1 > 0x7fffffff / B)
@@ -269,7 +269,7 @@ int gptoss_paged_attention_prefill(const uint16_t* q, int64_t q_stride, const in
   if (rc != GPTOSS_OK) return rc;
   if (num_tokens == 0 || num_seqs == 0) return ok();
   if (query_offsets == nullptr) return set_error(GPTOSS_ERR_INVALID, "null query_offsets");
-  HIP_TRY(launch_attend_rows(a, static_cast<hipStream_t>(stream)), "paged attention prefill launch");
+  HIP_TRY(launch_prefill(a, static_cast<hipStream_t>(stream)), "paged attention prefill launch");
   return ok();
 }
 

@@ -29,7 +29,6 @@ namespace gxmoe {
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 32;      // tokens per step of a wave
@@ -64,17 +63,6 @@ struct Piece {
   int b, t0, t1, chunks, first_slot;
   Seen seen;
 };
-
-// The sum over this lane and those before it.
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes before in the row of 16
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row 0's sum to row 1, row 2's to row 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // the lower half's to the upper
-  return v;
-}
 
 // Sequences are cut into pieces of `size` tiles, the size chosen from all
 // lengths so that the pieces of one kv head are about sp.slots in number; every
@@ -154,14 +142,6 @@ __device__ __forceinline__ void load_dwords(GlobalBytes p, uint32_t (&d)[N], int
       for (int c = 0; c < 4; ++c) d[4 * i + c] = x[c];
     }
   }
-}
-
-__device__ __forceinline__ uint32_t bits(bf16x2 v) { return __builtin_bit_cast(uint32_t, v); }
-
-// The four e4m3 codes of a dword as bf16 (exact).
-__device__ __forceinline__ void widen(uint32_t codes, uint32_t* out) {
-  out[0] = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false));
-  out[1] = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true));
 }
 
 template <int D, bool kE4m3, int W>

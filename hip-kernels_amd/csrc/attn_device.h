@@ -12,6 +12,23 @@ typedef uint32_t attn_u32x2 __attribute__((ext_vector_type(2)));
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// The sum over this lane and those before it.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes before in the row of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row 0's sum to row 1, row 2's to row 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // the lower half's to the upper
+  return v;
+}
+
+// The four e4m3 codes of a dword as bf16 (exact).
+__device__ __forceinline__ void widen(uint32_t codes, uint32_t* out) {
+  out[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false));
+  out[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true));
+}
+
 // Tokens of sequence b: negative lengths read as 0, longer ones than its
 // table holds are cut to that.
 __device__ __forceinline__ int seq_len(const AttendArgs& a, int b) {

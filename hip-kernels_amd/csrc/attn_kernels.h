@@ -60,6 +60,6 @@ hipError_t launch_rope_table(const RopeTableArgs& a, hipStream_t s);
 hipError_t launch_rope_append(const AppendArgs& a, hipStream_t s);
 size_t decode_workspace_bytes(int B, int heads, int kv_heads, int head_dim);
 hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s);
-hipError_t launch_attend_rows(const AttendArgs& a, hipStream_t s);
+hipError_t launch_prefill(const AttendArgs& a, hipStream_t s);
 
 }  // namespace gxmoe

@@ -1,0 +1,407 @@
+// attn_prefill.hip -- causal attention of prompt chunks over the paged cache
+// (gfx950).
+//
+// Mathematics: the softmax with a running reference and sum of attn_decode.hip,
+// for 128 rows at a time.  A row is one query head of one new token; the heads
+// that share a kv head lie side by side, so that a work-group's rows are few
+// tokens and what a window or the diagonal cuts off is cut off for all of them.
+//
+// A work-group is four waves of 32 rows over tiles of 64 tokens.  The products are
+// S^T = K Q^T and O^T = V^T P^T in 32 x 32 x 16 steps: S^T leaves a lane with its
+// own row and the tokens that the second product wants from it, so the weights
+// stay in registers.  K and V go through LDS, 16-byte pieces permuted by the
+// token so that neither the row reads of K nor the transposing reads of V meet
+// in a bank; the next tile is on its way to registers while one is worked on.
+#include "attn_device.h"
+
+namespace gxmoe {
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef const __attribute__((address_space(1))) uint8_t* GlobalBytes;
+typedef __attribute__((address_space(3))) uint8_t* LdsBytes;
+
+constexpr int kRows = 128;    // rows of a work-group
+constexpr int kTile = 64;     // tokens of a step
+constexpr float kSlack = 8.0f;  // how far a score may exceed the reference, in powers of two
+
+struct Chunk {
+  int b, row0;     // sequence, its first row of q
+  int tokens;      // new tokens of the tile
+  int tok0;        // the first one, within the sequence's new ones
+  int pos0;        // its position
+  int len;
+};
+
+// Tile `at` of all tiles of `per` tokens, the last one first: the longest rows
+// of a prompt begin earliest.
+__device__ __forceinline__ bool find_chunk(const AttendArgs& a, int at, int per, Chunk* c) {
+  const int lane = threadIdx.x & 63;
+  auto span = [&](int b, int* begin) {  // new tokens of sequence b, within the rows that there are
+    const int lo = min(max(a.offsets[b], 0), a.rows);
+    *begin = lo;
+    return max(0, min(a.offsets[b + 1], a.rows) - lo);
+  };
+  int total = 0, begin;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int tiles = b0 + lane < a.B ? (span(b0 + lane, &begin) + per - 1) / per : 0;
+    total += __builtin_amdgcn_readlane(wave_scan(tiles), 63);
+  }
+  at = total - 1 - at;
+  if (at < 0) return false;
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    begin = 0;
+    const int n = b0 + lane < a.B ? span(b0 + lane, &begin) : 0;
+    const int upto = before + wave_scan((n + per - 1) / per);
+    const uint64_t reached = __ballot(at < upto);
+    if (reached != 0) {
+      const int who = __builtin_ctzll(reached);
+      const int mine = __builtin_amdgcn_readlane(n, who);
+      const int first = __builtin_amdgcn_readlane(upto, who) - (mine + per - 1) / per;
+      c->b = b0 + who;
+      c->row0 = __builtin_amdgcn_readlane(begin, who);
+      c->tok0 = (at - first) * per;
+      c->tokens = min(per, mine - c->tok0);
+      c->len = __builtin_amdgcn_readfirstlane(seq_len(a, c->b));
+      c->pos0 = c->len - mine + c->tok0;
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+__device__ __forceinline__ bool not_finite(uint32_t two) {  // either of two bf16
+  return (((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0;
+}
+
+template <int D, bool kE4m3>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArgs a) {
+  constexpr int kSize = kE4m3 ? 1 : 2;
+  constexpr int kPieces = D * kSize / 16;      // 16-byte pieces of a token's row in memory
+  constexpr int kLoads = 16 * kPieces / 64;    // loads of a wave for its 16 tokens of K, and of V
+  constexpr int kRowBytes = 2 * D;             // of a token in LDS
+  constexpr int kHalf = kTile * kRowBytes;     // K, then V
+  constexpr int kSteps = D / 16, kDb = D / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t s_kv[2][2 * kHalf];
+  __shared__ int s_odd;  // whether put() left out a value
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, h = lane >> 5;
+  const int group = a.heads / a.kv.kv_heads, per = kRows / group;
+  const int kvh = blockIdx.x % a.kv.kv_heads;
+  Chunk c;
+  if (!find_chunk(a, blockIdx.x / a.kv.kv_heads, per, &c)) return;
+  for (int* x : {&c.b, &c.row0, &c.tokens, &c.tok0, &c.pos0, &c.len}) *x = __builtin_amdgcn_readfirstlane(*x);
+
+  // this lane's row
+  const int r = 32 * wave + n;
+  const int tok = r / group, head = kvh * group + r % group;
+  const bool mine = tok < c.tokens;
+  const int pos = mine ? c.pos0 + tok : -1;
+  const int64_t qrow = c.row0 + c.tok0 + (mine ? tok : 0);
+  bf16x8 q[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    attn_u32x4 x = *reinterpret_cast<const attn_u32x4*>(a.q + qrow * a.q_stride + static_cast<int64_t>(head) * D + 16 * s + 8 * h);
+    if (!mine) x = attn_u32x4{0, 0, 0, 0};
+    q[s] = __builtin_bit_cast(bf16x8, x);
+  }
+  const float scale = a.scale_log2 * (kE4m3 && a.kv.k_scale ? a.kv.k_scale[kvh] : 1.0f);
+
+  // the tiles that the rows see: the first tokens', then the window's
+  const int pmin = c.pos0, pmax = c.pos0 + c.tokens - 1;
+  const int low = a.window > 0 ? max(0, pmin - a.window + 1) : 0;
+  const int main = low / kTile, nf = min((min(a.first, low) + kTile - 1) / kTile, main);
+  const int tiles = pmax < 0 ? 0 : nf + pmax / kTile + 1 - main;
+  auto tile_at = [&](int i) { return (i < nf ? i : main + i - nf) * kTile; };
+
+  // Pages of 16 tiles at a time: lane 4 i + j has tokens 16 j on of tile i0 + i.
+  auto load_pages = [&](int i0) {
+    const int i = i0 + (lane >> 2);
+    int page = -1;
+    if (i < tiles) {
+      const int t = tile_at(i) + 16 * (lane & 3);
+      if (t < c.len) page = a.tables[c.b * a.table_stride + (t >> a.kv.bs_shift)];
+    }
+    return page;
+  };
+  const int mask = (1 << a.kv.bs_shift) - 1;
+  const int st = static_cast<int>(a.kv.st) * kSize;
+  int64_t off;     // where the lane's 16 tokens lie in K and in V
+  uint64_t paged;  // which of them have a page
+  auto locate = [&](int i0, int page) {
+    const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.num_blocks);
+    const int t = tile_at(i0 + (lane >> 2)) + 16 * (lane & 3);
+    off = (ok ? page : 0) * a.kv.sb * kSize + static_cast<int64_t>(t & mask) * st;
+    paged = __ballot(ok);
+  };
+  auto pages_of = [&](int i) { return static_cast<uint32_t>(paged >> (4 * (i & 15))) & 15u; };
+
+  // staging: wave w brings tokens 16 w to 16 w + 15, load j the rows from
+  // j * 64 / kPieces on
+  GlobalBytes kb = (GlobalBytes)(static_cast<const uint8_t*>(a.kv.k) + kvh * a.kv.sh * kSize);
+  GlobalBytes vb = (GlobalBytes)(static_cast<const uint8_t*>(a.kv.v) + kvh * a.kv.sh * kSize);
+  const int srow = lane / kPieces, spiece = lane % kPieces;
+  constexpr int kRowsPerLoad = 64 / kPieces;
+  const uint32_t goff = srow * st + spiece * 16;
+  attn_u32x4 kr[kLoads], vr[kLoads];
+  auto load = [&](int i) {
+    const int from = 4 * (i & 15) + wave;
+    const int64_t at = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(
+                                                __builtin_amdgcn_readlane(static_cast<int>(off >> 32), from)))
+                                            << 32) |
+                       static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(off), from));
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int64_t to = at + j * kRowsPerLoad * st;
+      kr[j] = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x4*>(kb + to + goff);
+      vr[j] = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x4*>(vb + to + goff);
+    }
+  };
+  // whole: every row of the work-group sees every token of the tile
+  auto is_whole = [&](int t, uint32_t pages) {
+    return pages == 15u && t + kTile - 1 <= pmin && (a.window == 0 || t > pmax - a.window || t + kTile <= a.first);
+  };
+  // To LDS.  0 times an infinity or a NaN is not 0, so in a tile that not every
+  // row sees whole such values become 0 here; the rows that do see one get it
+  // at the end.
+  auto put = [&](int buf, bool whole) {
+    uint8_t* kd = s_kv[buf];
+    uint8_t* vd = kd + kHalf;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int row = 16 * wave + j * kRowsPerLoad + srow;
+      uint32_t w[2][2][4];
+      if constexpr (kE4m3) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          widen(kr[j][e], &w[0][e >> 1][2 * (e & 1)]);
+          widen(vr[j][e], &w[1][e >> 1][2 * (e & 1)]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[0][0][e] = kr[j][e], w[1][0][e] = vr[j][e];
+      }
+#pragma unroll
+      for (int p = 0; p < (kE4m3 ? 2 : 1); ++p) {
+        if (!whole) {
+          bool odd = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd |= not_finite(w[1][p][e]);
+          if (__ballot(odd) != 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t x = w[1][p][e];
+              w[1][p][e] = ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) |
+                           ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
+            }
+            if (lane == 0) s_odd = 1;
+          }
+        }
+        const int piece = kE4m3 ? 2 * spiece + p : spiece;
+        const int at = row * kRowBytes + ((piece ^ (row & 7)) << 4);
+        *reinterpret_cast<attn_u32x4*>(kd + at) = attn_u32x4{w[0][p][0], w[0][p][1], w[0][p][2], w[0][p][3]};
+        *reinterpret_cast<attn_u32x4*>(vd + at) = attn_u32x4{w[1][p][0], w[1][p][1], w[1][p][2], w[1][p][3]};
+      }
+    }
+  };
+
+  float m = kNegInf, l = 0.0f;
+  bool any = false;
+  f32x16 o[kDb];
+#pragma unroll
+  for (int d = 0; d < kDb; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+
+  // LDS addresses.  K: token 32 b + n, piece 2 s + h.  V: the 16 lanes of a quarter
+  // read 4 tokens x 16 dims and are left with 4 tokens of one dim each.
+  const int krow = n * kRowBytes;
+  const int vrow = 4 * h + ((lane & 15) >> 2);  // and vrow + 8 and so on
+  const int vpiece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  auto value = [&](int buf, int d, int s) {  // dims 32 d on of the tokens of step s
+    bf16x8 x;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int at = (16 * s + 8 * e + vrow) * kRowBytes + (((4 * d + vpiece) ^ vrow) << 4) + 8 * (lane & 1);
+      const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)((LdsBytes)s_kv[buf] + kHalf + at));
+      reinterpret_cast<s16x4*>(&x)[e] = y;
+    }
+    return x;
+  };
+
+  auto compute = [&](int i, int buf, uint32_t pages) {
+    const int t = tile_at(i);
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const bf16x8 x = *reinterpret_cast<const bf16x8*>(&s_kv[buf][32 * b * kRowBytes + krow + (((2 * k + h) ^ (n & 7)) << 4)]);
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, q[k], s[b], 0, 0, 0);
+      }
+    }
+    const bool whole = is_whole(t, pages);
+    if (whole) {
+      any = true;
+    } else {
+      const int rel = pos - t - 4 * h, lowest = a.window > 0 ? rel - a.window : -1 - 4 * h, f = a.first - t - 4 * h;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int x = 32 * b + 8 * (e >> 2) + (e & 3);
+          const bool in = (pages >> (2 * b + (e >> 3)) & 1u) != 0 && x <= rel && (x > lowest || x < f);
+          any |= in;
+          s[b][e] = in ? s[b][e] : kNegInf;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 32; ++e) top = __builtin_fmaxf(top, s[e >> 4][e & 15]);
+    top *= scale;
+    if (__ballot(top > m + kSlack) != 0) {
+      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+      const float mn = __builtin_fmaxf(m, top);
+      const float keep = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
+      m = mn;
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < kDb; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] *= keep;
+    }
+    const float base = m == kNegInf ? 0.0f : m;
+    bf16x8 w[4];
+    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 1][8 * (k & 1) + e], scale, -base));
+        part[e & 3] += p[e];
+      }
+      w[k] = __builtin_bit_cast(bf16x8, attn_u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
+                                                   pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])});
+    }
+    l += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+    for (int d = 0; d < kDb; ++d)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value(buf, d, k), w[k], o[d], 0, 0, 0);
+  };
+
+  if (threadIdx.x == 0) s_odd = 0;
+  __syncthreads();
+  if (tiles > 0) {
+    locate(0, load_pages(0));
+    load(0);
+    uint32_t pages = pages_of(0);
+    put(0, is_whole(tile_at(0), pages));
+    __syncthreads();
+    int next = -1;
+    for (int i = 0; i < tiles; ++i) {
+      if ((i & 15) == 0) next = load_pages(i + 16);
+      if ((i & 15) == 15) locate(i + 1, next);
+      const uint32_t ahead = i + 1 < tiles ? pages_of(i + 1) : 0;
+      if (i + 1 < tiles) load(i + 1);
+      compute(i, i & 1, pages);
+      if (i + 1 < tiles) put((i + 1) & 1, is_whole(tile_at(i + 1), ahead));
+      pages = ahead;
+      __syncthreads();
+    }
+  }
+  if (s_odd != 0) {
+    // what put() left out, for the rows that see it
+    for (int i = 0; i < tiles; ++i) {
+      for (int x = 0; x < kTile; ++x) {
+        const int t = tile_at(i) + x;
+        if (t >= c.len) break;
+        const int page = a.tables[c.b * a.table_stride + (t >> a.kv.bs_shift)];
+        if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.kv.num_blocks)) continue;
+        uint32_t all = 0;  // whether this tile went through put() unchanged
+        for (int j = 0; j < 4; ++j) {
+          const int u = tile_at(i) + 16 * j;
+          const int g = u < c.len ? a.tables[c.b * a.table_stride + (u >> a.kv.bs_shift)] : -1;
+          all |= static_cast<uint32_t>(g) < static_cast<uint32_t>(a.kv.num_blocks) ? 1u << j : 0u;
+        }
+        if (is_whole(tile_at(i), all) || pos < 0 || !sees(a, pos, t)) continue;
+        GlobalBytes v = vb + page * a.kv.sb * kSize + static_cast<int64_t>(t & mask) * st + 4 * h * kSize;
+#pragma unroll
+        for (int d = 0; d < kDb; ++d)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t w[2];
+            if constexpr (kE4m3) {
+              widen(*reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(v + 32 * d + 8 * k), w);
+            } else {
+              const attn_u32x2 y = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x2*>(v + 64 * d + 16 * k);
+              w[0] = y[0], w[1] = y[1];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y = bf16_to_f32(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))));
+              o[d][4 * k + e] += (__float_as_uint(y) & 0x7f800000u) == 0x7f800000u ? y : 0.0f;
+            }
+          }
+      }
+    }
+  }
+
+  l += __shfl_xor(l, 32);
+  any |= __shfl_xor(static_cast<int>(any), 32) != 0;
+  if (!mine) return;
+  float sum = l;
+  if (a.sinks) {
+    const float sink = bf16_to_f32(a.sinks[head]) * kLog2e;
+    const float top = __builtin_fmaxf(m, sink), base = top == kNegInf ? 0.0f : top;
+    const float keep = __builtin_amdgcn_exp2f(m - base);
+    sum = l * keep + __builtin_amdgcn_exp2f(sink - base);
+#pragma unroll
+    for (int d = 0; d < kDb; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] *= keep;
+  }
+  const float vs = kE4m3 && a.kv.v_scale ? a.kv.v_scale[kvh] : 1.0f;
+  const float f = vs / sum;
+  uint16_t* to = a.out + qrow * a.out_stride + static_cast<int64_t>(head) * D + 4 * h;
+#pragma unroll
+  for (int d = 0; d < kDb; ++d)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = any ? o[d][4 * k + e] * f : 0.0f;
+      *reinterpret_cast<attn_u32x2*>(to + 32 * d + 8 * k) = attn_u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+    }
+}
+
+}  // namespace
+
+hipError_t launch_prefill(const AttendArgs& a, hipStream_t s) {
+  const int per = kRows / (a.heads / a.kv.kv_heads);
+  // sum of ceil(new tokens / per)
+  const int64_t tiles = (static_cast<int64_t>(a.rows) + per - 1) / per + a.B;
+  const dim3 grid(static_cast<unsigned>(tiles * a.kv.kv_heads));
+#define GX_PREFILL(D_, E_) hipLaunchKernelGGL((prefill_kernel<D_, E_>), grid, dim3(256), 0, s, a)
+  if (a.kv.head_dim == 64) {
+    if (a.kv.e4m3) GX_PREFILL(64, true);
+    else GX_PREFILL(64, false);
+  } else {
+    if (a.kv.e4m3) GX_PREFILL(128, true);
+    else GX_PREFILL(128, false);
+  }
+#undef GX_PREFILL
+  return hipGetLastError();
+}
+
+}  // namespace gxmoe

@@ -180,6 +180,37 @@ def test_visible_nan_and_infinities_follow_the_formula(gpu):
         assert got[2].isfinite().all()
 
 
+@pytest.mark.parametrize("shape,e4m3", [(GPT, False), (GPT, True), ((32, 8, 128, 32), False), ((32, 8, 128, 32), True)])
+@pytest.mark.parametrize("window", [0, 30])
+def test_values_reach_only_who_sees_them(gpu, shape, e4m3, window):
+    """NaN (and, in bf16, infinities) among the values of a prompt: in the rows that see their tokens and in no other,
+    also where both lie in one tile."""
+    H, Hk, D, bs = shape
+    n = 150
+    c = Case(gpu, 45, [n], *shape, e4m3=e4m3)
+    q = randn(c.gen, n, H * D, scale=1.5)
+    off = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    want = gpu.paged_attention_prefill(q, off, c.cache, c.tables, c.seq_lens, window=window).view(n, H, D).clone()
+    marks = [(0, 3, math.nan), (70, 7, math.nan), (100, 5, math.nan if e4m3 else math.inf), (149, 9, math.nan)]
+    for t, d, x in marks:
+        page = c.tables[0, t // bs].long()
+        raw = c.pages[1]
+        if e4m3:
+            raw.view(torch.uint8)[page, 1, t % bs, d] = 0x7f
+        else:
+            raw[page, 1, t % bs, d] = x
+    got = gpu.paged_attention_prefill(q, off, c.cache, c.tables, c.seq_lens, window=window).view(n, H, D)
+    G = H // Hk
+    bad = torch.zeros((n, H, D), dtype=torch.bool, device="cuda")
+    for t, d, x in marks:
+        rows = slice(t, n if not window else min(n, t + window))
+        bad[rows, G:2 * G, d] = True
+        if math.isinf(x):
+            assert (got[rows, G:2 * G, d] == math.inf).all()
+    assert (~got[bad].isfinite()).all()
+    assert torch.equal(got[~bad], want[~bad])
+
+
 def test_lengths_outside_the_table(gpu):
     """A length past the table's pages is cut to them, a negative one is 0."""
     c = Case(gpu, 18, [64, 48], *GPT)
