@@ -221,7 +221,10 @@ int gptoss_rope_kv_append(const uint16_t* qkv, int64_t qkv_stride, const int32_t
 size_t gptoss_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads,
                                               int head_dim) {
   if (num_tokens < 1 || num_seqs < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1) return 0;
-  return decode_workspace_bytes(num_seqs, num_heads, num_kv_heads, head_dim);
+  const int group = num_heads / num_kv_heads;
+  const size_t decode = decode_workspace_bytes(num_seqs, num_heads, num_kv_heads, head_dim);
+  const size_t prefill = group > kMaxGroup ? 0 : prefill_workspace_bytes(num_tokens, num_seqs, num_heads, num_kv_heads, head_dim);
+  return decode > prefill ? decode : prefill;
 }
 
 int gptoss_paged_attention_decode(const uint16_t* q, int64_t q_stride, const gptoss_kv_cache* cache,
@@ -269,7 +272,7 @@ int gptoss_paged_attention_prefill(const uint16_t* q, int64_t q_stride, const in
   if (rc != GPTOSS_OK) return rc;
   if (num_tokens == 0 || num_seqs == 0) return ok();
   if (query_offsets == nullptr) return set_error(GPTOSS_ERR_INVALID, "null query_offsets");
-  HIP_TRY(launch_prefill(a, static_cast<hipStream_t>(stream)), "paged attention prefill launch");
+  HIP_TRY(launch_prefill(a, workspace, static_cast<hipStream_t>(stream)), "paged attention prefill launch");
   return ok();
 }
 

@@ -408,92 +408,10 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
   }
 }
 
-// Joins the pieces of a sequence: T threads for each (sequence, head), 256 / T
-// of these to a work-group.  A lane takes four dims of the pieces row, row + R,
-// ..., with a reference of its own, so that nothing but the plan is waited for
-// before they are read.
-template <int D, int T>
-__global__ __launch_bounds__(256) void join_kernel(AttendArgs a, SplitArgs sp, bool e4m3) {
-  constexpr int kLanes = D / 4, R = T / kLanes;
-  __shared__ f32x4 s_o[256 / kLanes][kLanes];
-  __shared__ float s_m[256 / kLanes], s_l[256 / kLanes];
-  __shared__ int s_any[256 / kLanes];
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * (256 / T) + threadIdx.x / T;
-  const int d = threadIdx.x % kLanes, row = threadIdx.x / kLanes, r0 = row / R * R;
-  const bool in = at < static_cast<int64_t>(a.B) * a.heads;
-  const int b = in ? static_cast<int>(at / a.heads) : 0, head = in ? static_cast<int>(at % a.heads) : 0;
-  const int first = sp.plan[2 * b], chunks = in ? sp.plan[2 * b + 1] : 0;
-  const float sink = a.sinks ? bf16_to_f32(a.sinks[head]) * kLog2e : kNegInf;
-  const float vs = e4m3 && a.kv.v_scale ? a.kv.v_scale[head / (a.heads / a.kv.kv_heads)] : 1.0f;
-  if (chunks > 1) {  // otherwise written by its only work-group
-    const f32x4* ml = reinterpret_cast<const f32x4*>(sp.part_ml) + static_cast<int64_t>(first) * a.heads + head;
-    const f32x4* po = reinterpret_cast<const f32x4*>(sp.part_o + (static_cast<int64_t>(first) * a.heads + head) * D) + d;
-    float m = kNegInf, l = 0.0f;
-    f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    int any = 0;
-    constexpr int U = 8;
-    for (int c0 = row - r0; c0 < chunks; c0 += U * R) {
-      f32x4 x[U], y[U];
-      float top = m;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t c = min(c0 + u * R, chunks - 1);
-        x[u] = ml[c * a.heads];
-        y[u] = po[c * a.heads * kLanes];
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (c0 + u * R >= chunks) x[u] = f32x4{kNegInf, 0.0f, 0.0f, 0.0f};
-        top = __builtin_fmaxf(top, x[u][0]);
-      }
-      const float base = top == kNegInf ? 0.0f : top;
-      const float keep = __builtin_amdgcn_exp2f(m - base);
-      m = top;
-      l *= keep;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] *= keep;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (c0 + u * R >= chunks) continue;
-        const float f = __builtin_amdgcn_exp2f(x[u][0] - base);
-        l = __builtin_fmaf(x[u][1], f, l);
-        any |= x[u][2] != 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(y[u][e], f, o[e]);
-      }
-    }
-    s_o[row][d] = o;
-    if (d == 0) s_m[row] = m, s_l[row] = l, s_any[row] = any;
-  }
-  __syncthreads();
-  if (chunks <= 1 || row != r0) return;
-  float top = sink;
-#pragma unroll
-  for (int r = 0; r < R; ++r) top = __builtin_fmaxf(top, s_m[r0 + r]);
-  const float base = top == kNegInf ? 0.0f : top;
-  float sum = a.sinks ? __builtin_amdgcn_exp2f(sink - base) : 0.0f;
-  f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  int any = 0;
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const float f = __builtin_amdgcn_exp2f(s_m[r0 + r] - base);
-    sum = __builtin_fmaf(s_l[r0 + r], f, sum);
-    any |= s_any[r0 + r];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(s_o[r0 + r][d][e], f, acc[e]);
-  }
-  const float f = vs / sum;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) acc[e] = any ? acc[e] * f : 0.0f;
-  *reinterpret_cast<attn_u32x2*>(a.out + b * a.out_stride + static_cast<int64_t>(head) * D + 4 * d) =
-      attn_u32x2{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
-}
-
 // Work-groups of W waves.  With one piece to each sequence (a context or a
 // window that short) the call is one launch.
 constexpr int kWaves = 4;
 constexpr int kMinTiles = 8;       // tiles of the smallest piece of a cut sequence
-constexpr int kWideJoins = 1024;   // (sequence, head) pairs up to which a join is a whole work-group
 
 struct Cut {
   int slots;      // pieces aimed at for each tile of 16 heads; 0: none is cut
@@ -514,16 +432,6 @@ Cut cut_of(int B, int64_t most_tiles, int tiles_of_heads, int head_dim) {
 }
 
 int tiles_of_heads(int heads, int kv_heads) { return kv_heads * ((heads / kv_heads + 15) / 16); }
-
-template <int D>
-void launch_join(const AttendArgs& a, const SplitArgs& sp, hipStream_t s) {
-  const int64_t pairs = static_cast<int64_t>(a.B) * a.heads;
-  if (pairs <= kWideJoins)
-    hipLaunchKernelGGL((join_kernel<D, 256>), dim3(static_cast<unsigned>(pairs)), dim3(256), 0, s, a, sp, a.kv.e4m3);
-  else
-    hipLaunchKernelGGL((join_kernel<D, 64>), dim3(static_cast<unsigned>((pairs + 3) / 4)), dim3(256), 0, s, a, sp,
-                       a.kv.e4m3);
-}
 
 }  // namespace
 
@@ -559,9 +467,12 @@ hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
 #undef GX_DECODE
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || c.slots == 0) return e;
-  if (a.kv.head_dim == 64) launch_join<64>(a, sp, s);
-  else launch_join<128>(a, sp, s);
-  return hipGetLastError();
+  JoinArgs j{};
+  j.part_o = sp.part_o;
+  j.part_ml = sp.part_ml;
+  j.plan = sp.plan;
+  j.max_pieces = c.max_slots;
+  return launch_join(a, j, s);
 }
 
 }  // namespace gxmoe

@@ -50,6 +50,16 @@ struct AttendArgs {
   const uint16_t* sinks;  // [heads] or null
 };
 
+// Partial sums of rows that were cut into pieces.  Decode: piece c of row b is
+// number plan[2 b] + c of plan[2 b + 1].  Prefill (offsets set): piece c of row r
+// is number c * rows + r of plan[r].  One piece: the row is already written.
+struct JoinArgs {
+  const float* part_o;   // [piece][heads][head_dim] weighted sums
+  const float* part_ml;  // [piece][heads][4] reference, sum, whether any token was seen
+  const int* plan;
+  int max_pieces;  // no row has more
+};
+
 struct RopeTableArgs {
   float* table;
   int rotary, max_positions;
@@ -58,8 +68,10 @@ struct RopeTableArgs {
 
 hipError_t launch_rope_table(const RopeTableArgs& a, hipStream_t s);
 hipError_t launch_rope_append(const AppendArgs& a, hipStream_t s);
+hipError_t launch_join(const AttendArgs& a, const JoinArgs& j, hipStream_t s);
 size_t decode_workspace_bytes(int B, int heads, int kv_heads, int head_dim);
 hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s);
-hipError_t launch_prefill(const AttendArgs& a, hipStream_t s);
+size_t prefill_workspace_bytes(int rows, int B, int heads, int kv_heads, int head_dim);
+hipError_t launch_prefill(const AttendArgs& a, void* workspace, hipStream_t s);
 
 }  // namespace gxmoe

@@ -26,7 +26,17 @@ typedef __attribute__((address_space(3))) uint8_t* LdsBytes;
 
 constexpr int kRows = 128;    // rows of a work-group
 constexpr int kTile = 64;     // tokens of a step
+constexpr int kMinTiles = 4;  // tiles of the smallest piece
 constexpr float kSlack = 8.0f;  // how far a score may exceed the reference, in powers of two
+
+// With few rows and a long context the tokens are cut too: piece p of a tile of
+// rows takes its p-th part.
+struct PieceArgs {
+  int pieces;      // largest number
+  float* part_o;   // as JoinArgs
+  float* part_ml;
+  int* plan;       // [rows] pieces
+};
 
 struct Chunk {
   int b, row0;     // sequence, its first row of q
@@ -80,7 +90,7 @@ __device__ __forceinline__ bool not_finite(uint32_t two) {  // either of two bf1
 }
 
 template <int D, bool kE4m3>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArgs a, PieceArgs pa) {
   constexpr int kSize = kE4m3 ? 1 : 2;
   constexpr int kPieces = D * kSize / 16;      // 16-byte pieces of a token's row in memory
   constexpr int kLoads = 16 * kPieces / 64;    // loads of a wave for its 16 tokens of K, and of V
@@ -94,8 +104,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
   const int n = lane & 31, h = lane >> 5;
   const int group = a.heads / a.kv.kv_heads, per = kRows / group;
   const int kvh = blockIdx.x % a.kv.kv_heads;
+  const int piece = blockIdx.x / a.kv.kv_heads % pa.pieces;
   Chunk c;
-  if (!find_chunk(a, blockIdx.x / a.kv.kv_heads, per, &c)) return;
+  if (!find_chunk(a, blockIdx.x / a.kv.kv_heads / pa.pieces, per, &c)) return;
   for (int* x : {&c.b, &c.row0, &c.tokens, &c.tok0, &c.pos0, &c.len}) *x = __builtin_amdgcn_readfirstlane(*x);
 
   // this lane's row
@@ -117,8 +128,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
   const int pmin = c.pos0, pmax = c.pos0 + c.tokens - 1;
   const int low = a.window > 0 ? max(0, pmin - a.window + 1) : 0;
   const int main = low / kTile, nf = min((min(a.first, low) + kTile - 1) / kTile, main);
-  const int tiles = pmax < 0 ? 0 : nf + pmax / kTile + 1 - main;
-  auto tile_at = [&](int i) { return (i < nf ? i : main + i - nf) * kTile; };
+  const int all_tiles = pmax < 0 ? 0 : nf + pmax / kTile + 1 - main;
+  const int pieces = max(1, min(pa.pieces, all_tiles / kMinTiles));
+  if (piece >= pieces) return;
+  const int first_tile = static_cast<int>(static_cast<int64_t>(all_tiles) * piece / pieces);
+  const int tiles = static_cast<int>(static_cast<int64_t>(all_tiles) * (piece + 1) / pieces) - first_tile;
+  auto tile_at = [&](int i) {
+    const int t = first_tile + i;
+    return (t < nf ? t : main + t - nf) * kTile;
+  };
+  if (pa.pieces > 1 && piece == 0 && kvh == 0 && threadIdx.x < c.tokens) pa.plan[c.row0 + c.tok0 + threadIdx.x] = pieces;
 
   // Pages of 16 tiles at a time: lane 4 i + j has tokens 16 j on of tile i0 + i.
   auto load_pages = [&](int i0) {
@@ -360,6 +379,18 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
   l += __shfl_xor(l, 32);
   any |= __shfl_xor(static_cast<int>(any), 32) != 0;
   if (!mine) return;
+  if (pieces > 1) {
+    const int64_t at = (static_cast<int64_t>(piece) * a.rows + qrow) * a.heads + head;
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int d = 0; d < kDb; ++d)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<f32x4*>(pa.part_o + at * D + 32 * d + 8 * k + 4 * h) =
+            f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+    if (h == 0) reinterpret_cast<f32x4*>(pa.part_ml)[at] = f32x4{m, l, any ? 1.0f : 0.0f, 0.0f};
+    return;
+  }
   float sum = l;
   if (a.sinks) {
     const float sink = bf16_to_f32(a.sinks[head]) * kLog2e;
@@ -385,14 +416,43 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
     }
 }
 
+// Pieces: as many as fill the chip (work-groups that it holds at once: three on a
+// CU with heads of 64 dims, two with 128) when the tiles of rows alone do not.
+int most_pieces(int rows, int B, int heads, int kv_heads, int head_dim) {
+  const int per = kRows / (heads / kv_heads);
+  const int64_t tiles = (static_cast<int64_t>(rows) + per - 1) / per + (B < rows ? B : rows) - 1;
+  const int64_t pieces = (head_dim == 64 ? 768 : 512) / (tiles * kv_heads);
+  return pieces < 1 ? 1 : static_cast<int>(pieces);
+}
+
 }  // namespace
 
-hipError_t launch_prefill(const AttendArgs& a, hipStream_t s) {
+size_t prefill_workspace_bytes(int rows, int B, int heads, int kv_heads, int head_dim) {
+  const int pieces = most_pieces(rows, B, heads, kv_heads, head_dim);
+  if (pieces == 1) return 0;
+  return static_cast<size_t>(pieces) * rows * heads * (head_dim + 4) * sizeof(float) +
+         ((static_cast<size_t>(rows) * sizeof(int) + 15) & ~size_t{15});
+}
+
+hipError_t launch_prefill(const AttendArgs& a, void* workspace, hipStream_t s) {
   const int per = kRows / (a.heads / a.kv.kv_heads);
-  // sum of ceil(new tokens / per)
-  const int64_t tiles = (static_cast<int64_t>(a.rows) + per - 1) / per + a.B;
-  const dim3 grid(static_cast<unsigned>(tiles * a.kv.kv_heads));
-#define GX_PREFILL(D_, E_) hipLaunchKernelGGL((prefill_kernel<D_, E_>), grid, dim3(256), 0, s, a)
+  // no more tiles than the longest sequence, or a window over a tile's rows, has
+  const int64_t cap = static_cast<int64_t>(a.max_blocks) << a.kv.bs_shift;
+  int64_t most = (cap + kTile - 1) / kTile;
+  if (a.window > 0)
+    most = min(most, (static_cast<int64_t>(a.window) + per + kTile - 3) / kTile + 1 +
+                         (static_cast<int64_t>(a.first) + kTile - 1) / kTile);
+  PieceArgs pa{};
+  pa.pieces = most_pieces(a.rows, a.B, a.heads, a.kv.kv_heads, a.kv.head_dim);
+  if (pa.pieces > most / kMinTiles) pa.pieces = most / kMinTiles > 1 ? static_cast<int>(most / kMinTiles) : 1;
+  const size_t parts = static_cast<size_t>(pa.pieces) * a.rows * a.heads;
+  pa.part_o = static_cast<float*>(workspace);
+  pa.part_ml = pa.part_o + parts * a.kv.head_dim;
+  pa.plan = reinterpret_cast<int*>(pa.part_ml + parts * 4);
+  // sum of ceil(new tokens / per), at most one tile more for each sequence that has rows
+  const int64_t tiles = (static_cast<int64_t>(a.rows) + per - 1) / per + (a.B < a.rows ? a.B : a.rows);
+  const dim3 grid(static_cast<unsigned>(tiles * a.kv.kv_heads * pa.pieces));
+#define GX_PREFILL(D_, E_) hipLaunchKernelGGL((prefill_kernel<D_, E_>), grid, dim3(256), 0, s, a, pa)
   if (a.kv.head_dim == 64) {
     if (a.kv.e4m3) GX_PREFILL(64, true);
     else GX_PREFILL(64, false);
@@ -401,7 +461,14 @@ hipError_t launch_prefill(const AttendArgs& a, hipStream_t s) {
     else GX_PREFILL(128, false);
   }
 #undef GX_PREFILL
-  return hipGetLastError();
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || pa.pieces == 1) return e;
+  JoinArgs j{};
+  j.part_o = pa.part_o;
+  j.part_ml = pa.part_ml;
+  j.plan = pa.plan;
+  j.max_pieces = pa.pieces;
+  return launch_join(a, j, s);
 }
 
 }  // namespace gxmoe
