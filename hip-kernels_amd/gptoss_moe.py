@@ -877,35 +877,43 @@ def rope_table(cfg: RopeConfig | None = None, device="cuda", stream=None) -> tor
     cfg = cfg or default_rope_config()
     if cfg.rotary_dim < 2 or cfg.max_positions < 1:
         _bad(f"rotary_dim={cfg.rotary_dim} and max_positions={cfg.max_positions} must be positive")
-    device = torch.device(device)
-    with _alloc_on(stream, device):
-        table = torch.empty((cfg.max_positions, 2, cfg.rotary_dim // 2), dtype=torch.float32, device=device)
-    with _on(table):
-        check(_lib.gptoss_rope_table(ctypes.byref(cfg), _ptr(table), _stream(stream)))
+    table = _empty((cfg.max_positions, 2, cfg.rotary_dim // 2), torch.float32, torch.device(device), stream)
+    _needs_gpu(table.device)
+    _launch(table.device, stream, _lib.gptoss_rope_table, ctypes.byref(cfg), table.data_ptr())
     return table
 
 
 class _on:
-    """The device of `t` as the current one within the block."""
+    """The device of index `to` as the current one within the block."""
 
-    def __init__(self, t):
-        self._to = t.device.index if t.device.type == "cuda" else None
+    def __init__(self, to: int):
+        self._to = to
 
     def __enter__(self):
-        self._was = None
-        if self._to is not None and torch.cuda.current_device() != self._to:
-            self._was = torch.cuda.current_device()
-            torch.cuda.set_device(self._to)
+        self._was = torch.cuda.current_device()
+        torch.cuda.set_device(self._to)
 
     def __exit__(self, *exc):
-        if self._was is not None:
-            torch.cuda.set_device(self._was)
+        torch.cuda.set_device(self._was)
+
+
+def _launch(device, stream, fn, *args) -> None:
+    """Calls fn on `stream` (None: the current one) of `device`."""
+    if stream is None:
+        handle = torch._C._cuda_getCurrentRawStream(device.index)
+    else:
+        handle = stream if isinstance(stream, int) else stream.cuda_stream
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, handle))
+    else:
+        with _on(device.index):
+            check(fn(*args, handle))
 
 
 def _on_device(name: str, t, device, dtype=None, dim: int | None = None) -> None:
     if not isinstance(t, torch.Tensor):
         _bad(f"{name} must be a torch.Tensor, got {type(t).__name__}")
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         _bad(f"{name} has dtype {t.dtype}, expected {dtype}")
     if dim is not None and t.dim() != dim:
         _bad(f"{name} must be {dim}-D, got shape {tuple(t.shape)}")
@@ -913,13 +921,18 @@ def _on_device(name: str, t, device, dtype=None, dim: int | None = None) -> None
         _bad(f"{name} is on {t.device}, the cache is on {device}")
 
 
-def _row_tensor(name: str, t, device, cols: int) -> None:
-    """bf16 [rows, cols] on `device`, rows any distance apart."""
+def _row_tensor(name: str, t, device, cols: int) -> int:
+    """bf16 [rows, cols] on `device`, rows any distance apart: the distance."""
     _on_device(name, t, device, torch.bfloat16, 2)
-    if t.shape[1] != cols:
+    rows, width = t.shape
+    step, one = t.stride()
+    if width != cols:
         _bad(f"{name} has shape {tuple(t.shape)}, expected [rows, {cols}]")
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < cols):
+    if rows < 2:
+        step = (cols + 7) // 8 * 8  # torch gives a single row any stride
+    if one != 1 or step < cols:
         _bad(f"{name} must have contiguous rows, strides are {t.stride()}")
+    return step
 
 
 def _vector(name: str, t, device, n: int, dtype) -> None:
@@ -935,30 +948,15 @@ def _needs_gpu(device) -> None:
         _bad(f"the cache is on {device}, a GPU is needed")
 
 
-class _alloc_on:
-    """Allocations within the block belong to `stream` (None: the current one), where the kernels that use
-    them run: torch hands a freed block out again in the order of its own stream only."""
-
-    def __init__(self, stream, device):
-        self._with = None
-        if stream is not None and device.type == "cuda":
-            if isinstance(stream, int):
-                stream = torch.cuda.default_stream(device) if stream == 0 else \
-                    torch.cuda.ExternalStream(stream, device=device)
-            self._with = torch.cuda.stream(stream)
-
-    def __enter__(self):
-        if self._with is not None:
-            self._with.__enter__()
-
-    def __exit__(self, *exc):
-        if self._with is not None:
-            self._with.__exit__(*exc)
-
-
-def _row_stride(t) -> int:
-    # torch gives a single row any stride
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
+def _empty(shape, dtype, device, stream):
+    """torch.empty in the memory of `stream` (None: the current one), where the kernels that use it run: torch hands
+    a freed block out again in the order of its own stream only."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if isinstance(stream, int):
+        stream = torch.cuda.default_stream(device) if stream == 0 else torch.cuda.ExternalStream(stream, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 class KVCache:
@@ -1010,28 +1008,28 @@ def rope_kv_append(qkv, positions, slots, table, cache: KVCache, num_heads: int,
     Rows whose position is outside the table (rope_table()) write nothing.  Returns the queries
     [T, num_heads * head_dim]; q_out may be qkv[:, :num_heads * head_dim]."""
     dev, D = cache.device, cache.head_dim
-    _row_tensor("qkv", qkv, dev, (num_heads + 2 * cache.kv_heads) * D)
+    stride = _row_tensor("qkv", qkv, dev, (num_heads + 2 * cache.kv_heads) * D)
     T = qkv.shape[0]
     _vector("positions", positions, dev, T, torch.int32)
     _vector("slots", slots, dev, T, torch.int32)
     _on_device("table", table, dev, torch.float32, 3)
-    if table.shape[1] != 2 or not table.is_contiguous():
+    max_positions, two, half = table.shape
+    if two != 2 or not table.is_contiguous():
         _bad(f"table must be contiguous [max_positions, 2, rotary_dim / 2], got {tuple(table.shape)}")
+    cols = q_stride = num_heads * D
     if q_out is None:
-        with _alloc_on(stream, dev):
-            q_out = torch.empty((T, num_heads * D), dtype=torch.bfloat16, device=dev)
+        _needs_gpu(dev)
+        q_out = _empty((T, cols), torch.bfloat16, dev, stream)
     else:
-        _row_tensor("q_out", q_out, dev, num_heads * D)
+        q_stride = _row_tensor("q_out", q_out, dev, cols)
         if q_out.shape[0] != T:
             _bad(f"q_out has {q_out.shape[0]} rows, expected {T}")
-    _needs_gpu(dev)
-    q_stride = _row_stride(q_out)
-    if T == 1 and q_out.data_ptr() == qkv.data_ptr():
-        q_stride = _row_stride(qkv)
-    with _on(qkv):
-        check(_lib.gptoss_rope_kv_append(qkv.data_ptr(), _row_stride(qkv), positions.data_ptr(), slots.data_ptr(),
-                                         table.data_ptr(), 2 * table.shape[2], table.shape[0], 1 if interleaved else 0,
-                                         T, num_heads, q_out.data_ptr(), q_stride, cache._desc, _stream(stream)))
+        _needs_gpu(dev)
+        if T == 1 and q_out.data_ptr() == qkv.data_ptr():
+            q_stride = stride
+    _launch(dev, stream, _lib.gptoss_rope_kv_append, qkv.data_ptr(), stride, positions.data_ptr(), slots.data_ptr(),
+            table.data_ptr(), 2 * half, max_positions, 1 if interleaved else 0, T, num_heads, q_out.data_ptr(), q_stride,
+            cache._desc)
     return q_out
 
 
@@ -1044,46 +1042,48 @@ def _attend(q, offsets, cache, block_tables, seq_lens, scale, window, first_toke
     dev, D = cache.device, cache.head_dim
     if not isinstance(q, torch.Tensor) or q.dim() != 2 or q.shape[1] % D != 0 or q.shape[1] == 0:
         _bad(f"q must be [rows, num_heads * {D}]")
-    _row_tensor("q", q, dev, q.shape[1])
-    rows, H = q.shape[0], q.shape[1] // D
+    rows, cols = q.shape
+    q_stride = out_stride = _row_tensor("q", q, dev, cols)
+    H = cols // D
     _on_device("block_tables", block_tables, dev, torch.int32, 2)
     B, blocks = block_tables.shape
-    if blocks > 1 and block_tables.stride(1) != 1:
+    table_stride, one = block_tables.stride()
+    if B < 2:
+        table_stride = blocks
+    if blocks > 1 and one != 1:
         _bad("block_tables must have contiguous rows")
     _vector("seq_lens", seq_lens, dev, B, torch.int32)
     if sinks is not None:
         _vector("sinks", sinks, dev, H, torch.bfloat16)
+        sinks = sinks.data_ptr()
     if offsets is None:
         if rows != B:
             _bad(f"q has {rows} rows for {B} sequences")
     else:
         _vector("query_offsets", offsets, dev, B + 1, torch.int32)
     if out is None:
-        with _alloc_on(stream, dev):
-            out = torch.empty((rows, H * D), dtype=torch.bfloat16, device=dev)
+        _needs_gpu(dev)
+        out, out_stride = _empty((rows, cols), torch.bfloat16, dev, stream), cols
     else:
-        _row_tensor("out", out, dev, H * D)
+        out_stride = _row_tensor("out", out, dev, cols)
         if out.shape[0] != rows:
             _bad(f"out has {out.shape[0]} rows, expected {rows}")
-    _needs_gpu(dev)
-    need = _lib.gptoss_paged_attention_workspace_bytes(rows, B, H, cache.kv_heads, D)
+        _needs_gpu(dev)
     if workspace is None:
-        with _alloc_on(stream, dev):
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        size = _lib.gptoss_paged_attention_workspace_bytes(rows, B, H, cache.kv_heads, D)
+        workspace = _empty(size, torch.uint8, dev, stream)
     else:
         _on_device("workspace", workspace, dev)
         if not workspace.is_contiguous():
             _bad("workspace must be contiguous")
-    cfg = AttentionConfig(D ** -0.5 if scale is None else scale, window, first_tokens, _ptr(sinks))
-    tail = (cache._desc, block_tables.data_ptr(), block_tables.stride(0) if B > 1 else blocks, blocks, seq_lens.data_ptr(),
-            B, H, ctypes.addressof(cfg), out.data_ptr(), _row_stride(out), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size())
-    with _on(q):
-        if offsets is None:
-            check(_lib.gptoss_paged_attention_decode(q.data_ptr(), _row_stride(q), *tail, _stream(stream)))
-        else:
-            check(_lib.gptoss_paged_attention_prefill(q.data_ptr(), _row_stride(q), offsets.data_ptr(), rows, *tail,
-                                                      _stream(stream)))
+        size = workspace.numel() * workspace.element_size()
+    cfg = AttentionConfig(D ** -0.5 if scale is None else scale, window, first_tokens, sinks)
+    tail = (cache._desc, block_tables.data_ptr(), table_stride, blocks, seq_lens.data_ptr(), B, H, ctypes.addressof(cfg),
+            out.data_ptr(), out_stride, workspace.data_ptr(), size)
+    if offsets is None:
+        _launch(dev, stream, _lib.gptoss_paged_attention_decode, q.data_ptr(), q_stride, *tail)
+    else:
+        _launch(dev, stream, _lib.gptoss_paged_attention_prefill, q.data_ptr(), q_stride, offsets.data_ptr(), rows, *tail)
     return out
 
 
