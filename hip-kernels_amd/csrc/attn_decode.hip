@@ -53,6 +53,7 @@ __device__ __forceinline__ Seen seen_tiles(const AttendArgs& a, int len) {
 
 struct SplitArgs {
   int slots, min_tiles;  // pieces aimed at (0: one per sequence), smallest piece
+  bool whole_ok;         // sequences of about the same length need not be cut
   float* part_o;         // [piece][heads][D] sums of the cut sequences' pieces
   float* part_ml;        // [piece][heads][4] reference, sum, whether any token was seen
   int* plan;             // [B][2] first piece and number of pieces
@@ -71,15 +72,24 @@ struct Piece {
 __device__ __forceinline__ bool find_piece(const AttendArgs& a, const SplitArgs& sp, int slot, Piece* p) {
   const int lane = threadIdx.x & 63;
   const int len0 = lane < a.B ? seq_len(a, lane) : 0;
-  int total = lane < a.B ? seen_tiles(a, len0).tiles : 0;
-  for (int b0 = 64; b0 < a.B; b0 += 64) total += b0 + lane < a.B ? seen_tiles(a, seq_len(a, b0 + lane)).tiles : 0;
+  int total = lane < a.B ? seen_tiles(a, len0).tiles : 0, longest = total;
+  for (int b0 = 64; b0 < a.B; b0 += 64) {
+    const int tiles = b0 + lane < a.B ? seen_tiles(a, seq_len(a, b0 + lane)).tiles : 0;
+    total += tiles;
+    longest = max(longest, tiles);
+  }
   total = __builtin_amdgcn_readlane(wave_scan(total), 63);
-  const int size = max(sp.min_tiles, (total + sp.slots - 1) / sp.slots);
+  int size = max(sp.min_tiles, (total + sp.slots - 1) / sp.slots);
+  if (sp.whole_ok) {
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) longest = max(longest, __shfl_xor(longest, x));
+    if (2 * static_cast<int64_t>(longest) * a.B <= 3 * static_cast<int64_t>(total)) size = max(size, longest);
+  }
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const bool in = b0 + lane < a.B;
     const int len = b0 == 0 ? len0 : in ? seq_len(a, b0 + lane) : 0;
-    const int mine = in ? max(1, (seen_tiles(a, len).tiles + size - 1) / size) : 0;
+    const int mine = in ? max(1, (seen_tiles(a, len).tiles + size / 2) / size) : 0;
     const int upto = wave_scan(mine);
     const int all = __builtin_amdgcn_readlane(upto, 63);
     if (slot < before + all) {
@@ -90,8 +100,9 @@ __device__ __forceinline__ bool find_piece(const AttendArgs& a, const SplitArgs&
       const int first = __builtin_amdgcn_readlane(upto, who) - p->chunks;
       p->first_slot = before + first;
       p->seen = seen_tiles(a, __builtin_amdgcn_readlane(len, who));
-      p->t0 = (at - first) * size;
-      p->t1 = min(p->t0 + size, p->seen.tiles);
+      const int64_t n = p->seen.tiles;
+      p->t0 = static_cast<int>(n * (at - first) / p->chunks);
+      p->t1 = static_cast<int>(n * (at - first + 1) / p->chunks);
       return true;
     }
     before += all;
@@ -408,10 +419,19 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
   }
 }
 
-// Work-groups of W waves.  With one piece to each sequence (a context or a
-// window that short) the call is one launch.
+// Work-groups of W waves.  Where the table or the window holds no more than
+// kWholeTiles (1024 tokens) the call is one launch of a piece to each sequence
+// (cut or whole: one sequence of 1000 9.8 / 9.0 us, of 500 9.8 / 6.5, 32 of
+// 1000 20.5 / 15.1, 64 of up to 1000 16.7 / 13.3, 256 with a window of 512 63.8 /
+// 56.6; 8 of 1000 11.6 / 11.8.  Whole with eight waves instead of four is slower
+// in each).
 constexpr int kWaves = 4;
-constexpr int kMinTiles = 8;       // tiles of the smallest piece of a cut sequence
+constexpr int kMinTiles = 8;     // tiles of the smallest piece of a cut sequence
+// Work-groups that fill the chip: one to a CU.  From there on sequences whose mean
+// is two thirds of the longest are not cut either (cut or whole, join included:
+// 32 of 1500 27.5 / 22.6 us, 64 of 2000 56.5 / 50.6).
+constexpr int kFull = 256;
+constexpr int kWholeTiles = 32;  // no sequence is cut when the longest has no more tiles
 
 struct Cut {
   int slots;      // pieces aimed at for each tile of 16 heads; 0: none is cut
@@ -423,10 +443,10 @@ struct Cut {
 // slower (one sequence of 131072, bf16: 55.7 against 52.7 us; 32 of 2000: 33.3
 // against 29.7; fewer partial sums, and a CU's loads are enough in flight).
 Cut cut_of(int B, int64_t most_tiles, int tiles_of_heads, int head_dim) {
-  if (most_tiles <= kMinTiles) return Cut{0, B};
+  if (most_tiles <= kWholeTiles) return Cut{0, B};
   const int work_groups = head_dim == 64 ? 768 : 512;
   const int slots = (work_groups + tiles_of_heads - 1) / tiles_of_heads;
-  // sum of ceil(tiles / size) <= B + slots
+  // sum of max(1, (tiles + size / 2) / size) <= B + slots
   const int64_t pieces = static_cast<int64_t>(B) * ((most_tiles + kMinTiles - 1) / kMinTiles);
   return Cut{slots, static_cast<int>(pieces < B + slots ? pieces : B + slots)};
 }
@@ -451,6 +471,7 @@ hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
   SplitArgs sp{};
   sp.slots = c.slots;
   sp.min_tiles = kMinTiles;
+  sp.whole_ok = static_cast<int64_t>(a.B) * th >= kFull;
   const size_t pieces = static_cast<size_t>(c.max_slots) * a.heads;
   sp.part_o = static_cast<float*>(workspace);
   sp.part_ml = sp.part_o + pieces * a.kv.head_dim;

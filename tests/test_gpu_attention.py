@@ -117,6 +117,15 @@ def test_decode_batches_and_long_caches(gpu, B, L, e4m3):
     c.check_decode(window=128)
 
 
+@pytest.mark.parametrize("B,L", [(40, 0), (40, 1500), (100, 1300), (300, 0)])
+def test_decode_uniform_batches(gpu, B, L):
+    """Many sequences of one length, nothing at all among them, with a table that would hold more."""
+    c = Case(gpu, 46, [L] * B, *GPT, width=200)
+    q, got = c.check_decode(sinks=randn(c.gen, 64))
+    if L:
+        c.check_decode()
+
+
 @pytest.mark.parametrize("lens,new", [([1000], [1000]), ([2300], [260]), ([700, 5000], [700, 9]), ([64], [64]),
                                       ([300] * 9, [3] * 9), ([4100], [1]), ([90, 0, 91], [0, 0, 91])])
 @pytest.mark.parametrize("shape,e4m3", [(GPT, False), (GPT, True), ((32, 8, 128, 32), False), ((4, 4, 64, 16), False),
