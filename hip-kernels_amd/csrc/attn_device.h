@@ -23,6 +23,12 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
+// acc + both bf16 of a dword.
+__device__ __forceinline__ float add_two(uint32_t two, float acc) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), __builtin_bit_cast(bf16x2, 0x3f803f80u), acc, false);
+}
+
 // The four e4m3 codes of a dword as bf16 (exact).
 __device__ __forceinline__ void widen(uint32_t codes, uint32_t* out) {
   out[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false));

@@ -12,6 +12,8 @@
 // stay in registers.  K and V go through LDS, 16-byte pieces permuted by the
 // token so that neither the row reads of K nor the transposing reads of V meet
 // in a bank; the next tile is on its way to registers while one is worked on.
+#include <type_traits>
+
 #include "attn_device.h"
 
 namespace gxmoe {
@@ -27,7 +29,7 @@ typedef __attribute__((address_space(3))) uint8_t* LdsBytes;
 constexpr int kRows = 128;    // rows of a work-group
 constexpr int kTile = 64;     // tokens of a step
 constexpr int kMinTiles = 4;  // tiles of the smallest piece
-constexpr float kSlack = 8.0f;  // how far a score may exceed the reference, in powers of two
+constexpr float kMost = 4096.0f;  // a lane's sum of weights from which on the reference moves
 
 // With few rows and a long context the tokens are cut too: piece p of a tile of
 // rows takes its p-th part.
@@ -85,8 +87,29 @@ __device__ __forceinline__ bool find_chunk(const AttendArgs& a, int at, int per,
   return false;
 }
 
-__device__ __forceinline__ bool not_finite(uint32_t two) {  // either of two bf16
-  return (((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0;
+// The bits of the infinities and NaN among two bf16 or four e4m3.
+template <bool kE4m3>
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) {
+  if constexpr (kE4m3) return (((x & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0xffu;
+  return (((x & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u) * 0xffffu;
+}
+
+__device__ __forceinline__ uint32_t here(uint32_t x) {  // an offset as the block at hand sees it, not hoisted as 64 bits
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+__device__ __forceinline__ GlobalBytes scalar(GlobalBytes p) {
+  asm("" : "+s"(p));
+  return p;
+}
+
+// Where in its row of LDS a 16-byte piece of token t lies: the 16 tokens that
+// take part in a read of K, and the four of a read of V, meet in no bank.
+template <int D>
+__device__ __forceinline__ int piece_at(int t, int piece) {
+  if constexpr (D == 64) return piece ^ ((t >> 1 & 1) << 2 | (t >> 2 & 3));
+  return piece ^ ((t & 3) << 2 | (t >> 2 & 3));
 }
 
 template <int D, bool kE4m3>
@@ -103,8 +126,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
   const int group = a.heads / a.kv.kv_heads, per = kRows / group;
-  const int kvh = blockIdx.x % a.kv.kv_heads;
-  const int piece = blockIdx.x / a.kv.kv_heads % pa.pieces;
+  const int kvh = __builtin_amdgcn_readfirstlane(blockIdx.x % a.kv.kv_heads);
+  const int piece = __builtin_amdgcn_readfirstlane(blockIdx.x / a.kv.kv_heads % pa.pieces);
   Chunk c;
   if (!find_chunk(a, blockIdx.x / a.kv.kv_heads / pa.pieces, per, &c)) return;
   for (int* x : {&c.b, &c.row0, &c.tokens, &c.tok0, &c.pos0, &c.len}) *x = __builtin_amdgcn_readfirstlane(*x);
@@ -131,12 +154,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
   const int all_tiles = pmax < 0 ? 0 : nf + pmax / kTile + 1 - main;
   const int pieces = max(1, min(pa.pieces, all_tiles / kMinTiles));
   if (piece >= pieces) return;
-  const int first_tile = static_cast<int>(static_cast<int64_t>(all_tiles) * piece / pieces);
-  const int tiles = static_cast<int>(static_cast<int64_t>(all_tiles) * (piece + 1) / pieces) - first_tile;
+  const int first_tile = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(all_tiles) * piece / pieces));
+  const int tiles = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(all_tiles) * (piece + 1) / pieces) - first_tile);
   auto tile_at = [&](int i) {
     const int t = first_tile + i;
     return (t < nf ? t : main + t - nf) * kTile;
   };
+  auto begin_of = [&](int i) { return __builtin_amdgcn_readfirstlane(tile_at(i)); };
   if (pa.pieces > 1 && piece == 0 && kvh == 0 && threadIdx.x < c.tokens) pa.plan[c.row0 + c.tok0 + threadIdx.x] = pieces;
 
   // Pages of 16 tiles at a time: lane 4 i + j has tokens 16 j on of tile i0 + i.
@@ -175,11 +199,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
                                                 __builtin_amdgcn_readlane(static_cast<int>(off >> 32), from)))
                                             << 32) |
                        static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(off), from));
+    const uint32_t go = here(goff);
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int64_t to = at + j * kRowsPerLoad * st;
-      kr[j] = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x4*>(kb + to + goff);
-      vr[j] = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x4*>(vb + to + goff);
+      kr[j] = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x4*>(scalar(kb + to) + go);
+      vr[j] = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x4*>(scalar(vb + to) + go);
     }
   };
   // whole: every row of the work-group sees every token of the tile
@@ -189,48 +214,46 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
   // To LDS.  0 times an infinity or a NaN is not 0, so in a tile that not every
   // row sees whole such values become 0 here; the rows that do see one get it
   // at the end.
-  auto put = [&](int buf, bool whole) {
+  auto put = [&](int buf, bool whole) __attribute__((always_inline)) {
     uint8_t* kd = s_kv[buf];
     uint8_t* vd = kd + kHalf;
+    if (!whole) {
+      uint32_t odd = 0;
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= not_finite<kE4m3>(vr[j][e]);
+      if (__ballot(odd != 0) != 0) {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vr[j][e] &= ~not_finite<kE4m3>(vr[j][e]);
+        if (lane == 0) s_odd = 1;
+      }
+    }
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int row = 16 * wave + j * kRowsPerLoad + srow;
-      uint32_t w[2][2][4];
       if constexpr (kE4m3) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          widen(kr[j][e], &w[0][e >> 1][2 * (e & 1)]);
-          widen(vr[j][e], &w[1][e >> 1][2 * (e & 1)]);
+        for (int p = 0; p < 2; ++p) {
+          uint32_t w[8];
+          widen(kr[j][2 * p], w), widen(kr[j][2 * p + 1], w + 2), widen(vr[j][2 * p], w + 4), widen(vr[j][2 * p + 1], w + 6);
+          const int at = row * kRowBytes + (piece_at<D>(row, 2 * spiece + p) << 4);
+          *reinterpret_cast<attn_u32x4*>(kd + at) = attn_u32x4{w[0], w[1], w[2], w[3]};
+          *reinterpret_cast<attn_u32x4*>(vd + at) = attn_u32x4{w[4], w[5], w[6], w[7]};
         }
       } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[0][0][e] = kr[j][e], w[1][0][e] = vr[j][e];
-      }
-#pragma unroll
-      for (int p = 0; p < (kE4m3 ? 2 : 1); ++p) {
-        if (!whole) {
-          bool odd = false;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) odd |= not_finite(w[1][p][e]);
-          if (__ballot(odd) != 0) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t x = w[1][p][e];
-              w[1][p][e] = ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) |
-                           ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
-            }
-            if (lane == 0) s_odd = 1;
-          }
-        }
-        const int piece = kE4m3 ? 2 * spiece + p : spiece;
-        const int at = row * kRowBytes + ((piece ^ (row & 7)) << 4);
-        *reinterpret_cast<attn_u32x4*>(kd + at) = attn_u32x4{w[0][p][0], w[0][p][1], w[0][p][2], w[0][p][3]};
-        *reinterpret_cast<attn_u32x4*>(vd + at) = attn_u32x4{w[1][p][0], w[1][p][1], w[1][p][2], w[1][p][3]};
+        const int at = row * kRowBytes + (piece_at<D>(row, spiece) << 4);
+        *reinterpret_cast<attn_u32x4*>(kd + at) = kr[j];
+        *reinterpret_cast<attn_u32x4*>(vd + at) = vr[j];
       }
     }
   };
 
-  float m = kNegInf, l = 0.0f;
+  // The reference of a row, its negative as the scores' products take it (+inf: none
+  // yet, so that the first score of the row leads to one), the sum.
+  float m = kNegInf, less = mine ? __builtin_inff() : 0.0f, l = 0.0f;
   bool any = false;
   f32x16 o[kDb];
 #pragma unroll
@@ -240,23 +263,26 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
 
   // LDS addresses.  K: token 32 b + n, piece 2 s + h.  V: the 16 lanes of a quarter
   // read 4 tokens x 16 dims and are left with 4 tokens of one dim each.
-  const int krow = n * kRowBytes;
   const int vrow = 4 * h + ((lane & 15) >> 2);  // and vrow + 8 and so on
   const int vpiece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  auto value = [&](int buf, int d, int s) {  // dims 32 d on of the tokens of step s
+  int kat[kSteps], vat[kDb][2];
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) kat[k] = n * kRowBytes + (piece_at<D>(n, 2 * k + h) << 4);
+#pragma unroll
+  for (int d = 0; d < kDb; ++d)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      vat[d][e] = kHalf + (vrow + 8 * e) * kRowBytes + (piece_at<D>(vrow + 8 * e, 4 * d + vpiece) << 4) + 8 * (lane & 1);
+  auto value = [&](int buf, int d, int s) __attribute__((always_inline)) {  // dims 32 d on of the tokens of step s
     bf16x8 x;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int at = (16 * s + 8 * e + vrow) * kRowBytes + (((4 * d + vpiece) ^ vrow) << 4) + 8 * (lane & 1);
-      const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4*)((LdsBytes)s_kv[buf] + kHalf + at));
-      reinterpret_cast<s16x4*>(&x)[e] = y;
-    }
+    for (int e = 0; e < 2; ++e)
+      reinterpret_cast<s16x4*>(&x)[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)((LdsBytes)s_kv[buf] + vat[d][e] + 16 * s * kRowBytes));
     return x;
   };
 
-  auto compute = [&](int i, int buf, uint32_t pages) {
-    const int t = tile_at(i);
+  auto compute = [&](int t, int buf, uint32_t pages) __attribute__((always_inline)) {
     f32x16 s[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -264,12 +290,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
       for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
-        const bf16x8 x = *reinterpret_cast<const bf16x8*>(&s_kv[buf][32 * b * kRowBytes + krow + (((2 * k + h) ^ (n & 7)) << 4)]);
+        const bf16x8 x = *reinterpret_cast<const bf16x8*>(&s_kv[buf][32 * b * kRowBytes + kat[k]]);
         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, q[k], s[b], 0, 0, 0);
       }
     }
-    const bool whole = is_whole(t, pages);
-    if (whole) {
+    if (is_whole(t, pages)) {
       any = true;
     } else {
       const int rel = pos - t - 4 * h, lowest = a.window > 0 ? rel - a.window : -1 - 4 * h, f = a.first - t - 4 * h;
@@ -283,36 +308,45 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
           s[b][e] = in ? s[b][e] : kNegInf;
         }
     }
-    float top = s[0][0];
+    // Weights against the reference there is; only if they come out large (or
+    // there is none) the tile's maximum is looked for and they are formed again.
+    bf16x8 w[4];
+    float sum;
+    auto weigh = [&](float off) __attribute__((always_inline)) {
+      float part[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int e = 1; e < 32; ++e) top = __builtin_fmaxf(top, s[e >> 4][e & 15]);
-    top *= scale;
-    if (__ballot(top > m + kSlack) != 0) {
+      for (int k = 0; k < 4; ++k) {
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float lo = s[k >> 1][8 * (k & 1) + 2 * e], hi = s[k >> 1][8 * (k & 1) + 2 * e + 1];
+          x[e] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(lo, scale, off)),
+                             __builtin_amdgcn_exp2f(__builtin_fmaf(hi, scale, off)));
+          part[e & 1] = add_two(x[e], part[e & 1]);
+        }
+        w[k] = __builtin_bit_cast(bf16x8, attn_u32x4{x[0], x[1], x[2], x[3]});
+      }
+      sum = part[0] + part[1];
+    };
+    weigh(less);
+    if (__ballot(!(sum < kMost)) != 0) {
+      float top = s[0][0];
+#pragma unroll
+      for (int e = 1; e < 32; ++e) top = __builtin_fmaxf(top, s[e >> 4][e & 15]);
+      top *= scale;
       top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-      const float mn = __builtin_fmaxf(m, top);
-      const float keep = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
+      const float mn = __builtin_fmaxf(m, top), base = mn == kNegInf ? 0.0f : mn;
+      const float keep = __builtin_amdgcn_exp2f(m - base);
       m = mn;
+      less = mn == kNegInf && mine ? __builtin_inff() : -base;
       l *= keep;
 #pragma unroll
       for (int d = 0; d < kDb; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] *= keep;
+      weigh(-base);
     }
-    const float base = m == kNegInf ? 0.0f : m;
-    bf16x8 w[4];
-    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float p[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 1][8 * (k & 1) + e], scale, -base));
-        part[e & 3] += p[e];
-      }
-      w[k] = __builtin_bit_cast(bf16x8, attn_u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
-                                                   pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])});
-    }
-    l += (part[0] + part[1]) + (part[2] + part[3]);
+    l += sum;
 #pragma unroll
     for (int d = 0; d < kDb; ++d)
 #pragma unroll
@@ -325,18 +359,27 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
     locate(0, load_pages(0));
     load(0);
     uint32_t pages = pages_of(0);
-    put(0, is_whole(tile_at(0), pages));
+    int t = begin_of(0);
+    put(0, is_whole(t, pages));
     __syncthreads();
     int next = -1;
-    for (int i = 0; i < tiles; ++i) {
+    auto step = [&](auto B, int i) __attribute__((always_inline)) {
+      constexpr int buf = decltype(B)::value;
       if ((i & 15) == 0) next = load_pages(i + 16);
       if ((i & 15) == 15) locate(i + 1, next);
-      const uint32_t ahead = i + 1 < tiles ? pages_of(i + 1) : 0;
-      if (i + 1 < tiles) load(i + 1);
-      compute(i, i & 1, pages);
-      if (i + 1 < tiles) put((i + 1) & 1, is_whole(tile_at(i + 1), ahead));
+      const bool more = i + 1 < tiles;
+      const uint32_t ahead = pages_of(i + 1);
+      const int u = begin_of(i + 1);
+      if (more) load(i + 1);
+      compute(t, buf, pages);
+      if (more) put(buf ^ 1, is_whole(u, ahead));
       pages = ahead;
+      t = u;
       __syncthreads();
+    };
+    for (int i = 0; i < tiles; i += 2) {
+      step(std::integral_constant<int, 0>{}, i);
+      if (i + 1 < tiles) step(std::integral_constant<int, 1>{}, i + 1);
     }
   }
   if (s_odd != 0) {
