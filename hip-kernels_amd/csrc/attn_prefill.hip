@@ -118,9 +118,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
   constexpr int kPieces = D * kSize / 16;      // 16-byte pieces of a token's row in memory
   constexpr int kLoads = 16 * kPieces / 64;    // loads of a wave for its 16 tokens of K, and of V
   constexpr int kRowBytes = 2 * D;             // of a token in LDS
-  constexpr int kHalf = kTile * kRowBytes;     // K, then V
+  constexpr int kBytes = kTile * kRowBytes;
   constexpr int kSteps = D / 16, kDb = D / 32;
-  __shared__ __attribute__((aligned(16))) uint8_t s_kv[2][2 * kHalf];
+  __shared__ __attribute__((aligned(16))) uint8_t s_k[2][kBytes], s_v[2][kBytes];
   __shared__ int s_odd;  // whether put() left out a value
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -183,7 +183,21 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
     off = (ok ? page : 0) * a.kv.sb * kSize + static_cast<int64_t>(t & mask) * st;
     paged = __ballot(ok);
   };
-  auto pages_of = [&](int i) { return static_cast<uint32_t>(paged >> (4 * (i & 15))) & 15u; };
+  int next = -1;
+  // Tile i, in order: where this wave's part of it lies, and which of its pages
+  // there are (past the last tile: the cache's first page, and none).
+  auto fetch = [&](int i, uint32_t* pages) __attribute__((always_inline)) {
+    if ((i & 15) == 0) {
+      if (i == 0) next = load_pages(0);
+      locate(i, next);
+      next = load_pages(i + 16);
+    }
+    *pages = static_cast<uint32_t>(paged >> (4 * (i & 15))) & 15u;
+    const int from = 4 * (i & 15) + wave;
+    return static_cast<int64_t>(
+        static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(off >> 32), from))) << 32 |
+        static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(off), from)));
+  };
 
   // staging: wave w brings tokens 16 w to 16 w + 15, load j the rows from
   // j * 64 / kPieces on
@@ -193,30 +207,37 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
   constexpr int kRowsPerLoad = 64 / kPieces;
   const uint32_t goff = srow * st + spiece * 16;
   attn_u32x4 kr[kLoads], vr[kLoads];
-  auto load = [&](int i) {
-    const int from = 4 * (i & 15) + wave;
-    const int64_t at = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(
-                                                __builtin_amdgcn_readlane(static_cast<int>(off >> 32), from)))
-                                            << 32) |
-                       static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(off), from));
+  auto load = [&](GlobalBytes base, int64_t at, attn_u32x4 (&r)[kLoads]) __attribute__((always_inline)) {
     const uint32_t go = here(goff);
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int64_t to = at + j * kRowsPerLoad * st;
-      kr[j] = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x4*>(scalar(kb + to) + go);
-      vr[j] = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x4*>(scalar(vb + to) + go);
-    }
+    for (int j = 0; j < kLoads; ++j)
+      r[j] = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x4*>(scalar(base + at + j * kRowsPerLoad * st) + go);
   };
   // whole: every row of the work-group sees every token of the tile
   auto is_whole = [&](int t, uint32_t pages) {
     return pages == 15u && t + kTile - 1 <= pmin && (a.window == 0 || t > pmax - a.window || t + kTile <= a.first);
   };
-  // To LDS.  0 times an infinity or a NaN is not 0, so in a tile that not every
+  // To LDS.  0 times an infinity or a NaN is not 0, so of a tile that not every
   // row sees whole such values become 0 here; the rows that do see one get it
   // at the end.
-  auto put = [&](int buf, bool whole) __attribute__((always_inline)) {
-    uint8_t* kd = s_kv[buf];
-    uint8_t* vd = kd + kHalf;
+  auto put = [&](uint8_t* to, attn_u32x4 (&r)[kLoads]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int row = 16 * wave + j * kRowsPerLoad + srow;
+      if constexpr (kE4m3) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          uint32_t w[4];
+          widen(r[j][2 * p], w), widen(r[j][2 * p + 1], w + 2);
+          *reinterpret_cast<attn_u32x4*>(to + row * kRowBytes + (piece_at<D>(row, 2 * spiece + p) << 4)) =
+              attn_u32x4{w[0], w[1], w[2], w[3]};
+        }
+      } else {
+        *reinterpret_cast<attn_u32x4*>(to + row * kRowBytes + (piece_at<D>(row, spiece) << 4)) = r[j];
+      }
+    }
+  };
+  auto put_values = [&](int buf, bool whole) __attribute__((always_inline)) {
     if (!whole) {
       uint32_t odd = 0;
 #pragma unroll
@@ -231,24 +252,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
         if (lane == 0) s_odd = 1;
       }
     }
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int row = 16 * wave + j * kRowsPerLoad + srow;
-      if constexpr (kE4m3) {
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          uint32_t w[8];
-          widen(kr[j][2 * p], w), widen(kr[j][2 * p + 1], w + 2), widen(vr[j][2 * p], w + 4), widen(vr[j][2 * p + 1], w + 6);
-          const int at = row * kRowBytes + (piece_at<D>(row, 2 * spiece + p) << 4);
-          *reinterpret_cast<attn_u32x4*>(kd + at) = attn_u32x4{w[0], w[1], w[2], w[3]};
-          *reinterpret_cast<attn_u32x4*>(vd + at) = attn_u32x4{w[4], w[5], w[6], w[7]};
-        }
-      } else {
-        const int at = row * kRowBytes + (piece_at<D>(row, spiece) << 4);
-        *reinterpret_cast<attn_u32x4*>(kd + at) = kr[j];
-        *reinterpret_cast<attn_u32x4*>(vd + at) = vr[j];
-      }
-    }
+    put(s_v[buf], vr);
   };
 
   // The reference of a row, its negative as the scores' products take it (+inf: none
@@ -272,67 +276,83 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
   for (int d = 0; d < kDb; ++d)
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      vat[d][e] = kHalf + (vrow + 8 * e) * kRowBytes + (piece_at<D>(vrow + 8 * e, 4 * d + vpiece) << 4) + 8 * (lane & 1);
-  auto value = [&](int buf, int d, int s) __attribute__((always_inline)) {  // dims 32 d on of the tokens of step s
-    bf16x8 x;
+      vat[d][e] = (vrow + 8 * e) * kRowBytes + (piece_at<D>(vrow + 8 * e, 4 * d + vpiece) << 4) + 8 * (lane & 1);
+  f32x16 s[2];   // scores of the two halves of a tile
+  bf16x8 w[2];   // weights of a half
+  float half_sum;  // and their sum
+  // Scores of half b of the tile in buffer buf.
+  auto score = [&](int buf, int b) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-      reinterpret_cast<s16x4*>(&x)[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4*)((LdsBytes)s_kv[buf] + vat[d][e] + 16 * s * kRowBytes));
-    return x;
+    for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+      s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+          *reinterpret_cast<const bf16x8*>(&s_k[buf][32 * b * kRowBytes + kat[k]]), q[k], s[b], 0, 0, 0);
   };
-
-  auto compute = [&](int t, int buf, uint32_t pages) __attribute__((always_inline)) {
-    f32x16 s[2];
+  // What the rows see of half b of the tile at t.
+  auto hide = [&](int t, int b, uint32_t pages) __attribute__((always_inline)) {
+    const int rel = pos - t - 4 * h - 32 * b, lowest = a.window > 0 ? rel - a.window : -1000, f = a.first - t - 4 * h - 32 * b;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        const bf16x8 x = *reinterpret_cast<const bf16x8*>(&s_kv[buf][32 * b * kRowBytes + kat[k]]);
-        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, q[k], s[b], 0, 0, 0);
-      }
+    for (int e = 0; e < 16; ++e) {
+      const int x = 8 * (e >> 2) + (e & 3);
+      const bool in = (pages >> (2 * b + (e >> 3)) & 1u) != 0 && x <= rel && (x > lowest || x < f);
+      any |= in;
+      s[b][e] = in ? s[b][e] : kNegInf;
     }
-    if (is_whole(t, pages)) {
+  };
+  // Weights of half b against 2^-off.
+  auto weigh = [&](int b, float off, bf16x8 (&to)[2]) __attribute__((always_inline)) {
+    float part[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * k + 2 * e], scale, off)),
+                           __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * k + 2 * e + 1], scale, off)));
+        part[e & 1] = add_two(x[e], part[e & 1]);
+      }
+      to[k] = __builtin_bit_cast(bf16x8, attn_u32x4{x[0], x[1], x[2], x[3]});
+    }
+    half_sum = part[0] + part[1];
+  };
+  // The values of half b in buffer buf, weighted.
+  auto add = [&](int buf, int b, const bf16x8 (&by)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < kDb; ++d)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        bf16x8 x;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          reinterpret_cast<s16x4*>(&x)[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)((LdsBytes)s_v[buf] + vat[d][e] + (32 * b + 16 * k) * kRowBytes));
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, by[k], o[d], 0, 0, 0);
+      }
+  };
+  // Half b of the tile at t in buffer buf: its weights, beside the products of
+  // the half before (values) and of the one after (scores).  These three do not
+  // depend on each other, so that matrix and vector instructions run together.
+  auto half = [&](int buf, int b, int t, uint32_t pages, bool whole) __attribute__((always_inline)) {
+    if (whole)
       any = true;
+    else
+      hide(t, b, pages);
+    bf16x8 now[2];
+    if (b == 0) {
+      score(buf, 1);
+      add(buf ^ 1, 1, w);
     } else {
-      const int rel = pos - t - 4 * h, lowest = a.window > 0 ? rel - a.window : -1 - 4 * h, f = a.first - t - 4 * h;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int x = 32 * b + 8 * (e >> 2) + (e & 3);
-          const bool in = (pages >> (2 * b + (e >> 3)) & 1u) != 0 && x <= rel && (x > lowest || x < f);
-          any |= in;
-          s[b][e] = in ? s[b][e] : kNegInf;
-        }
+      score(buf ^ 1, 0);
+      add(buf, 0, w);
     }
-    // Weights against the reference there is; only if they come out large (or
-    // there is none) the tile's maximum is looked for and they are formed again.
-    bf16x8 w[4];
-    float sum;
-    auto weigh = [&](float off) __attribute__((always_inline)) {
-      float part[2] = {0.0f, 0.0f};
+    weigh(b, less, now);
+    // Only if the weights come out large (or there is no reference) the half's
+    // maximum is looked for, and they are formed again.
+    if (__ballot(!(half_sum < kMost)) != 0) {
+      float top = s[b][0];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float lo = s[k >> 1][8 * (k & 1) + 2 * e], hi = s[k >> 1][8 * (k & 1) + 2 * e + 1];
-          x[e] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(lo, scale, off)),
-                             __builtin_amdgcn_exp2f(__builtin_fmaf(hi, scale, off)));
-          part[e & 1] = add_two(x[e], part[e & 1]);
-        }
-        w[k] = __builtin_bit_cast(bf16x8, attn_u32x4{x[0], x[1], x[2], x[3]});
-      }
-      sum = part[0] + part[1];
-    };
-    weigh(less);
-    if (__ballot(!(sum < kMost)) != 0) {
-      float top = s[0][0];
-#pragma unroll
-      for (int e = 1; e < 32; ++e) top = __builtin_fmaxf(top, s[e >> 4][e & 15]);
+      for (int e = 1; e < 16; ++e) top = __builtin_fmaxf(top, s[b][e]);
       top *= scale;
       top = __builtin_fmaxf(top, __shfl_xor(top, 32));
       const float mn = __builtin_fmaxf(m, top), base = mn == kNegInf ? 0.0f : mn;
@@ -344,43 +364,56 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
       for (int d = 0; d < kDb; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] *= keep;
-      weigh(-base);
+      weigh(b, -base, now);
     }
-    l += sum;
-#pragma unroll
-    for (int d = 0; d < kDb; ++d)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value(buf, d, k), w[k], o[d], 0, 0, 0);
+    l += half_sum;
+    w[0] = now[0], w[1] = now[1];
   };
 
   if (threadIdx.x == 0) s_odd = 0;
   __syncthreads();
   if (tiles > 0) {
-    locate(0, load_pages(0));
-    load(0);
-    uint32_t pages = pages_of(0);
-    int t = begin_of(0);
-    put(0, is_whole(t, pages));
+    // Tile i: K of tile i + 1 and V of tile i go to LDS, K of i + 2 and V of i + 1
+    // are asked for; then its two halves, with the only barrier between them: it
+    // shows what was put, and what is put next takes the place of K of tile i - 1
+    // and V of i - 2, which no wave reads behind it.
+    uint32_t pages, ahead;
+    int64_t at = fetch(0, &pages);
+    load(kb, at, kr);
+    load(vb, at, vr);
+    at = fetch(1, &ahead);
+    put(s_k[0], kr);
+    load(kb, at, kr);
+    for (int x = threadIdx.x; x < kBytes / 16; x += 256)  // taken with weights of 0 by the first half
+      reinterpret_cast<attn_u32x4*>(s_v[1])[x] = attn_u32x4{0, 0, 0, 0};
     __syncthreads();
-    int next = -1;
+    score(0, 0);
+    w[0] = w[1] = __builtin_bit_cast(bf16x8, attn_u32x4{0, 0, 0, 0});
     auto step = [&](auto B, int i) __attribute__((always_inline)) {
       constexpr int buf = decltype(B)::value;
-      if ((i & 15) == 0) next = load_pages(i + 16);
-      if ((i & 15) == 15) locate(i + 1, next);
-      const bool more = i + 1 < tiles;
-      const uint32_t ahead = pages_of(i + 1);
-      const int u = begin_of(i + 1);
-      if (more) load(i + 1);
-      compute(t, buf, pages);
-      if (more) put(buf ^ 1, is_whole(u, ahead));
-      pages = ahead;
-      t = u;
+      const int t = begin_of(i);
+      const bool whole = is_whole(t, pages);
+      put(s_k[buf ^ 1], kr);
+      put_values(buf, whole);
+      uint32_t later;
+      const int64_t to = fetch(i + 2, &later);
+      load(vb, at, vr);
+      load(kb, to, kr);
+      at = to;
+      half(buf, 0, t, pages, whole);
       __syncthreads();
+      half(buf, 1, t, pages, whole);
+      pages = ahead;
+      ahead = later;
     };
     for (int i = 0; i < tiles; i += 2) {
       step(std::integral_constant<int, 0>{}, i);
       if (i + 1 < tiles) step(std::integral_constant<int, 1>{}, i + 1);
     }
+    if (tiles & 1)
+      add(0, 1, w);
+    else
+      add(1, 1, w);
   }
   if (s_odd != 0) {
     // what put() left out, for the rows that see it
