@@ -21,12 +21,12 @@ namespace gxmoe {
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(1))) uint8_t* GlobalBytes;
 typedef __attribute__((address_space(3))) uint8_t* LdsBytes;
 
-constexpr int kRows = 128;    // rows of a work-group
 constexpr int kTile = 64;     // tokens of a step
 constexpr int kMinTiles = 4;  // tiles of the smallest piece
 constexpr float kMost = 4096.0f;  // a lane's sum of weights from which on the reference moves
@@ -49,37 +49,43 @@ struct Chunk {
 };
 
 // Tile `at` of all tiles of `per` tokens, the last one first: the longest rows
-// of a prompt begin earliest.
+// of a prompt begin earliest.  (64 sequences at a time, a lane each; what is read of
+// the first 64 is read once, lengths and offsets together.)
 __device__ __forceinline__ bool find_chunk(const AttendArgs& a, int at, int per, Chunk* c) {
   const int lane = threadIdx.x & 63;
-  auto span = [&](int b, int* begin) {  // new tokens of sequence b, within the rows that there are
-    const int lo = min(max(a.offsets[b], 0), a.rows);
-    *begin = lo;
-    return max(0, min(a.offsets[b + 1], a.rows) - lo);
+  struct Span {
+    int begin, n, len;  // new tokens of a sequence, within the rows that there are
   };
-  int total = 0, begin;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int tiles = b0 + lane < a.B ? (span(b0 + lane, &begin) + per - 1) / per : 0;
-    total += __builtin_amdgcn_readlane(wave_scan(tiles), 63);
-  }
-  at = total - 1 - at;
+  auto span = [&](int b) {
+    Span s{0, 0, 0};
+    if (b < a.B) {
+      const int lo = a.offsets[b], hi = a.offsets[b + 1];
+      s.len = seq_len(a, b);
+      s.begin = min(max(lo, 0), a.rows);
+      s.n = max(0, min(hi, a.rows) - s.begin);
+    }
+    return s;
+  };
+  const Span mine = span(lane);
+  int total = wave_scan((mine.n + per - 1) / per);
+  for (int b0 = 64; b0 < a.B; b0 += 64) total += wave_scan((span(b0 + lane).n + per - 1) / per);
+  at = __builtin_amdgcn_readlane(total, 63) - 1 - at;
   if (at < 0) return false;
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    begin = 0;
-    const int n = b0 + lane < a.B ? span(b0 + lane, &begin) : 0;
-    const int upto = before + wave_scan((n + per - 1) / per);
+    const Span s = b0 == 0 ? mine : span(b0 + lane);
+    const int upto = before + wave_scan((s.n + per - 1) / per);
     const uint64_t reached = __ballot(at < upto);
     if (reached != 0) {
       const int who = __builtin_ctzll(reached);
-      const int mine = __builtin_amdgcn_readlane(n, who);
-      const int first = __builtin_amdgcn_readlane(upto, who) - (mine + per - 1) / per;
+      const int n = __builtin_amdgcn_readlane(s.n, who);
+      const int first = __builtin_amdgcn_readlane(upto, who) - (n + per - 1) / per;
       c->b = b0 + who;
-      c->row0 = __builtin_amdgcn_readlane(begin, who);
+      c->row0 = __builtin_amdgcn_readlane(s.begin, who);
       c->tok0 = (at - first) * per;
-      c->tokens = min(per, mine - c->tok0);
-      c->len = __builtin_amdgcn_readfirstlane(seq_len(a, c->b));
-      c->pos0 = c->len - mine + c->tok0;
+      c->tokens = min(per, n - c->tok0);
+      c->len = __builtin_amdgcn_readlane(s.len, who);
+      c->pos0 = c->len - n + c->tok0;
       return true;
     }
     before = __builtin_amdgcn_readlane(upto, 63);
@@ -112,8 +118,8 @@ __device__ __forceinline__ int piece_at(int t, int piece) {
   return piece ^ ((t & 3) << 2 | (t >> 2 & 3));
 }
 
-template <int D, bool kE4m3>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArgs a, PieceArgs pa) {
+template <int D, bool kE4m3, int kCols>
+__global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_kernel(AttendArgs a, PieceArgs pa) {
   constexpr int kSize = kE4m3 ? 1 : 2;
   constexpr int kPieces = D * kSize / 16;      // 16-byte pieces of a token's row in memory
   constexpr int kLoads = 16 * kPieces / 64;    // loads of a wave for its 16 tokens of K, and of V
@@ -125,25 +131,31 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
-  const int group = a.heads / a.kv.kv_heads, per = kRows / group;
+  const int group = a.heads / a.kv.kv_heads, per = 128 * kCols / group;
   const int kvh = __builtin_amdgcn_readfirstlane(blockIdx.x % a.kv.kv_heads);
   const int piece = __builtin_amdgcn_readfirstlane(blockIdx.x / a.kv.kv_heads % pa.pieces);
   Chunk c;
   if (!find_chunk(a, blockIdx.x / a.kv.kv_heads / pa.pieces, per, &c)) return;
   for (int* x : {&c.b, &c.row0, &c.tokens, &c.tok0, &c.pos0, &c.len}) *x = __builtin_amdgcn_readfirstlane(*x);
 
-  // this lane's row
-  const int r = 32 * wave + n;
-  const int tok = r / group, head = kvh * group + r % group;
-  const bool mine = tok < c.tokens;
-  const int pos = mine ? c.pos0 + tok : -1;
-  const int64_t qrow = c.row0 + c.tok0 + (mine ? tok : 0);
-  bf16x8 q[kSteps];
+  // this lane's rows: 32 y + n of the wave's 32 kCols
+  int head[kCols], pos[kCols];
+  bool mine[kCols];
+  int64_t qrow[kCols];
+  bf16x8 q[kCols][kSteps];
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    attn_u32x4 x = *reinterpret_cast<const attn_u32x4*>(a.q + qrow * a.q_stride + static_cast<int64_t>(head) * D + 16 * s + 8 * h);
-    if (!mine) x = attn_u32x4{0, 0, 0, 0};
-    q[s] = __builtin_bit_cast(bf16x8, x);
+  for (int y = 0; y < kCols; ++y) {
+    const int r = 32 * (kCols * wave + y) + n, tok = r / group;
+    head[y] = kvh * group + r % group;
+    mine[y] = tok < c.tokens;
+    pos[y] = mine[y] ? c.pos0 + tok : -1;
+    qrow[y] = c.row0 + c.tok0 + (mine[y] ? tok : 0);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      attn_u32x4 x = *reinterpret_cast<const attn_u32x4*>(a.q + qrow[y] * a.q_stride + static_cast<int64_t>(head[y]) * D + 16 * s + 8 * h);
+      if (!mine[y]) x = attn_u32x4{0, 0, 0, 0};
+      q[y][s] = __builtin_bit_cast(bf16x8, x);
+    }
   }
   const float scale = a.scale_log2 * (kE4m3 && a.kv.k_scale ? a.kv.k_scale[kvh] : 1.0f);
 
@@ -257,13 +269,17 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
 
   // The reference of a row, its negative as the scores' products take it (+inf: none
   // yet, so that the first score of the row leads to one), the sum.
-  float m = kNegInf, less = mine ? __builtin_inff() : 0.0f, l = 0.0f;
-  bool any = false;
-  f32x16 o[kDb];
+  float m[kCols], less[kCols], l[kCols];
+  bool any[kCols];
+  f32x16 o[kCols][kDb];
 #pragma unroll
-  for (int d = 0; d < kDb; ++d)
+  for (int y = 0; y < kCols; ++y) {
+    m[y] = kNegInf, less[y] = mine[y] ? __builtin_inff() : 0.0f, l[y] = 0.0f, any[y] = false;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+    for (int d = 0; d < kDb; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[y][d][e] = 0.0f;
+  }
 
   // LDS addresses.  K: token 32 b + n, piece 2 s + h.  V: the 16 lanes of a quarter
   // read 4 tokens x 16 dims and are left with 4 tokens of one dim each.
@@ -277,97 +293,122 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       vat[d][e] = (vrow + 8 * e) * kRowBytes + (piece_at<D>(vrow + 8 * e, 4 * d + vpiece) << 4) + 8 * (lane & 1);
-  f32x16 s[2];   // scores of the two halves of a tile
-  bf16x8 w[2];   // weights of a half
-  float half_sum;  // and their sum
-  // Scores of half b of the tile in buffer buf.
-  auto score = [&](int buf, int b) __attribute__((always_inline)) {
+  f32x16 s[2][kCols];   // scores of the two halves of a tile
+  bf16x8 w[kCols][2];   // weights of a half
+  // One of the kSteps products of the scores of half b of the tile in buffer buf.
+  auto score = [&](int buf, int b, int k) __attribute__((always_inline)) {
+    const bf16x8 x = *reinterpret_cast<const bf16x8*>(&s_k[buf][32 * b * kRowBytes + kat[k]]);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k)
-      s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-          *reinterpret_cast<const bf16x8*>(&s_k[buf][32 * b * kRowBytes + kat[k]]), q[k], s[b], 0, 0, 0);
+    for (int y = 0; y < kCols; ++y) s[b][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, q[y][k], s[b][y], 0, 0, 0);
   };
-  // What the rows see of half b of the tile at t.
+  auto clear = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int y = 0; y < kCols; ++y)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[b][y][e] = 0.0f;
+  };
+  // What the rows see of half b of the tile at t: a bit for each of its 32
+  // tokens, the lane's own at the places that its scores have.
   auto hide = [&](int t, int b, uint32_t pages) __attribute__((always_inline)) {
-    const int rel = pos - t - 4 * h - 32 * b, lowest = a.window > 0 ? rel - a.window : -1000, f = a.first - t - 4 * h - 32 * b;
+    auto below = [](int x) { return x >= 32 ? ~0u : x <= 0 ? 0u : (1u << x) - 1u; };  // tokens 0 to x - 1
+    const int at = t + 32 * b;
+    const uint32_t there = (pages >> (2 * b) & 1u ? 0xffffu : 0u) | (pages >> (2 * b + 1) & 1u ? 0xffff0000u : 0u);
+    const uint32_t first = below(min(a.first, 0x40000000) - at);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int x = 8 * (e >> 2) + (e & 3);
-      const bool in = (pages >> (2 * b + (e >> 3)) & 1u) != 0 && x <= rel && (x > lowest || x < f);
-      any |= in;
-      s[b][e] = in ? s[b][e] : kNegInf;
+    for (int y = 0; y < kCols; ++y) {
+      const int rel = pos[y] - at;
+      const uint32_t old = a.window > 0 ? below(rel - a.window + 1) & ~first : 0u;
+      const uint32_t in = (pos[y] < 0 ? 0u : below(rel + 1) & ~old & there) >> (4 * h);
+      any[y] |= (in & 0x0f0f0f0fu) != 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t keep = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(in), 8 * (e >> 2) + (e & 3), 1));
+        s[b][y][e] = __uint_as_float((__float_as_uint(s[b][y][e]) & keep) | (0xff800000u & ~keep));
+      }
     }
   };
-  // Weights of half b against 2^-off.
-  auto weigh = [&](int b, float off, bf16x8 (&to)[2]) __attribute__((always_inline)) {
-    float part[2] = {0.0f, 0.0f};
+  // Weights number x to x + n - 1 of half b against 2^-off, and their sum.
+  float part[kCols][2];
+  uint32_t now[kCols][8];
+  auto weigh = [&](int b, int y, float off, int x, int n) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      uint32_t x[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * k + 2 * e], scale, off)),
-                           __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * k + 2 * e + 1], scale, off)));
-        part[e & 1] = add_two(x[e], part[e & 1]);
-      }
-      to[k] = __builtin_bit_cast(bf16x8, attn_u32x4{x[0], x[1], x[2], x[3]});
+    for (int e = x; e < x + n; e += 2) {
+      now[y][e / 2] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[b][y][e], scale, off)),
+                                  __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][y][e + 1], scale, off)));
+      part[y][e / 2 & 1] = add_two(now[y][e / 2], part[y][e / 2 & 1]);
     }
-    half_sum = part[0] + part[1];
   };
-  // The values of half b in buffer buf, weighted.
-  auto add = [&](int buf, int b, const bf16x8 (&by)[2]) __attribute__((always_inline)) {
+  // One of the kSteps products of the weighted values of half b in buffer buf: 16
+  // tokens, 32 dims, the dims in turn so that a sum is not waited for.
+  auto add = [&](int buf, int b, int x) __attribute__((always_inline)) {
+    const int d = x % kDb, k = x / kDb;
+    bf16x8 v;
 #pragma unroll
-    for (int d = 0; d < kDb; ++d)
+    for (int e = 0; e < 2; ++e)
+      reinterpret_cast<s16x4*>(&v)[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)((LdsBytes)s_v[buf] + vat[d][e] + (32 * b + 16 * k) * kRowBytes));
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        bf16x8 x;
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          reinterpret_cast<s16x4*>(&x)[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s16x4*)((LdsBytes)s_v[buf] + vat[d][e] + (32 * b + 16 * k) * kRowBytes));
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, by[k], o[d], 0, 0, 0);
-      }
+    for (int y = 0; y < kCols; ++y) o[y][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w[y][k], o[y][d], 0, 0, 0);
   };
   // Half b of the tile at t in buffer buf: its weights, beside the products of
   // the half before (values) and of the one after (scores).  These three do not
   // depend on each other, so that matrix and vector instructions run together.
   auto half = [&](int buf, int b, int t, uint32_t pages, bool whole) __attribute__((always_inline)) {
-    if (whole)
-      any = true;
-    else
-      hide(t, b, pages);
-    bf16x8 now[2];
-    if (b == 0) {
-      score(buf, 1);
-      add(buf ^ 1, 1, w);
-    } else {
-      score(buf ^ 1, 0);
-      add(buf, 0, w);
+    if (!whole) hide(t, b, pages);
+    clear(b ^ 1);
+#pragma unroll
+    for (int y = 0; y < kCols; ++y) any[y] |= whole, part[y][0] = part[y][1] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) {
+      score(b == 0 ? buf : buf ^ 1, b ^ 1, x);
+      add(b == 0 ? buf ^ 1 : buf, b ^ 1, x);
+#pragma unroll
+      for (int y = 0; y < kCols; ++y) weigh(b, y, less[y], 16 / kSteps * x, 16 / kSteps);
     }
-    weigh(b, less, now);
+    // the order to issue them in: the LDS reads of a step, then its products with
+    // vector instructions behind each
+    __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) {
+#pragma unroll
+      for (int y = 0; y < 2 * kCols; ++y) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, kSteps == 4 ? 6 : 3, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+    }
     // Only if the weights come out large (or there is no reference) the half's
     // maximum is looked for, and they are formed again.
-    if (__ballot(!(half_sum < kMost)) != 0) {
-      float top = s[b][0];
+    bool large = false;
 #pragma unroll
-      for (int e = 1; e < 16; ++e) top = __builtin_fmaxf(top, s[b][e]);
-      top *= scale;
-      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-      const float mn = __builtin_fmaxf(m, top), base = mn == kNegInf ? 0.0f : mn;
-      const float keep = __builtin_amdgcn_exp2f(m - base);
-      m = mn;
-      less = mn == kNegInf && mine ? __builtin_inff() : -base;
-      l *= keep;
+    for (int y = 0; y < kCols; ++y) large |= !(part[y][0] + part[y][1] < kMost);
+    if (__ballot(large) != 0) {
 #pragma unroll
-      for (int d = 0; d < kDb; ++d)
+      for (int y = 0; y < kCols; ++y) {
+        float top = s[b][y][0];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] *= keep;
-      weigh(b, -base, now);
+        for (int e = 1; e < 16; ++e) top = __builtin_fmaxf(top, s[b][y][e]);
+        top *= scale;
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+        const float mn = __builtin_fmaxf(m[y], top), base = mn == kNegInf ? 0.0f : mn;
+        const float keep = __builtin_amdgcn_exp2f(m[y] - base);
+        m[y] = mn;
+        less[y] = mn == kNegInf && mine[y] ? __builtin_inff() : -base;
+        l[y] *= keep;
+#pragma unroll
+        for (int d = 0; d < kDb; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[y][d][e] *= keep;
+        part[y][0] = part[y][1] = 0.0f;
+        weigh(b, y, -base, 0, 16);
+      }
     }
-    l += half_sum;
-    w[0] = now[0], w[1] = now[1];
+#pragma unroll
+    for (int y = 0; y < kCols; ++y) {
+      l[y] += part[y][0] + part[y][1];
+      w[y][0] = __builtin_bit_cast(bf16x8, attn_u32x4{now[y][0], now[y][1], now[y][2], now[y][3]});
+      w[y][1] = __builtin_bit_cast(bf16x8, attn_u32x4{now[y][4], now[y][5], now[y][6], now[y][7]});
+    }
   };
 
   if (threadIdx.x == 0) s_odd = 0;
@@ -387,8 +428,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
     for (int x = threadIdx.x; x < kBytes / 16; x += 256)  // taken with weights of 0 by the first half
       reinterpret_cast<attn_u32x4*>(s_v[1])[x] = attn_u32x4{0, 0, 0, 0};
     __syncthreads();
-    score(0, 0);
-    w[0] = w[1] = __builtin_bit_cast(bf16x8, attn_u32x4{0, 0, 0, 0});
+    clear(0);
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) score(0, 0, x);
+#pragma unroll
+    for (int y = 0; y < kCols; ++y) w[y][0] = w[y][1] = __builtin_bit_cast(bf16x8, attn_u32x4{0, 0, 0, 0});
     auto step = [&](auto B, int i) __attribute__((always_inline)) {
       constexpr int buf = decltype(B)::value;
       const int t = begin_of(i);
@@ -410,10 +454,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
       step(std::integral_constant<int, 0>{}, i);
       if (i + 1 < tiles) step(std::integral_constant<int, 1>{}, i + 1);
     }
-    if (tiles & 1)
-      add(0, 1, w);
-    else
-      add(1, 1, w);
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) {
+      if (tiles & 1)
+        add(0, 1, x);
+      else
+        add(1, 1, x);
+    }
   }
   if (s_odd != 0) {
     // what put() left out, for the rows that see it
@@ -429,73 +476,83 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefill_kernel(AttendArg
           const int g = u < c.len ? a.tables[c.b * a.table_stride + (u >> a.kv.bs_shift)] : -1;
           all |= static_cast<uint32_t>(g) < static_cast<uint32_t>(a.kv.num_blocks) ? 1u << j : 0u;
         }
-        if (is_whole(tile_at(i), all) || pos < 0 || !sees(a, pos, t)) continue;
+        if (is_whole(tile_at(i), all)) continue;
         GlobalBytes v = vb + page * a.kv.sb * kSize + static_cast<int64_t>(t & mask) * st + 4 * h * kSize;
 #pragma unroll
-        for (int d = 0; d < kDb; ++d)
+        for (int y = 0; y < kCols; ++y) {
+          if (pos[y] < 0 || !sees(a, pos[y], t)) continue;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t w[2];
-            if constexpr (kE4m3) {
-              widen(*reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(v + 32 * d + 8 * k), w);
-            } else {
-              const attn_u32x2 y = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x2*>(v + 64 * d + 16 * k);
-              w[0] = y[0], w[1] = y[1];
-            }
+          for (int d = 0; d < kDb; ++d)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float y = bf16_to_f32(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))));
-              o[d][4 * k + e] += (__float_as_uint(y) & 0x7f800000u) == 0x7f800000u ? y : 0.0f;
+            for (int k = 0; k < 4; ++k) {
+              uint32_t w[2];
+              if constexpr (kE4m3) {
+                widen(*reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(v + 32 * d + 8 * k), w);
+              } else {
+                const attn_u32x2 x = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x2*>(v + 64 * d + 16 * k);
+                w[0] = x[0], w[1] = x[1];
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = bf16_to_f32(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))));
+                o[y][d][4 * k + e] += (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? x : 0.0f;
+              }
             }
-          }
+        }
       }
     }
   }
 
-  l += __shfl_xor(l, 32);
-  any |= __shfl_xor(static_cast<int>(any), 32) != 0;
-  if (!mine) return;
-  if (pieces > 1) {
-    const int64_t at = (static_cast<int64_t>(piece) * a.rows + qrow) * a.heads + head;
-    typedef float f32x4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-    for (int d = 0; d < kDb; ++d)
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        *reinterpret_cast<f32x4*>(pa.part_o + at * D + 32 * d + 8 * k + 4 * h) =
-            f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
-    if (h == 0) reinterpret_cast<f32x4*>(pa.part_ml)[at] = f32x4{m, l, any ? 1.0f : 0.0f, 0.0f};
-    return;
-  }
-  float sum = l;
-  if (a.sinks) {
-    const float sink = bf16_to_f32(a.sinks[head]) * kLog2e;
-    const float top = __builtin_fmaxf(m, sink), base = top == kNegInf ? 0.0f : top;
-    const float keep = __builtin_amdgcn_exp2f(m - base);
-    sum = l * keep + __builtin_amdgcn_exp2f(sink - base);
-#pragma unroll
-    for (int d = 0; d < kDb; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[d][e] *= keep;
-  }
   const float vs = kE4m3 && a.kv.v_scale ? a.kv.v_scale[kvh] : 1.0f;
-  const float f = vs / sum;
-  uint16_t* to = a.out + qrow * a.out_stride + static_cast<int64_t>(head) * D + 4 * h;
 #pragma unroll
-  for (int d = 0; d < kDb; ++d)
+  for (int y = 0; y < kCols; ++y) {
+    float sum = l[y] + __shfl_xor(l[y], 32);
+    const bool seen = any[y] | (__shfl_xor(static_cast<int>(any[y]), 32) != 0);
+    if (!mine[y]) continue;
+    if (pieces > 1) {
+      const int64_t at = (static_cast<int64_t>(piece) * a.rows + qrow[y]) * a.heads + head[y];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float x[4];
+      for (int d = 0; d < kDb; ++d)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = any ? o[d][4 * k + e] * f : 0.0f;
-      *reinterpret_cast<attn_u32x2*>(to + 32 * d + 8 * k) = attn_u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<f32x4*>(pa.part_o + at * D + 32 * d + 8 * k + 4 * h) =
+              f32x4{o[y][d][4 * k], o[y][d][4 * k + 1], o[y][d][4 * k + 2], o[y][d][4 * k + 3]};
+      if (h == 0) reinterpret_cast<f32x4*>(pa.part_ml)[at] = f32x4{m[y], sum, seen ? 1.0f : 0.0f, 0.0f};
+      continue;
     }
+    float keep = 1.0f;
+    if (a.sinks) {
+      const float sink = bf16_to_f32(a.sinks[head[y]]) * kLog2e;
+      const float top = __builtin_fmaxf(m[y], sink), base = top == kNegInf ? 0.0f : top;
+      keep = __builtin_amdgcn_exp2f(m[y] - base);
+      sum = sum * keep + __builtin_amdgcn_exp2f(sink - base);
+    }
+    const float f = vs / sum;
+    uint16_t* to = a.out + qrow[y] * a.out_stride + static_cast<int64_t>(head[y]) * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < kDb; ++d)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = seen ? o[y][d][4 * k + e] * keep * f : 0.0f;
+        *reinterpret_cast<attn_u32x2*>(to + 32 * d + 8 * k) = attn_u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+      }
+  }
+}
+
+// Rows of a wave: 64 where the registers allow it and there are rows to fill the
+// chip with, else 32.
+constexpr int kTwoCols = 2048;
+int cols_of(int rows, int heads, int head_dim) {
+  return head_dim == 64 && static_cast<int64_t>(rows) * heads >= 256 * kTwoCols ? 2 : 1;
 }
 
 // Pieces: as many as fill the chip (work-groups that it holds at once: three on a
 // CU with heads of 64 dims, two with 128) when the tiles of rows alone do not.
 int most_pieces(int rows, int B, int heads, int kv_heads, int head_dim) {
-  const int per = kRows / (heads / kv_heads);
+  if (cols_of(rows, heads, head_dim) == 2) return 1;
+  const int per = 128 / (heads / kv_heads);
   const int64_t tiles = (static_cast<int64_t>(rows) + per - 1) / per + (B < rows ? B : rows) - 1;
   const int64_t pieces = (head_dim == 64 ? 768 : 512) / (tiles * kv_heads);
   return pieces < 1 ? 1 : static_cast<int>(pieces);
@@ -511,7 +568,7 @@ size_t prefill_workspace_bytes(int rows, int B, int heads, int kv_heads, int hea
 }
 
 hipError_t launch_prefill(const AttendArgs& a, void* workspace, hipStream_t s) {
-  const int per = kRows / (a.heads / a.kv.kv_heads);
+  const int cols = cols_of(a.rows, a.heads, a.kv.head_dim), per = 128 * cols / (a.heads / a.kv.kv_heads);
   // no more tiles than the longest sequence, or a window over a tile's rows, has
   const int64_t cap = static_cast<int64_t>(a.max_blocks) << a.kv.bs_shift;
   int64_t most = (cap + kTile - 1) / kTile;
@@ -528,13 +585,16 @@ hipError_t launch_prefill(const AttendArgs& a, void* workspace, hipStream_t s) {
   // sum of ceil(new tokens / per), at most one tile more for each sequence that has rows
   const int64_t tiles = (static_cast<int64_t>(a.rows) + per - 1) / per + (a.B < a.rows ? a.B : a.rows);
   const dim3 grid(static_cast<unsigned>(tiles * a.kv.kv_heads * pa.pieces));
-#define GX_PREFILL(D_, E_) hipLaunchKernelGGL((prefill_kernel<D_, E_>), grid, dim3(256), 0, s, a, pa)
-  if (a.kv.head_dim == 64) {
-    if (a.kv.e4m3) GX_PREFILL(64, true);
-    else GX_PREFILL(64, false);
+#define GX_PREFILL(D_, E_, C_) hipLaunchKernelGGL((prefill_kernel<D_, E_, C_>), grid, dim3(256), 0, s, a, pa)
+  if (a.kv.head_dim == 64 && cols == 2) {
+    if (a.kv.e4m3) GX_PREFILL(64, true, 2);
+    else GX_PREFILL(64, false, 2);
+  } else if (a.kv.head_dim == 64) {
+    if (a.kv.e4m3) GX_PREFILL(64, true, 1);
+    else GX_PREFILL(64, false, 1);
   } else {
-    if (a.kv.e4m3) GX_PREFILL(128, true);
-    else GX_PREFILL(128, false);
+    if (a.kv.e4m3) GX_PREFILL(128, true, 1);
+    else GX_PREFILL(128, false, 1);
   }
 #undef GX_PREFILL
   const hipError_t e = hipGetLastError();
