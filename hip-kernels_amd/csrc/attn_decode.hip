@@ -337,8 +337,21 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
 #pragma unroll
     for (int c = 0; c < 8; ++c) w[c] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c >> 2][c & 3], scale, -base));
     l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-    const bf16x8 wb = __builtin_bit_cast(
-        bf16x8, attn_u32x4{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]), pack_bf16x2(w[4], w[5]), pack_bf16x2(w[6], w[7])});
+    // The weights as two bf16 each, cut off and what that leaves: 16 bits of them
+    // count, for a product that the loads hide.  The second is kept above 0: 0
+    // times an infinite value would be NaN where the weight is not 0.
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float rest[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        rest[e] = __builtin_fmaxf(w[2 * c + e] - __uint_as_float(__float_as_uint(w[2 * c + e]) & 0xffff0000u), 1e-36f);
+      hi[c] = __builtin_amdgcn_perm(__float_as_uint(w[2 * c + 1]), __float_as_uint(w[2 * c]), 0x07060302u);
+      lo[c] = pack_bf16x2(rest[0], rest[1]);
+    }
+    const bf16x8 wb = __builtin_bit_cast(bf16x8, attn_u32x4{hi[0], hi[1], hi[2], hi[3]});
+    const bf16x8 wl = __builtin_bit_cast(bf16x8, attn_u32x4{lo[0], lo[1], lo[2], lo[3]});
 #pragma unroll
     for (int d = 0; d < kDt; ++d) {
       const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;  // the high or the low halves of two dwords
@@ -346,6 +359,7 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
 #pragma unroll
       for (int c = 0; c < 4; ++c) x[c] = __builtin_amdgcn_perm(vd[2 * c + 1][d >> 1], vd[2 * c][d >> 1], sel);
       o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), wb, o[d], 0, 0, 0);
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), wl, o[d], 0, 0, 0);
     }
   };
 

@@ -539,8 +539,9 @@ typedef struct gptoss_attention_config {
  * sequence, at position seq_lens[b] - 1; q and out are [num_seqs][num_heads *
  * head_dim] bf16, rows q_stride and out_stride elements apart (multiples of
  * 8), apart from each other, 16-byte aligned.  num_heads is a multiple of the
- * kv heads, at most 128 per kv head.  The scores and sums are fp32, the
- * weights bf16 against bf16 values.
+ * kv heads, at most 128 per kv head.  Scores and sums are fp32; the softmax's
+ * weights meet the values with 16 significant bits here and rounded to bf16 in
+ * the prefill call.
  * workspace: gptoss_paged_attention_workspace_bytes bytes, 16-byte aligned,
  * that no call running at the same time uses (two graphs that may overlap need
  * two); nothing is kept in it between calls. */
