@@ -110,6 +110,16 @@ __device__ __forceinline__ GlobalBytes scalar(GlobalBytes p) {
   return p;
 }
 
+typedef attn_u32x4 __attribute__((may_alias)) Piece;
+typedef attn_u32x2 __attribute__((may_alias)) HalfPiece;
+
+// Orders a wave's LDS traffic: what its lanes wrote before is what they read
+// behind it.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Where in its row of LDS a 16-byte piece of token t lies: the 16 tokens that
 // take part in a read of K, and the four of a read of V, meet in no bank.
 template <int D>
@@ -126,7 +136,12 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
   constexpr int kRowBytes = 2 * D;             // of a token in LDS
   constexpr int kBytes = kTile * kRowBytes;
   constexpr int kSteps = D / 16, kDb = D / 32;
-  __shared__ __attribute__((aligned(16))) uint8_t s_k[2][kBytes], s_v[2][kBytes];
+  constexpr int kOutRow = 144;                 // of a row's 128 bytes on their way out, in LDS
+  // K of two tiles, then V of two; the queries pass through the middle half of it
+  // before, the results through its beginning afterwards
+  __shared__ __attribute__((aligned(16))) uint8_t s_kv[4][kBytes];
+  uint8_t(*const s_k)[kBytes] = s_kv;
+  uint8_t(*const s_v)[kBytes] = s_kv + 2;
   __shared__ int s_odd;  // whether put() left out a value
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -138,10 +153,13 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
   if (!find_chunk(a, blockIdx.x / a.kv.kv_heads / pa.pieces, per, &c)) return;
   for (int* x : {&c.b, &c.row0, &c.tokens, &c.tok0, &c.pos0, &c.len}) *x = __builtin_amdgcn_readfirstlane(*x);
 
-  // this lane's rows: 32 y + n of the wave's 32 kCols
+  // This lane's rows: 32 y + n of the wave's 32 kCols.  Rows move between memory
+  // and LDS in 128-byte pieces, eight lanes to each (a lane to a row: 16 and 8
+  // bytes of a line at a time, and the store of 8192 rows alone took 38 us).
   int head[kCols], pos[kCols];
   bool mine[kCols];
   int64_t qrow[kCols];
+  attn_u32x4 qt[kCols][D / 64][4];
   bf16x8 q[kCols][kSteps];
 #pragma unroll
   for (int y = 0; y < kCols; ++y) {
@@ -150,27 +168,35 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
     mine[y] = tok < c.tokens;
     pos[y] = mine[y] ? c.pos0 + tok : -1;
     qrow[y] = c.row0 + c.tok0 + (mine[y] ? tok : 0);
+    const int64_t from = qrow[y] * a.q_stride + static_cast<int64_t>(head[y]) * D;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      attn_u32x4 x = *reinterpret_cast<const attn_u32x4*>(a.q + qrow[y] * a.q_stride + static_cast<int64_t>(head[y]) * D + 16 * s + 8 * h);
-      if (!mine[y]) x = attn_u32x4{0, 0, 0, 0};
-      q[y][s] = __builtin_bit_cast(bf16x8, x);
+    for (int i = 0; i < 4; ++i) {
+      const uint16_t* row = a.q + __shfl(from, 8 * i + (lane >> 3));
+      const bool in = __shfl(static_cast<int>(mine[y]), 8 * i + (lane >> 3)) != 0;
+#pragma unroll
+      for (int g = 0; g < D / 64; ++g) {
+        qt[y][g][i] = reinterpret_cast<const attn_u32x4*>(row + 64 * g)[lane & 7];
+        if (!in) qt[y][g][i] = attn_u32x4{0, 0, 0, 0};
+      }
     }
   }
   const float scale = a.scale_log2 * (kE4m3 && a.kv.k_scale ? a.kv.k_scale[kvh] : 1.0f);
 
+  const bool work = 32 * kCols * wave < c.tokens * group;  // whether any of the wave's rows is one
   // the tiles that the rows see: the first tokens', then the window's
   const int pmin = c.pos0, pmax = c.pos0 + c.tokens - 1;
   const int low = a.window > 0 ? max(0, pmin - a.window + 1) : 0;
-  const int main = low / kTile, nf = min((min(a.first, low) + kTile - 1) / kTile, main);
-  const int all_tiles = pmax < 0 ? 0 : nf + pmax / kTile + 1 - main;
+  // (from a page's 16 tokens on, where no first tokens lie on the same grid)
+  const int begin = a.first > 0 ? low & ~(kTile - 1) : low & ~15;
+  const int nf = min((min(a.first, low) + kTile - 1) / kTile, begin / kTile);
+  const int all_tiles = pmax < 0 ? 0 : nf + (pmax - begin) / kTile + 1;
   const int pieces = max(1, min(pa.pieces, all_tiles / kMinTiles));
   if (piece >= pieces) return;
   const int first_tile = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(all_tiles) * piece / pieces));
   const int tiles = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(all_tiles) * (piece + 1) / pieces) - first_tile);
   auto tile_at = [&](int i) {
     const int t = first_tile + i;
-    return (t < nf ? t : main + t - nf) * kTile;
+    return t < nf ? t * kTile : begin + (t - nf) * kTile;
   };
   auto begin_of = [&](int i) { return __builtin_amdgcn_readfirstlane(tile_at(i)); };
   if (pa.pieces > 1 && piece == 0 && kvh == 0 && threadIdx.x < c.tokens) pa.plan[c.row0 + c.tok0 + threadIdx.x] = pieces;
@@ -365,17 +391,21 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
 #pragma unroll
       for (int y = 0; y < kCols; ++y) weigh(b, y, less[y], 16 / kSteps * x, 16 / kSteps);
     }
-    // the order to issue them in: the LDS reads of a step, then its products with
-    // vector instructions behind each
-    __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+    // The order to issue them in with 64 dims: LDS reads of a step ahead, or all
+    // of them where two products share each, then every product with vector
+    // instructions behind it.  (As the compiler has them: prompts of 1024 and 8192
+    // 24.8 and 605 us, 23.0 and 584 so; with 128 dims its order is the best one.)
+    if constexpr (D == 64) {
+      __builtin_amdgcn_sched_group_barrier(0x100, kCols == 1 ? 3 : 12, 0);
 #pragma unroll
-    for (int x = 0; x < kSteps; ++x) {
+      for (int x = 0; x < kSteps; ++x) {
 #pragma unroll
-      for (int y = 0; y < 2 * kCols; ++y) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, kSteps == 4 ? 6 : 3, 0);
+        for (int y = 0; y < 2 * kCols; ++y) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, kCols == 1 ? 3 : 0, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
     }
     // Only if the weights come out large (or there is no reference) the half's
     // maximum is looked for, and they are formed again.
@@ -411,6 +441,25 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
     }
   };
 
+  {
+    uint8_t* mid = s_kv[1] + wave * 4096;  // the wave's own
+#pragma unroll
+    for (int y = 0; y < kCols; ++y)
+#pragma unroll
+      for (int g = 0; g < D / 64; ++g) {
+        wave_order();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 8 * i + (lane >> 3);
+          *reinterpret_cast<Piece*>(mid + row * 128 + (((lane & 7) ^ (row & 7)) << 4)) = qt[y][g][i];
+        }
+        wave_order();
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          q[y][4 * g + k] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const Piece*>(mid + n * 128 + (((2 * k + h) ^ (n & 7)) << 4)));
+      }
+  }
+
   if (threadIdx.x == 0) s_odd = 0;
   __syncthreads();
   if (tiles > 0) {
@@ -418,6 +467,7 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
     // are asked for; then its two halves, with the only barrier between them: it
     // shows what was put, and what is put next takes the place of K of tile i - 1
     // and V of i - 2, which no wave reads behind it.
+    const bool two = pmax - begin_of(tiles - 1) >= 32;  // whether any row sees the last tile's second half
     uint32_t pages, ahead;
     int64_t at = fetch(0, &pages);
     load(kb, at, kr);
@@ -444,9 +494,9 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
       load(vb, at, vr);
       load(kb, to, kr);
       at = to;
-      half(buf, 0, t, pages, whole);
+      if (work) half(buf, 0, t, pages, whole);
       __syncthreads();
-      half(buf, 1, t, pages, whole);
+      if (work && (i + 1 < tiles || two)) half(buf, 1, t, pages, whole);
       pages = ahead;
       ahead = later;
     };
@@ -454,12 +504,20 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
       step(std::integral_constant<int, 0>{}, i);
       if (i + 1 < tiles) step(std::integral_constant<int, 1>{}, i + 1);
     }
+    // the values of the last half
 #pragma unroll
     for (int x = 0; x < kSteps; ++x) {
-      if (tiles & 1)
-        add(0, 1, x);
-      else
-        add(1, 1, x);
+      if (tiles & 1) {
+        if (two)
+          add(0, 1, x);
+        else
+          add(0, 0, x);
+      } else {
+        if (two)
+          add(1, 1, x);
+        else
+          add(1, 0, x);
+      }
     }
   }
   if (s_odd != 0) {
@@ -503,41 +561,60 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
     }
   }
 
+  // A 128-byte piece of 32 rows from the wave's part of LDS: row r to at(r) bytes
+  // from `to`, rows of no token left out.
+  __syncthreads();
+  uint8_t* mid = s_kv[0] + wave * 32 * kOutRow;
+  auto emit = [&](void* to, int64_t at, bool in) __attribute__((always_inline)) {
+    wave_order();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 8 * i + (lane >> 3);
+      const Piece x = *reinterpret_cast<const Piece*>(mid + row * kOutRow + 16 * (lane & 7));
+      const int64_t there = __shfl(at, row);
+      if (__shfl(static_cast<int>(in), row) != 0) *reinterpret_cast<attn_u32x4*>(static_cast<uint8_t*>(to) + there + 16 * (lane & 7)) = x;
+    }
+    wave_order();
+  };
   const float vs = kE4m3 && a.kv.v_scale ? a.kv.v_scale[kvh] : 1.0f;
 #pragma unroll
   for (int y = 0; y < kCols; ++y) {
     float sum = l[y] + __shfl_xor(l[y], 32);
     const bool seen = any[y] | (__shfl_xor(static_cast<int>(any[y]), 32) != 0);
-    if (!mine[y]) continue;
     if (pieces > 1) {
       const int64_t at = (static_cast<int64_t>(piece) * a.rows + qrow[y]) * a.heads + head[y];
 #pragma unroll
-      for (int d = 0; d < kDb; ++d)
+      for (int d = 0; d < kDb; ++d) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<f32x4*>(pa.part_o + at * D + 32 * d + 8 * k + 4 * h) =
-              f32x4{o[y][d][4 * k], o[y][d][4 * k + 1], o[y][d][4 * k + 2], o[y][d][4 * k + 3]};
-      if (h == 0) reinterpret_cast<f32x4*>(pa.part_ml)[at] = f32x4{m[y], sum, seen ? 1.0f : 0.0f, 0.0f};
+          *reinterpret_cast<Piece*>(mid + n * kOutRow + 32 * k + 16 * h) =
+              __builtin_bit_cast(attn_u32x4, f32x4{o[y][d][4 * k], o[y][d][4 * k + 1], o[y][d][4 * k + 2], o[y][d][4 * k + 3]});
+        emit(pa.part_o, (at * D + 32 * d) * 4, mine[y]);
+      }
+      if (h == 0 && mine[y]) reinterpret_cast<f32x4*>(pa.part_ml)[at] = f32x4{m[y], sum, seen ? 1.0f : 0.0f, 0.0f};
       continue;
     }
-    float keep = 1.0f;
+    float f = vs / sum;
     if (a.sinks) {
       const float sink = bf16_to_f32(a.sinks[head[y]]) * kLog2e;
       const float top = __builtin_fmaxf(m[y], sink), base = top == kNegInf ? 0.0f : top;
-      keep = __builtin_amdgcn_exp2f(m[y] - base);
-      sum = sum * keep + __builtin_amdgcn_exp2f(sink - base);
+      const float keep = __builtin_amdgcn_exp2f(m[y] - base);
+      f = keep * (vs / (sum * keep + __builtin_amdgcn_exp2f(sink - base)));
     }
-    const float f = vs / sum;
-    uint16_t* to = a.out + qrow[y] * a.out_stride + static_cast<int64_t>(head[y]) * D + 4 * h;
 #pragma unroll
-    for (int d = 0; d < kDb; ++d)
+    for (int g = 0; g < D / 64; ++g) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float x[4];
+      for (int d = 0; d < 2; ++d)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = seen ? o[y][d][4 * k + e] * keep * f : 0.0f;
-        *reinterpret_cast<attn_u32x2*>(to + 32 * d + 8 * k) = attn_u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
-      }
+        for (int k = 0; k < 4; ++k) {
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = seen ? o[y][2 * g + d][4 * k + e] * f : 0.0f;
+          *reinterpret_cast<HalfPiece*>(mid + n * kOutRow + 64 * d + 16 * k + 8 * h) =
+              attn_u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+        }
+      emit(a.out, (qrow[y] * a.out_stride + static_cast<int64_t>(head[y]) * D + 64 * g) * 2, mine[y]);
+    }
   }
 }
 
