@@ -33,6 +33,8 @@ bool apart(const void* a, size_t na, const void* b, size_t nb) {
 }
 
 constexpr int kMaxGroup = 128;  // query heads per kv head
+constexpr int64_t kMaxRowHeads = 1 << 26, kMaxSeqHeads = 1 << 22;  // rows and sequences of a call, times heads
+constexpr int64_t kMaxTokens = 1 << 30;                            // of a sequence
 
 int check_cache(const gptoss_kv_cache* c, KvPages* kv) {
   if (c == nullptr) return set_error(GPTOSS_ERR_INVALID, "cache is NULL");
@@ -121,6 +123,13 @@ int check_attend(AttendArgs* a, const gptoss_kv_cache* cache, const gptoss_atten
   if (a->max_blocks < 1 || a->table_stride < a->max_blocks)
     return set_error(GPTOSS_ERR_INVALID, "max_blocks=%d must be positive and at most table_stride=%lld", a->max_blocks,
                      static_cast<long long>(a->table_stride));
+  // grids and counts of tiles stay within 32 bits
+  if (static_cast<int64_t>(rows) * a->heads > kMaxRowHeads || static_cast<int64_t>(B) * a->heads > kMaxSeqHeads)
+    return set_error(GPTOSS_ERR_UNSUPPORTED, "%d rows and %d sequences of %d heads in one call (at most 2^26 and 2^22)",
+                     rows, B, a->heads);
+  const int64_t cap = static_cast<int64_t>(a->max_blocks) << a->kv.bs_shift;
+  if (cap > kMaxTokens || cap / 16 + 1 > 0x7fffffff / B)
+    return set_error(GPTOSS_ERR_UNSUPPORTED, "tables of %d pages for %d sequences", a->max_blocks, B);
   const size_t need = gptoss_paged_attention_workspace_bytes(rows, B, a->heads, a->kv.kv_heads, a->kv.head_dim);
   if (need > 0) {
     if (workspace == nullptr || workspace_bytes < need)
@@ -128,15 +137,10 @@ int check_attend(AttendArgs* a, const gptoss_kv_cache* cache, const gptoss_atten
                        need);
     if (!aligned16(workspace)) return set_error(GPTOSS_ERR_INVALID, "workspace must be 16-byte aligned");
   }
-  if (static_cast<int64_t>(rows > B ? rows : B) * a->heads > 0x7fffffff - 65536 || a->heads > 65535)
-    return set_error(GPTOSS_ERR_UNSUPPORTED, "%d rows of %d heads in one call", rows, a->heads);
-  // all sequences' tokens, in units of 16, are counted in 32 bits
-  if (static_cast<int64_t>(a->max_blocks) * (1 << a->kv.bs_shift) / 16 + 1 > 0x7fffffff / B)
-    return set_error(GPTOSS_ERR_UNSUPPORTED, "tables of %d pages for %d sequences", a->max_blocks, B);
   a->B = B;
   a->rows = rows;
   a->scale_log2 = cfg->scale * 1.44269504088896340736f;
-  a->window = cfg->window;
+  a->window = cfg->window < cap ? cfg->window : 0;  // one that holds every token is none
   a->first = cfg->first_tokens;
   a->sinks = cfg->sinks;
   return GPTOSS_OK;
@@ -191,8 +195,9 @@ int gptoss_rope_kv_append(const uint16_t* qkv, int64_t qkv_stride, const int32_t
   if (rotary_dim < 16 || rotary_dim % 16 != 0 || rotary_dim > D)
     return set_error(GPTOSS_ERR_INVALID, "rotary_dim=%d must be a positive multiple of 16 and at most %d", rotary_dim, D);
   if (max_positions < 1) return set_error(GPTOSS_ERR_INVALID, "max_positions=%d must be positive", max_positions);
+  if (T > 1 << 25) return set_error(GPTOSS_ERR_UNSUPPORTED, "%d rows in one call (at most 2^25)", T);  // a work-group each
   if (T == 0) return ok();
-  const int64_t cols = static_cast<int64_t>(H + 2 * a.kv.kv_heads) * D, q_cols = static_cast<int64_t>(H) * D;
+  const int64_t cols = (static_cast<int64_t>(H) + 2 * static_cast<int64_t>(a.kv.kv_heads)) * D, q_cols = static_cast<int64_t>(H) * D;
   rc = check_rows("qkv", qkv, qkv_stride, cols);
   if (rc == GPTOSS_OK) rc = check_rows("q_out", q_out, q_stride, q_cols);
   if (rc != GPTOSS_OK) return rc;
@@ -223,7 +228,7 @@ size_t gptoss_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int 
   if (num_tokens < 1 || num_seqs < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1) return 0;
   const int group = num_heads / num_kv_heads;
   const size_t decode = decode_workspace_bytes(num_seqs, num_heads, num_kv_heads, head_dim);
-  const size_t prefill = group > kMaxGroup ? 0 : prefill_workspace_bytes(num_tokens, num_seqs, num_heads, num_kv_heads, head_dim);
+  const size_t prefill = group > kMaxGroup ? 0 : prefill_workspace_bytes(num_tokens, num_heads, num_kv_heads, head_dim);
   return decode > prefill ? decode : prefill;
 }
 

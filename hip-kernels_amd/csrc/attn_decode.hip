@@ -449,7 +449,7 @@ constexpr int kWholeTiles = 32;  // no sequence is cut when the longest has no m
 
 struct Cut {
   int slots;      // pieces aimed at for each tile of 16 heads; 0: none is cut
-  int max_slots;  // and their largest number
+  int64_t max_slots;  // and their largest number
 };
 
 // Work-groups aimed at: three for each CU with heads of 64 dims, two with 128,
@@ -462,7 +462,8 @@ Cut cut_of(int B, int64_t most_tiles, int tiles_of_heads, int head_dim) {
   const int slots = (work_groups + tiles_of_heads - 1) / tiles_of_heads;
   // sum of max(1, (tiles + size / 2) / size) <= B + slots
   const int64_t pieces = static_cast<int64_t>(B) * ((most_tiles + kMinTiles - 1) / kMinTiles);
-  return Cut{slots, static_cast<int>(pieces < B + slots ? pieces : B + slots)};
+  const int64_t most = static_cast<int64_t>(B) + slots;
+  return Cut{slots, pieces < most ? pieces : most};
 }
 
 int tiles_of_heads(int heads, int kv_heads) { return kv_heads * ((heads / kv_heads + 15) / 16); }
@@ -490,7 +491,7 @@ hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
   sp.part_o = static_cast<float*>(workspace);
   sp.part_ml = sp.part_o + pieces * a.kv.head_dim;
   sp.plan = reinterpret_cast<int*>(sp.part_ml + pieces * 4);
-  const dim3 grid(static_cast<unsigned>(c.max_slots) * th);
+  const dim3 grid(static_cast<unsigned>(c.max_slots * th));
 #define GX_DECODE(D_, E_) hipLaunchKernelGGL((decode_kernel<D_, E_, kWaves>), grid, dim3(64 * kWaves), 0, s, a, sp)
   if (a.kv.head_dim == 64) {
     if (a.kv.e4m3) GX_DECODE(64, true);
@@ -506,7 +507,7 @@ hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
   j.part_o = sp.part_o;
   j.part_ml = sp.part_ml;
   j.plan = sp.plan;
-  j.max_pieces = c.max_slots;
+  j.max_pieces = static_cast<int>(c.max_slots);
   return launch_join(a, j, s);
 }
 

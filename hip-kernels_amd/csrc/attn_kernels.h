@@ -71,7 +71,7 @@ hipError_t launch_rope_append(const AppendArgs& a, hipStream_t s);
 hipError_t launch_join(const AttendArgs& a, const JoinArgs& j, hipStream_t s);
 size_t decode_workspace_bytes(int B, int heads, int kv_heads, int head_dim);
 hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s);
-size_t prefill_workspace_bytes(int rows, int B, int heads, int kv_heads, int head_dim);
+size_t prefill_workspace_bytes(int rows, int heads, int kv_heads, int head_dim);
 hipError_t launch_prefill(const AttendArgs& a, void* workspace, hipStream_t s);
 
 }  // namespace gxmoe

@@ -627,21 +627,26 @@ int cols_of(int rows, int heads, int head_dim) {
 
 // Pieces: as many as fill the chip (work-groups that it holds at once: three on a
 // CU with heads of 64 dims, two with 128) when the tiles of rows alone do not.
+int fill_of(int head_dim) { return head_dim == 64 ? 768 : 512; }
+
 int most_pieces(int rows, int B, int heads, int kv_heads, int head_dim) {
   if (cols_of(rows, heads, head_dim) == 2) return 1;
   const int per = 128 / (heads / kv_heads);
   const int64_t tiles = (static_cast<int64_t>(rows) + per - 1) / per + (B < rows ? B : rows) - 1;
-  const int64_t pieces = (head_dim == 64 ? 768 : 512) / (tiles * kv_heads);
+  const int64_t pieces = fill_of(head_dim) / (tiles * kv_heads);
   return pieces < 1 ? 1 : static_cast<int>(pieces);
 }
 
 }  // namespace
 
-size_t prefill_workspace_bytes(int rows, int B, int heads, int kv_heads, int head_dim) {
-  const int pieces = most_pieces(rows, B, heads, kv_heads, head_dim);
-  if (pieces == 1) return 0;
-  return static_cast<size_t>(pieces) * rows * heads * (head_dim + 4) * sizeof(float) +
-         ((static_cast<size_t>(rows) * sizeof(int) + 15) & ~size_t{15});
+// For any call of up to `rows` rows: with t tiles there are at most fill / (t
+// kv_heads) pieces of at most t * per rows.
+size_t prefill_workspace_bytes(int rows, int heads, int kv_heads, int head_dim) {
+  const int per = 128 / (heads / kv_heads);
+  const size_t pieces = fill_of(head_dim) / kv_heads;
+  if (pieces < 2) return 0;
+  const size_t part_rows = min(static_cast<size_t>(rows) * pieces, static_cast<size_t>(per) * fill_of(head_dim) / kv_heads);
+  return part_rows * heads * (head_dim + 4) * sizeof(float) + ((static_cast<size_t>(rows) * sizeof(int) + 15) & ~size_t{15});
 }
 
 hipError_t launch_prefill(const AttendArgs& a, void* workspace, hipStream_t s) {

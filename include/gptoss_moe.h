@@ -509,7 +509,8 @@ int gptoss_rope_table(const gptoss_rope_config* cfg, float* table, void* stream)
  * writes nothing at all.  Slots of one call are distinct: of rows that share
  * one, any may be found there, in pieces.  q_out may be the queries' place in
  * qkv (same pointer and stride) and otherwise lies apart from qkv.
- * qkv, q_out and rope_table are 16-byte aligned; rotary_dim <= head_dim. */
+ * qkv, q_out and rope_table are 16-byte aligned; rotary_dim <= head_dim;
+ * num_tokens is at most 2^25. */
 int gptoss_rope_kv_append(const uint16_t* qkv, int64_t qkv_stride, const int32_t* positions,
                           const int32_t* slots, const float* rope_table, int rotary_dim, int max_positions,
                           int interleaved, int num_tokens, int num_heads, uint16_t* q_out, int64_t q_stride,
@@ -544,7 +545,11 @@ typedef struct gptoss_attention_config {
  * the prefill call.
  * workspace: gptoss_paged_attention_workspace_bytes bytes, 16-byte aligned,
  * that no call running at the same time uses (two graphs that may overlap need
- * two); nothing is kept in it between calls. */
+ * two); nothing is kept in it between calls.  The bytes for num_tokens rows and
+ * num_seqs sequences are enough for calls of fewer.
+ * Limits of a call (GPTOSS_ERR_UNSUPPORTED): num_tokens * num_heads 2^26, num_seqs
+ * * num_heads 2^22, max_blocks * block_size 2^30, num_seqs * max_blocks *
+ * block_size 2^35, token_stride 2^24. */
 size_t gptoss_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads,
                                               int head_dim);
 int gptoss_paged_attention_decode(const uint16_t* q, int64_t q_stride, const gptoss_kv_cache* cache,

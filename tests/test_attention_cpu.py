@@ -152,6 +152,30 @@ def test_workspace_refused(g):
         assert decode(g, cache(g), ws=16 * A + 8) == g.GPTOSS_ERR_INVALID and b"aligned" in g.lib.gptoss_last_error()
 
 
+@pytest.mark.parametrize("H,Hk,D", [(64, 8, 64), (32, 8, 128), (5, 1, 64), (128, 1, 128), (6, 6, 128), (1, 1, 64)])
+def test_workspace_is_enough_for_smaller_calls(g, H, Hk, D):
+    size = lambda T, B: g.lib.gptoss_paged_attention_workspace_bytes(T, B, H, Hk, D)
+    sizes = [size(T, 1) for T in range(1, 3000)]
+    assert sizes == sorted(sizes) and sizes[0] > 0
+    assert [size(4096, B) for B in range(1, 300)] == sorted(size(4096, B) for B in range(1, 300))
+    assert size(0, 1) == size(1, 0) == 0
+
+
+def test_limits_refused(g):
+    def refused(rc, message):
+        assert rc == g.GPTOSS_ERR_UNSUPPORTED and message in g.lib.gptoss_last_error()
+
+    far = dict(out=1 << 60, ws=1 << 62, ws_bytes=1 << 62)
+    refused(decode(g, cache(g), B=(1 << 16) + 1, **far), b"sequences of 64 heads")
+    refused(prefill(g, cache(g), T=(1 << 20) + 1, **far), b"rows and")
+    refused(prefill(g, cache(g), B=(1 << 16) + 1, **far), b"sequences of 64 heads")
+    for call in (decode, prefill):
+        refused(call(g, cache(g), max_blocks=(1 << 26) + 1, table_stride=1 << 27, B=1, T=1, **far), b"tables of")
+        refused(call(g, cache(g), max_blocks=1 << 26, table_stride=1 << 27, B=33, T=33, **far), b"tables of")
+        refused(call(g, cache(g, token_stride=(1 << 24) + 64, head_stride=64, block_stride=64), **far), b"token_stride")
+    refused(append(g, cache(g), T=(1 << 25) + 1, q=1 << 60), b"rows in one call")
+
+
 # ---------------------------------------------------------------------------
 # the binding
 # ---------------------------------------------------------------------------

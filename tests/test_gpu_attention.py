@@ -126,6 +126,27 @@ def test_decode_uniform_batches(gpu, B, L):
         c.check_decode()
 
 
+def test_window_of_every_token_is_none(gpu):
+    """A window no sequence can outgrow, up to the largest number, gives the bits of no window."""
+    lens = [70, 0, 1000, 2048]
+    c = Case(gpu, 61, lens, *GPT)
+    for window in (2048, 2 ** 31 - 1):
+        q, got = c.check_decode()
+        assert got.equal(gpu.paged_attention_decode(q, c.cache, c.tables, c.seq_lens, window=window, first_tokens=2 ** 31 - 1))
+        q, offsets, got = c.check_prefill([70, 0, 90, 1])
+        assert got.equal(gpu.paged_attention_prefill(q, offsets, c.cache, c.tables, c.seq_lens, window=window,
+                                                     first_tokens=2 ** 31 - 1))
+
+
+def test_one_workspace_for_fewer_rows(gpu):
+    """A workspace sized once for the largest call serves every smaller one."""
+    c = Case(gpu, 62, [3000, 900, 2200], *GPT)
+    ws = torch.zeros(gpu.paged_attention_workspace_bytes(9000, 3, 64, c.cache), dtype=torch.uint8, device="cuda")
+    for new in ([1, 1, 1], [700, 0, 2], [3000, 900, 2200], [40, 40, 40]):
+        c.check_prefill(new, workspace=ws)
+    c.check_decode(workspace=ws)
+
+
 @pytest.mark.parametrize("lens,new", [([1000], [1000]), ([2300], [260]), ([700, 5000], [700, 9]), ([64], [64]),
                                       ([300] * 9, [3] * 9), ([4100], [1]), ([90, 0, 91], [0, 0, 91])])
 @pytest.mark.parametrize("shape,e4m3", [(GPT, False), (GPT, True), ((32, 8, 128, 32), False), ((4, 4, 64, 16), False),
