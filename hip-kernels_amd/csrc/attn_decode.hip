@@ -32,6 +32,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 32;      // tokens per step of a wave
+constexpr int kClasses = 2;    // of a piece's length, a factor of 4 each
 constexpr float kSlack = 8.0f;  // how far a score may exceed the reference, in powers of two
 
 // The tiles of a sequence that its new token sees: the first nf tiles (first
@@ -67,16 +68,25 @@ struct Piece {
 
 // Sequences are cut into pieces of `size` tiles, the size chosen from all
 // lengths so that the pieces of one kv head are about sp.slots in number; every
-// wave works it out from the lengths, which only the device knows (64 at a
-// time, with scans over the lanes' registers).
+// wave works it out from the lengths, which only the device knows (64 kSeqs at a
+// time, kSeqs to a lane, with scans over the lanes' registers).  The pieces are
+// numbered by classes of their length, the longest first: late in the grid they
+// would run when little else does.
+template <int kSeqs>
 __device__ __forceinline__ bool find_piece(const AttendArgs& a, const SplitArgs& sp, int slot, Piece* p) {
   const int lane = threadIdx.x & 63;
-  const int len0 = lane < a.B ? seq_len(a, lane) : 0;
-  int total = lane < a.B ? seen_tiles(a, len0).tiles : 0, longest = total;
-  for (int b0 = 64; b0 < a.B; b0 += 64) {
-    const int tiles = b0 + lane < a.B ? seen_tiles(a, seq_len(a, b0 + lane)).tiles : 0;
-    total += tiles;
-    longest = max(longest, tiles);
+  int len[kSeqs], tiles[kSeqs];  // -1: no sequence
+  auto read = [&](int b0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kSeqs; ++j) len[j] = b0 + 64 * j + lane < a.B ? seq_len(a, b0 + 64 * j + lane) : -1;
+#pragma unroll
+    for (int j = 0; j < kSeqs; ++j) tiles[j] = len[j] < 0 ? -1 : seen_tiles(a, len[j]).tiles;
+  };
+  int total = 0, longest = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64 * kSeqs) {
+    read(b0);
+#pragma unroll
+    for (int j = 0; j < kSeqs; ++j) total += max(tiles[j], 0), longest = max(longest, tiles[j]);
   }
   total = __builtin_amdgcn_readlane(wave_scan(total), 63);
   int size = max(sp.min_tiles, (total + sp.slots - 1) / sp.slots);
@@ -85,27 +95,48 @@ __device__ __forceinline__ bool find_piece(const AttendArgs& a, const SplitArgs&
     for (int x = 32; x >= 1; x >>= 1) longest = max(longest, __shfl_xor(longest, x));
     if (2 * static_cast<int64_t>(longest) * a.B <= 3 * static_cast<int64_t>(total)) size = max(size, longest);
   }
+  const float per_size = 1.0f / static_cast<float>(size);  // (all waves divide alike: no more is asked of it)
+  int cuts[kSeqs];
+  auto cut = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kSeqs; ++j) cuts[j] = max(1, static_cast<int>(__builtin_fmaf(static_cast<float>(tiles[j]), per_size, 0.5f)));
+  };
+  cut();
   int before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const bool in = b0 + lane < a.B;
-    const int len = b0 == 0 ? len0 : in ? seq_len(a, b0 + lane) : 0;
-    const int mine = in ? max(1, (seen_tiles(a, len).tiles + size / 2) / size) : 0;
-    const int upto = wave_scan(mine);
-    const int all = __builtin_amdgcn_readlane(upto, 63);
-    if (slot < before + all) {
-      const int at = slot - before;
-      const int who = __builtin_ctzll(__ballot(at < upto));
-      p->b = b0 + who;
-      p->chunks = __builtin_amdgcn_readlane(mine, who);
-      const int first = __builtin_amdgcn_readlane(upto, who) - p->chunks;
-      p->first_slot = before + first;
-      p->seen = seen_tiles(a, __builtin_amdgcn_readlane(len, who));
-      const int64_t n = p->seen.tiles;
-      p->t0 = static_cast<int>(n * (at - first) / p->chunks);
-      p->t1 = static_cast<int>(n * (at - first + 1) / p->chunks);
-      return true;
+  for (int k = 0; k < kClasses; ++k) {
+    // tiles of a sequence of class k: at least `least`, and less than the class before
+    const int least = k == kClasses - 1 ? 0 : size >> (2 * k + 1), below = k == 0 ? 0x7fffffff : size >> (2 * k - 1);
+    for (int b0 = 0; b0 < a.B; b0 += 64 * kSeqs) {
+      if (a.B > 64 * kSeqs) read(b0), cut();
+      int mine[kSeqs], sum = 0;
+#pragma unroll
+      for (int j = 0; j < kSeqs; ++j) {
+        mine[j] = tiles[j] >= least && tiles[j] < below ? cuts[j] : 0;
+        sum += mine[j];
+      }
+      const int upto = wave_scan(sum);
+      const int all = __builtin_amdgcn_readlane(upto, 63);
+      if (slot < before + all) {
+        const int at = slot - before;
+        const int who = __builtin_ctzll(__ballot(at < upto));
+        int first = __builtin_amdgcn_readlane(upto, who) - __builtin_amdgcn_readlane(sum, who);
+#pragma unroll
+        for (int j = 0; j < kSeqs; ++j) {
+          const int n = __builtin_amdgcn_readlane(mine[j], who);
+          if (at >= first && at < first + n) {
+            p->b = b0 + 64 * j + who;
+            p->chunks = n;
+            p->first_slot = before + first;
+            p->seen = seen_tiles(a, __builtin_amdgcn_readlane(len[j], who));
+            p->t0 = static_cast<int>(static_cast<int64_t>(p->seen.tiles) * (at - first) / n);
+            p->t1 = static_cast<int>(static_cast<int64_t>(p->seen.tiles) * (at - first + 1) / n);
+          }
+          first += n;
+        }
+        return true;
+      }
+      before += all;
     }
-    before += all;
   }
   return false;
 }
@@ -180,7 +211,7 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
 
   Piece p;
   if (sp.slots > 0) {
-    if (!find_piece(a, sp, piece, &p)) return;
+    if (!(a.B <= 64 ? find_piece<1>(a, sp, piece, &p) : find_piece<4>(a, sp, piece, &p))) return;
     for (int* x : {&p.b, &p.t0, &p.t1, &p.chunks, &p.first_slot, &p.seen.len, &p.seen.low, &p.seen.nf, &p.seen.main,
                    &p.seen.tiles})
       *x = __builtin_amdgcn_readfirstlane(*x);  // the same in all lanes: addresses in scalar registers

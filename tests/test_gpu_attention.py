@@ -117,6 +117,13 @@ def test_decode_batches_and_long_caches(gpu, B, L, e4m3):
     c.check_decode(window=128)
 
 
+@pytest.mark.parametrize("B,L", [(63, 3000), (64, 3000), (65, 3000), (257, 2100), (520, 1300)])
+def test_decode_ragged_batches(gpu, B, L):
+    """Lengths from nothing to L in no order, as many as are found in one, four and more reads."""
+    c = Case(gpu, 47, [L * (37 * b % 101) // 101 // (1 + b % 7) + (b == B - 1) * L for b in range(B)], 16, 2, 64, 16)
+    c.check_decode(sinks=randn(c.gen, 16))
+
+
 @pytest.mark.parametrize("B,L", [(40, 0), (40, 1500), (100, 1300), (300, 0)])
 def test_decode_uniform_batches(gpu, B, L):
     """Many sequences of one length, nothing at all among them, with a table that would hold more."""
