@@ -13,8 +13,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // T threads for each (row, head), 256 / T of these to a work-group.  A lane
 // takes four dims of the pieces r, r + R, ..., with a reference of its own, so
-// that nothing but the plan is waited for before they are read.
-template <int D, int T>
+// that nothing but the plan is waited for before they are read, U at a time.
+template <int D, int T, int U>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, JoinArgs j) {
   constexpr int kLanes = D / 4, R = T / kLanes;
   __shared__ f32x4 s_o[256 / kLanes][kLanes];
@@ -36,7 +36,6 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, JoinArgs j) {
     float m = kNegInf, l = 0.0f;
     f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     int any = 0;
-    constexpr int U = 8;
     for (int c0 = row - r0; c0 < chunks; c0 += U * R) {
       f32x4 x[U], y[U];
       float top = m;
@@ -97,14 +96,23 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, JoinArgs j) {
 // (row, head) pairs up to which a pair is a whole work-group
 constexpr int kWide = 1024;
 
+template <int D, int T>
+hipError_t launch(const AttendArgs& a, const JoinArgs& j, hipStream_t s) {
+  constexpr int R = T / (D / 4);
+  const int64_t pairs = static_cast<int64_t>(a.rows) * a.heads;
+  const dim3 grid(static_cast<unsigned>((pairs + 256 / T - 1) / (256 / T)));
+  // (no more reads than there can be pieces: 16384 pairs of four pieces of 128
+  // dims 11 us, 16.5 with 8 at a time)
+  if (j.max_pieces <= 2 * R)
+    hipLaunchKernelGGL((join_kernel<D, T, 2>), grid, dim3(256), 0, s, a, j);
+  else
+    hipLaunchKernelGGL((join_kernel<D, T, 8>), grid, dim3(256), 0, s, a, j);
+  return hipGetLastError();
+}
+
 template <int D>
 hipError_t launch(const AttendArgs& a, const JoinArgs& j, hipStream_t s) {
-  const int64_t pairs = static_cast<int64_t>(a.rows) * a.heads;
-  if (pairs <= kWide)
-    hipLaunchKernelGGL((join_kernel<D, 256>), dim3(static_cast<unsigned>(pairs)), dim3(256), 0, s, a, j);
-  else
-    hipLaunchKernelGGL((join_kernel<D, 64>), dim3(static_cast<unsigned>((pairs + 3) / 4)), dim3(256), 0, s, a, j);
-  return hipGetLastError();
+  return static_cast<int64_t>(a.rows) * a.heads <= kWide ? launch<D, 256>(a, j, s) : launch<D, 64>(a, j, s);
 }
 
 }  // namespace
