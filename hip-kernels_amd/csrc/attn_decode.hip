@@ -32,7 +32,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 32;      // tokens per step of a wave
-constexpr int kClasses = 2;    // of a piece's length, a factor of 4 each
+constexpr int kClasses = 2;     // of a piece's length
+constexpr int kWholeTiles = 32;  // tiles up to which many sequences are not cut
 constexpr float kSlack = 8.0f;  // how far a score may exceed the reference, in powers of two
 
 // The tiles of a sequence that its new token sees: the first nf tiles (first
@@ -93,7 +94,7 @@ __device__ __forceinline__ bool find_piece(const AttendArgs& a, const SplitArgs&
   if (sp.whole_ok) {
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) longest = max(longest, __shfl_xor(longest, x));
-    if (2 * static_cast<int64_t>(longest) * a.B <= 3 * static_cast<int64_t>(total)) size = max(size, longest);
+    if (longest <= 2 * kWholeTiles && 2 * static_cast<int64_t>(longest) * a.B <= 3 * static_cast<int64_t>(total)) size = max(size, longest);
   }
   const float per_size = 1.0f / static_cast<float>(size);  // (all waves divide alike: no more is asked of it)
   int cuts[kSeqs];
@@ -464,31 +465,36 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
   }
 }
 
-// Work-groups of W waves.  Where the table or the window holds no more than
-// kWholeTiles (1024 tokens) the call is one launch of a piece to each sequence
-// (cut or whole: one sequence of 1000 9.8 / 9.0 us, of 500 9.8 / 6.5, 32 of
-// 1000 20.5 / 15.1, 64 of up to 1000 16.7 / 13.3, 256 with a window of 512 63.8 /
-// 56.6; 8 of 1000 11.6 / 11.8.  Whole with eight waves instead of four is slower
-// in each).
-constexpr int kWaves = 4;
-constexpr int kMinTiles = 8;     // tiles of the smallest piece of a cut sequence
-// Work-groups that fill the chip: one to a CU.  From there on sequences whose mean
-// is two thirds of the longest are not cut either (cut or whole, join included:
-// 32 of 1500 27.5 / 22.6 us, 64 of 2000 56.5 / 50.6).
+// Waves of a work-group.  Two leave more, smaller work-groups to a CU, which short
+// and ragged sequences want; four (or one) are better for few long ones and for
+// many long ones of the same length.  us with 2 and 4 waves: 64 ragged of up to 2000
+// 18.3 / 19.8, of up to 8192 28.4 / 30.3, 256 of 1000 23.6 / 27.3, 64 of 4000 96.4 /
+// 88.1, one of 131072 54 / 53; 185 of two tokens 9.2 / 12.6; one wave loses where
+// sequences are whole (32 of 1000 15.1 / 15.5, and 22.8 with one).
+constexpr int kWaves = 2;
+constexpr int kMinTiles = 6;  // tiles of the smallest piece of a cut sequence
+// Work-groups from which on, one to a CU, sequences of up to 2 kWholeTiles whose
+// mean is two thirds of the longest are not cut either (cut or whole, join
+// included: 32 of 2000 31.6 / 28.4 us, 64 of 2000 56.2 / 53; 40 of 3000 55 / 65).
 constexpr int kFull = 256;
-constexpr int kWholeTiles = 32;  // no sequence is cut when the longest has no more tiles
+// Where the table or the window holds no more than kWholeTiles (1024 tokens), or
+// half of that or so when there are few work-groups, the call is one launch of a
+// piece to each sequence (cut or whole: 16 sequences of 1000 16.2 / 14.1 us, 8 of
+// 1000 13.7 / 12.3, 8 ragged of up to 1000 10.5 / 11.9, 4 of 900 with 128 dims 12 /
+// 16.5, one of 1000 9.4 / 11.4, of 500 9.3 / 8; 8 with a window of 512 10 / 8).
+constexpr int kMany = 128;
 
 struct Cut {
-  int slots;      // pieces aimed at for each tile of 16 heads; 0: none is cut
+  int slots;          // pieces aimed at for each tile of 16 heads; 0: none is cut
   int64_t max_slots;  // and their largest number
 };
 
-// Work-groups aimed at: three for each CU with heads of 64 dims, two with 128,
-// which is what the registers leave there.  Four with 64 dims are possible and
-// slower (one sequence of 131072, bf16: 55.7 against 52.7 us; 32 of 2000: 33.3
-// against 29.7; fewer partial sums, and a CU's loads are enough in flight).
+// Work-groups aimed at: three for each CU with heads of 64 dims, two with 128.
+// The registers hold twice as many, and one sequence of 131072 takes 58.0 us so
+// against 54.8 (fewer partial sums, and a CU's loads are enough in flight).
 Cut cut_of(int B, int64_t most_tiles, int tiles_of_heads, int head_dim) {
-  if (most_tiles <= kWholeTiles) return Cut{0, B};
+  const bool many = static_cast<int64_t>(B) * tiles_of_heads >= kMany;
+  if (most_tiles <= (many ? kWholeTiles : head_dim == 64 ? 24 : 16)) return Cut{0, B};
   const int work_groups = head_dim == 64 ? 768 : 512;
   const int slots = (work_groups + tiles_of_heads - 1) / tiles_of_heads;
   // sum of max(1, (tiles + size / 2) / size) <= B + slots
