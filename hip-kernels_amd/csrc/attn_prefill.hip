@@ -128,8 +128,8 @@ __device__ __forceinline__ int piece_at(int t, int piece) {
   return piece ^ ((t & 3) << 2 | (t >> 2 & 3));
 }
 
-template <int D, bool kE4m3, int kCols>
-__global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_kernel(AttendArgs a, PieceArgs pa) {
+template <int D, bool kE4m3, int kCols, int G>
+__global__ __launch_bounds__(256 * G, D == 64 && kCols == 1 && G == 1 ? 3 : 2) void prefill_kernel(AttendArgs a, PieceArgs pa) {
   constexpr int kSize = kE4m3 ? 1 : 2;
   constexpr int kPieces = D * kSize / 16;      // 16-byte pieces of a token's row in memory
   constexpr int kLoads = 16 * kPieces / 64;    // loads of a wave for its 16 tokens of K, and of V
@@ -137,14 +137,16 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
   constexpr int kBytes = kTile * kRowBytes;
   constexpr int kSteps = D / 16, kDb = D / 32;
   constexpr int kOutRow = 144;                 // of a row's 128 bytes on their way out, in LDS
-  // K of two tiles, then V of two; the queries pass through the middle half of it
-  // before, the results through its beginning afterwards
-  __shared__ __attribute__((aligned(16))) uint8_t s_kv[4][kBytes];
-  uint8_t(*const s_k)[kBytes] = s_kv;
-  uint8_t(*const s_v)[kBytes] = s_kv + 2;
+  // of each group K of two tiles, then V of two; the queries pass through the middle
+  // half of it before, the results through its beginning afterwards
+  __shared__ __attribute__((aligned(16))) uint8_t s_all[4 * G][kBytes];
   __shared__ int s_odd;  // whether put() left out a value
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+  const int part_of = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);  // the group
+  uint8_t(*const s_kv)[kBytes] = s_all + 4 * part_of;
+  uint8_t(*const s_k)[kBytes] = s_kv;
+  uint8_t(*const s_v)[kBytes] = s_kv + 2;
   const int n = lane & 31, h = lane >> 5;
   const int group = a.heads / a.kv.kv_heads, per = 128 * kCols / group;
   const int kvh = __builtin_amdgcn_readfirstlane(blockIdx.x % a.kv.kv_heads);
@@ -190,10 +192,14 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
   const int begin = a.first > 0 ? low & ~(kTile - 1) : low & ~15;
   const int nf = min((min(a.first, low) + kTile - 1) / kTile, begin / kTile);
   const int all_tiles = pmax < 0 ? 0 : nf + (pmax - begin) / kTile + 1;
-  const int pieces = max(1, min(pa.pieces, all_tiles / kMinTiles));
+  const int pieces = max(1, min(pa.pieces, all_tiles / (G * kMinTiles)));
   if (piece >= pieces) return;
-  const int first_tile = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(all_tiles) * piece / pieces));
-  const int tiles = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(all_tiles) * (piece + 1) / pieces) - first_tile);
+  // the piece's tiles [t0, t1) go to the groups in equal parts, whose number of
+  // steps is the same: what a group has past its last tile is hidden
+  const int t0 = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(all_tiles) * piece / pieces));
+  const int t1 = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(all_tiles) * (piece + 1) / pieces));
+  const int steps = (t1 - t0 + G - 1) / G, first_tile = t0 + part_of * steps;
+  const int tiles = max(0, min(steps, t1 - first_tile));
   auto tile_at = [&](int i) {
     const int t = first_tile + i;
     return t < nf ? t * kTile : begin + (t - nf) * kTile;
@@ -462,12 +468,12 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
 
   if (threadIdx.x == 0) s_odd = 0;
   __syncthreads();
-  if (tiles > 0) {
+  if (steps > 0) {
     // Tile i: K of tile i + 1 and V of tile i go to LDS, K of i + 2 and V of i + 1
     // are asked for; then its two halves, with the only barrier between them: it
     // shows what was put, and what is put next takes the place of K of tile i - 1
     // and V of i - 2, which no wave reads behind it.
-    const bool two = pmax - begin_of(tiles - 1) >= 32;  // whether any row sees the last tile's second half
+    const bool two = pmax - begin_of(steps - 1) >= 32;  // whether any row sees the last tile's second half
     uint32_t pages, ahead;
     int64_t at = fetch(0, &pages);
     load(kb, at, kr);
@@ -475,7 +481,7 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
     at = fetch(1, &ahead);
     put(s_k[0], kr);
     load(kb, at, kr);
-    for (int x = threadIdx.x; x < kBytes / 16; x += 256)  // taken with weights of 0 by the first half
+    for (int x = threadIdx.x & 255; x < kBytes / 16; x += 256)  // taken with weights of 0 by the first half
       reinterpret_cast<attn_u32x4*>(s_v[1])[x] = attn_u32x4{0, 0, 0, 0};
     __syncthreads();
     clear(0);
@@ -496,18 +502,18 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
       at = to;
       if (work) half(buf, 0, t, pages, whole);
       __syncthreads();
-      if (work && (i + 1 < tiles || two)) half(buf, 1, t, pages, whole);
+      if (work && (i + 1 < steps || two)) half(buf, 1, t, pages, whole);
       pages = ahead;
       ahead = later;
     };
-    for (int i = 0; i < tiles; i += 2) {
+    for (int i = 0; i < steps; i += 2) {
       step(std::integral_constant<int, 0>{}, i);
-      if (i + 1 < tiles) step(std::integral_constant<int, 1>{}, i + 1);
+      if (i + 1 < steps) step(std::integral_constant<int, 1>{}, i + 1);
     }
     // the values of the last half
 #pragma unroll
     for (int x = 0; x < kSteps; ++x) {
-      if (tiles & 1) {
+      if (steps & 1) {
         if (two)
           add(0, 1, x);
         else
@@ -564,6 +570,36 @@ __global__ __launch_bounds__(256, D == 64 && kCols == 1 ? 3 : 2) void prefill_ke
   // A 128-byte piece of 32 rows from the wave's part of LDS: row r to at(r) bytes
   // from `to`, rows of no token left out.
   __syncthreads();
+  if constexpr (G == 2) {
+    // the second group's sums to the first, lane by lane
+    static_assert(kCols == 1, "32 rows a wave");
+    Piece* at = reinterpret_cast<Piece*>(s_all[4 + wave]) + lane;
+    float* ml = reinterpret_cast<float*>(s_all[3]) + 192 * wave + lane;
+    if (part_of == 1) {
+#pragma unroll
+      for (int d = 0; d < kDb; ++d)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          at[64 * (4 * d + k)] = __builtin_bit_cast(attn_u32x4, f32x4{o[0][d][4 * k], o[0][d][4 * k + 1], o[0][d][4 * k + 2], o[0][d][4 * k + 3]});
+      ml[0] = m[0], ml[64] = l[0], ml[128] = any[0] ? 1.0f : 0.0f;
+    }
+    __syncthreads();
+    if (part_of == 1) return;
+    const float m1 = ml[0], top = __builtin_fmaxf(m[0], m1), base = top == kNegInf ? 0.0f : top;
+    const float f0 = __builtin_amdgcn_exp2f(m[0] - base), f1 = __builtin_amdgcn_exp2f(m1 - base);
+    m[0] = top;
+    l[0] = __builtin_fmaf(ml[64], f1, l[0] * f0);
+    any[0] |= ml[128] != 0.0f;
+#pragma unroll
+    for (int d = 0; d < kDb; ++d)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f32x4 x = __builtin_bit_cast(f32x4, at[64 * (4 * d + k)]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][d][4 * k + e] = __builtin_fmaf(x[e], f1, o[0][d][4 * k + e] * f0);
+      }
+    wave_order();
+  }
   uint8_t* mid = s_kv[0] + wave * 32 * kOutRow;
   auto emit = [&](void* to, int64_t at, bool in) __attribute__((always_inline)) {
     wave_order();
@@ -630,14 +666,24 @@ int cols_of(int rows, int heads, int head_dim) {
 
 // Pieces: as many as fill the chip (work-groups that it holds at once: three on a
 // CU with heads of 64 dims, two with 128) when the tiles of rows alone do not.
+constexpr int kCus = 256;
 int fill_of(int head_dim) { return head_dim == 64 ? 768 : 512; }
 
-int most_pieces(int rows, int B, int heads, int kv_heads, int head_dim) {
-  if (cols_of(rows, heads, head_dim) == 2) return 1;
+struct Split {
+  int groups, pieces;
+};
+
+Split split_of(int rows, int B, int heads, int kv_heads, int head_dim, int64_t most) {
+  if (cols_of(rows, heads, head_dim) == 2) return {1, 1};
   const int per = 128 / (heads / kv_heads);
   const int64_t tiles = (static_cast<int64_t>(rows) + per - 1) / per + (B < rows ? B : rows) - 1;
-  const int64_t pieces = fill_of(head_dim) / (tiles * kv_heads);
-  return pieces < 1 ? 1 : static_cast<int>(pieces);
+  const int64_t wgs = tiles * kv_heads;
+  auto pieces = [&](int64_t fill, int groups) {
+    return static_cast<int>(max(int64_t{1}, min(fill / wgs, most / (groups * kMinTiles))));
+  };
+  Split s{1, pieces(fill_of(head_dim), 1)};
+  if (wgs <= kCus && wgs * s.pieces > kCus && 2 * static_cast<int64_t>(rows) >= tiles * per) s = {2, pieces(kCus, 2)};
+  return s;
 }
 
 }  // namespace
@@ -661,8 +707,8 @@ hipError_t launch_prefill(const AttendArgs& a, void* workspace, hipStream_t s) {
     most = min(most, (static_cast<int64_t>(a.window) + per + kTile - 3) / kTile + 1 +
                          (static_cast<int64_t>(a.first) + kTile - 1) / kTile);
   PieceArgs pa{};
-  pa.pieces = most_pieces(a.rows, a.B, a.heads, a.kv.kv_heads, a.kv.head_dim);
-  if (pa.pieces > most / kMinTiles) pa.pieces = most / kMinTiles > 1 ? static_cast<int>(most / kMinTiles) : 1;
+  const Split split = split_of(a.rows, a.B, a.heads, a.kv.kv_heads, a.kv.head_dim, most);
+  pa.pieces = split.pieces;
   const size_t parts = static_cast<size_t>(pa.pieces) * a.rows * a.heads;
   pa.part_o = static_cast<float*>(workspace);
   pa.part_ml = pa.part_o + parts * a.kv.head_dim;
@@ -670,17 +716,19 @@ hipError_t launch_prefill(const AttendArgs& a, void* workspace, hipStream_t s) {
   // sum of ceil(new tokens / per), at most one tile more for each sequence that has rows
   const int64_t tiles = (static_cast<int64_t>(a.rows) + per - 1) / per + (a.B < a.rows ? a.B : a.rows);
   const dim3 grid(static_cast<unsigned>(tiles * a.kv.kv_heads * pa.pieces));
-#define GX_PREFILL(D_, E_, C_) hipLaunchKernelGGL((prefill_kernel<D_, E_, C_>), grid, dim3(256), 0, s, a, pa)
-  if (a.kv.head_dim == 64 && cols == 2) {
-    if (a.kv.e4m3) GX_PREFILL(64, true, 2);
-    else GX_PREFILL(64, false, 2);
-  } else if (a.kv.head_dim == 64) {
-    if (a.kv.e4m3) GX_PREFILL(64, true, 1);
-    else GX_PREFILL(64, false, 1);
-  } else {
-    if (a.kv.e4m3) GX_PREFILL(128, true, 1);
-    else GX_PREFILL(128, false, 1);
-  }
+#define GX_PREFILL(D_, E_, C_, G_) \
+  hipLaunchKernelGGL((prefill_kernel<D_, E_, C_, G_>), grid, dim3(256 * G_), 0, s, a, pa)
+#define GX_PREFILL_E(D_, C_, G_)               \
+  do {                                         \
+    if (a.kv.e4m3) GX_PREFILL(D_, true, C_, G_); \
+    else GX_PREFILL(D_, false, C_, G_);        \
+  } while (0)
+  if (a.kv.head_dim == 64 && cols == 2) GX_PREFILL_E(64, 2, 1);
+  else if (a.kv.head_dim == 64 && split.groups == 1) GX_PREFILL_E(64, 1, 1);
+  else if (a.kv.head_dim == 64) GX_PREFILL_E(64, 1, 2);
+  else if (split.groups == 1) GX_PREFILL_E(128, 1, 1);
+  else GX_PREFILL_E(128, 1, 2);
+#undef GX_PREFILL_E
 #undef GX_PREFILL
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || pa.pieces == 1) return e;
