@@ -21,7 +21,11 @@
 //                 as long as both operands agree).
 // The reference m of a head moves only when a score exceeds it by 2^8: until
 // then weights up to 256 lose nothing in bf16 or fp32, and the tile needs no
-// exchange between lanes.
+// exchange between lanes.  The weights meet the values as two bf16 each.
+//
+// With 64 heads on 8 of 64 dims in bf16: one sequence of 131072 54 us, 4.95 TB/s
+// (a kernel that only reads the same, 44 us); 64 of 4000 5.5 TB/s; 64 of very
+// different lengths up to 8192 28.5 us, 3.5 TB/s, of which the join takes 4.3.
 #include "attn_device.h"
 
 namespace gxmoe {
@@ -153,21 +157,6 @@ struct TileRegs {
   uint32_t k[2][kKd];
   uint32_t v[8][kVd];
 };
-
-typedef const __attribute__((address_space(1))) uint8_t* GlobalBytes;
-
-// A lane's offset as the block at hand sees it: 32 bits on a pointer in scalar
-// registers.  (Hoisted out of the loop it would be a 64-bit sum per load.)
-__device__ __forceinline__ uint32_t here(uint32_t x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
-// A pointer that is the same in all lanes, kept apart from their offsets.
-__device__ __forceinline__ GlobalBytes scalar(GlobalBytes p) {
-  asm("" : "+s"(p));
-  return p;
-}
 
 // N dwords, 16 bytes at a time `step` bytes apart.
 template <int N>

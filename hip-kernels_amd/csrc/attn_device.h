@@ -9,6 +9,21 @@ namespace gxmoe {
 typedef uint32_t attn_u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t attn_u32x2 __attribute__((ext_vector_type(2)));
 
+typedef const __attribute__((address_space(1))) uint8_t* GlobalBytes;
+
+// A lane's offset as the block at hand sees it: 32 bits on a pointer in scalar
+// registers.  (Hoisted out of the loop it would be a 64-bit sum per load.)
+__device__ __forceinline__ uint32_t here(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// A pointer that is the same in all lanes, kept apart from their offsets.
+__device__ __forceinline__ GlobalBytes scalar(GlobalBytes p) {
+  asm("" : "+s"(p));
+  return p;
+}
+
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f;
 

@@ -1,17 +1,32 @@
 // attn_prefill.hip -- causal attention of prompt chunks over the paged cache
 // (gfx950).
 //
-// Mathematics: the softmax with a running reference and sum of attn_decode.hip,
-// for 128 rows at a time.  A row is one query head of one new token; the heads
-// that share a kv head lie side by side, so that a work-group's rows are few
-// tokens and what a window or the diagonal cuts off is cut off for all of them.
+// Mathematics: the triples (reference m, sum l, weighted values O) of
+// attn_decode.hip, for 128 or 256 rows at a time.  A row is one query head of one
+// new token; the heads that share a kv head lie side by side, so that a
+// work-group's rows are few tokens and what a window or the diagonal cuts off is
+// cut off for all of them.
 //
-// A work-group is four waves of 32 rows over tiles of 64 tokens.  The products are
-// S^T = K Q^T and O^T = V^T P^T in 32 x 32 x 16 steps: S^T leaves a lane with its
-// own row and the tokens that the second product wants from it, so the weights
-// stay in registers.  K and V go through LDS, 16-byte pieces permuted by the
-// token so that neither the row reads of K nor the transposing reads of V meet
-// in a bank; the next tile is on its way to registers while one is worked on.
+// A work-group is four waves of 32 or 64 rows (with few rows eight, see G) over
+// tiles of 64 tokens.  The products are S^T = K Q^T and O^T = V^T P^T in
+// 32 x 32 x 16 steps: S^T leaves a lane with its own row and the tokens that the
+// second product wants from it, so the weights stay in registers.  K and V go
+// through LDS, 16-byte pieces permuted by the token so that neither the row reads
+// of K nor the transposing reads of V meet in a bank; the next tile is on its way
+// to registers while one is worked on.
+//
+// The weights 2^(s - m) of a tile's half are formed, rounded to bf16 for the
+// matrix cores (l sums them as rounded, so that what they share of the rounding
+// leaves the result), while the products of the half before and the half after
+// run.  m moves only when a lane's weights of a half sum to kMost or more: until
+// then bf16 and fp32 lose nothing, and no maximum is looked for.
+//
+// Bound by the matrix cores with the vector and LDS work beside them, all 40 to 50 %
+// busy, and for large calls by power (2.09 GHz then): a prompt of 8192 with 64
+// heads of 64 takes 567 us, 970 TFLOP/s, where a matrix product of 8192^3 reaches
+// 1250; 512 tokens over 16000 in e4m3 with 32 heads of 128 153 us, 890 TFLOP/s.  A
+// short window is bound by the queries and results instead: 8192 tokens with a
+// window of 128 60 us, of which these take 29.
 #include <type_traits>
 
 #include "attn_device.h"
@@ -24,7 +39,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef const __attribute__((address_space(1))) uint8_t* GlobalBytes;
 typedef __attribute__((address_space(3))) uint8_t* LdsBytes;
 
 constexpr int kTile = 64;     // tokens of a step
@@ -100,16 +114,6 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t x) {
   return (((x & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u) * 0xffffu;
 }
 
-__device__ __forceinline__ uint32_t here(uint32_t x) {  // an offset as the block at hand sees it, not hoisted as 64 bits
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
-__device__ __forceinline__ GlobalBytes scalar(GlobalBytes p) {
-  asm("" : "+s"(p));
-  return p;
-}
-
 typedef attn_u32x4 __attribute__((may_alias)) Piece;
 typedef attn_u32x2 __attribute__((may_alias)) HalfPiece;
 
@@ -128,6 +132,8 @@ __device__ __forceinline__ int piece_at(int t, int piece) {
   return piece ^ ((t & 3) << 2 | (t >> 2 & 3));
 }
 
+// kCols * 32 rows a wave.  G groups of four waves have the same rows and each its
+// part of the tokens; the second one's sums join the first's through LDS.
 template <int D, bool kE4m3, int kCols, int G>
 __global__ __launch_bounds__(256 * G, D == 64 && kCols == 1 && G == 1 ? 3 : 2) void prefill_kernel(AttendArgs a, PieceArgs pa) {
   constexpr int kSize = kE4m3 ? 1 : 2;
@@ -143,7 +149,7 @@ __global__ __launch_bounds__(256 * G, D == 64 && kCols == 1 && G == 1 ? 3 : 2) v
   __shared__ int s_odd;  // whether put() left out a value
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
-  const int part_of = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);  // the group
+  const int part_of = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);  // its group
   uint8_t(*const s_kv)[kBytes] = s_all + 4 * part_of;
   uint8_t(*const s_k)[kBytes] = s_kv;
   uint8_t(*const s_v)[kBytes] = s_kv + 2;
@@ -658,7 +664,7 @@ __global__ __launch_bounds__(256 * G, D == 64 && kCols == 1 && G == 1 ? 3 : 2) v
 }
 
 // Rows of a wave: 64 where the registers allow it and there are rows to fill the
-// chip with, else 32.
+// chip with, else 32 (a prompt of 8192 573 / 618 us, of 2048 60.7 / 54.3).
 constexpr int kTwoCols = 2048;
 int cols_of(int rows, int heads, int head_dim) {
   return head_dim == 64 && static_cast<int64_t>(rows) * heads >= 256 * kTwoCols ? 2 : 1;
@@ -669,6 +675,15 @@ int cols_of(int rows, int heads, int head_dim) {
 constexpr int kCus = 256;
 int fill_of(int head_dim) { return head_dim == 64 ? 768 : 512; }
 
+// Where that gives more than one work-group to a CU and most rows of the tiles are
+// there, two groups of waves in one work-group do what two pieces would, with half
+// the partial sums or none and no join (one group and two: 512 tokens 21.6 / 13.8
+// us, 430 over 2889 52.6 / 43.2, 64 over 8000 30.0 / 27.7, five of up to 200 over
+// 634 with 128 dims in e4m3 31.2 / 23.0).  With tiles hardly filled or a CU to each
+// piece the pieces are better (eight of up to 24 over 2000 19.1 / 22.3, 1055 with 4
+// heads of 128 21.0 / 27.0), and with many tiles, where work-groups of four waves
+// follow each other (1024 tokens 23.2 / 25.3; two of up to 1117 with 128 dims, the
+// shorter chain for once, 34 / 28.5).
 struct Split {
   int groups, pieces;
 };
@@ -682,7 +697,8 @@ Split split_of(int rows, int B, int heads, int kv_heads, int head_dim, int64_t m
     return static_cast<int>(max(int64_t{1}, min(fill / wgs, most / (groups * kMinTiles))));
   };
   Split s{1, pieces(fill_of(head_dim), 1)};
-  if (wgs <= kCus && wgs * s.pieces > kCus && 2 * static_cast<int64_t>(rows) >= tiles * per) s = {2, pieces(kCus, 2)};
+  const bool few = wgs <= kCus || (head_dim == 128 && wgs <= 2 * kCus && most >= 2 * kMinTiles);
+  if (few && wgs * s.pieces > kCus && 2 * static_cast<int64_t>(rows) >= tiles * per) s = {2, pieces(kCus, 2)};
   return s;
 }
 
