@@ -248,6 +248,49 @@ def test_values_reach_only_who_sees_them(gpu, shape, e4m3, window):
     assert torch.equal(got[~bad], want[~bad])
 
 
+# few rows over many tokens: 1 and 2 pieces of the tokens, each shared by two groups of waves
+GQA4 = (32, 8, 128, 32)
+FEW = [(GPT, 270), (GPT, 90), (GQA4, 540), (GQA4, 180), ((34, 2, 64, 64), 500), ((9, 3, 128, 16), 2700)]
+
+
+@pytest.mark.parametrize("shape,new", FEW)
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("window,first,sink", [(0, 0, False), (1500, 0, True), (1501, 70, False)])
+def test_prefill_few_rows_over_many_tokens(gpu, shape, new, e4m3, window, first, sink):
+    say("prefill, few rows", shape, new, e4m3, window, first, sink)
+    c = Case(gpu, 48, [2900, 40, max(2101, new)], *shape, e4m3=e4m3)
+    c.tables[0, 20] = -1
+    c.check_prefill([new // 2, 7, new // 2 + 1], window, first, randn(c.gen, shape[0], scale=2.0) if sink else None)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("window,first,sink", [(0, 0, True), (100, 20, False), (700, 0, True)])
+def test_prefill_many_rows(gpu, e4m3, window, first, sink):
+    """Enough rows for a wave to take 64 of them."""
+    c = Case(gpu, 50, [2000, 1, 1501, 1500], 128, 4, 64, 16, e4m3=e4m3)
+    c.tables[2, 5] = -1
+    c.check_prefill([1990, 1, 1501, 700], window, first, randn(c.gen, 128, scale=2.0) if sink else None)
+
+
+@pytest.mark.parametrize("shape,new", FEW[:4] + [((128, 4, 64, 16), 4120)])
+def test_values_reach_only_who_sees_them_in_few_rows(gpu, shape, new):
+    H, Hk, D, bs = shape
+    n, G, window = max(2000, new + 100), H // Hk, 1200
+    c = Case(gpu, 49, [n], *shape)
+    q = randn(c.gen, new, H * D, scale=1.5)
+    off = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    want = gpu.paged_attention_prefill(q, off, c.cache, c.tables, c.seq_lens, window=window).view(new, H, D).clone()
+    bad = torch.zeros((new, H, D), dtype=torch.bool, device="cuda")
+    for t, d, x in [(10, 1, math.nan), (max(0, n - new - 1190), 3, math.nan), (n - 1200, 5, math.inf), (n - 60, 7, math.nan),
+                    (n - 1, 9, math.inf)]:
+        c.pages[1][c.tables[0, t // bs].long(), 1, t % bs, d] = x
+        rows = slice(max(0, t - n + new), max(0, min(new, t + window - n + new)))
+        bad[rows, G:2 * G, d] = True
+    got = gpu.paged_attention_prefill(q, off, c.cache, c.tables, c.seq_lens, window=window).view(new, H, D)
+    assert bad.any() and (~got[bad].isfinite()).all()
+    assert torch.equal(got[~bad], want[~bad])
+
+
 def test_lengths_outside_the_table(gpu):
     """A length past the table's pages is cut to them, a negative one is 0."""
     c = Case(gpu, 18, [64, 48], *GPT)
