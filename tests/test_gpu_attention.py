@@ -124,6 +124,15 @@ def test_decode_ragged_batches(gpu, B, L):
     c.check_decode(sinks=randn(c.gen, 16))
 
 
+@pytest.mark.parametrize("B,L", [(1, 1), (1, 6000), (3, 200), (9, 3000), (30, 700)])
+@pytest.mark.parametrize("H,Hk", [(8, 8), (40, 2), (64, 8)])
+def test_decode_rows_of_half_a_line(gpu, B, L, H, Hk):
+    """Token-major rows of 64 bytes, whose lines two heads share."""
+    c = Case(gpu, 51, [max(1, L - 97 * b) for b in range(B)], H, Hk, 64, 32, e4m3=True, layout="tokens")
+    c.check_decode(sinks=randn(c.gen, H))
+    c.check_decode(window=100)
+
+
 @pytest.mark.parametrize("B,L", [(40, 0), (40, 1500), (100, 1300), (300, 0)])
 def test_decode_uniform_batches(gpu, B, L):
     """Many sequences of one length, nothing at all among them, with a table that would hold more."""
