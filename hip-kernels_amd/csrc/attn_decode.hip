@@ -461,28 +461,30 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
   }
 }
 
-// Waves of a work-group.  Two leave more, smaller work-groups to a CU, which short
-// and ragged sequences want; four (or one) are better for few long ones and for
-// many long ones of the same length.  us with 2 and 4 waves: 64 ragged of up to 2000
-// 18.3 / 19.8, of up to 8192 28.4 / 30.3, 256 of 1000 23.6 / 27.3, 64 of 4000 96.4 /
-// 88.1, one of 131072 54 / 53; 185 of two tokens 9.2 / 12.6; one wave loses where
-// sequences are whole (32 of 1000 15.1 / 15.5, and 22.8 with one).
-constexpr int kWaves = 2;
+// A work-group has two waves, which leaves more of them to a CU and suits short and
+// ragged sequences; four (or one) would be better for many long ones of the same
+// length.  us with 2 and 4 waves: 64 ragged of up to 2000 18.3 / 19.8, of up to 8192
+// 28.4 / 30.3, 256 of 1000 23.6 / 27.3, 64 of 4000 96.4 / 88.1, one of 131072 54 / 53;
+// 185 of two tokens 9.2 / 12.6; 32 of 1000 15.1 / 15.5, and 22.8 with one.  Where the
+// chip is not filled and nothing is cut it has four (one of 1000 11.4 / 10.1, of
+// 500 7.9 / 7.5; 8 with a window of 128 4.6 / 4.8, so not for the shortest).
 constexpr int kMinTiles = 6;  // tiles of the smallest piece of a cut sequence
 // Work-groups from which on, one to a CU, sequences of up to 2 kWholeTiles whose
 // mean is two thirds of the longest are not cut either (cut or whole, join
 // included: 32 of 2000 31.6 / 28.4 us, 64 of 2000 56.2 / 53; 40 of 3000 55 / 65).
 constexpr int kFull = 256;
 // Where the table or the window holds no more than kWholeTiles (1024 tokens), or
-// half of that or so when there are few work-groups, the call is one launch of a
-// piece to each sequence (cut or whole: 16 sequences of 1000 16.2 / 14.1 us, 8 of
-// 1000 13.7 / 12.3, 8 ragged of up to 1000 10.5 / 11.9, 4 of 900 with 128 dims 12 /
-// 16.5, one of 1000 9.4 / 11.4, of 500 9.3 / 8; 8 with a window of 512 10 / 8).
+// with 128 dims and few work-groups half of that, the call is one launch of a piece
+// to each sequence (cut or whole: 16 sequences of 1000 16.2 / 14.1 us, 8 of 1000 13.7
+// / 11.8, 8 ragged of up to 1000 10.5 / 11.0, 8 with a window of 512 10 / 8, one of
+// 500 9.3 / 7.5; with 128 dims 4 of 900 12 / 16.5, 8 of 500 12.3 / 11.3; one of 1000
+// 9.4 / 10.1 in a graph, 13.1 / 10.7 where each launch is the host's).
 constexpr int kMany = 128;
 
 struct Cut {
   int slots;          // pieces aimed at for each tile of 16 heads; 0: none is cut
   int64_t max_slots;  // and their largest number
+  int waves;          // of a work-group
 };
 
 // Work-groups aimed at: three for each CU with heads of 64 dims, two with 128.
@@ -490,13 +492,13 @@ struct Cut {
 // against 54.8 (fewer partial sums, and a CU's loads are enough in flight).
 Cut cut_of(int B, int64_t most_tiles, int tiles_of_heads, int head_dim) {
   const bool many = static_cast<int64_t>(B) * tiles_of_heads >= kMany;
-  if (most_tiles <= (many ? kWholeTiles : head_dim == 64 ? 24 : 16)) return Cut{0, B};
+  if (most_tiles <= (many || head_dim == 64 ? kWholeTiles : kWholeTiles / 2)) return Cut{0, B, !many && most_tiles > 8 ? 4 : 2};
   const int work_groups = head_dim == 64 ? 768 : 512;
   const int slots = (work_groups + tiles_of_heads - 1) / tiles_of_heads;
   // sum of max(1, (tiles + size / 2) / size) <= B + slots
   const int64_t pieces = static_cast<int64_t>(B) * ((most_tiles + kMinTiles - 1) / kMinTiles);
   const int64_t most = static_cast<int64_t>(B) + slots;
-  return Cut{slots, pieces < most ? pieces : most};
+  return Cut{slots, pieces < most ? pieces : most, 2};
 }
 
 int tiles_of_heads(int heads, int kv_heads) { return kv_heads * ((heads / kv_heads + 15) / 16); }
@@ -530,14 +532,20 @@ hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
   sp.same_die = a.kv.sh * (a.kv.e4m3 ? 1 : 2) < 128;
   sp.max_slots = static_cast<int>(c.max_slots);
   const dim3 grid(static_cast<unsigned>((sp.same_die ? (c.max_slots + 7) / 8 * 8 : c.max_slots) * th));
-#define GX_DECODE(D_, E_) hipLaunchKernelGGL((decode_kernel<D_, E_, kWaves>), grid, dim3(64 * kWaves), 0, s, a, sp)
+#define GX_DECODE(D_, E_, W_) hipLaunchKernelGGL((decode_kernel<D_, E_, W_>), grid, dim3(64 * W_), 0, s, a, sp)
+#define GX_DECODE_W(D_, E_)               \
+  do {                                    \
+    if (c.waves == 4) GX_DECODE(D_, E_, 4); \
+    else GX_DECODE(D_, E_, 2);            \
+  } while (0)
   if (a.kv.head_dim == 64) {
-    if (a.kv.e4m3) GX_DECODE(64, true);
-    else GX_DECODE(64, false);
+    if (a.kv.e4m3) GX_DECODE_W(64, true);
+    else GX_DECODE_W(64, false);
   } else {
-    if (a.kv.e4m3) GX_DECODE(128, true);
-    else GX_DECODE(128, false);
+    if (a.kv.e4m3) GX_DECODE_W(128, true);
+    else GX_DECODE_W(128, false);
   }
+#undef GX_DECODE_W
 #undef GX_DECODE
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || c.slots == 0) return e;

@@ -12,6 +12,7 @@ bf16 tensors are passed as torch.bfloat16 (or their int16/uint16 bit views).
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 
@@ -1033,9 +1034,14 @@ def rope_kv_append(qkv, positions, slots, table, cache: KVCache, num_heads: int,
     return q_out
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(rows: int, seqs: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    return _lib.gptoss_paged_attention_workspace_bytes(rows, seqs, heads, kv_heads, head_dim)
+
+
 def paged_attention_workspace_bytes(num_tokens: int, num_seqs: int, num_heads: int, cache: KVCache) -> int:
     """Bytes of workspace that suffice for a call on num_tokens rows of num_seqs sequences."""
-    return _lib.gptoss_paged_attention_workspace_bytes(num_tokens, num_seqs, num_heads, cache.kv_heads, cache.head_dim)
+    return _workspace_bytes(num_tokens, num_seqs, num_heads, cache.kv_heads, cache.head_dim)
 
 
 def _attend(q, offsets, cache, block_tables, seq_lens, scale, window, first_tokens, sinks, out, workspace, stream):
@@ -1070,7 +1076,7 @@ def _attend(q, offsets, cache, block_tables, seq_lens, scale, window, first_toke
             _bad(f"out has {out.shape[0]} rows, expected {rows}")
         _needs_gpu(dev)
     if workspace is None:
-        size = _lib.gptoss_paged_attention_workspace_bytes(rows, B, H, cache.kv_heads, D)
+        size = _workspace_bytes(rows, B, H, cache.kv_heads, D)
         workspace = _empty(size, torch.uint8, dev, stream)
     else:
         _on_device("workspace", workspace, dev)
