@@ -904,11 +904,13 @@ def _launch(device, stream, fn, *args) -> None:
         handle = torch._C._cuda_getCurrentRawStream(device.index)
     else:
         handle = stream if isinstance(stream, int) else stream.cuda_stream
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, handle))
+    if torch._C._cuda_getDevice() == device.index:
+        rc = fn(*args, handle)
     else:
         with _on(device.index):
-            check(fn(*args, handle))
+            rc = fn(*args, handle)
+    if rc:
+        check(rc)
 
 
 def _on_device(name: str, t, device, dtype=None, dim: int | None = None) -> None:
@@ -924,7 +926,8 @@ def _on_device(name: str, t, device, dtype=None, dim: int | None = None) -> None
 
 def _row_tensor(name: str, t, device, cols: int) -> int:
     """bf16 [rows, cols] on `device`, rows any distance apart: the distance."""
-    _on_device(name, t, device, torch.bfloat16, 2)
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.dim() == 2 and t.device == device):
+        _on_device(name, t, device, torch.bfloat16, 2)
     rows, width = t.shape
     step, one = t.stride()
     if width != cols:
@@ -937,6 +940,9 @@ def _row_tensor(name: str, t, device, cols: int) -> int:
 
 
 def _vector(name: str, t, device, n: int, dtype) -> None:
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous() \
+            and t.device == device:
+        return
     _on_device(name, t, device, dtype, 1)
     if t.shape[0] != n:
         _bad(f"{name} has {t.shape[0]} entries, expected {n}")
