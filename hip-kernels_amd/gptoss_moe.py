@@ -3,7 +3,8 @@
 Mirrors the reference's MoE operator interface (src/model/moe_layer.cu:
 1556-1615: moe_layer_create / init / forward / forward_prenormed /
 get_ffn_norm_weight / destroy) and its kernel launchers, over the C ABI
-declared in include/gptoss_moe.h.  Device memory is held in torch tensors
+declared in include/gptoss_moe.h; and attention over a paged key-value cache
+(KVCache, rope_kv_append, paged_attention_decode, paged_attention_prefill).  Device memory is held in torch tensors
 (plumbing only); every computation runs in the HIP library, and importing
 this module without the built library raises immediately.
 
