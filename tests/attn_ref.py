@@ -48,7 +48,8 @@ def attend64(q, pos, length, pages, scales, table, bs, scale, window=0, first=0,
     """q [n, H, D] at positions pos (list) over the first `length` tokens; table entries outside the pages hide
     their tokens.  Returns (out, tol) [n, H, D]: the result and the largest error that the kernels' arithmetic
     allows.  With A = sum p |v| / l and half a bf16 step h = 2^-8 relative: the weights' rounding moves the result by
-    up to h A, the result's own by h |out|; the scores' fp32 sums of D products (and the product with the scale) by a
+    up to h A (where the sum is of the rounded weights too the bound is h sum p |v - out| / l, at most h (A + |out|);
+    that is counted as h A all the same), the result's own by h |out|; the scores' fp32 sums of D products (and the product with the scale) by a
     relative 2 (D + 8) 2^-24 max sum |q k| scale of each weight, and the fp32 sums over the tokens by L 2^-23."""
     n, H, D = q.shape
     Hk = pages[0].shape[1]

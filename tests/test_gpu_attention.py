@@ -630,6 +630,68 @@ def test_captured_step_follows_its_buffers(gpu):
     assert torch.equal(a.out, other.out) and torch.equal(a.out, got)
 
 
+def test_captured_prompt_follows_its_buffers(gpu):
+    """A captured prompt chunk: replays follow offsets and lengths, whatever its pieces were joined from before; eager
+    calls of the same workspace's size run between them and on another stream beside them."""
+    c = Case(gpu, 52, [2600, 1900, 700], *GPT)
+    rows = 100
+    ws, beside = (torch.zeros(gpu.paged_attention_workspace_bytes(rows, 3, 64, c.cache), dtype=torch.uint8, device="cuda")
+                  for _ in range(2))
+    q, off = torch.zeros((rows, 4096), dtype=BF16, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    lens, out = c.seq_lens.clone(), torch.zeros((rows, 4096), dtype=BF16, device="cuda")
+
+    def run(out, ws):
+        gpu.paged_attention_prefill(q, off, c.cache, c.tables, lens, window=0, out=out, workspace=ws)
+
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        run(out, ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(out, ws)
+    for step, (new, ends) in enumerate([([100, 0, 0], [2600, 5, 5]), ([1, 98, 1], [2600, 1900, 700]),
+                                        ([40, 40, 20], [64, 1900, 20]), ([0, 0, 100], [1, 1, 700]),
+                                        ([33, 33, 34], [2600, 1900, 700])]):
+        q.copy_(randn(gen_of(300 + step), rows, 4096))
+        off.copy_(torch.tensor([0] + new).cumsum(0))
+        lens.copy_(torch.tensor(ends))
+        torch.cuda.synchronize()
+        want = torch.zeros_like(out)
+        with torch.cuda.stream(s):
+            run(want, beside)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), step
+        c.lens = ends
+        o, tol = c.want(q, new)
+        assert ref.within(out, o, tol) is None, step
+
+
+def test_many_sequences(gpu):
+    """Thousands of sequences in one call, most of them without a new token in a prompt's."""
+    B = 5000
+    lens = [1 + 37 * b % 90 for b in range(B)]
+    lens[77], lens[4321] = 2000, 1100
+    c = Case(gpu, 53, lens, 8, 1, 64, 16)
+    q = randn(c.gen, B, 512, scale=1.5)
+    got = gpu.paged_attention_decode(q, c.cache, c.tables, c.seq_lens)
+    new = [0] * B
+    picked = [0, 63, 64, 77, 255, 256, 1000, 4321, B - 1]
+    for b in picked:
+        new[b] = min(lens[b], 20)
+    rows = sum(new)
+    p = randn(c.gen, rows, 512, scale=1.5)
+    off = torch.tensor([0] + new, device="cuda").cumsum(0).to(torch.int32)
+    chunk = gpu.paged_attention_prefill(p, off, c.cache, c.tables, c.seq_lens)
+    torch.cuda.synchronize()
+    for b in picked:
+        n, at = lens[b], int(off[b])
+        for x, out, pos in ((q[b:b + 1], got[b:b + 1], [n - 1]), (p[at:at + new[b]], chunk[at:at + new[b]], range(n - new[b], n))):
+            o, tol = ref.attend64(x.view(-1, 8, 64), list(pos), n, c.pages, c.scales, c.tables[b], 16, 0.125)
+            assert ref.within(out.view(-1, 8, 64), o, tol) is None, b
+
+
 def test_on_a_given_stream(gpu):
     """stream= runs the call there, on buffers that it allocates there."""
     c = Case(gpu, 43, [3000, 100], *GPT)
