@@ -107,8 +107,9 @@ int check_attend(AttendArgs* a, const gptoss_kv_cache* cache, const gptoss_atten
   if (rc == GPTOSS_OK) rc = check_heads(a->heads, a->kv);
   if (rc != GPTOSS_OK) return rc;
   if (cfg == nullptr) return set_error(GPTOSS_ERR_INVALID, "cfg is NULL");
-  if (!(cfg->scale > 0.0f) || std::isinf(cfg->scale))
-    return set_error(GPTOSS_ERR_INVALID, "scale=%g must be positive and finite", static_cast<double>(cfg->scale));
+  a->scale_log2 = cfg->scale * 1.44269504088896340736f;
+  if (!(cfg->scale > 0.0f) || std::isinf(a->scale_log2))
+    return set_error(GPTOSS_ERR_INVALID, "scale=%g must be positive and below 2.3e38", static_cast<double>(cfg->scale));
   if (cfg->window < 0 || cfg->first_tokens < 0)
     return set_error(GPTOSS_ERR_INVALID, "window=%d and first_tokens=%d must not be negative", cfg->window,
                      cfg->first_tokens);
@@ -139,7 +140,6 @@ int check_attend(AttendArgs* a, const gptoss_kv_cache* cache, const gptoss_atten
   }
   a->B = B;
   a->rows = rows;
-  a->scale_log2 = cfg->scale * 1.44269504088896340736f;
   a->window = cfg->window < cap ? cfg->window : 0;  // one that holds every token is none
   a->first = cfg->first_tokens;
   a->sinks = cfg->sinks;
@@ -226,9 +226,9 @@ int gptoss_rope_kv_append(const uint16_t* qkv, int64_t qkv_stride, const int32_t
 size_t gptoss_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads,
                                               int head_dim) {
   if (num_tokens < 1 || num_seqs < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1) return 0;
-  const int group = num_heads / num_kv_heads;
+  if (num_heads / num_kv_heads > kMaxGroup || num_heads > kMaxSeqHeads) return 0;  // no call takes these
   const size_t decode = decode_workspace_bytes(num_seqs, num_heads, num_kv_heads, head_dim);
-  const size_t prefill = group > kMaxGroup ? 0 : prefill_workspace_bytes(num_tokens, num_heads, num_kv_heads, head_dim);
+  const size_t prefill = prefill_workspace_bytes(num_tokens, num_heads, num_kv_heads, head_dim);
   return decode > prefill ? decode : prefill;
 }
 

@@ -522,7 +522,7 @@ int gptoss_rope_kv_append(const uint16_t* qkv, int64_t qkv_stride, const int32_t
  * adds exp(sinks[head]) to the softmax's sum, as a token without a value.  A
  * query that sees nothing gives zeros. */
 typedef struct gptoss_attention_config {
-  float scale;       /* of the scores; > 0 */
+  float scale;       /* of the scores; > 0, below 2.3e38 */
   int window;        /* 0: no window */
   int first_tokens;
   const uint16_t* sinks;

@@ -104,7 +104,7 @@ def test_prefill_arguments_refused(g):
     assert decode(g, cache(g, num_kv_heads=1), H=129, q_stride=129 * 64, out_stride=129 * 64) == g.GPTOSS_ERR_UNSUPPORTED
 
 
-@pytest.mark.parametrize("cfg", [(0.0, 0, 0), (-1.0, 0, 0), (float("nan"), 0, 0), (float("inf"), 0, 0), (1.0, -1, 0),
+@pytest.mark.parametrize("cfg", [(0.0, 0, 0), (-1.0, 0, 0), (float("nan"), 0, 0), (float("inf"), 0, 0), (3e38, 0, 0), (1.0, -1, 0),
                                  (1.0, 4, -1)])
 def test_attention_config_refused(g, cfg):
     for call in (decode, prefill):
@@ -159,6 +159,10 @@ def test_workspace_is_enough_for_smaller_calls(g, H, Hk, D):
     assert sizes == sorted(sizes) and sizes[0] > 0
     assert [size(4096, B) for B in range(1, 300)] == sorted(size(4096, B) for B in range(1, 300))
     assert size(0, 1) == size(1, 0) == 0
+    big = 2 ** 31 - 1
+    assert g.lib.gptoss_paged_attention_workspace_bytes(big, big, big, big, D) == 0
+    assert g.lib.gptoss_paged_attention_workspace_bytes(big, big, big, 1, D) == 0
+    assert size(big, big) > 0
 
 
 def test_limits_refused(g):
