@@ -391,7 +391,8 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
     }
   };
 
-  // Two tiles in turn: the next one is on its way while one is worked on.  The
+  // Two tiles in turn: the next one is on its way while one is worked on (two on
+  // their way: 32 of 2000 28.6 / 27.6 us, 256 of 1000 23.7 / 29.2).  The
   // loads stand outside of any branch, since a wait counts the loads behind it
   // and a branch would make that number the smaller one (a wave's last load is
   // its last tile again).
@@ -468,7 +469,10 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
 // 185 of two tokens 9.2 / 12.6; 32 of 1000 15.1 / 15.5, and 22.8 with one.  Where the
 // chip is not filled and nothing is cut it has four (one of 1000 11.4 / 10.1, of
 // 500 7.9 / 7.5; 8 with a window of 128 4.6 / 4.8, so not for the shortest).
-constexpr int kMinTiles = 6;  // tiles of the smallest piece of a cut sequence
+// Tiles of the smallest piece of a cut sequence (of 128 dims a tile has twice the
+// work; us with 6 and 4: one of 1000 with 128 dims 10.7 / 9.4, 32 ragged of up to
+// 1500 with 64 13.9 / 15.3).
+int min_tiles(int head_dim) { return head_dim == 64 ? 6 : 4; }
 // Work-groups from which on, one to a CU, sequences of up to 2 kWholeTiles whose
 // mean is two thirds of the longest are not cut either (cut or whole, join
 // included: 32 of 2000 31.6 / 28.4 us, 64 of 2000 56.2 / 53; 40 of 3000 55 / 65).
@@ -496,7 +500,7 @@ Cut cut_of(int B, int64_t most_tiles, int tiles_of_heads, int head_dim) {
   const int work_groups = head_dim == 64 ? 768 : 512;
   const int slots = (work_groups + tiles_of_heads - 1) / tiles_of_heads;
   // sum of max(1, (tiles + size / 2) / size) <= B + slots
-  const int64_t pieces = static_cast<int64_t>(B) * ((most_tiles + kMinTiles - 1) / kMinTiles);
+  const int64_t pieces = static_cast<int64_t>(B) * ((most_tiles + min_tiles(head_dim) - 1) / min_tiles(head_dim));
   const int64_t most = static_cast<int64_t>(B) + slots;
   return Cut{slots, pieces < most ? pieces : most, 2};
 }
@@ -520,7 +524,7 @@ hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
   const Cut c = cut_of(a.B, most, th, a.kv.head_dim);
   SplitArgs sp{};
   sp.slots = c.slots;
-  sp.min_tiles = kMinTiles;
+  sp.min_tiles = min_tiles(a.kv.head_dim);
   sp.whole_ok = static_cast<int64_t>(a.B) * th >= kFull;
   const size_t pieces = static_cast<size_t>(c.max_slots) * a.heads;
   sp.part_o = static_cast<float*>(workspace);
