@@ -558,7 +558,7 @@ hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
   j.part_ml = sp.part_ml;
   j.plan = sp.plan;
   j.max_pieces = static_cast<int>(c.max_slots);
-  return launch_join(a, j, s);
+  return launch_join(a, j, c.max_slots / a.B, s);
 }
 
 }  // namespace gxmoe

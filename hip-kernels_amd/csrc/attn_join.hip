@@ -97,13 +97,15 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, JoinArgs j) {
 constexpr int kWide = 1024;
 
 template <int D, int T>
-hipError_t launch(const AttendArgs& a, const JoinArgs& j, hipStream_t s) {
+hipError_t launch(const AttendArgs& a, const JoinArgs& j, int64_t mean, hipStream_t s) {
   constexpr int R = T / (D / 4);
   const int64_t pairs = static_cast<int64_t>(a.rows) * a.heads;
   const dim3 grid(static_cast<unsigned>((pairs + 256 / T - 1) / (256 / T)));
-  // (no more reads than there can be pieces: 16384 pairs of four pieces of 128
-  // dims 11 us, 16.5 with 8 at a time)
-  if (j.max_pieces <= 2 * R)
+  // No more reads at a time than most rows have pieces, which a lane without
+  // pieces waits for as well: 16384 pairs of four pieces of 128 dims 11 us, 16.5 with
+  // 8 at a time; decode of 8 ragged sequences of up to 4000 10.6 / 11.4, of 4 of up to
+  // 32000 with 128 dims, 17 pieces each, 38.6 / 37.4.
+  if (mean <= 2 * R)
     hipLaunchKernelGGL((join_kernel<D, T, 2>), grid, dim3(256), 0, s, a, j);
   else
     hipLaunchKernelGGL((join_kernel<D, T, 8>), grid, dim3(256), 0, s, a, j);
@@ -111,14 +113,14 @@ hipError_t launch(const AttendArgs& a, const JoinArgs& j, hipStream_t s) {
 }
 
 template <int D>
-hipError_t launch(const AttendArgs& a, const JoinArgs& j, hipStream_t s) {
-  return static_cast<int64_t>(a.rows) * a.heads <= kWide ? launch<D, 256>(a, j, s) : launch<D, 64>(a, j, s);
+hipError_t launch(const AttendArgs& a, const JoinArgs& j, int64_t mean, hipStream_t s) {
+  return static_cast<int64_t>(a.rows) * a.heads <= kWide ? launch<D, 256>(a, j, mean, s) : launch<D, 64>(a, j, mean, s);
 }
 
 }  // namespace
 
-hipError_t launch_join(const AttendArgs& a, const JoinArgs& j, hipStream_t s) {
-  return a.kv.head_dim == 64 ? launch<64>(a, j, s) : launch<128>(a, j, s);
+hipError_t launch_join(const AttendArgs& a, const JoinArgs& j, int64_t mean, hipStream_t s) {
+  return a.kv.head_dim == 64 ? launch<64>(a, j, mean, s) : launch<128>(a, j, mean, s);
 }
 
 }  // namespace gxmoe

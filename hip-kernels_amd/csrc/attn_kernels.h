@@ -68,7 +68,7 @@ struct RopeTableArgs {
 
 hipError_t launch_rope_table(const RopeTableArgs& a, hipStream_t s);
 hipError_t launch_rope_append(const AppendArgs& a, hipStream_t s);
-hipError_t launch_join(const AttendArgs& a, const JoinArgs& j, hipStream_t s);
+hipError_t launch_join(const AttendArgs& a, const JoinArgs& j, int64_t mean, hipStream_t s);  // mean: pieces of a row
 size_t decode_workspace_bytes(int B, int heads, int kv_heads, int head_dim);
 hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s);
 size_t prefill_workspace_bytes(int rows, int heads, int kv_heads, int head_dim);

@@ -753,7 +753,7 @@ hipError_t launch_prefill(const AttendArgs& a, void* workspace, hipStream_t s) {
   j.part_ml = pa.part_ml;
   j.plan = pa.plan;
   j.max_pieces = pa.pieces;
-  return launch_join(a, j, s);
+  return launch_join(a, j, pa.pieces, s);
 }
 
 }  // namespace gxmoe
