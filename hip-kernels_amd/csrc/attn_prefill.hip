@@ -683,7 +683,15 @@ int fill_of(int head_dim) { return head_dim == 64 ? 768 : 512; }
 // piece the pieces are better (eight of up to 24 over 2000 19.1 / 22.3, 1055 with 4
 // heads of 128 21.0 / 27.0), and with many tiles, where work-groups of four waves
 // follow each other (1024 tokens 23.2 / 25.3; two of up to 1117 with 128 dims, the
-// shorter chain for once, 34 / 28.5).
+// shorter chain for once, 34 / 28.5).  Nor for several sequences whose lengths may
+// be very different, which fewer work-groups balance worse: kAlike is the tiles by
+// which one may miss the longest, and half of those by which all together may
+// (seven of up to 39 over up to 10753 62 / 117 us, two of up to 200 over up to 8000
+// 64.5 / 90.5, eight of up to 128 over up to 4000 38 / 51, eight of up to 60 over up to
+// 1900 23.4 / 29.2; eight of up to 128 over up to 900 23.8 / 19.7, two of up to 256 over
+// up to 1800 34.5 / 30.6, three of up to 258 over up to 4563 with a window 56.3 / 49.0).
+constexpr int64_t kAlike = 80;
+
 struct Split {
   int groups, pieces;
 };
@@ -698,7 +706,8 @@ Split split_of(int rows, int B, int heads, int kv_heads, int head_dim, int64_t m
   };
   Split s{1, pieces(fill_of(head_dim), 1)};
   const bool few = wgs <= kCus || (head_dim == 128 && wgs <= 2 * kCus && most >= 2 * kMinTiles);
-  if (few && wgs * s.pieces > kCus && 2 * static_cast<int64_t>(rows) >= tiles * per) s = {2, pieces(kCus, 2)};
+  const bool even = B == 1 || (most <= kAlike && (B - 1) * most <= 2 * kAlike);
+  if (few && even && wgs * s.pieces > kCus && 2 * static_cast<int64_t>(rows) >= tiles * per) s = {2, pieces(kCus, 2)};
   return s;
 }
 
