@@ -670,7 +670,7 @@ int cols_of(int rows, int heads, int head_dim) {
   return head_dim == 64 && static_cast<int64_t>(rows) * heads >= 256 * kTwoCols ? 2 : 1;
 }
 
-// Pieces: as many as fill the chip (work-groups that it holds at once: three on a
+// Pieces: no more than fill the chip (work-groups that it holds at once: three on a
 // CU with heads of 64 dims, two with 128) when the tiles of rows alone do not.
 constexpr int kCus = 256;
 int fill_of(int head_dim) { return head_dim == 64 ? 768 : 512; }
@@ -692,6 +692,11 @@ int fill_of(int head_dim) { return head_dim == 64 ? 768 : 512; }
 // up to 1800 34.5 / 30.6, three of up to 258 over up to 4563 with a window 56.3 / 49.0).
 constexpr int64_t kAlike = 80;
 
+// How long a tile of 64 dims takes a work-group, a join, and a partial sum's float on
+// its way to it and back: a piece more has to save more than it costs (680 tokens in
+// two pieces 27.2 us, in one 16.4; four of up to 120 over up to 1000 20.7 / 19.2).
+constexpr double kTileUs = 1.2, kJoinUs = 4.0, kPartUs = 2e-6;
+
 struct Split {
   int groups, pieces;
 };
@@ -701,13 +706,17 @@ Split split_of(int rows, int B, int heads, int kv_heads, int head_dim, int64_t m
   const int per = 128 / (heads / kv_heads);
   const int64_t tiles = (static_cast<int64_t>(rows) + per - 1) / per + (B < rows ? B : rows) - 1;
   const int64_t wgs = tiles * kv_heads;
-  auto pieces = [&](int64_t fill, int groups) {
-    return static_cast<int>(max(int64_t{1}, min(fill / wgs, most / (groups * kMinTiles))));
-  };
-  Split s{1, pieces(fill_of(head_dim), 1)};
+  auto top = [&](int64_t fill, int groups) { return max(int64_t{1}, min(fill / wgs, most / (groups * kMinTiles))); };
   const bool few = wgs <= kCus || (head_dim == 128 && wgs <= 2 * kCus && most >= 2 * kMinTiles);
   const bool even = B == 1 || (most <= kAlike && (B - 1) * most <= 2 * kAlike);
-  if (few && even && wgs * s.pieces > kCus && 2 * static_cast<int64_t>(rows) >= tiles * per) s = {2, pieces(kCus, 2)};
+  const bool two = few && even && wgs * top(fill_of(head_dim), 1) > kCus && 2 * static_cast<int64_t>(rows) >= tiles * per;
+  Split s{two ? 2 : 1, 1};
+  double least = 0.0;
+  for (int p = 1; p <= top(two ? kCus : fill_of(head_dim), s.groups); ++p) {
+    const double chain = kTileUs * head_dim / 64 * static_cast<double>(most) / (s.groups * p);
+    const double join = p == 1 ? 0.0 : kJoinUs + kPartUs * p * rows * heads * (head_dim + 4);
+    if (p == 1 || chain + join < least) s.pieces = p, least = chain + join;
+  }
   return s;
 }
 
