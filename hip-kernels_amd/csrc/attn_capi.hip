@@ -34,7 +34,6 @@ bool apart(const void* a, size_t na, const void* b, size_t nb) {
 
 constexpr int kMaxGroup = 128;  // query heads per kv head
 constexpr int64_t kMaxRowHeads = 1 << 26, kMaxSeqHeads = 1 << 22;  // rows and sequences of a call, times heads
-constexpr int64_t kMaxTokens = 1 << 30;                            // of a sequence
 
 int check_cache(const gptoss_kv_cache* c, KvPages* kv) {
   if (c == nullptr) return set_error(GPTOSS_ERR_INVALID, "cache is NULL");
@@ -131,7 +130,8 @@ int check_attend(AttendArgs* a, const gptoss_kv_cache* cache, const gptoss_atten
   const int64_t cap = static_cast<int64_t>(a->max_blocks) << a->kv.bs_shift;
   if (cap > kMaxTokens || cap / 16 + 1 > 0x7fffffff / B)
     return set_error(GPTOSS_ERR_UNSUPPORTED, "tables of %d pages for %d sequences", a->max_blocks, B);
-  const size_t need = gptoss_paged_attention_workspace_bytes(rows, B, a->heads, a->kv.kv_heads, a->kv.head_dim);
+  const size_t need = gptoss_paged_attention_call_bytes(a->offsets == nullptr ? 0 : rows, B, a->heads, a->kv.kv_heads,
+                                                        a->kv.head_dim, cap, cfg->window, cfg->first_tokens);
   if (need > 0) {
     if (workspace == nullptr || workspace_bytes < need)
       return set_error(GPTOSS_ERR_INVALID, "workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : 0,
@@ -232,6 +232,16 @@ size_t gptoss_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int 
   return decode > prefill ? decode : prefill;
 }
 
+size_t gptoss_paged_attention_call_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                         int64_t max_tokens, int window, int first_tokens) {
+  if (num_tokens < 0 || num_seqs < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1) return 0;
+  if (num_heads / num_kv_heads > kMaxGroup || num_heads > kMaxSeqHeads) return 0;
+  if (max_tokens < 1 || max_tokens > kMaxTokens || window < 0 || first_tokens < 0) return 0;
+  const Reach r{max_tokens, window < max_tokens ? window : 0, first_tokens};
+  return num_tokens == 0 ? decode_call_bytes(num_seqs, num_heads, num_kv_heads, head_dim, r)
+                         : prefill_call_bytes(num_tokens, num_seqs, num_heads, num_kv_heads, head_dim, r);
+}
+
 int gptoss_paged_attention_decode(const uint16_t* q, int64_t q_stride, const gptoss_kv_cache* cache,
                                   const int32_t* block_tables, int64_t table_stride, int max_blocks,
                                   const int32_t* seq_lens, int num_seqs, int num_heads,
@@ -273,10 +283,11 @@ int gptoss_paged_attention_prefill(const uint16_t* q, int64_t q_stride, const in
   a.lens = seq_lens;
   a.offsets = query_offsets;
   a.heads = num_heads;
+  if (query_offsets == nullptr && num_tokens > 0 && num_seqs > 0)
+    return set_error(GPTOSS_ERR_INVALID, "null query_offsets");
   const int rc = check_attend(&a, cache, cfg, num_tokens, num_seqs, workspace, workspace_bytes);
   if (rc != GPTOSS_OK) return rc;
   if (num_tokens == 0 || num_seqs == 0) return ok();
-  if (query_offsets == nullptr) return set_error(GPTOSS_ERR_INVALID, "null query_offsets");
   HIP_TRY(launch_prefill(a, workspace, static_cast<hipStream_t>(stream)), "paged attention prefill launch");
   return ok();
 }

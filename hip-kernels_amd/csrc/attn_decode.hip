@@ -505,23 +505,30 @@ Cut cut_of(int B, int64_t most_tiles, int tiles_of_heads, int head_dim) {
   return Cut{slots, pieces < most ? pieces : most, 2};
 }
 
+// No more tiles than the longest sequence, or its window and first tokens, has.
+int64_t most_tiles(const Reach& r) {
+  const int64_t all = (r.tokens + kTile - 1) / kTile;
+  return r.window == 0 ? all : min(all, (r.window + kTile - 2) / kTile + 1 + (r.first + kTile - 1) / kTile);
+}
+
 int tiles_of_heads(int heads, int kv_heads) { return kv_heads * ((heads / kv_heads + 15) / 16); }
 
 }  // namespace
 
-size_t decode_workspace_bytes(int B, int heads, int kv_heads, int head_dim) {
-  const Cut c = cut_of(B, 1 << 30, tiles_of_heads(heads, kv_heads), head_dim);
+size_t decode_call_bytes(int B, int heads, int kv_heads, int head_dim, const Reach& r) {
+  const Cut c = cut_of(B, most_tiles(r), tiles_of_heads(heads, kv_heads), head_dim);
+  if (c.slots == 0) return 0;
   const size_t pieces = static_cast<size_t>(c.max_slots) * heads;
   return pieces * (head_dim + 4) * sizeof(float) + ((static_cast<size_t>(B) * 2 * sizeof(int) + 15) & ~size_t{15});
 }
 
+size_t decode_workspace_bytes(int B, int heads, int kv_heads, int head_dim) {
+  return decode_call_bytes(B, heads, kv_heads, head_dim, Reach{kMaxTokens, 0, 0});
+}
+
 hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
-  const int64_t cap = static_cast<int64_t>(a.max_blocks) << a.kv.bs_shift;
-  int64_t most = (cap + kTile - 1) / kTile;
-  if (a.window > 0) most = min(most, (static_cast<int64_t>(a.window) + kTile - 2) / kTile + 1 +
-                                         (static_cast<int64_t>(a.first) + kTile - 1) / kTile);
   const int th = tiles_of_heads(a.heads, a.kv.kv_heads);
-  const Cut c = cut_of(a.B, most, th, a.kv.head_dim);
+  const Cut c = cut_of(a.B, most_tiles(reach_of(a)), th, a.kv.head_dim);
   SplitArgs sp{};
   sp.slots = c.slots;
   sp.min_tiles = min_tiles(a.kv.head_dim);

@@ -69,6 +69,20 @@ struct RopeTableArgs {
 hipError_t launch_rope_table(const RopeTableArgs& a, hipStream_t s);
 hipError_t launch_rope_append(const AppendArgs& a, hipStream_t s);
 hipError_t launch_join(const AttendArgs& a, const JoinArgs& j, int64_t mean, hipStream_t s);  // mean: pieces of a row
+constexpr int64_t kMaxTokens = 1 << 30;  // of a sequence
+
+// What a sequence of a call can hold and a query of it see, as the host knows it.
+struct Reach {
+  int64_t tokens, window, first;  // window 0: all
+};
+
+inline Reach reach_of(const AttendArgs& a) {
+  return Reach{static_cast<int64_t>(a.max_blocks) << a.kv.bs_shift, a.window, a.first};
+}
+
+// Bytes for one call, and for any of at most its counts.
+size_t decode_call_bytes(int B, int heads, int kv_heads, int head_dim, const Reach& r);
+size_t prefill_call_bytes(int rows, int B, int heads, int kv_heads, int head_dim, const Reach& r);
 size_t decode_workspace_bytes(int B, int heads, int kv_heads, int head_dim);
 hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s);
 size_t prefill_workspace_bytes(int rows, int heads, int kv_heads, int head_dim);

@@ -697,6 +697,14 @@ constexpr int64_t kAlike = 80;
 // two pieces 27.2 us, in one 16.4; four of up to 120 over up to 1000 20.7 / 19.2).
 constexpr double kTileUs = 1.2, kJoinUs = 4.0, kPartUs = 2e-6;
 
+// No more tiles than the longest sequence, or the window over a tile's rows and the
+// first tokens, has.
+int64_t most_tiles(const Reach& r, int rows, int heads, int kv_heads, int head_dim) {
+  const int per = 128 * cols_of(rows, heads, head_dim) / (heads / kv_heads);
+  const int64_t all = (r.tokens + kTile - 1) / kTile;
+  return r.window == 0 ? all : min(all, (r.window + per + kTile - 3) / kTile + 1 + (r.first + kTile - 1) / kTile);
+}
+
 struct Split {
   int groups, pieces;
 };
@@ -722,6 +730,13 @@ Split split_of(int rows, int B, int heads, int kv_heads, int head_dim, int64_t m
 
 }  // namespace
 
+size_t prefill_call_bytes(int rows, int B, int heads, int kv_heads, int head_dim, const Reach& r) {
+  const int pieces = split_of(rows, B, heads, kv_heads, head_dim, most_tiles(r, rows, heads, kv_heads, head_dim)).pieces;
+  if (pieces == 1) return 0;
+  return static_cast<size_t>(pieces) * rows * heads * (head_dim + 4) * sizeof(float) +
+         ((static_cast<size_t>(rows) * sizeof(int) + 15) & ~size_t{15});
+}
+
 // For any call of up to `rows` rows: with t tiles there are at most fill / (t
 // kv_heads) pieces of at most t * per rows.
 size_t prefill_workspace_bytes(int rows, int heads, int kv_heads, int head_dim) {
@@ -734,14 +749,9 @@ size_t prefill_workspace_bytes(int rows, int heads, int kv_heads, int head_dim) 
 
 hipError_t launch_prefill(const AttendArgs& a, void* workspace, hipStream_t s) {
   const int cols = cols_of(a.rows, a.heads, a.kv.head_dim), per = 128 * cols / (a.heads / a.kv.kv_heads);
-  // no more tiles than the longest sequence, or a window over a tile's rows, has
-  const int64_t cap = static_cast<int64_t>(a.max_blocks) << a.kv.bs_shift;
-  int64_t most = (cap + kTile - 1) / kTile;
-  if (a.window > 0)
-    most = min(most, (static_cast<int64_t>(a.window) + per + kTile - 3) / kTile + 1 +
-                         (static_cast<int64_t>(a.first) + kTile - 1) / kTile);
   PieceArgs pa{};
-  const Split split = split_of(a.rows, a.B, a.heads, a.kv.kv_heads, a.kv.head_dim, most);
+  const Split split = split_of(a.rows, a.B, a.heads, a.kv.kv_heads, a.kv.head_dim,
+                               most_tiles(reach_of(a), a.rows, a.heads, a.kv.kv_heads, a.kv.head_dim));
   pa.pieces = split.pieces;
   const size_t parts = static_cast<size_t>(pa.pieces) * a.rows * a.heads;
   pa.part_o = static_cast<float*>(workspace);

@@ -165,6 +165,7 @@ _sig("gptoss_rope_config_default", [ctypes.POINTER(RopeConfig)])
 _sig("gptoss_rope_table", [ctypes.POINTER(RopeConfig), _P, _P])
 _sig("gptoss_rope_kv_append", [_P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _P, _L, _P, _P])
 _sig("gptoss_paged_attention_workspace_bytes", [_I, _I, _I, _I, _I], _SZ)
+_sig("gptoss_paged_attention_call_bytes", [_I, _I, _I, _I, _I, ctypes.c_int64, _I, _I], _SZ)
 _sig("gptoss_paged_attention_decode", [_P, _L, _P, _P, _L, _I, _P, _I, _I, _P, _P, _L, _P, _SZ, _P])
 _sig("gptoss_paged_attention_prefill", [_P, _L, _P, _I, _P, _P, _L, _I, _P, _I, _I, _P, _P, _L, _P, _SZ, _P])
 
@@ -1027,7 +1028,7 @@ def rope_kv_append(qkv, positions, slots, table, cache: KVCache, num_heads: int,
     cols = q_stride = num_heads * D
     if q_out is None:
         _needs_gpu(dev)
-        q_out = _empty((T, cols), torch.bfloat16, dev, stream)
+        q_out = qkv.new_empty((T, cols)) if stream is None else _empty((T, cols), torch.bfloat16, dev, stream)
     else:
         q_stride = _row_tensor("q_out", q_out, dev, cols)
         if q_out.shape[0] != T:
@@ -1041,14 +1042,13 @@ def rope_kv_append(qkv, positions, slots, table, cache: KVCache, num_heads: int,
     return q_out
 
 
-@functools.lru_cache(maxsize=1024)
-def _workspace_bytes(rows: int, seqs: int, heads: int, kv_heads: int, head_dim: int) -> int:
-    return _lib.gptoss_paged_attention_workspace_bytes(rows, seqs, heads, kv_heads, head_dim)
-
-
 def paged_attention_workspace_bytes(num_tokens: int, num_seqs: int, num_heads: int, cache: KVCache) -> int:
-    """Bytes of workspace that suffice for a call on num_tokens rows of num_seqs sequences."""
-    return _workspace_bytes(num_tokens, num_seqs, num_heads, cache.kv_heads, cache.head_dim)
+    """Bytes of workspace that suffice for any call on up to num_tokens rows of up to num_seqs sequences."""
+    return _lib.gptoss_paged_attention_workspace_bytes(num_tokens, num_seqs, num_heads, cache.kv_heads, cache.head_dim)
+
+
+# (rows, 0 for decode; sequences; heads; kv heads; head_dim; tokens of a table; window; first tokens)
+_call_bytes = functools.lru_cache(maxsize=4096)(_lib.gptoss_paged_attention_call_bytes)
 
 
 def _attend(q, offsets, cache, block_tables, seq_lens, scale, window, first_tokens, sinks, out, workspace, stream):
@@ -1058,7 +1058,9 @@ def _attend(q, offsets, cache, block_tables, seq_lens, scale, window, first_toke
     rows, cols = q.shape
     q_stride = out_stride = _row_tensor("q", q, dev, cols)
     H = cols // D
-    _on_device("block_tables", block_tables, dev, torch.int32, 2)
+    if not (isinstance(block_tables, torch.Tensor) and block_tables.dtype is torch.int32 and block_tables.dim() == 2
+            and block_tables.device == dev):
+        _on_device("block_tables", block_tables, dev, torch.int32, 2)
     B, blocks = block_tables.shape
     table_stride, one = block_tables.stride()
     if B < 2:
@@ -1076,23 +1078,29 @@ def _attend(q, offsets, cache, block_tables, seq_lens, scale, window, first_toke
         _vector("query_offsets", offsets, dev, B + 1, torch.int32)
     if out is None:
         _needs_gpu(dev)
-        out, out_stride = _empty((rows, cols), torch.bfloat16, dev, stream), cols
+        out_stride = cols
+        out = torch.empty_like(q) if stream is None and q.is_contiguous() else _empty((rows, cols), torch.bfloat16, dev, stream)
     else:
         out_stride = _row_tensor("out", out, dev, cols)
         if out.shape[0] != rows:
             _bad(f"out has {out.shape[0]} rows, expected {rows}")
         _needs_gpu(dev)
+    where = None
     if workspace is None:
-        size = _workspace_bytes(rows, B, H, cache.kv_heads, D)
-        workspace = _empty(size, torch.uint8, dev, stream)
+        size = _call_bytes(rows if offsets is not None else 0, B, H, cache.kv_heads, D, blocks * cache.block_size, window,
+                           first_tokens) if rows else 0
+        if size:
+            workspace = _empty((size,), torch.uint8, dev, stream)
+            where = workspace.data_ptr()
     else:
         _on_device("workspace", workspace, dev)
         if not workspace.is_contiguous():
             _bad("workspace must be contiguous")
         size = workspace.numel() * workspace.element_size()
+        where = workspace.data_ptr()
     cfg = AttentionConfig(D ** -0.5 if scale is None else scale, window, first_tokens, sinks)
     tail = (cache._desc, block_tables.data_ptr(), table_stride, blocks, seq_lens.data_ptr(), B, H, ctypes.addressof(cfg),
-            out.data_ptr(), out_stride, workspace.data_ptr(), size)
+            out.data_ptr(), out_stride, where, size)
     if offsets is None:
         _launch(dev, stream, _lib.gptoss_paged_attention_decode, q.data_ptr(), q_stride, *tail)
     else:
@@ -1105,8 +1113,8 @@ def paged_attention_decode(q, cache: KVCache, block_tables, seq_lens, scale: flo
     """Attention of one new token per sequence (already appended): q [B, num_heads * head_dim] over the pages
     block_tables (int32 [B, max_blocks], -1: none) of seq_lens (int32 [B]) tokens.  scale: head_dim ** -0.5 when
     None.  window: 0, or how many of the last tokens are seen, besides the first first_tokens.  sinks: bf16
-    [num_heads], a logit that joins the softmax's sum.  workspace: of paged_attention_workspace_bytes(); when None it
-    is allocated, like out."""
+    [num_heads], a logit that joins the softmax's sum.  workspace: of paged_attention_workspace_bytes(); when None what
+    the call needs is allocated, like out."""
     return _attend(q, None, cache, block_tables, seq_lens, scale, window, first_tokens, sinks, out, workspace, stream)
 
 

@@ -546,12 +546,17 @@ typedef struct gptoss_attention_config {
  * workspace: gptoss_paged_attention_workspace_bytes bytes, 16-byte aligned,
  * that no call running at the same time uses (two graphs that may overlap need
  * two); nothing is kept in it between calls.  The bytes for num_tokens rows and
- * num_seqs sequences are enough for calls of fewer.
+ * num_seqs sequences are enough for calls of fewer, whatever their lengths.
+ * What one call needs is less, and 0 where nothing is split (workspace may be NULL
+ * then): gptoss_paged_attention_call_bytes, with max_tokens = max_blocks *
+ * block_size and num_tokens = 0 for decode.
  * Limits of a call (GPTOSS_ERR_UNSUPPORTED): num_tokens * num_heads 2^26, num_seqs
  * * num_heads 2^22, max_blocks * block_size 2^30, num_seqs * max_blocks *
  * block_size 2^35, token_stride 2^24. */
 size_t gptoss_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads,
                                               int head_dim);
+size_t gptoss_paged_attention_call_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                         int64_t max_tokens, int window, int first_tokens);
 int gptoss_paged_attention_decode(const uint16_t* q, int64_t q_stride, const gptoss_kv_cache* cache,
                                   const int32_t* block_tables, int64_t table_stride, int max_blocks,
                                   const int32_t* seq_lens, int num_seqs, int num_heads,

@@ -145,11 +145,30 @@ def test_rope_table_refused(g, change):
 
 
 def test_workspace_refused(g):
-    need = g.lib.gptoss_paged_attention_workspace_bytes(3, 3, 64, 8, 64)
-    if need:
-        assert decode(g, cache(g), ws_bytes=need - 1) == g.GPTOSS_ERR_INVALID and b"workspace" in g.lib.gptoss_last_error()
-        assert decode(g, cache(g), ws=None) == g.GPTOSS_ERR_INVALID
-        assert decode(g, cache(g), ws=16 * A + 8) == g.GPTOSS_ERR_INVALID and b"aligned" in g.lib.gptoss_last_error()
+    """Calls that are cut: less than they need, none, and one that is not aligned."""
+    wide = dict(max_blocks=2000, table_stride=2000)
+    for call, T in ((decode, 0), (prefill, 20)):
+        need = g.lib.gptoss_paged_attention_call_bytes(T, 3, 64, 8, 64, 32000, 0, 0)
+        assert 0 < need <= g.lib.gptoss_paged_attention_workspace_bytes(max(T, 3), 3, 64, 8, 64)
+        assert call(g, cache(g), ws_bytes=need - 1, **wide) == g.GPTOSS_ERR_INVALID and b"workspace" in g.lib.gptoss_last_error()
+        assert call(g, cache(g), ws=None, **wide) == g.GPTOSS_ERR_INVALID
+        assert call(g, cache(g), ws=16 * A + 8, **wide) == g.GPTOSS_ERR_INVALID and b"aligned" in g.lib.gptoss_last_error()
+
+
+@pytest.mark.parametrize("H,Hk,D", [(64, 8, 64), (32, 8, 128), (5, 1, 64), (128, 1, 128), (6, 6, 128), (1, 1, 64)])
+def test_call_bytes(g, H, Hk, D):
+    """No call needs more than the workspace for its counts; short ones need none."""
+    one, top = g.lib.gptoss_paged_attention_call_bytes, g.lib.gptoss_paged_attention_workspace_bytes
+    for B in (1, 2, 7, 64, 700):
+        for tokens in (1, 512, 513, 1024, 1025, 4000, 131072, 1 << 30):
+            for window, first in ((0, 0), (128, 0), (3000, 4), (2 ** 31 - 1, 2 ** 31 - 1)):
+                assert one(0, B, H, Hk, D, tokens, window, first) <= top(B, B, H, Hk, D)
+                for T in (1, B, 90, 680, 5000):
+                    assert one(T, B, H, Hk, D, tokens, window, first) <= top(T, B, H, Hk, D)
+    assert one(0, 3, H, Hk, D, 512, 0, 0) == one(20, 3, H, Hk, D, 400, 0, 0) == 0
+    for bad in ((-1, 1, H, Hk, D, 9, 0, 0), (0, 0, H, Hk, D, 9, 0, 0), (0, 1, H, 0, D, 9, 0, 0), (0, 1, H, Hk, D, 0, 0, 0),
+                (0, 1, H, Hk, D, 9999, -1, 0), (0, 1, H, Hk, D, 1 << 40, 0, 0)):
+        assert one(*bad) == 0
 
 
 @pytest.mark.parametrize("H,Hk,D", [(64, 8, 64), (32, 8, 128), (5, 1, 64), (128, 1, 128), (6, 6, 128), (1, 1, 64)])
