@@ -902,14 +902,15 @@ class _on:
 
 def _launch(device, stream, fn, *args) -> None:
     """Calls fn on `stream` (None: the current one) of `device`."""
+    index = device.index
     if stream is None:
-        handle = torch._C._cuda_getCurrentRawStream(device.index)
+        handle = torch._C._cuda_getCurrentRawStream(index)
     else:
         handle = stream if isinstance(stream, int) else stream.cuda_stream
-    if torch._C._cuda_getDevice() == device.index:
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args, handle)
     else:
-        with _on(device.index):
+        with _on(index):
             rc = fn(*args, handle)
     if rc:
         check(rc)
@@ -1021,7 +1022,8 @@ def rope_kv_append(qkv, positions, slots, table, cache: KVCache, num_heads: int,
     T = qkv.shape[0]
     _vector("positions", positions, dev, T, torch.int32)
     _vector("slots", slots, dev, T, torch.int32)
-    _on_device("table", table, dev, torch.float32, 3)
+    if not (isinstance(table, torch.Tensor) and table.dtype is torch.float32 and table.dim() == 3 and table.device == dev):
+        _on_device("table", table, dev, torch.float32, 3)
     max_positions, two, half = table.shape
     if two != 2 or not table.is_contiguous():
         _bad(f"table must be contiguous [max_positions, 2, rotary_dim / 2], got {tuple(table.shape)}")
@@ -1053,11 +1055,13 @@ _call_bytes = functools.lru_cache(maxsize=4096)(_lib.gptoss_paged_attention_call
 
 def _attend(q, offsets, cache, block_tables, seq_lens, scale, window, first_tokens, sinks, out, workspace, stream):
     dev, D = cache.device, cache.head_dim
-    if not isinstance(q, torch.Tensor) or q.dim() != 2 or q.shape[1] % D != 0 or q.shape[1] == 0:
+    if not isinstance(q, torch.Tensor) or q.dim() != 2:
         _bad(f"q must be [rows, num_heads * {D}]")
     rows, cols = q.shape
-    q_stride = out_stride = _row_tensor("q", q, dev, cols)
-    H = cols // D
+    H, rest = divmod(cols, D)
+    if rest or not H:
+        _bad(f"q must be [rows, num_heads * {D}]")
+    q_stride = _row_tensor("q", q, dev, cols)
     if not (isinstance(block_tables, torch.Tensor) and block_tables.dtype is torch.int32 and block_tables.dim() == 2
             and block_tables.device == dev):
         _on_device("block_tables", block_tables, dev, torch.int32, 2)
