@@ -974,7 +974,7 @@ class KVCache:
     [num_blocks, kv_heads, block_size, head_dim], bfloat16 or float8_e4m3fn with
     the last dim contiguous and the same strides, so a permuted view covers
     token-major pages and k = slab[:, 0], v = slab[:, 1] an interleaved slab.
-    8-bit caches stand for code * scale, scales float32 [kv_heads] (None: 1)."""
+    8-bit caches stand for code * scale, scales float32 [kv_heads], positive (None: 1)."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None):

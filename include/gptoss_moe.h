@@ -461,8 +461,8 @@ enum { GPTOSS_KV_BF16 = 0, GPTOSS_KV_E4M3 = 1 };
  * multiples of 16 bytes and at least head_dim, k and v are 16-byte aligned, so
  * token-major pages and K / V interleaved by page are covered.  head_dim is 64
  * or 128, block_size a power of two from 16 to 256.  E4M3 (OCP, gfx950's own)
- * elements stand for code * scale[kv head]; a null scale is 1, and bf16 caches
- * have none. */
+ * elements stand for code * scale[kv head], scales positive; a null scale is 1,
+ * and bf16 caches have none. */
 typedef struct gptoss_kv_cache {
   void* k;
   void* v;
