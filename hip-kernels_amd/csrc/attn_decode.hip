@@ -238,7 +238,7 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
       q[s] = __builtin_bit_cast(bf16x8, x);
     }
   }
-  const float scale = a.scale_log2 * (kE4m3 && a.kv.k_scale ? a.kv.k_scale[kvh] : 1.0f);
+  const float scale = score_scale<kE4m3>(a, kvh);
 
   // Pages of 32 of this wave's tiles at a time: lane 2 i + j has half j of
   // the i-th (tile t0 + wave + W i).

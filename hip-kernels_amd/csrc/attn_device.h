@@ -58,6 +58,15 @@ __device__ __forceinline__ int seq_len(const AttendArgs& a, int b) {
   return cap < n ? static_cast<int>(cap) : n;
 }
 
+// What scores of a kv head are multiplied by.  Not 0 where the product underflows:
+// a hidden token's -inf would become NaN (so small a scale gives every seen token
+// the same weight, and the smallest number does too).
+template <bool kE4m3>
+__device__ __forceinline__ float score_scale(const AttendArgs& a, int kvh) {
+  const float scale = a.scale_log2 * (kE4m3 && a.kv.k_scale ? a.kv.k_scale[kvh] : 1.0f);
+  return scale == 0.0f ? 0x1p-149f : scale;
+}
+
 // Whether the token at position t is seen from position p: not a later one,
 // and within the window or among the first tokens.
 __device__ __forceinline__ bool sees(const AttendArgs& a, int p, int t) {

@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256 * G, D == 64 && kCols == 1 && G == 1 ? 3 : 2) v
       }
     }
   }
-  const float scale = a.scale_log2 * (kE4m3 && a.kv.k_scale ? a.kv.k_scale[kvh] : 1.0f);
+  const float scale = score_scale<kE4m3>(a, kvh);
 
   const bool work = 32 * kCols * wave < c.tokens * group;  // whether any of the wave's rows is one
   // the tiles that the rows see: the first tokens', then the window's

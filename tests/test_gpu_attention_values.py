@@ -36,3 +36,15 @@ def test_large_values_without_weight(gpu, shape, n):
                       ("prefill", gpu.paged_attention_prefill(q, off, c.cache, c.tables, c.seq_lens, scale=8.0))):
         bad = ref.within(got, want, tol)
         assert bad is None, (name, bad)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("scale", [1e-44, 1e-40, 1e-20])
+def test_smallest_scales(gpu, e4m3, scale):
+    """Scales so small that the product with an 8-bit cache's underflows: every seen token counts alike."""
+    c = Case(gpu, 72, [50, 333, 3], *GPT, e4m3=e4m3)
+    if e4m3:
+        c.scales[0].fill_(0.01)
+    for window in (0, 20):
+        c.check_decode(window=window, scale=scale)
+        c.check_prefill([50, 70, 1], window=window, scale=scale)
