@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256 * G, D == 64 && kCols == 1 && G == 1 ? 3 : 2) v
   // of each group K of two tiles, then V of two; the queries pass through the middle
   // half of it before, the results through its beginning afterwards
   __shared__ __attribute__((aligned(16))) uint8_t s_all[4 * G][kBytes];
-  __shared__ int s_odd;  // whether put() left out a value
+  __shared__ uint32_t s_odd[2];  // the tiles (of 64 in turn) of which put() left out a value
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
   const int part_of = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);  // its group
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(256 * G, D == 64 && kCols == 1 && G == 1 ? 3 : 2) v
       }
     }
   };
-  auto put_values = [&](int buf, bool whole) __attribute__((always_inline)) {
+  auto put_values = [&](int buf, int tile, bool whole) __attribute__((always_inline)) {
     if (!whole) {
       uint32_t odd = 0;
 #pragma unroll
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(256 * G, D == 64 && kCols == 1 && G == 1 ? 3 : 2) v
         for (int j = 0; j < kLoads; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) vr[j][e] &= ~not_finite<kE4m3>(vr[j][e]);
-        if (lane == 0) s_odd = 1;
+        if (lane == 0) atomicOr(&s_odd[tile >> 5 & 1], 1u << (tile & 31));
       }
     }
     put(s_v[buf], vr);
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(256 * G, D == 64 && kCols == 1 && G == 1 ? 3 : 2) v
       }
   }
 
-  if (threadIdx.x == 0) s_odd = 0;
+  if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
   __syncthreads();
   if (steps > 0) {
     // Tile i: K of tile i + 1 and V of tile i go to LDS, K of i + 2 and V of i + 1
@@ -500,7 +500,7 @@ __global__ __launch_bounds__(256 * G, D == 64 && kCols == 1 && G == 1 ? 3 : 2) v
       const int t = begin_of(i);
       const bool whole = is_whole(t, pages);
       put(s_k[buf ^ 1], kr);
-      put_values(buf, whole);
+      put_values(buf, first_tile + i, whole);
       uint32_t later;
       const int64_t to = fetch(i + 2, &later);
       load(vb, at, vr);
@@ -532,22 +532,35 @@ __global__ __launch_bounds__(256 * G, D == 64 && kCols == 1 && G == 1 ? 3 : 2) v
       }
     }
   }
-  if (s_odd != 0) {
-    // what put() left out, for the rows that see it
+  if (work && (s_odd[0] | s_odd[1]) != 0) {
+    // What put() left out, for the rows that see it.  Only tiles that it marked are
+    // looked at, a lane to a token, and of these only tokens that do hold something:
+    // most often it lies past the sequence's end (a prompt of 2048 with NaN there
+    // 53 us, as without; 975 with every token of every tile looked at).
     for (int i = 0; i < tiles; ++i) {
-      for (int x = 0; x < kTile; ++x) {
-        const int t = tile_at(i) + x;
-        if (t >= c.len) break;
-        const int page = a.tables[c.b * a.table_stride + (t >> a.kv.bs_shift)];
-        if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.kv.num_blocks)) continue;
-        uint32_t all = 0;  // whether this tile went through put() unchanged
-        for (int j = 0; j < 4; ++j) {
-          const int u = tile_at(i) + 16 * j;
-          const int g = u < c.len ? a.tables[c.b * a.table_stride + (u >> a.kv.bs_shift)] : -1;
-          all |= static_cast<uint32_t>(g) < static_cast<uint32_t>(a.kv.num_blocks) ? 1u << j : 0u;
+      const int tile = first_tile + i, from = begin_of(i);
+      if ((s_odd[tile >> 5 & 1] >> (tile & 31) & 1) == 0) continue;
+      const int mine_t = from + lane;
+      int page = mine_t < c.len ? a.tables[c.b * a.table_stride + (mine_t >> a.kv.bs_shift)] : -1;
+      const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.num_blocks);
+      const uint64_t there = __ballot(ok);
+      uint32_t all = 0;  // as fetch() has them
+#pragma unroll
+      for (int j = 0; j < 4; ++j) all |= static_cast<uint32_t>(there >> (16 * j) & 1) << j;
+      if (is_whole(from, all)) continue;
+      uint32_t odd = 0;
+      if (ok && mine_t <= pmax) {
+        GlobalBytes v = vb + page * a.kv.sb * kSize + static_cast<int64_t>(mine_t & mask) * st;
+#pragma unroll 2
+        for (int k = 0; k < kPieces; ++k) {
+          const attn_u32x4 x = *reinterpret_cast<const __attribute__((address_space(1))) attn_u32x4*>(v + 16 * k);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd |= not_finite<kE4m3>(x[e]);
         }
-        if (is_whole(tile_at(i), all)) continue;
-        GlobalBytes v = vb + page * a.kv.sb * kSize + static_cast<int64_t>(t & mask) * st + 4 * h * kSize;
+      }
+      for (uint64_t left = __ballot(odd != 0); left != 0; left &= left - 1) {
+        const int x = __builtin_ctzll(left), t = from + x;
+        GlobalBytes v = vb + __builtin_amdgcn_readlane(page, x) * a.kv.sb * kSize + static_cast<int64_t>(t & mask) * st + 4 * h * kSize;
 #pragma unroll
         for (int y = 0; y < kCols; ++y) {
           if (pos[y] < 0 || !sees(a, pos[y], t)) continue;

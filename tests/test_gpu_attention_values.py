@@ -48,3 +48,66 @@ def test_smallest_scales(gpu, e4m3, scale):
     for window in (0, 20):
         c.check_decode(window=window, scale=scale)
         c.check_prefill([50, 70, 1], window=window, scale=scale)
+
+
+@pytest.mark.parametrize("shape,e4m3,new,n", [(GPT, False, 2048, 2048), (GPT, False, 60, 9000), (GQA4, True, 300, 6000)])
+def test_what_lies_past_the_end_costs_nothing(gpu, shape, e4m3, new, n):
+    """NaN in the last page's slots past the end, as memory that nothing was written to may hold: the same results, in
+    about the same time (looking at every token took 13 to 18 times as long)."""
+    H, Hk, D, bs = shape
+    c = Case(gpu, 73, [n - 3], *shape, e4m3=e4m3)
+    pages = [p.clone() for p in c.pages]
+    raw = pages[1].view(torch.uint8) if e4m3 else pages[1]
+    page = c.tables[0, -1].long()
+    raw[page, :, (n - 3) % bs:] = 0
+    clean = gpu.KVCache(pages[0], pages[1], *c.scales)
+    q = randn(c.gen, new, H * D, scale=1.5)
+    off = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+
+    def took(cache):
+        best = float("inf")
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(10):
+                out = gpu.paged_attention_prefill(q, off, cache, c.tables, c.seq_lens)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return out, best
+
+    (want, fast), (got, slow) = took(clean), took(c.cache)
+    say("past the end", shape, e4m3, new, n, f"{100 * fast:.1f} us, with NaN {100 * slow:.1f}")
+    assert torch.equal(got, want) and want.isfinite().all()
+    assert slow < 3 * fast
+
+
+@pytest.mark.parametrize("shape,e4m3", [(GPT, False), (GPT, True), (GQA4, False), (GQA4, True), ((128, 4, 64, 16), False)])
+@pytest.mark.parametrize("window,first", [(0, 0), (1200, 0), (5000, 70)])
+def test_values_of_far_tiles_reach_only_who_sees_them(gpu, shape, e4m3, window, first):
+    """NaN and infinities among the values of a long context, 64 tiles apart and in one tile, in seen places, between
+    window and first tokens and past the end: in the rows that see them and in no other."""
+    say("far values", shape, e4m3, window, first)
+    H, Hk, D, bs = shape
+    n, new, G = 9000, 4200 if H == 128 else 150, H // Hk
+    c = Case(gpu, 74, [n], *shape, e4m3=e4m3)
+    q = randn(c.gen, new, H * D, scale=1.5)
+    off = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    call = lambda: gpu.paged_attention_prefill(q, off, c.cache, c.tables, c.seq_lens, window=window,  # noqa: E731
+                                               first_tokens=first).view(new, H, D)
+    want = call().clone()
+    assert want.isfinite().all()
+    pos = torch.arange(n - new, n, device="cuda")
+    bad = torch.zeros((new, H, D), dtype=torch.bool, device="cuda")
+    for i, t in enumerate([2, 69, 70, 4850, 4850 - 4096, n - 1 - 4096, n - 130, n - 130 + 1, n - 100, n - 64, n - 1, n - 1]):
+        d = 5 * i % D
+        page = c.tables[0, t // bs].long()
+        if e4m3:
+            c.pages[1].view(torch.uint8)[page, 1, t % bs, d] = 0x7f
+        else:
+            c.pages[1][page, 1, t % bs, d] = float("inf") if i % 2 else float("nan")
+        sees = (t <= pos) & ((window == 0) | (pos - t < window) | (t < first))
+        bad[:, G:2 * G, d] |= sees[:, None]
+    got = call()
+    assert (~got[bad].isfinite()).all()
+    assert torch.equal(got[~bad], want[~bad])
