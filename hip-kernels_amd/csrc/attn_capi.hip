@@ -1,5 +1,6 @@
 // attn_capi.hip -- C ABI of the attention operators (include/gptoss_moe.h):
-// argument checks, then one or two launches on the caller's stream.
+// argument checks, then one or two launches (for each 8192 sequences) on the
+// caller's stream.
 #include <cmath>
 
 #include "attn_kernels.h"

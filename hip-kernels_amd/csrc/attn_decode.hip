@@ -529,9 +529,11 @@ size_t decode_workspace_bytes(int B, int heads, int kv_heads, int head_dim) {
   return decode_call_bytes(B, heads, kv_heads, head_dim, Reach{kMaxTokens, 0, 0});
 }
 
-hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
+namespace {
+
+// The sequences of `a`, cut as c says, in one launch and the join behind it.
+hipError_t launch(const AttendArgs& a, const Cut& c, void* workspace, hipStream_t s) {
   const int th = tiles_of_heads(a.heads, a.kv.kv_heads);
-  const Cut c = cut_of(a.B, most_tiles(reach_of(a)), th, a.kv.head_dim);
   SplitArgs sp{};
   sp.slots = c.slots;
   sp.min_tiles = min_tiles(a.kv.head_dim);
@@ -569,6 +571,27 @@ hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
   j.plan = sp.plan;
   j.max_pieces = static_cast<int>(c.max_slots);
   return launch_join(a, j, c.max_slots / a.B, s);
+}
+
+}  // namespace
+
+hipError_t launch_decode(const AttendArgs& a, void* workspace, hipStream_t s) {
+  const int th = tiles_of_heads(a.heads, a.kv.kv_heads);
+  const int64_t most = most_tiles(reach_of(a));
+  const Cut c = cut_of(a.B, most, th, a.kv.head_dim);
+  if (c.slots == 0 || a.B <= kSearch) return launch(a, c, workspace, s);
+  const int parts = (a.B + kSearch - 1) / kSearch, per = (a.B + parts - 1) / parts;
+  for (int b = 0; b < a.B; b += per) {
+    AttendArgs x = a;
+    x.B = x.rows = min(per, a.B - b);
+    x.q += b * a.q_stride;
+    x.out += b * a.out_stride;
+    x.tables += b * a.table_stride;
+    x.lens += b;
+    const hipError_t e = launch(x, cut_of(x.B, most, th, a.kv.head_dim), workspace, s);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace gxmoe

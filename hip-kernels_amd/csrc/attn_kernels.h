@@ -71,6 +71,11 @@ hipError_t launch_rope_append(const AppendArgs& a, hipStream_t s);
 hipError_t launch_join(const AttendArgs& a, const JoinArgs& j, int64_t mean, hipStream_t s);  // mean: pieces of a row
 constexpr int64_t kMaxTokens = 1 << 30;  // of a sequence
 
+// Every work-group finds its part among the lengths of all sequences of its launch,
+// in a time that grows with them.  Calls of more go in several launches (65536
+// sequences of 8 heads in one and in eight: decode 19.1 / 3.2 ms, prefill 50.9 / 8.3).
+constexpr int kSearch = 8192;
+
 // What a sequence of a call can hold and a query of it see, as the host knows it.
 struct Reach {
   int64_t tokens, window, first;  // window 0: all

@@ -770,25 +770,33 @@ hipError_t launch_prefill(const AttendArgs& a, void* workspace, hipStream_t s) {
   pa.part_o = static_cast<float*>(workspace);
   pa.part_ml = pa.part_o + parts * a.kv.head_dim;
   pa.plan = reinterpret_cast<int*>(pa.part_ml + parts * 4);
-  // sum of ceil(new tokens / per), at most one tile more for each sequence that has rows
-  const int64_t tiles = (static_cast<int64_t>(a.rows) + per - 1) / per + (a.B < a.rows ? a.B : a.rows);
-  const dim3 grid(static_cast<unsigned>(tiles * a.kv.kv_heads * pa.pieces));
+  AttendArgs x = a;  // kSearch of its sequences at a time
 #define GX_PREFILL(D_, E_, C_, G_) \
-  hipLaunchKernelGGL((prefill_kernel<D_, E_, C_, G_>), grid, dim3(256 * G_), 0, s, a, pa)
+  hipLaunchKernelGGL((prefill_kernel<D_, E_, C_, G_>), grid, dim3(256 * G_), 0, s, x, pa)
 #define GX_PREFILL_E(D_, C_, G_)               \
   do {                                         \
     if (a.kv.e4m3) GX_PREFILL(D_, true, C_, G_); \
     else GX_PREFILL(D_, false, C_, G_);        \
   } while (0)
-  if (a.kv.head_dim == 64 && cols == 2) GX_PREFILL_E(64, 2, 1);
-  else if (a.kv.head_dim == 64 && split.groups == 1) GX_PREFILL_E(64, 1, 1);
-  else if (a.kv.head_dim == 64) GX_PREFILL_E(64, 1, 2);
-  else if (split.groups == 1) GX_PREFILL_E(128, 1, 1);
-  else GX_PREFILL_E(128, 1, 2);
+  for (int b = 0; b < a.B; b += kSearch) {
+    x.B = min(kSearch, a.B - b);
+    x.offsets = a.offsets + b;
+    x.lens = a.lens + b;
+    x.tables = a.tables + b * a.table_stride;
+    // sum of ceil(new tokens / per), at most one tile more for each sequence that has rows
+    const int64_t tiles = (static_cast<int64_t>(a.rows) + per - 1) / per + min(x.B, a.rows);
+    const dim3 grid(static_cast<unsigned>(tiles * a.kv.kv_heads * pa.pieces));
+    if (a.kv.head_dim == 64 && cols == 2) GX_PREFILL_E(64, 2, 1);
+    else if (a.kv.head_dim == 64 && split.groups == 1) GX_PREFILL_E(64, 1, 1);
+    else if (a.kv.head_dim == 64) GX_PREFILL_E(64, 1, 2);
+    else if (split.groups == 1) GX_PREFILL_E(128, 1, 1);
+    else GX_PREFILL_E(128, 1, 2);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
 #undef GX_PREFILL_E
 #undef GX_PREFILL
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || pa.pieces == 1) return e;
+  if (pa.pieces == 1) return hipSuccess;
   JoinArgs j{};
   j.part_o = pa.part_o;
   j.part_ml = pa.part_ml;
