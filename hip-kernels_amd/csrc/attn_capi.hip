@@ -168,6 +168,10 @@ int gptoss_rope_table(const gptoss_rope_config* cfg, float* table, void* stream)
   if (cfg->scaling_factor != 1.0 && !(cfg->original_positions > 0.0 && cfg->beta_fast > 0.0 && cfg->beta_slow > 0.0))
     return set_error(GPTOSS_ERR_INVALID, "original_positions=%g, beta_fast=%g and beta_slow=%g must be positive",
                      cfg->original_positions, cfg->beta_fast, cfg->beta_slow);
+  // (no dim turns that often, and a ramp from none has no slope)
+  if (cfg->scaling_factor != 1.0 && !(cfg->original_positions / (cfg->beta_fast * 6.283185307179586) > 0.0))
+    return set_error(GPTOSS_ERR_INVALID, "beta_fast=%g is too large for original_positions=%g", cfg->beta_fast,
+                     cfg->original_positions);
   if (table == nullptr) return set_error(GPTOSS_ERR_INVALID, "null table");
   if (!aligned16(table)) return set_error(GPTOSS_ERR_INVALID, "table must be 16-byte aligned");
   RopeTableArgs a{};

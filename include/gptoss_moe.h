@@ -484,7 +484,7 @@ typedef struct gptoss_rope_config {
   int max_positions;
   double theta;        /* > 1 */
   double scaling_factor; /* >= 1 */
-  double original_positions, beta_fast, beta_slow; /* > 0; unused at factor 1 */
+  double original_positions, beta_fast, beta_slow; /* > 0, original_positions / beta_fast too; unused at factor 1 */
 } gptoss_rope_config;
 
 /* GPT-OSS: rotary_dim 64, 131072 positions, theta 150000, factor 32 over 4096,
