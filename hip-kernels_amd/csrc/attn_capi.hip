@@ -33,6 +33,19 @@ bool apart(const void* a, size_t na, const void* b, size_t nb) {
   return x + na <= y || y + nb <= x;
 }
 
+// Whether n bytes at p lie outside of what K's and V's pages span.
+bool clear_of(const KvPages& kv, const void* p, size_t n) {
+  typedef unsigned __int128 Wide;  // strides may be anything
+  const Wide last = Wide(kv.num_blocks - 1) * static_cast<uint64_t>(kv.sb) + Wide(kv.kv_heads - 1) * static_cast<uint64_t>(kv.sh) +
+                    ((Wide(1) << kv.bs_shift) - 1) * static_cast<uint64_t>(kv.st);
+  const Wide span = (last + kv.head_dim) * (kv.e4m3 ? 1 : 2), x = reinterpret_cast<uintptr_t>(p);
+  for (const void* pages : {kv.k, kv.v}) {
+    const Wide y = reinterpret_cast<uintptr_t>(pages);
+    if (x < y + span && y < x + n) return false;
+  }
+  return true;
+}
+
 constexpr int kMaxGroup = 128;  // query heads per kv head
 constexpr int64_t kMaxRowHeads = 1 << 26, kMaxSeqHeads = 1 << 22;  // rows and sequences of a call, times heads
 
@@ -120,6 +133,8 @@ int check_attend(AttendArgs* a, const gptoss_kv_cache* cache, const gptoss_atten
   if (rc != GPTOSS_OK) return rc;
   if (!apart(a->q, extent(rows, a->q_stride, cols), a->out, extent(rows, a->out_stride, cols)))
     return set_error(GPTOSS_ERR_INVALID, "out overlaps q");
+  if (!clear_of(a->kv, a->out, extent(rows, a->out_stride, cols)))
+    return set_error(GPTOSS_ERR_INVALID, "out overlaps the cache");
   if (a->tables == nullptr || a->lens == nullptr) return set_error(GPTOSS_ERR_INVALID, "null block_tables / seq_lens");
   if (a->max_blocks < 1 || a->table_stride < a->max_blocks)
     return set_error(GPTOSS_ERR_INVALID, "max_blocks=%d must be positive and at most table_stride=%lld", a->max_blocks,
@@ -212,6 +227,8 @@ int gptoss_rope_kv_append(const uint16_t* qkv, int64_t qkv_stride, const int32_t
   const bool in_place = q_out == qkv && q_stride == qkv_stride;
   if (!in_place && !apart(qkv, extent(T, qkv_stride, cols), q_out, extent(T, q_stride, q_cols)))
     return set_error(GPTOSS_ERR_INVALID, "q_out overlaps qkv without being its queries' place");
+  if (!clear_of(a.kv, qkv, extent(T, qkv_stride, cols)) || !clear_of(a.kv, q_out, extent(T, q_stride, q_cols)))
+    return set_error(GPTOSS_ERR_INVALID, "qkv or q_out overlaps the cache");
   a.qkv = qkv;
   a.qkv_stride = qkv_stride;
   a.positions = positions;

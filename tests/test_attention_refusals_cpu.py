@@ -27,3 +27,54 @@ def test_rope_ramp_without_a_beginning_refused(g, change):
     cfg.scaling_factor = 1.0  # unused then: what is refused is the table's alignment
     assert g.lib.gptoss_rope_table(ctypes.byref(cfg), A + 4, None) == g.GPTOSS_ERR_INVALID
     assert b"aligned" in g.lib.gptoss_last_error()
+
+
+def cache(g, **kw):
+    d = g.KvCacheDesc(64 * A, 80 * A, None, None, 0, 0, 0, g.GPTOSS_KV_BF16, 100, 16, 8, 64)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+SPAN = 100 * 16 * 8 * 64 * 2  # bytes of K, and of V
+
+
+def attend(g, desc, prefill=False, **kw):
+    a = dict(q=4 * A, q_stride=4096, off=7 * A, T=3, tables=8 * A, table_stride=10, max_blocks=10, lens=9 * A, B=3, H=64,
+             out=5 * A, out_stride=4096, ws=16 * A + 8, ws_bytes=0)
+    a.update(kw)
+    c = g.AttentionConfig(0.125, 0, 0, None)
+    head = (a["q"], a["q_stride"]) + ((a["off"], a["T"]) if prefill else ())
+    f = g.lib.gptoss_paged_attention_prefill if prefill else g.lib.gptoss_paged_attention_decode
+    return f(*head, ctypes.byref(desc), a["tables"], a["table_stride"], a["max_blocks"], a["lens"], a["B"], a["H"],
+             ctypes.byref(c), a["out"], a["out_stride"], a["ws"], a["ws_bytes"], None)
+
+
+def append(g, desc, **kw):
+    a = dict(qkv=4 * A, stride=5120, pos=8 * A, slots=9 * A, table=10 * A, rotary=64, positions=1000, pairs=0, T=7, H=64,
+             q=6 * A, q_stride=4096)
+    a.update(kw)
+    return g.lib.gptoss_rope_kv_append(a["qkv"], a["stride"], a["pos"], a["slots"], a["table"], a["rotary"], a["positions"],
+                                       a["pairs"], a["T"], a["H"], a["q"], a["q_stride"], ctypes.byref(desc), None)
+
+
+@pytest.mark.parametrize("at", [64 * A, 64 * A + SPAN - 16, 64 * A - 16, 80 * A + 4096, 80 * A - 2 * 8192 - 8192 + 16])
+def test_results_in_the_cache_refused(g, at):
+    for prefill in (False, True):
+        assert attend(g, cache(g), prefill, out=at) == g.GPTOSS_ERR_INVALID
+        assert g.lib.gptoss_last_error() == b"out overlaps the cache"
+    for kw in (dict(q=at), dict(qkv=at, q=at, q_stride=5120), dict(qkv=at, T=3)):
+        assert append(g, cache(g), **kw) == g.GPTOSS_ERR_INVALID
+        assert b"overlaps the cache" in g.lib.gptoss_last_error()
+
+
+def test_results_beside_the_cache(g):
+    """Right before and behind K and V (what is refused is the next argument); strides past any address do not wrap."""
+    for at in (64 * A - 3 * 8192, 64 * A + SPAN, 80 * A - 3 * 8192, 80 * A + SPAN):
+        for prefill in (False, True):
+            assert attend(g, cache(g), prefill, out=at, tables=None) == g.GPTOSS_ERR_INVALID
+            assert b"null block_tables" in g.lib.gptoss_last_error()
+    far = cache(g, num_blocks=1 << 20, block_stride=1 << 60, head_stride=1 << 40, token_stride=64)
+    for prefill in (False, True):
+        assert attend(g, far, prefill, out=128 * A) == g.GPTOSS_ERR_INVALID
+        assert g.lib.gptoss_last_error() == b"out overlaps the cache"
