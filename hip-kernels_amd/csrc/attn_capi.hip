@@ -33,6 +33,17 @@ bool apart(const void* a, size_t na, const void* b, size_t nb) {
   return x + na <= y || y + nb <= x;
 }
 
+// Whether no row of a is one of b's: their spans are apart, or the rows of one lie
+// between the other's, the same distance apart.
+bool rows_apart(const void* a, int64_t a_stride, int64_t a_cols, const void* b, int64_t b_stride, int64_t b_cols, int rows) {
+  if (apart(a, extent(rows, a_stride, a_cols), b, extent(rows, b_stride, b_cols))) return true;
+  if (a_stride != b_stride) return false;
+  const int64_t step = 2 * a_stride;
+  int64_t from = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a)) % step;
+  if (from < 0) from += step;  // where b's rows begin, of a step from a's rows on
+  return from >= 2 * a_cols && from + 2 * b_cols <= step;
+}
+
 // Whether n bytes at p lie outside of what K's and V's pages span.
 bool clear_of(const KvPages& kv, const void* p, size_t n) {
   typedef unsigned __int128 Wide;  // strides may be anything
@@ -131,7 +142,7 @@ int check_attend(AttendArgs* a, const gptoss_kv_cache* cache, const gptoss_atten
   rc = check_rows("q", a->q, a->q_stride, cols);
   if (rc == GPTOSS_OK) rc = check_rows("out", a->out, a->out_stride, cols);
   if (rc != GPTOSS_OK) return rc;
-  if (!apart(a->q, extent(rows, a->q_stride, cols), a->out, extent(rows, a->out_stride, cols)))
+  if (!rows_apart(a->q, a->q_stride, cols, a->out, a->out_stride, cols, rows))
     return set_error(GPTOSS_ERR_INVALID, "out overlaps q");
   if (!clear_of(a->kv, a->out, extent(rows, a->out_stride, cols)))
     return set_error(GPTOSS_ERR_INVALID, "out overlaps the cache");
@@ -225,7 +236,7 @@ int gptoss_rope_kv_append(const uint16_t* qkv, int64_t qkv_stride, const int32_t
     return set_error(GPTOSS_ERR_INVALID, "null positions / slots / rope_table");
   if (!aligned16(rope_table)) return set_error(GPTOSS_ERR_INVALID, "rope_table must be 16-byte aligned");
   const bool in_place = q_out == qkv && q_stride == qkv_stride;
-  if (!in_place && !apart(qkv, extent(T, qkv_stride, cols), q_out, extent(T, q_stride, q_cols)))
+  if (!in_place && !rows_apart(qkv, qkv_stride, cols, q_out, q_stride, q_cols, T))
     return set_error(GPTOSS_ERR_INVALID, "q_out overlaps qkv without being its queries' place");
   if (!clear_of(a.kv, qkv, extent(T, qkv_stride, cols)) || !clear_of(a.kv, q_out, extent(T, q_stride, q_cols)))
     return set_error(GPTOSS_ERR_INVALID, "qkv or q_out overlaps the cache");

@@ -508,7 +508,8 @@ int gptoss_rope_table(const gptoss_rope_config* cfg, float* table, void* stream)
  * key or value; one whose position is not in the table [0, max_positions)
  * writes nothing at all.  Slots of one call are distinct: of rows that share
  * one, any may be found there, in pieces.  q_out may be the queries' place in
- * qkv (same pointer and stride) and otherwise lies apart from qkv; both lie
+ * qkv (same pointer and stride) and otherwise lies apart from qkv (or its rows
+ * between qkv's, at the same stride); both lie
  * outside of what the cache's pages span.
  * qkv, q_out and rope_table are 16-byte aligned; rotary_dim <= head_dim;
  * num_tokens is at most 2^25. */
@@ -540,7 +541,8 @@ typedef struct gptoss_attention_config {
  * Decode (the reference's: paged_attention.cu:112-717): one new token per
  * sequence, at position seq_lens[b] - 1; q and out are [num_seqs][num_heads *
  * head_dim] bf16, rows q_stride and out_stride elements apart (multiples of
- * 8), apart from each other, 16-byte aligned; out lies outside of what the
+ * 8), apart from each other (rows of one may lie between the other's, at the
+ * same stride), 16-byte aligned; out lies outside of what the
  * cache's pages span.  num_heads is a multiple of the
  * kv heads, at most 128 per kv head.  Scores and sums are fp32; the softmax's
  * weights meet the values with 16 significant bits here and rounded to bf16 in

@@ -78,3 +78,25 @@ def test_results_beside_the_cache(g):
     for prefill in (False, True):
         assert attend(g, far, prefill, out=128 * A) == g.GPTOSS_ERR_INVALID
         assert g.lib.gptoss_last_error() == b"out overlaps the cache"
+
+
+@pytest.mark.parametrize("at,fits", [(4096, True), (4096 + 96, True), (-4096 - 96, True), (4096 - 8, False), (4096 + 104, False),
+                                     (8, False), (-8, False), (2 * 8288 - 8, False), (2 * 8288 + 4096, True), (-4096 - 104, False)])
+def test_rows_between_rows(g, at, fits):
+    """q and out as columns of one buffer: rows of either lie between the other's (what is refused then is the next
+    argument).  `at`: elements from q to out; a buffer's row has 8288, each of the two 4096."""
+    for prefill in (False, True):
+        kw = dict(q=20 * A, q_stride=8288, out=20 * A + 2 * at, out_stride=8288, B=3, T=3, tables=None)
+        assert attend(g, cache(g), prefill, **kw) == g.GPTOSS_ERR_INVALID
+        assert (b"null block_tables" if fits else b"out overlaps q") in g.lib.gptoss_last_error()
+
+
+@pytest.mark.parametrize("at,fits", [(5120, True), (5120 + 128, True), (-4096, True), (-4096 - 128, True), (5112, False),
+                                     (5120 + 136, False), (8, False), (-8, False)])
+def test_queries_between_rows(g, at, fits):
+    kw = dict(qkv=20 * A, stride=9344, q=20 * A + 2 * at, q_stride=9344)
+    if fits:  # accepted as far as the cache, which is made to hold it
+        d = cache(g, k=20 * A)
+        assert append(g, d, **kw) == g.GPTOSS_ERR_INVALID and b"overlaps the cache" in g.lib.gptoss_last_error()
+    else:
+        assert append(g, cache(g), **kw) == g.GPTOSS_ERR_INVALID and b"overlaps qkv" in g.lib.gptoss_last_error()
