@@ -974,7 +974,8 @@ class KVCache:
     [num_blocks, kv_heads, block_size, head_dim], bfloat16 or float8_e4m3fn with
     the last dim contiguous and the same strides, so a permuted view covers
     token-major pages and k = slab[:, 0], v = slab[:, 1] an interleaved slab.
-    8-bit caches stand for code * scale, scales float32 [kv_heads], positive (None: 1)."""
+    8-bit caches stand for code * scale, scales float32 [kv_heads], positive (None: 1).
+    Fixed once made: other tensors need another KVCache."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None):
@@ -1004,11 +1005,16 @@ class KVCache:
             if k.dtype == torch.bfloat16:
                 _bad(f"{name}: a bfloat16 cache has no scales")
             _vector(name, t, k.device, heads, torch.float32)
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device, self.num_blocks, self.kv_heads, self.block_size, self.head_dim = k.device, blocks, heads, size, dim
-        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), _ptr(k_scale), _ptr(v_scale), stride[0], stride[1], stride[2],
-                                GPTOSS_KV_BF16 if k.dtype == torch.bfloat16 else GPTOSS_KV_E4M3, blocks, size, heads, dim)
-        self._desc = ctypes.addressof(self.desc)
+        desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), _ptr(k_scale), _ptr(v_scale), stride[0], stride[1], stride[2],
+                           GPTOSS_KV_BF16 if k.dtype == torch.bfloat16 else GPTOSS_KV_E4M3, blocks, size, heads, dim)
+        vars(self).update(k=k, v=v, k_scale=k_scale, v_scale=v_scale, device=k.device, num_blocks=blocks, kv_heads=heads,
+                          block_size=size, head_dim=dim, desc=desc, _desc=ctypes.addressof(desc))
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"KVCache.{name} is fixed: calls use the tensors it was made with")
+
+    def __delattr__(self, name):
+        raise AttributeError(f"KVCache.{name} is fixed: calls use the tensors it was made with")
 
 
 def rope_kv_append(qkv, positions, slots, table, cache: KVCache, num_heads: int, interleaved: bool = False, q_out=None,

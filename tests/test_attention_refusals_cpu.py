@@ -100,3 +100,23 @@ def test_queries_between_rows(g, at, fits):
         assert append(g, d, **kw) == g.GPTOSS_ERR_INVALID and b"overlaps the cache" in g.lib.gptoss_last_error()
     else:
         assert append(g, cache(g), **kw) == g.GPTOSS_ERR_INVALID and b"overlaps qkv" in g.lib.gptoss_last_error()
+
+
+# ---------------------------------------------------------------------------
+# the binding
+# ---------------------------------------------------------------------------
+def pages(blocks=6):
+    import torch
+    return torch.zeros((blocks, 8, 16, 64), dtype=torch.bfloat16)
+
+
+def test_kv_cache_is_fixed(g):
+    """Another tensor would not be what calls use: their descriptor holds the addresses of the first."""
+    k, v = pages(), pages()
+    c = g.KVCache(k, v)
+    for name, x in (("k", pages(9)), ("v", pages(9)), ("k_scale", None), ("num_blocks", 9), ("desc", None), ("other", 1)):
+        with pytest.raises(AttributeError, match="fixed"):
+            setattr(c, name, x)
+    with pytest.raises(AttributeError, match="fixed"):
+        del c.k
+    assert c.k is k and c.v is v and c.desc.k == k.data_ptr() and c.desc.num_blocks == c.num_blocks == 6
