@@ -1051,9 +1051,14 @@ def rope_kv_append(qkv, positions, slots, table, cache: KVCache, num_heads: int,
 
 
 def paged_attention_workspace_bytes(num_tokens: int, num_seqs: int, num_heads: int, cache: KVCache) -> int:
-    """Bytes of workspace that suffice for any call on up to num_tokens rows of up to num_seqs sequences."""
+    """Bytes of workspace that suffice for any call on up to num_tokens rows of up to num_seqs sequences; a decode call
+    has a row for each sequence, so a caller that only decodes gives num_tokens = num_seqs."""
+    if max(num_tokens, num_seqs, num_heads) > _INT_MAX:
+        _bad(f"num_tokens={num_tokens}, num_seqs={num_seqs} and num_heads={num_heads} must be below 2^31")
     return _lib.gptoss_paged_attention_workspace_bytes(num_tokens, num_seqs, num_heads, cache.kv_heads, cache.head_dim)
 
+
+_INT_MAX = 2 ** 31 - 1  # of the library's int arguments: ctypes would cut larger numbers
 
 # (rows, 0 for decode; sequences; heads; kv heads; head_dim; tokens of a table; window; first tokens)
 _call_bytes = functools.lru_cache(maxsize=4096)(_lib.gptoss_paged_attention_call_bytes)
@@ -1078,6 +1083,8 @@ def _attend(q, offsets, cache, block_tables, seq_lens, scale, window, first_toke
     if blocks > 1 and one != 1:
         _bad("block_tables must have contiguous rows")
     _vector("seq_lens", seq_lens, dev, B, torch.int32)
+    if not (0 <= window <= _INT_MAX and 0 <= first_tokens <= _INT_MAX):
+        _bad(f"window={window} and first_tokens={first_tokens} must not be negative and below 2^31")
     if sinks is not None:
         _vector("sinks", sinks, dev, H, torch.bfloat16)
         sinks = sinks.data_ptr()

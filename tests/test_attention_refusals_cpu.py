@@ -120,3 +120,21 @@ def test_kv_cache_is_fixed(g):
     with pytest.raises(AttributeError, match="fixed"):
         del c.k
     assert c.k is k and c.v is v and c.desc.k == k.data_ptr() and c.desc.num_blocks == c.num_blocks == 6
+
+
+def test_numbers_past_32_bits_refused(g):
+    """A window of 2^32 + 128 is not one of 128."""
+    import torch
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    c, q = g.KVCache(pages(), pages()), torch.zeros((3, 4096), dtype=torch.bfloat16)
+    for bad in (2 ** 32 + 128, 2 ** 31, -1, -2 ** 32):
+        for kw in (dict(window=bad), dict(window=4, first_tokens=bad)):
+            with pytest.raises(ValueError, match="2\\^31"):
+                g.paged_attention_decode(q, c, i32(3, 5), i32(3), **kw)
+            with pytest.raises(ValueError, match="2\\^31"):
+                g.paged_attention_prefill(q, i32(4), c, i32(3, 5), i32(3), **kw)
+    with pytest.raises(ValueError, match="GPU is needed"):
+        g.paged_attention_decode(q, c, i32(3, 5), i32(3), window=2 ** 31 - 1, first_tokens=2 ** 31 - 1)
+    for bad in ((2 ** 32 + 5, 3, 64), (5, 2 ** 32 + 3, 64), (5, 3, 2 ** 32 + 64)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            g.paged_attention_workspace_bytes(*bad, c)
