@@ -591,8 +591,8 @@ class PyInferenceEngine {
   }
 
   // generate / generate_batch (bindings.cpp:100-185): the same argument
-  // checks, then RuntimeError -- attention, sampling and the tokenizer are not
-  // part of this build.
+  // checks, then RuntimeError -- the engine loads the MoE block's weights only, and
+  // sampling and the tokenizer are not part of this build.
   std::vector<int32_t> generate(const std::vector<int32_t>& prompt, int max_tokens, float temperature, float top_p) {
     if (prompt.empty()) throw py::value_error("prompt_tokens must not be empty");
     if (max_tokens <= 0) throw py::value_error("max_tokens must be positive");
@@ -614,8 +614,9 @@ class PyInferenceEngine {
 
  private:
   std::string not_built() const {
-    return std::string("Generation failed: this gptoss build runs the MoE block only (attention, sampling and the "
-                       "tokenizer are not part of it); use decode_step() for the MoE half of a decode step") +
+    return std::string("Generation failed: this engine runs the MoE block only (the weights of attention, sampling and "
+                       "the tokenizer are not part of it); use decode_step() for the MoE half of a decode step and "
+                       "gptoss_moe's rope_kv_append and paged_attention_decode for the attention of the other half") +
            (stack_ ? "" : " [InferenceEngine] Not initialized");
   }
   void shutdown_impl() {
@@ -689,8 +690,8 @@ PYBIND11_MODULE(gptoss, m) {
            "Raises:\n    RuntimeError: if the weights cannot be loaded.")
       .def("generate", &PyInferenceEngine::generate, py::arg("prompt_tokens"), py::arg("max_tokens") = 512,
            py::arg("temperature") = 0.8f, py::arg("top_p") = 0.95f,
-           "Checks its arguments (ValueError), then raises RuntimeError: generation needs attention and sampling, "
-           "which this build does not contain.")
+           "Checks its arguments (ValueError), then raises RuntimeError: generation needs the attention's weights and "
+           "sampling, which the engine does not have (attention over a paged cache is in gptoss_moe).")
       .def("generate_batch", &PyInferenceEngine::generate_batch, py::arg("prompts"), py::arg("max_tokens") = 512,
            py::arg("temperature") = 0.0f, py::arg("top_p") = 1.0f,
            "Checks its arguments (ValueError), then raises RuntimeError (see generate).")

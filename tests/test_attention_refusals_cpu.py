@@ -138,3 +138,12 @@ def test_numbers_past_32_bits_refused(g):
     for bad in ((2 ** 32 + 5, 3, 64), (5, 2 ** 32 + 3, 64), (5, 3, 2 ** 32 + 64)):
         with pytest.raises(ValueError, match="2\\^31"):
             g.paged_attention_workspace_bytes(*bad, c)
+
+
+def test_engine_names_the_attention_there_is():
+    """The engine's refusal to generate points to the attention operators instead of denying them."""
+    import torch  # noqa: F401  (first: the library binds to torch's HIP runtime)
+    import gptoss
+    with pytest.raises(RuntimeError, match="gptoss_moe's rope_kv_append and paged_attention_decode"):
+        gptoss.InferenceEngine().generate([1, 2, 3])
+    assert "does not contain" not in gptoss.InferenceEngine.generate.__doc__
