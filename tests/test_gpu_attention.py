@@ -257,7 +257,7 @@ def test_values_reach_only_who_sees_them(gpu, shape, e4m3, window):
     assert torch.equal(got[~bad], want[~bad])
 
 
-# few rows over many tokens: 1 and 2 pieces of the tokens, each shared by two groups of waves
+# few rows over many tokens: 1, 3 and 4 pieces of the tokens, each shared by two groups of waves
 GQA4 = (32, 8, 128, 32)
 FEW = [(GPT, 270), (GPT, 90), (GQA4, 540), (GQA4, 180), ((34, 2, 64, 64), 500), ((9, 3, 128, 16), 2700)]
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import attn_ref as ref
-from test_gpu_attention import BF16, gen_of, randn, say
+from test_gpu_attention import BF16, GPT, GQA4, Case, gen_of, randn, say
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +72,38 @@ def test_time_grows_with_the_sequences(gpu):
             say(name, B, f"{best:.2f} ms")
     for name in ("decode", "prefill"):
         assert took[name, 65536] < 24 * took[name, 8192]
+
+
+# tables as a serving engine has them, of the longest context that it allows
+WIDE = [(GPT, [680], [680]), (GPT, [512], [512]), (GPT, [1120, 900, 500, 300], [120, 110, 60, 40]),
+        (GPT, [1028, 900, 800, 700, 500, 300, 200, 128], [128, 100, 60, 40, 100, 20, 30, 28]), (GQA4, [680], [680]),
+        (GPT, [1], [1]), (GPT, [17, 0, 2], [5, 0, 2]), (GQA4, [100, 3000], [1, 1]), ((6, 6, 128, 16), [300, 20], [31, 20])]
+
+
+@pytest.mark.parametrize("shape,lens,new", WIDE)
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_wide_tables(gpu, shape, lens, new, e4m3):
+    """Tables of 131072 tokens over short sequences."""
+    say("wide tables", shape, lens, new, e4m3)
+    c = Case(gpu, 83, lens, *shape, e4m3=e4m3, width=131072 // shape[3])
+    sinks = randn(c.gen, shape[0])
+    c.check_prefill(new, sinks=sinks)
+    c.check_prefill(new, window=100, first=3)
+    c.check_decode(sinks=sinks)
+    c.check_decode(window=100, first=3)
+
+
+@pytest.mark.parametrize("B,L", [(1, 1000), (1, 500), (64, 1000), (40, 30)])
+def test_wide_tables_of_single_tokens(gpu, B, L):
+    c = Case(gpu, 84, [L - 3 * b for b in range(min(B, L // 3))], *GPT, width=131072 // 16)
+    c.check_decode(sinks=randn(c.gen, 64))
+
+
+@pytest.mark.parametrize("shape,new", [(GPT, 210), (GQA4, 340)])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_prefill_two_groups_in_two_pieces(gpu, shape, new, e4m3):
+    say("two groups in two pieces", shape, new, e4m3)
+    c = Case(gpu, 85, [4090], *shape, e4m3=e4m3)
+    c.tables[0, 20] = -1
+    c.check_prefill([new], sinks=randn(c.gen, shape[0], scale=2.0))
+    c.check_prefill([new], window=3500, first=70)
