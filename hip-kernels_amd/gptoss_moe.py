@@ -1083,7 +1083,7 @@ def _attend(q, offsets, cache, block_tables, seq_lens, scale, window, first_toke
     if blocks > 1 and one != 1:
         _bad("block_tables must have contiguous rows")
     _vector("seq_lens", seq_lens, dev, B, torch.int32)
-    if not (0 <= window <= _INT_MAX and 0 <= first_tokens <= _INT_MAX):
+    if (window | first_tokens) >> 31:  # negative, or past _INT_MAX
         _bad(f"window={window} and first_tokens={first_tokens} must not be negative and below 2^31")
     if sinks is not None:
         _vector("sinks", sinks, dev, H, torch.bfloat16)
