@@ -7,7 +7,8 @@
 //   M = max(m1, m2), l = l1 2^(m1 - M) + l2 2^(m2 - M), O likewise,
 // so tokens are split over tiles, waves and work-groups in any way.
 //
-// Bound by reading K and V once: 8 heads on a kv head take 16 flops per byte.
+// Bound by reading K and V once: 8 heads on a kv head take 8 flops per byte in
+// bf16, 16 in e4m3.
 // Everything else is laid out so that nothing but the loads is slow: K and V go
 // from memory to registers, whole 128-byte rows, and from there into the
 // matrix cores without passing through LDS.
@@ -23,9 +24,12 @@
 // then weights up to 256 lose nothing in bf16 or fp32, and the tile needs no
 // exchange between lanes.  The weights meet the values as two bf16 each.
 //
-// With 64 heads on 8 of 64 dims in bf16: one sequence of 131072 54 us, 4.95 TB/s
-// (a kernel that only reads the same, 44 us); 64 of 4000 5.5 TB/s; 64 of very
-// different lengths up to 8192 28.4 us, 3.6 TB/s, of which the join takes 4.
+// With 64 heads on 8 of 64 dims in bf16, joins included: one sequence of 131072 51
+// us, 5.3 TB/s (a kernel that only reads the same, 44 us and 6.1); four of them 6.3
+// TB/s; 64 of 4000 96 us, 5.5 TB/s; 64 of very different lengths up to 8192 27.4 us,
+// 3.7 TB/s, of which the join takes 4.  With 32 heads on 8 of 128 one of 131072 88.6
+// us, 6.1 TB/s; with 64 dims in e4m3 31.2 us, 4.3 TB/s.
+// (Pairs of times beside the choices below are of one run each, and may be older.)
 #include "attn_device.h"
 
 namespace gxmoe {
@@ -482,10 +486,12 @@ int min_tiles(int head_dim) { return head_dim == 64 ? 6 : 4; }
 constexpr int kFull = 256;
 // Where the table or the window holds no more than kWholeTiles (1024 tokens), or
 // with 128 dims and few work-groups half of that, the call is one launch of a piece
-// to each sequence (cut or whole: 16 sequences of 1000 16.2 / 14.1 us, 8 of 1000 13.7
-// / 11.8, 8 ragged of up to 1000 10.5 / 11.0, 8 with a window of 512 10 / 8, one of
-// 500 9.3 / 7.5; with 128 dims 4 of 900 12 / 16.5, 8 of 500 12.3 / 11.3; one of 1000
-// 9.4 / 10.1 in a graph, 13.1 / 10.7 where each launch is the host's).
+// to each sequence.  us cut (where the table would hold more) and whole, in a graph:
+//   64 dims: one of 1000 10.7 / 9.6, of 500 9.9 / 7.0; 64 of 1000 28.6 / 25.9; 16 of
+//   1000 16.2 / 14.1, 8 of 1000 13.7 / 11.8, 8 ragged of up to 1000 10.5 / 11.0, 8 with
+//   a window of 512 10 / 8; one of 1000 launched by the host 13.8 / 9.5
+//   128 dims: 4 of 900 12 / 16.5; 8 of 500 10.5 / 12.4, launched by the host 13.7 /
+//   12.4
 constexpr int kMany = 128;
 
 struct Cut {

@@ -23,10 +23,11 @@
 //
 // Bound by the matrix cores with the vector and LDS work beside them, all 40 to 50 %
 // busy, and for large calls by power (2.09 GHz then): a prompt of 8192 with 64
-// heads of 64 takes 567 us, 970 TFLOP/s, where a matrix product of 8192^3 reaches
-// 1250; 512 tokens over 16000 in e4m3 with 32 heads of 128 153 us, 890 TFLOP/s.  A
-// short window is bound by the queries and results instead: 8192 tokens with a
-// window of 128 60 us, of which these take 29.
+// heads of 64 takes 569 us, 966 TFLOP/s, where a matrix product of 8192^3 reaches
+// 1250; 512 tokens over 16000 in e4m3 with 32 heads of 128 148 us, 923 TFLOP/s.  A
+// short window is bound by the queries and results instead: a prompt of 8192 with a
+// window of 128 64 us, of which these take 29.
+// (Pairs of times beside the choices below are of one run each, and may be older.)
 #include <type_traits>
 
 #include "attn_device.h"

@@ -546,17 +546,26 @@ typedef struct gptoss_attention_config {
  * cache's pages span.  num_heads is a multiple of the
  * kv heads, at most 128 per kv head.  Scores and sums are fp32; the softmax's
  * weights meet the values with 16 significant bits here and rounded to bf16 in
- * the prefill call.
+ * the prefill call; one below 2^-126 of the largest is 0.  Values are summed
+ * before the division, weights reaching 2^12: bf16 values whose magnitude times
+ * the number of tokens is past 2^115 may give infinities.
  * workspace: gptoss_paged_attention_workspace_bytes bytes, 16-byte aligned,
  * that no call running at the same time uses (two graphs that may overlap need
  * two); nothing is kept in it between calls.  The bytes for num_tokens rows and
- * num_seqs sequences are enough for calls of fewer, whatever their lengths.
+ * num_seqs sequences are enough for calls of fewer, whatever their lengths (rows
+ * of any call: a decode call has num_seqs of them, and 0 rows need 0 bytes).
  * What one call needs is less, and 0 where nothing is split (workspace may be NULL
  * then): gptoss_paged_attention_call_bytes, with max_tokens = max_blocks *
  * block_size and num_tokens = 0 for decode.
+ * The host knows of the lengths only that they fit into max_blocks pages, and
+ * cuts sequences into pieces (a second launch joins these) where that many tokens
+ * would want it.  Tables no wider than the longest sequence needs are faster for
+ * short ones: one token over 1000 9.6 us, with a table of 131072 10.7; a prompt of
+ * 680 17 and 27.
  * Limits of a call (GPTOSS_ERR_UNSUPPORTED): num_tokens * num_heads 2^26, num_seqs
  * * num_heads 2^22, max_blocks * block_size 2^30, num_seqs * max_blocks *
- * block_size 2^35, token_stride 2^24. */
+ * block_size 2^35, token_stride 2^24.  More than 8192 sequences go in several
+ * launches. */
 size_t gptoss_paged_attention_workspace_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads,
                                               int head_dim);
 size_t gptoss_paged_attention_call_bytes(int num_tokens, int num_seqs, int num_heads, int num_kv_heads, int head_dim,

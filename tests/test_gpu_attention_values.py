@@ -111,3 +111,15 @@ def test_values_of_far_tiles_reach_only_who_sees_them(gpu, shape, e4m3, window, 
     got = call()
     assert (~got[bad].isfinite()).all()
     assert torch.equal(got[~bad], want[~bad])
+
+
+@pytest.mark.parametrize("shape", [GPT, GQA4])
+@pytest.mark.parametrize("lens", [[40, 500], [9000]])
+def test_values_up_to_the_limit(gpu, shape, lens):
+    """Values times tokens up to 2^115 give no infinities on the way: 4.5 * 1.5 sigma * 2^98 * 9000 is below it."""
+    c = Case(gpu, 75, lens, *shape)
+    for b, n in enumerate(lens):  # NaN past the ends stays NaN
+        c.pages[1][c.tables[b, : (n + shape[3] - 1) // shape[3]].long()] *= 2.0 ** 98
+    c.check_decode(sinks=randn(c.gen, shape[0]))
+    c.check_prefill([min(n, 70) for n in lens])
+    c.check_prefill([min(n, 5) for n in lens], window=200, first=10)
