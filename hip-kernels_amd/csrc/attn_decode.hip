@@ -370,9 +370,10 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
     for (int c = 0; c < 8; ++c) w[c] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c >> 2][c & 3], scale, -base));
     l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
     // The weights as two bf16 each, cut off and what that leaves: 16 bits of them
-    // count, for a product that the loads hide.  The second is kept above 0 where the
-    // weight is: 0 times an infinite value would be NaN.  A weight of 0, one below
-    // 2^-126, stays 0: a large value of such a token counts for nothing.
+    // count, for a product that the loads hide.  The second is not 0 where the weight
+    // is not, or 0 times an infinite value would be NaN: it is at least 2^-17 of the
+    // weight, which is less than these bits, and bf16's smallest number.  A weight of
+    // 0, one below 2^-126, stays 0: a large value of such a token counts for nothing.
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -380,7 +381,8 @@ __global__ __launch_bounds__(64 * W, 2) void decode_kernel(AttendArgs a, SplitAr
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float x = w[2 * c + e];
-        rest[e] = __builtin_fmaxf(x - __uint_as_float(__float_as_uint(x) & 0xffff0000u), __builtin_fminf(x, 0x1p-126f));
+        rest[e] = __builtin_fmaxf(x - __uint_as_float(__float_as_uint(x) & 0xffff0000u),
+                                 __builtin_fmaxf(x * 0x1p-17f, __builtin_fminf(x, 0x1p-133f)));
       }
       hi[c] = __builtin_amdgcn_perm(__float_as_uint(w[2 * c + 1]), __float_as_uint(w[2 * c]), 0x07060302u);
       lo[c] = pack_bf16x2(rest[0], rest[1]);

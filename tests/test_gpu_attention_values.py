@@ -123,3 +123,38 @@ def test_values_up_to_the_limit(gpu, shape, lens):
     c.check_decode(sinks=randn(c.gen, shape[0]))
     c.check_prefill([min(n, 70) for n in lens])
     c.check_prefill([min(n, 5) for n in lens], window=200, first=10)
+
+
+@pytest.mark.parametrize("shape", [GPT, GQA4])
+@pytest.mark.parametrize("n", [2, 300, 3000])
+def test_large_values_of_small_weights(gpu, shape, n):
+    """The largest values where their weights are the smallest powers of two: as precise as any.  With a scale of ln 2 a
+    key of -g in one dim of a query of ones is a weight of 2^-g; the other tokens but one have none at all."""
+    H, Hk, D, bs = shape
+    gaps = [90, 100, 110, 116, 118, 120, 122, 124, 125]
+    c = Case(gpu, 76, [n] * len(gaps), *shape)
+    for b, gap in enumerate(gaps):
+        for t in range(n):
+            page = c.tables[b, t // bs].long()
+            c.pages[0][page, :, t % bs] = -4.0
+            if t in (0, n // 2):
+                c.pages[0][page, :, t % bs] = 0.0
+        page = c.tables[b, n // 2 // bs].long()
+        c.pages[0][page, :, n // 2 % bs, 5] = -float(gap)
+        c.pages[1][page, :, n // 2 % bs] = 3.25e38
+    q = torch.ones((len(gaps), H * D), dtype=BF16, device="cuda")
+    want, tol = c.want(q, [1] * len(gaps), scale=0.6931471805599453)
+    off = torch.arange(len(gaps) + 1, dtype=torch.int32, device="cuda")
+    for name, got in (("decode", gpu.paged_attention_decode(q, c.cache, c.tables, c.seq_lens, scale=0.6931471805599453)),
+                      ("prefill", gpu.paged_attention_prefill(q, off, c.cache, c.tables, c.seq_lens, scale=0.6931471805599453))):
+        bad = ref.within(got, want, tol)
+        assert bad is None, (name, bad)
+    # an infinite value is infinite with all of these weights
+    for b, gap in enumerate(gaps):
+        c.pages[1][c.tables[b, n // 2 // bs].long(), :, n // 2 % bs, 7] = float("inf")
+    for name, call in (("decode", lambda: gpu.paged_attention_decode(q, c.cache, c.tables, c.seq_lens, scale=0.6931471805599453)),
+                       ("prefill", lambda: gpu.paged_attention_prefill(q, off, c.cache, c.tables, c.seq_lens,
+                                                                       scale=0.6931471805599453))):
+        got = call().view(len(gaps), H, D)
+        say(name, [(gap, got[b, 0, 7].item()) for b, gap in enumerate(gaps)])
+        assert (got[..., 7] == float("inf")).all() and got[..., :7].isfinite().all() and got[..., 8:].isfinite().all()
