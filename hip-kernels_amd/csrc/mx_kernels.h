@@ -1,0 +1,62 @@
+// mx_kernels.h -- launchers of the expert selection and of the MXFP4 operators (internal).
+//
+// MXFP4 here is row-major: a matrix of [rows][K] values is packed [rows][K / 2]
+// (low nibble = even k) and scales [rows][K / 32], value = e2m1 * 2^(scale - 127),
+// a scale byte of 255 is NaN.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace gxmoe {
+
+constexpr int kSelectMaxExperts = 1024;
+constexpr int kSelectMaxTopK = 32;
+constexpr int kSelectMaxGroups = 64;
+
+struct SelectArgs {
+  const void* logits;  // [T] rows of E, `stride` elements apart
+  int64_t stride;
+  const float* bias;   // [E] or null
+  int32_t* idx;        // [T][k]
+  float* w;            // [T][k]
+  int T, E, k;
+  int groups, top_groups, group_rank;
+  bool fp32, sigmoid, renormalize;
+  float scale;
+};
+hipError_t launch_select_experts(const SelectArgs& a, hipStream_t s);
+
+// x: rows of K bf16 or fp32 values, `stride` elements apart.
+hipError_t launch_mx_quantize(const void* x, int64_t stride, bool fp32, int rows, int K, uint8_t* packed, uint8_t* scales,
+                              hipStream_t s);
+hipError_t launch_mx_dequantize(const uint8_t* packed, const uint8_t* scales, int rows, int K, void* out, int64_t stride,
+                                bool fp32, hipStream_t s);
+
+constexpr int kMxMaxExperts = 1024;
+
+// y[p][n] = sum_k a[row(p)][k] * w_e[n][k] + bias[e][n] for the rows p of expert
+// e, [offsets[e], offsets[e + 1]); one expert of all rows without offsets.
+struct MxProductArgs {
+  const uint8_t* a;     // packed, [a_rows][K / 2]
+  const uint8_t* as;    // scales, [a_rows][K / 32]
+  const int32_t* row_index;  // [rows] or null: row(p) = p
+  const int32_t* offsets;    // [E + 1] or null
+  int a_rows, rows, E;
+  const uint8_t* w;     // [E][N][K / 2]
+  const uint8_t* ws;    // [E][N][K / 32]
+  const uint16_t* bias; // [E][N] or null
+  int N, K;
+  bool swiglu;
+  float alpha, limit;
+  // One of: values (bf16, or fp32), rows `stride` elements apart; or MXFP4.
+  void* out;
+  int64_t stride;
+  bool out_fp32;
+  uint8_t* out_packed;
+  uint8_t* out_scales;
+};
+hipError_t launch_mx_product(const MxProductArgs& a, hipStream_t s);
+
+}  // namespace gxmoe

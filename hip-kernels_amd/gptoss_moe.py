@@ -3,8 +3,10 @@
 Mirrors the reference's MoE operator interface (src/model/moe_layer.cu:
 1556-1615: moe_layer_create / init / forward / forward_prenormed /
 get_ffn_norm_weight / destroy) and its kernel launchers, over the C ABI
-declared in include/gptoss_moe.h; and attention over a paged key-value cache
-(KVCache, rope_kv_append, paged_attention_decode, paged_attention_prefill).  Device memory is held in torch tensors
+declared in include/gptoss_moe.h; attention over a paged key-value cache
+(KVCache, rope_kv_append, paged_attention_decode, paged_attention_prefill); routing by scores, bias and groups
+(select_experts); and MXFP4 matrices (MXFP4Matrix, mxfp4_quantize, mxfp4_dequantize, mxfp4_matmul,
+grouped_mxfp4_matmul).  Device memory is held in torch tensors
 (plumbing only); every computation runs in the HIP library, and importing
 this module without the built library raises immediately.
 
@@ -103,6 +105,16 @@ class AttentionConfig(ctypes.Structure):
     _fields_ = [("scale", _F), ("window", _I), ("first_tokens", _I), ("sinks", _P)]
 
 
+class RoutingConfig(ctypes.Structure):
+    _fields_ = [("score", _I), ("top_k", _I), ("num_groups", _I), ("top_groups", _I), ("group_rank", _I),
+                ("renormalize", _I), ("scale", _F)]
+
+
+class Mxfp4Result(ctypes.Structure):
+    _fields_ = [("swiglu", _I), ("alpha", _F), ("limit", _F), ("out_fp32", _I), ("out", _P),
+                ("out_stride", ctypes.c_int64), ("out_packed", _P), ("out_scales", _P)]
+
+
 def _sig(name, args, res=_I):
     f = getattr(_lib, name)
     f.argtypes = args
@@ -168,6 +180,11 @@ _sig("gptoss_paged_attention_workspace_bytes", [_I, _I, _I, _I, _I], _SZ)
 _sig("gptoss_paged_attention_call_bytes", [_I, _I, _I, _I, _I, ctypes.c_int64, _I, _I], _SZ)
 _sig("gptoss_paged_attention_decode", [_P, _L, _P, _P, _L, _I, _P, _I, _I, _P, _P, _L, _P, _SZ, _P])
 _sig("gptoss_paged_attention_prefill", [_P, _L, _P, _I, _P, _P, _L, _I, _P, _I, _I, _P, _P, _L, _P, _SZ, _P])
+_sig("gptoss_moe_select_experts", [_P, _L, _I, _P, _I, _I, _P, _P, _P, _P])
+_sig("gptoss_mxfp4_quantize", [_P, _L, _I, _I, _I, _P, _P, _P])
+_sig("gptoss_mxfp4_dequantize", [_P, _P, _I, _I, _P, _L, _I, _P])
+_sig("gptoss_mxfp4_matmul", [_P, _P, _I, _P, _P, _P, _I, _I, _P, _P])
+_sig("gptoss_moe_grouped_mxfp4_matmul", [_P, _P, _I, _P, _P, _I, _I, _P, _P, _P, _I, _I, _P, _P])
 
 lib = _lib
 
@@ -924,7 +941,7 @@ def _on_device(name: str, t, device, dtype=None, dim: int | None = None) -> None
     if dim is not None and t.dim() != dim:
         _bad(f"{name} must be {dim}-D, got shape {tuple(t.shape)}")
     if t.device != device:
-        _bad(f"{name} is on {t.device}, the cache is on {device}")
+        _bad(f"{name} is on {t.device}, expected {device}")
 
 
 def _row_tensor(name: str, t, device, cols: int) -> int:
@@ -1144,3 +1161,264 @@ def paged_attention_prefill(q, query_offsets, cache: KVCache, block_tables, seq_
         _bad("query_offsets must be a tensor")
     return _attend(q, query_offsets, cache, block_tables, seq_lens, scale, window, first_tokens, sinks, out, workspace,
                    stream)
+
+
+# ---------------------------------------------------------------------------
+# routing by scores, bias and groups
+# ---------------------------------------------------------------------------
+GPTOSS_SCORE_SOFTMAX = 0
+GPTOSS_SCORE_SIGMOID = 1
+_SCORES = {"softmax": GPTOSS_SCORE_SOFTMAX, "sigmoid": GPTOSS_SCORE_SIGMOID}
+
+
+@functools.lru_cache(maxsize=256)
+def _routing_config(score, top_k, num_groups, top_groups, group_rank, renormalize, scale):
+    if score not in _SCORES:
+        _bad(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    for name, n in (("top_k", top_k), ("num_groups", num_groups), ("top_groups", top_groups), ("group_rank", group_rank)):
+        if n >> 31:
+            _bad(f"{name}={n} must not be negative and below 2^31")
+    cfg = RoutingConfig(_SCORES[score], top_k, num_groups, top_groups, group_rank, 1 if renormalize else 0, scale)
+    return cfg, ctypes.addressof(cfg)
+
+
+def _strided_rows(name: str, t, dtypes, device=None):
+    """[rows, cols] of one of dtypes with contiguous rows: rows, cols and the distance between rows in elements."""
+    if not isinstance(t, torch.Tensor):
+        _bad(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.dtype not in dtypes:
+        _bad(f"{name} has dtype {t.dtype}, expected one of {', '.join(str(d) for d in dtypes)}")
+    if t.dim() != 2:
+        _bad(f"{name} must be 2-D, got shape {tuple(t.shape)}")
+    if device is not None and t.device != device:
+        _bad(f"{name} is on {t.device}, expected {device}")
+    rows, cols = t.shape
+    step, one = t.stride()
+    if (one != 1 and cols > 1) or (step < cols and rows > 1):
+        _bad(f"{name} must have contiguous rows, strides are {t.stride()}")
+    if rows > _INT_MAX or cols > _INT_MAX:
+        _bad(f"{name} of shape {tuple(t.shape)} is too large")
+    return rows, cols, step if rows > 1 else 0  # torch gives a single row any stride
+
+
+def _gpu(name: str, device) -> None:
+    if device.type != "cuda":
+        _bad(f"{name} is on {device}, a GPU is needed")
+
+
+def select_experts(logits, top_k: int, score: str = "softmax", bias=None, num_groups: int = 1, top_groups: int = 1,
+                   group_rank: int = 2, renormalize: bool = True, scale: float = 1.0, out=None, stream=None):
+    """The top_k experts of each token and their weights, (int32 [T, top_k], float32 [T, top_k]), from the router's
+    logits [T, E] (bfloat16 or float32, rows any distance apart).  score: "softmax" over the experts or "sigmoid" of
+    each.  bias (float32 [E]): added for the choice, not to the weights.  num_groups > 1: of that many groups of
+    neighbours only the top_groups stay whose group_rank (1 or 2) best choices sum highest.  renormalize: weights over
+    their sum; scale: a factor of them.  Ties go to the lower index; a logit or bias of -inf switches an expert off (it
+    has weight 0 and comes after the others).  out: preallocated (indices, weights)."""
+    T, E, stride = _strided_rows("logits", logits, (torch.bfloat16, torch.float32))
+    dev = logits.device
+    _, cfg = _routing_config(score, top_k, num_groups, top_groups, group_rank, bool(renormalize), float(scale))
+    if bias is not None:
+        _vector("bias", bias, dev, E, torch.float32)
+        bias = bias.data_ptr()
+    if out is None:
+        _gpu("logits", dev)
+        if top_k > E:
+            _bad(f"top_k={top_k} of {E} experts")
+        idx = _empty((T, top_k), torch.int32, dev, stream)
+        w = _empty((T, top_k), torch.float32, dev, stream)
+    else:
+        idx, w = out
+        for name, t, dtype in (("indices", idx, torch.int32), ("weights", w, torch.float32)):
+            _on_device(name, t, dev, dtype, 2)
+            if tuple(t.shape) != (T, top_k) or not t.is_contiguous():
+                _bad(f"{name} must be contiguous of shape {(T, top_k)}, got {tuple(t.shape)}")
+        _gpu("logits", dev)
+    _launch(dev, stream, _lib.gptoss_moe_select_experts, logits.data_ptr(), stride or E,
+            1 if logits.dtype is torch.float32 else 0, bias, T, E, cfg, idx.data_ptr(), w.data_ptr())
+    return idx, w
+
+
+# ---------------------------------------------------------------------------
+# MXFP4 matrices
+# ---------------------------------------------------------------------------
+class MXFP4Matrix:
+    """A matrix of [rows, K] values, or a stack of them for [experts], in the reference layout: packed uint8
+    [.., rows, K / 2] (low nibble = even k) and scales uint8 [.., rows, K / 32], both contiguous.  Value = e2m1 *
+    2^(scale - 127).  Fixed once made."""
+
+    __slots__ = ("packed", "scales", "device", "experts", "rows", "K", "_packed", "_scales")
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor):
+        for name, t in (("packed", packed), ("scales", scales)):
+            if not isinstance(t, torch.Tensor) or t.dtype is not torch.uint8:
+                _bad(f"{name} must be a torch.uint8 tensor")
+            if not t.is_contiguous():
+                _bad(f"{name} must be contiguous")
+        if packed.dim() not in (2, 3) or packed.shape[:-1] != scales.shape[:-1] or packed.shape[-1] != 16 * scales.shape[-1]:
+            _bad(f"packed must be [.., rows, K / 2] and scales [.., rows, K / 32], got {tuple(packed.shape)} and "
+                 f"{tuple(scales.shape)}")
+        if packed.shape[-1] == 0:
+            _bad("K must be positive")
+        if packed.device != scales.device:
+            _bad(f"packed is on {packed.device}, scales are on {scales.device}")
+        self._set(packed, scales, packed.shape[0] if packed.dim() == 3 else None, packed.shape[-2], 2 * packed.shape[-1])
+
+    def _set(self, packed, scales, experts, rows, K):
+        put = object.__setattr__
+        put(self, "packed", packed)
+        put(self, "scales", scales)
+        put(self, "device", packed.device)
+        put(self, "experts", experts)
+        put(self, "rows", rows)
+        put(self, "K", K)
+        put(self, "_packed", packed.data_ptr())
+        put(self, "_scales", scales.data_ptr())
+        return self
+
+    @classmethod
+    def _empty(cls, rows, K, device, stream):
+        return cls.__new__(cls)._set(_empty((rows, K // 2), torch.uint8, device, stream),
+                                     _empty((rows, K // 32), torch.uint8, device, stream), None, rows, K)
+
+    @property
+    def shape(self):
+        return (self.rows, self.K) if self.experts is None else (self.experts, self.rows, self.K)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"MXFP4Matrix.{name} is fixed: calls use the tensors it was made with")
+
+    __delattr__ = lambda self, name: self.__setattr__(name, None)  # noqa: E731
+
+    def __repr__(self):
+        return f"<gptoss_moe.MXFP4Matrix {'x'.join(str(n) for n in self.shape)} on {self.device}>"
+
+
+def _matrix(name: str, m, device=None) -> "MXFP4Matrix":
+    if not isinstance(m, MXFP4Matrix):
+        _bad(f"{name} must be an MXFP4Matrix, got {type(m).__name__}")
+    if device is not None and m.device != device:
+        _bad(f"{name} is on {m.device}, expected {device}")
+    return m
+
+
+def mxfp4_quantize(x, out: MXFP4Matrix | None = None, stream=None) -> MXFP4Matrix:
+    """x [rows, K] (bfloat16 or float32, rows a multiple of 16 bytes apart, K a multiple of 32) as MXFP4: each 32 values
+    share the power of two 2^(floor(log2(largest)) - 2) and are rounded to the nearest e2m1 value, at most 6 of it.  A
+    block with an infinity or NaN becomes NaN.  out: a matrix of that shape to write to."""
+    rows, K, stride = _strided_rows("x", x, (torch.bfloat16, torch.float32))
+    dev = x.device
+    if K % 32 or not K:
+        _bad(f"x has {K} columns, a positive multiple of 32 is needed")
+    if out is None:
+        _gpu("x", dev)
+        out = MXFP4Matrix._empty(rows, K, dev, stream)
+    else:
+        _matrix("out", out, dev)
+        if out.shape != (rows, K):
+            _bad(f"out has shape {out.shape}, expected {(rows, K)}")
+        _gpu("x", dev)
+    _launch(dev, stream, _lib.gptoss_mxfp4_quantize, x.data_ptr(), stride or K, 1 if x.dtype is torch.float32 else 0, rows, K,
+            out._packed, out._scales)
+    return out
+
+
+def mxfp4_dequantize(m: MXFP4Matrix, dtype=torch.bfloat16, out=None, stream=None):
+    """The values of m, [rows, K] ([experts, rows, K] of a stack), bfloat16 or float32 (exact in both).  out: a 2-D
+    tensor [experts * rows, K], rows a multiple of 16 bytes apart."""
+    _matrix("m", m)
+    rows, K = (m.experts or 1) * m.rows if m.experts is None or m.experts else 0, m.K
+    if out is None:
+        if dtype is not torch.bfloat16 and dtype is not torch.float32:
+            _bad(f"dtype must be torch.bfloat16 or torch.float32, got {dtype}")
+        _gpu("m", m.device)
+        out, stride = _empty(m.shape, dtype, m.device, stream), K
+    else:
+        have, cols, stride = _strided_rows("out", out, (torch.bfloat16, torch.float32), m.device)
+        if (have, cols) != (rows, K):
+            _bad(f"out has shape {tuple(out.shape)}, expected {(rows, K)}")
+        stride, dtype = stride or K, out.dtype
+        _gpu("m", m.device)
+    _launch(m.device, stream, _lib.gptoss_mxfp4_dequantize, m._packed, m._scales, rows, K, out.data_ptr(), stride,
+            1 if dtype is torch.float32 else 0)
+    return out
+
+
+def _product(a, w, rows, offsets, row_index, bias, swiglu, alpha, limit, dtype, quantize, out, stream):
+    _matrix("a", a)
+    dev = a.device
+    _matrix("w", w, dev)
+    if a.experts is not None:
+        _bad(f"a must be one matrix, got a stack of shape {a.shape}")
+    if a.K != w.K:
+        _bad(f"a has K={a.K}, w has K={w.K}")
+    N = w.rows
+    cols = N // 2 if swiglu else N
+    if bias is not None:
+        want = (N,) if w.experts is None else (w.experts, N)
+        if not (isinstance(bias, torch.Tensor) and bias.dtype is torch.bfloat16 and bias.shape == want
+                and bias.is_contiguous() and bias.device == dev):
+            _on_device("bias", bias, dev, torch.bfloat16)
+            _bad(f"bias must be contiguous of shape {want}, got {tuple(bias.shape)}")
+        bias = bias.data_ptr()
+    if quantize:
+        if cols % 32 or not cols:
+            _bad(f"MXFP4 results of {cols} columns, a positive multiple of 32 is needed")
+        if out is None:
+            _gpu("a", dev)
+            out = MXFP4Matrix._empty(rows, cols, dev, stream)
+        else:
+            _matrix("out", out, dev)
+            if out.shape != (rows, cols):
+                _bad(f"out has shape {out.shape}, expected {(rows, cols)}")
+            _gpu("a", dev)
+        res = Mxfp4Result(1 if swiglu else 0, alpha, limit, 0, None, 0, out._packed, out._scales)
+    else:
+        if out is None:
+            if dtype is not torch.bfloat16 and dtype is not torch.float32:
+                _bad(f"dtype must be torch.bfloat16 or torch.float32, got {dtype}")
+            _gpu("a", dev)
+            out, stride = _empty((rows, cols), dtype, dev, stream), cols
+        else:
+            have, wide, stride = _strided_rows("out", out, (torch.bfloat16, torch.float32), dev)
+            if (have, wide) != (rows, cols):
+                _bad(f"out has shape {tuple(out.shape)}, expected {(rows, cols)}")
+            stride, dtype = stride or cols, out.dtype
+            _gpu("a", dev)
+        res = Mxfp4Result(1 if swiglu else 0, alpha, limit, 1 if dtype is torch.float32 else 0, out.data_ptr(), stride, None,
+                          None)
+    where = ctypes.addressof(res)
+    if offsets is None:
+        _launch(dev, stream, _lib.gptoss_mxfp4_matmul, a._packed, a._scales, rows, w._packed, w._scales, bias, N, a.K, where)
+    else:
+        _launch(dev, stream, _lib.gptoss_moe_grouped_mxfp4_matmul, a._packed, a._scales, a.rows, row_index,
+                offsets.data_ptr(), w.experts, rows, w._packed, w._scales, bias, N, a.K, where)
+    return out
+
+
+def mxfp4_matmul(a: MXFP4Matrix, w: MXFP4Matrix, bias=None, swiglu: bool = False, alpha: float = 1.702, limit: float = 7.0,
+                 dtype=torch.bfloat16, quantize: bool = False, out=None, stream=None):
+    """a [M, K] times w [N, K] transposed, plus bias (bfloat16 [N]): [M, N], summed in fp32.  swiglu: column pairs (gate,
+    up) through the clamped SwiGLU, [M, N / 2].  The result is of dtype (bfloat16 or float32), or with quantize an
+    MXFP4Matrix.  out: a tensor (rows any distance apart; its dtype counts) or an MXFP4Matrix."""
+    if _matrix("w", w).experts is not None:
+        _bad(f"w is a stack of shape {w.shape}: grouped_mxfp4_matmul takes these")
+    return _product(a, w, _matrix("a", a).rows, None, None, bias, swiglu, alpha, limit, dtype, quantize, out, stream)
+
+
+def grouped_mxfp4_matmul(a: MXFP4Matrix, w: MXFP4Matrix, offsets, rows: int, row_index=None, bias=None,
+                         swiglu: bool = False, alpha: float = 1.702, limit: float = 7.0, dtype=torch.bfloat16,
+                         quantize: bool = False, out=None, stream=None):
+    """mxfp4_matmul of each expert's rows with its own matrix: w is a stack [E, N, K], bias bfloat16 [E, N], and result
+    row p of [rows, N], offsets[e] <= p < offsets[e + 1] (int32 [E + 1], permute_plan's), that of row row_index[p] (int32
+    [rows], its perm_token; None: p) of a.  Rows of no expert are left as they were (unset where out is allocated
+    here)."""
+    if _matrix("w", w).experts is None:
+        _bad(f"w must be a stack [experts, N, K], got shape {w.shape}")
+    dev = _matrix("a", a).device
+    if not 0 <= rows <= _INT_MAX:
+        _bad(f"rows={rows} must not be negative and below 2^31")
+    _vector("offsets", offsets, dev, w.experts + 1, torch.int32)
+    if row_index is not None:
+        _vector("row_index", row_index, dev, rows, torch.int32)
+        row_index = row_index.data_ptr()
+    return _product(a, w, rows, offsets, row_index, bias, swiglu, alpha, limit, dtype, quantize, out, stream)

@@ -587,6 +587,101 @@ int gptoss_paged_attention_prefill(const uint16_t* q, int64_t q_stride, const in
                                    int num_heads, const gptoss_attention_config* cfg, uint16_t* out,
                                    int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Routing of other models, and products of MXFP4 with MXFP4 ------------
+ * None of these calls synchronises the host, allocates or needs a workspace;
+ * routing, offsets and row numbers are read on the device.  They are additions:
+ * the ABI version stays.  The reference has no counterpart: it routes by the
+ * top logits (topk_softmax.cu:47-432), only reads MXFP4
+ * (mxfp4_dequant.cu:32-71) and multiplies bf16 with it
+ * (fused_mxfp4_gemv.cu:76-310). */
+
+enum { GPTOSS_SCORE_SOFTMAX = 0, GPTOSS_SCORE_SIGMOID = 1 };
+
+/* How a token's experts are chosen.  score: the softmax over all experts, or the
+ * sigmoid of each.  choice: score + bias.  groups: num_groups contiguous ones of
+ * equal size; a group counts the sum of its group_rank (1 or 2) highest choices,
+ * and the top_groups highest groups stay (num_groups 1: no groups).  Of their
+ * experts the top_k highest choices are taken, in descending order.  Equal ones:
+ * the lower index.  Weights are the scores, without the bias; over the sum of the
+ * chosen ones if renormalize (0 where that sum is 0); times scale.
+ * Scores, choices and sums are those of 64 bits (choices that are closer
+ * than that may come in either order), weights rounded once.
+ * An expert whose logit or bias is -inf is switched off: it counts 0 in
+ * its group's sum (a group of these alone comes last), is chosen only where the
+ * kept groups have no other left, lower index first, and has weight 0, so
+ * indices are distinct and valid in any case.  A choice of NaN is last too, with its
+ * score as the weight; a NaN logit makes a softmax row's weights NaN. */
+typedef struct gptoss_routing_config {
+  int score;        /* GPTOSS_SCORE_SOFTMAX or GPTOSS_SCORE_SIGMOID */
+  int top_k;        /* 1 to 32, at most the experts of top_groups groups */
+  int num_groups;   /* 1 to 64, divides num_experts */
+  int top_groups;   /* 1 to num_groups */
+  int group_rank;   /* 1 or 2 */
+  int renormalize;
+  float scale;      /* finite */
+} gptoss_routing_config;
+
+/* logits: num_tokens rows of num_experts (1 to 1024) bf16 or fp32 values,
+ * logits_stride elements apart, as gptoss_moe_route writes them.  bias: device fp32
+ * [num_experts] or NULL.  expert_indices and expert_weights ([num_tokens][top_k])
+ * are what gptoss_moe_permute_plan, gptoss_moe_layer_forward_routed and
+ * gptoss_moe_combine_forward take. */
+int gptoss_moe_select_experts(const void* logits, int64_t logits_stride, int logits_fp32, const float* bias,
+                              int num_tokens, int num_experts, const gptoss_routing_config* cfg,
+                              int32_t* expert_indices, float* expert_weights, void* stream);
+
+/* Rows to MXFP4 in the reference layout (packed [rows][K/2], low nibble = even k;
+ * scales [rows][K/32]), which gptoss_mxfp4_pack_tiled and the layer's expert
+ * tables take.  A block of 32 values has the scale byte e + 127,
+ * e = max(floor(log2(largest magnitude)) - 2, -126), and each value over 2^e
+ * rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with its sign (half way: the
+ * even code; above 6: 6).  A block with an infinity or NaN has the byte 255 and zero
+ * nibbles: NaN throughout.  x: bf16 or fp32 rows, x_stride elements apart, a multiple
+ * of 16 bytes; x and packed are 16-byte aligned; K is a multiple of 32. */
+int gptoss_mxfp4_quantize(const void* x, int64_t x_stride, int x_fp32, int rows, int K, uint8_t* packed, uint8_t* scales,
+                          void* stream);
+
+/* The values of such a matrix, e2m1 * 2^(scale byte - 127), exact in bf16 and in fp32
+ * (past the types' range: infinity; below 2^-133 rounded in bf16); NaN for a byte of 255.  out:
+ * rows out_stride elements apart, a multiple of 16 bytes; 16-byte aligned.  (Of a
+ * tiled matrix: gptoss_mxfp4_dequant.) */
+int gptoss_mxfp4_dequantize(const uint8_t* packed, const uint8_t* scales, int rows, int K, void* out, int64_t out_stride,
+                            int out_fp32, void* stream);
+
+/* Where a product's results go.  swiglu: columns 2i (gate) and 2i + 1 (up) give
+ * column i, (clamp(up, -limit, limit) + 1) * g * sigmoid(alpha * g),
+ * g = min(gate, limit); NaN is kept.  Then either values, bf16 or fp32 in rows out_stride
+ * elements apart, or (out NULL) MXFP4 as gptoss_mxfp4_quantize makes it of the
+ * fp32 results, a multiple of 32 columns, out_packed 16-byte aligned.  Nothing is rounded in between. */
+typedef struct gptoss_mxfp4_result {
+  int swiglu;
+  float alpha, limit;
+  int out_fp32;
+  void* out;
+  int64_t out_stride;
+  uint8_t* out_packed;
+  uint8_t* out_scales;
+} gptoss_mxfp4_result;
+
+/* y[m][n] = sum_k a[m][k] * w[n][k] + bias[n], a [M][K] and w [N][K] in MXFP4, row-major
+ * (16-byte aligned packed values), bias bf16 or NULL.  Products are exact and summed in
+ * fp32 on the block-scaled matrix cores; a scale byte of 255 makes its row's
+ * results NaN, and byte 0 is 2^-127. */
+int gptoss_mxfp4_matmul(const uint8_t* a_packed, const uint8_t* a_scales, int M, const uint8_t* w_packed,
+                        const uint8_t* w_scales, const uint16_t* bias, int N, int K, const gptoss_mxfp4_result* result,
+                        void* stream);
+
+/* The same for each expert e's rows p in [expert_offsets[e], expert_offsets[e + 1]), as
+ * gptoss_moe_permute_plan sorts them: result row p is that of row row_index[p] of
+ * a (perm_token; NULL: row p) with w_e and bias_e, w [num_experts][N][K],
+ * bias [num_experts][N].  expert_offsets (device, [num_experts + 1], at most 1024
+ * experts) is nondecreasing within [0, rows]; result rows outside of it are left as they
+ * were.  A row number outside [0, a_rows) stands for a row of zeros. */
+int gptoss_moe_grouped_mxfp4_matmul(const uint8_t* a_packed, const uint8_t* a_scales, int a_rows, const int32_t* row_index,
+                                    const int32_t* expert_offsets, int num_experts, int rows, const uint8_t* w_packed,
+                                    const uint8_t* w_scales, const uint16_t* bias, int N, int K,
+                                    const gptoss_mxfp4_result* result, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,236 @@
+"""GPU: the expert selection against its definition in 64 bits (mx_ref.py, where the tolerances are derived)."""
+import math
+
+import pytest
+import torch
+
+import mx_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def gen_of(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def check(gpu, logits, k, **kw):
+    got = gpu.select_experts(logits, k, score=kw.get("score", "softmax"), bias=kw.get("bias"),
+                             num_groups=kw.get("groups", 1), top_groups=kw.get("top_groups", 1),
+                             group_rank=kw.get("rank", 2), renormalize=kw.get("renormalize", True),
+                             scale=kw.get("scale", 1.0))
+    torch.cuda.synchronize()
+    ref.assert_selected(got, ref.select(logits, k, **kw), (tuple(logits.shape), k, kw.get("score"), kw.get("groups")))
+    return got
+
+
+GROUPS = [(1, 1, 2), (4, 2, 2), (4, 3, 1), (4, 4, 2)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups, top_groups, rank", GROUPS)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("E, k", [(4, 1), (8, 2), (60, 5), (64, 8), (128, 4), (192, 6), (256, 8), (512, 10), (1000, 7),
+                                  (1024, 32)])
+def test_against_64_bits(gpu, E, k, bias, groups, top_groups, rank, score, dtype):
+    gen = gen_of(E + k)
+    logits = (2 * torch.randn((37, E), device="cuda", generator=gen)).to(dtype)
+    b = 0.1 * torch.randn(E, device="cuda", generator=gen) if bias else None
+    check(gpu, logits, min(k, top_groups * (E // groups)), score=score, bias=b, groups=groups, top_groups=top_groups, rank=rank,
+          renormalize=E % 128 != 0, scale=2.5 if E % 3 else 1.0)
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 5, 63, 64, 65, 257, 2000])
+@pytest.mark.parametrize("E, groups", [(256, 8), (128, 1), (24, 3)])
+def test_token_counts(gpu, T, E, groups):
+    logits = (2 * torch.randn((T, E), device="cuda", generator=gen_of(T))).to(BF16)
+    bias = 0.1 * torch.randn(E, device="cuda", generator=gen_of(T + 1))
+    check(gpu, logits, 6, score="sigmoid", bias=bias, groups=groups, top_groups=(groups + 1) // 2, scale=2.5)
+    check(gpu, logits, 4)
+
+
+@pytest.mark.parametrize("E", [1, 2, 3, 7, 33, 65, 127, 130, 257, 1023])
+def test_odd_expert_counts(gpu, E):
+    logits = torch.randn((9, E), device="cuda", generator=gen_of(E))
+    for k in {1, min(E, 5), min(E, 32)}:
+        for score in ("softmax", "sigmoid"):
+            check(gpu, logits, k, score=score)
+            check(gpu, logits.to(BF16), k, score=score, renormalize=False)
+            check(gpu, logits, k, score=score, bias=torch.linspace(-1, 1, E, device="cuda"))
+
+
+@pytest.mark.parametrize("groups, top_groups", [(2, 1), (8, 3), (16, 5), (32, 32), (64, 17)])
+@pytest.mark.parametrize("rank", [1, 2])
+def test_group_sizes(gpu, groups, top_groups, rank):
+    for size in (1, 2, 3, 16):
+        E = groups * size
+        logits = (3 * torch.randn((21, E), device="cuda", generator=gen_of(E + rank))).to(BF16)
+        k = min(top_groups * size, 8)
+        for score in ("softmax", "sigmoid"):
+            check(gpu, logits, k, score=score, groups=groups, top_groups=top_groups, rank=rank)
+            check(gpu, logits, k, score=score, groups=groups, top_groups=top_groups, rank=rank,
+                  bias=torch.randn(E, device="cuda", generator=gen_of(E)))
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_ties_go_to_the_lower_index(gpu, score, bias, groups):
+    E = 64
+    b = torch.full((E,), 0.25, device="cuda") if bias else None
+    few = torch.randint(0, 3, (50, E), device="cuda", generator=gen_of(1)).float()  # three different values
+    for logits in (torch.zeros((3, E), device="cuda"), few, few.to(BF16), -few):
+        check(gpu, logits, 8, score=score, bias=b, groups=groups, top_groups=(groups + 1) // 2)
+    zeros = torch.zeros((2, E), device="cuda")
+    zeros[:, ::2] = -0.0
+    idx, _ = check(gpu, zeros, 4, score=score, bias=b)
+    assert idx.cpu().tolist() == [[0, 1, 2, 3]] * 2
+
+
+@pytest.mark.parametrize("groups", [1, 4])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_choices_that_32_bits_do_not_tell_apart(gpu, score, groups):
+    """The order is that of the exact choices: the bias makes up for the score but for a few 1e-9."""
+    E, T = 64, 40
+    logits = torch.randn((T, E), device="cuda", generator=gen_of(3))
+    logits = logits[:1].expand(T, E).contiguous()  # one row, so that one bias nearly evens it out
+    x = logits[0].double()
+    s = torch.softmax(x, 0) if score == "softmax" else torch.sigmoid(x)
+    bias = (0.9 - s).float()
+    # what rounding the bias to 32 bits leaves is of the size of 2^-26 to 2^-25, and never a tie
+    left = s + bias.double()
+    assert 0 < float((left.sort().values.diff()).min()) < 1e-8 and float(left.max() - left.min()) < 1e-6
+    check(gpu, logits, 8, score=score, bias=bias, groups=groups, top_groups=(groups + 1) // 2)
+
+
+def test_close_choices_among_others(gpu):
+    """Pairs of nearly equal choices here and there in ordinary rows."""
+    E, T = 256, 64
+    gen = gen_of(5)
+    logits = 2 * torch.randn((T, E), device="cuda", generator=gen)
+    top = logits.argsort(1, descending=True)
+    for t in range(T):  # the eighth and ninth, or two in the middle of the chosen
+        a, b = top[t, 7 if t % 2 else 3], top[t, 8 if t % 2 else 4]
+        logits[t, a] = torch.nextafter(logits[t, b], torch.tensor(math.inf, device="cuda"))
+    bias = torch.full((E,), 0.125, device="cuda")
+    for score in ("softmax", "sigmoid"):
+        check(gpu, logits, 8, score=score, bias=bias)
+        check(gpu, logits, 8, score=score, bias=bias, groups=8, top_groups=4)
+        check(gpu, logits, 8, score=score, groups=8, top_groups=4)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_experts_switched_off(gpu, score, groups):
+    E, k = 32, 8
+    gen = gen_of(7)
+    logits = torch.randn((60, E), device="cuda", generator=gen)
+    keep = torch.rand((60, E), device="cuda", generator=gen) < torch.linspace(0, 1, 60, device="cuda")[:, None]
+    masked = torch.where(keep, logits, -math.inf)  # the first rows have few or none left
+    masked[0], masked[1] = -math.inf, -math.inf
+    masked[1, E - 1] = 0.5
+    kw = dict(score=score, groups=groups, top_groups=(groups + 1) // 2)
+    for dtype in (F32, BF16):
+        idx, w = check(gpu, masked.to(dtype), k, **kw)
+        assert idx.sort(1).values.diff(dim=1).min() > 0 and idx.min() >= 0 and idx.max() < E  # distinct and valid
+        assert not w[0].any()
+    for off in (1, 20, 31, 32):
+        bias = 0.1 * torch.randn(E, device="cuda", generator=gen)
+        bias[torch.randperm(E, device="cuda", generator=gen)[:off]] = -math.inf
+        check(gpu, logits, k, bias=bias, **kw)
+        check(gpu, masked, k, bias=bias, renormalize=False, **kw)
+    check(gpu, torch.full((2, E), torch.finfo(BF16).min, device="cuda", dtype=BF16), k, **kw)  # the lowest value is one
+    check(gpu, torch.full((2, E), -1e38, device="cuda"), k, bias=torch.linspace(0, 1, E, device="cuda"), **kw)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups", [1, 4])
+@pytest.mark.parametrize("bias", [False, True])
+def test_infinite_and_nan_logits(gpu, score, groups, bias):
+    E = 32
+    logits = torch.randn((8, E), device="cuda", generator=gen_of(9))
+    logits[0, 5] = math.inf
+    logits[1, 5], logits[1, 29] = math.inf, math.inf
+    logits[2, 7] = math.nan
+    logits[3] = math.nan
+    logits[4, 3], logits[4, 4], logits[4, 20] = math.nan, -math.inf, math.inf
+    logits[5] = math.inf
+    logits[6, :8] = math.nan
+    b = 0.1 * torch.randn(E, device="cuda", generator=gen_of(10)) if bias else None
+    if bias:
+        b[11] = math.nan
+        b[12] = math.inf
+    for dtype in (F32, BF16):
+        check(gpu, logits.to(dtype), 6, score=score, groups=groups, top_groups=(groups + 1) // 2, bias=b)
+
+
+def test_wide_logits(gpu):
+    """Far apart, and all far below zero: shares of a vanishing sum."""
+    for scale in (30.0, 100.0):
+        logits = scale * torch.randn((40, 64), device="cuda", generator=gen_of(11))
+        check(gpu, logits, 4)
+        check(gpu, logits, 4, renormalize=False)
+    check(gpu, torch.randn((40, 64), device="cuda", generator=gen_of(12)) - 300, 4, score="sigmoid")
+    check(gpu, torch.randn((40, 64), device="cuda", generator=gen_of(12)) - 95, 4, score="sigmoid", groups=4, top_groups=2)
+
+
+def test_strided_logits_and_given_results(gpu):
+    wide = torch.randn((33, 300), device="cuda", generator=gen_of(13))
+    idx = torch.empty((33, 4), dtype=torch.int32, device="cuda")
+    w = torch.empty((33, 4), device="cuda")
+    for view in (wide[:, 100:228], wide[:, 1:129], wide[::2, 3:131], wide.to(BF16)[:, 7:135]):
+        n = view.shape[0]
+        got = gpu.select_experts(view, 4, out=(idx[:n], w[:n]))
+        assert got[0].data_ptr() == idx.data_ptr()
+        ref.assert_selected(got, ref.select(view, 4))
+    one = wide[5:6, 200:264]
+    ref.assert_selected(gpu.select_experts(one, 3), ref.select(one, 3))
+    assert gpu.select_experts(wide[:0], 4)[0].shape == (0, 4)
+
+
+def test_a_prefix_gives_the_same(gpu):
+    """A token's choice is its own: the same bits in a smaller call, and in another place of it."""
+    logits = (2 * torch.randn((3000, 256), device="cuda", generator=gen_of(14))).to(BF16)
+    bias = 0.1 * torch.randn(256, device="cuda", generator=gen_of(15))
+    kw = dict(score="sigmoid", bias=bias, num_groups=8, top_groups=4, scale=2.5)
+    idx, w = gpu.select_experts(logits, 8, **kw)
+    for n in (1, 7, 64, 1000):
+        a, b = gpu.select_experts(logits[:n], 8, **kw)
+        assert torch.equal(a, idx[:n]) and torch.equal(b, w[:n])
+        a, b = gpu.select_experts(logits[-n:], 8, **kw)
+        assert torch.equal(a, idx[-n:]) and torch.equal(b, w[-n:])
+
+
+@pytest.mark.parametrize("E, k", [(32, 4), (128, 4), (128, 8), (256, 2)])
+def test_like_the_top_k_softmax(gpu, E, k):
+    """Softmax scores, renormalised: what gptoss_topk_softmax_forward computes."""
+    for dtype in (BF16, F32):
+        logits = (2 * torch.randn((300, E), device="cuda", generator=gen_of(16))).to(dtype)
+        idx, w = gpu.select_experts(logits, k)
+        idx2, w2 = gpu.topk_softmax(logits, k)
+        assert torch.equal(idx, idx2)
+        assert float(((w - w2).abs() / w).max()) < 40 * 2.0 ** -23  # arguments up to 16, both off by 2^-23 of them
+
+
+def test_streams_and_graphs(gpu):
+    logits = 2 * torch.randn((64, 256), device="cuda", generator=gen_of(17))
+    bias = 0.1 * torch.randn(256, device="cuda", generator=gen_of(18))
+    kw = dict(score="sigmoid", bias=bias, num_groups=8, top_groups=4)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = gpu.select_experts(logits, 8, stream=side, **kw)
+    side.synchronize()
+    want = gpu.select_experts(logits, 8, **kw)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    out = (torch.empty_like(want[0]), torch.empty_like(want[1]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu.select_experts(logits, 8, out=out, **kw)
+    for seed in range(3):
+        logits.copy_(2 * torch.randn((64, 256), device="cuda", generator=gen_of(seed)))
+        want = gpu.select_experts(logits, 8, **kw)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
