@@ -56,7 +56,9 @@ struct MxProductArgs {
   bool out_fp32;
   uint8_t* out_packed;
   uint8_t* out_scales;
+  bool vec;  // out's rows and their pieces of 16 bytes are on 16 bytes
 };
+hipError_t launch_mx_tile(const MxProductArgs& a, hipStream_t s);
 hipError_t launch_mx_product(const MxProductArgs& a, hipStream_t s);
 
 }  // namespace gxmoe

@@ -191,6 +191,7 @@ __global__ __launch_bounds__(kWaves * kWave) void product_kernel(MxProductArgs a
 }  // namespace
 
 hipError_t launch_mx_product(const MxProductArgs& a, hipStream_t s) {
+  if (a.rows > 64) return launch_mx_tile(a, s);
   const int tiles = a.offsets ? a.rows / kTileM + (a.E < a.rows ? a.E : a.rows) : (a.rows + kTileM - 1) / kTileM;
   const int n_groups = (a.N + kWaves * kTileN - 1) / (kWaves * kTileN);
   hipLaunchKernelGGL(product_kernel, dim3(static_cast<uint32_t>(tiles) * static_cast<uint32_t>(n_groups)),

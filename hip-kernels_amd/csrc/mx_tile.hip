@@ -1,0 +1,350 @@
+// mx_tile.hip -- MXFP4 products of many rows: tiles through LDS.
+//
+// A work-group of eight waves computes TM rows x 256 columns.  K goes in chunks of
+// four blocks: 64 bytes of each of the tile's rows and weight rows reach an LDS ring of
+// four chunks by direct global -> LDS loads, 16 bytes a lane; the 16-byte piece of
+// block b of row r lies at b ^ (r / 4) % 4 of the row's 64 bytes, so that the operand
+// reads (one block of 16 rows at a time) meet all banks.  The scales of 16 blocks of every
+// row come through registers into LDS, one 16-byte load per row and four chunks, since
+// single dwords of the rows would cost the address unit as much as the data.
+//
+// Per chunk a wave runs two steps of NT x MT products on operands that it read during
+// the step before; between the steps of a chunk it waits for its loads of the next one
+// and meets the others once, after which the chunk's stage is free for the loads of
+// the chunk four ahead.
+#include <type_traits>
+
+#include "mx_product.h"
+
+namespace gxmoe {
+
+namespace {
+
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+constexpr int kTileWaves = 8;
+constexpr int kTileThreads = kTileWaves * kWave;
+constexpr int kStages = 4;
+constexpr int kStageBytes = 512 * 64;                      // up to 512 rows of four blocks
+constexpr int kScaleOff = kStages * kStageBytes;           // [2][512 rows][16]
+constexpr int kBiasOff = kScaleOff + 2 * 512 * 16;         // [256] floats
+constexpr int kLdsBytes = kBiasOff + 1024;
+constexpr int kTileN = 256;
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {  // vmcnt(N), the other counters as they are
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0f70);
+}
+
+typedef u32x4_t __attribute__((aligned(1))) loose_u32x4;
+
+// 16 bytes of a row's scales from `from` on, zeros past the row's nb bytes: in two
+// parts, so that the load is one that nothing waits for.  The load ends within the row
+// (nb >= 16); what it holds too early is shifted out.
+__device__ __forceinline__ u32x4_t shift_bytes(u32x4_t v, int n) {  // 0 < n < 16 bytes, uniform
+  for (; n >= 4; n -= 4) v = u32x4_t{v[1], v[2], v[3], 0u};
+  if (n > 0) {
+    const int k = 8 * n;
+    v = u32x4_t{v[0] >> k | v[1] << (32 - k), v[1] >> k | v[2] << (32 - k), v[2] >> k | v[3] << (32 - k), v[3] >> k};
+  }
+  return v;
+}
+
+__device__ __forceinline__ u32x4_t load_short_row(const uint8_t* row, int nb) {  // nb < 16
+  u32x4_t v{0u, 0u, 0u, 0u};
+  for (int i = 0; i < nb; ++i) {
+    const uint32_t x = static_cast<uint32_t>(row[i]) << (8 * (i & 3));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] |= (i >> 2) == j ? x : 0u;
+  }
+  return v;
+}
+
+// WN x WM waves, each NT x MT products of 32 columns x 32 rows.
+template <int NT, int MT, int WN, int WM>
+__device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, int n0, uint8_t* lds) {
+  static_assert(WN * WM == kTileWaves && 32 * NT * WN == kTileN, "");
+  constexpr int kTM = 32 * MT * WM;
+  constexpr int kRows = kTileN + kTM;               // the weights', then a's
+  constexpr int kPieces = kRows / 16;               // of 1 KiB
+  constexpr int L = (kPieces + kTileWaves - 1) / kTileWaves;  // loads per wave and chunk
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = w % WN, wm = w / WN;
+  const int r = lane & 31, half = lane >> 5;
+  const int nb = a.K / 32, nch = (nb + 3) / 4;
+  const size_t row_bytes = static_cast<size_t>(a.K) / 2;
+  const size_t wrow = static_cast<size_t>(mt.e) * a.N;
+
+  // The lane's row of each piece that its wave loads.  A wave without a piece of its own
+  // left loads its first one once more, so that all waves have as many loads in flight.
+  const uint8_t* src[L];
+  int piece[L];
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    piece[i] = w + kTileWaves * i < kPieces ? w + kTileWaves * i : w;
+    const int row = 16 * piece[i] + (lane >> 2);
+    if (row < kTileN) {
+      src[i] = a.w + (wrow + min(n0 + row, a.N - 1)) * row_bytes;
+    } else {
+      const int p = mt.lo + row - kTileN;
+      src[i] = a.a + static_cast<size_t>(max(p < mt.hi ? source_row(a, p) : 0, 0)) * row_bytes;
+    }
+  }
+  const int blk = (lane & 3) ^ ((lane >> 4) & 3);
+  auto issue = [&](int c) __attribute__((always_inline)) {
+    // blocks past the end: the last one again (its scale there is 0)
+    const int b = min(4 * c + blk, nb - 1);
+    uint8_t* stage = lds + (c & (kStages - 1)) * kStageBytes;
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      __builtin_amdgcn_global_load_lds(src[i] + 16 * static_cast<size_t>(b), (lds_void_t*)(stage + 1024 * piece[i]), 16, 0, 0);
+  };
+  // The thread's row of the scales.
+  const bool scaled = tid < kRows;
+  const uint8_t* ssrc;
+  if (tid < kTileN) {
+    ssrc = a.ws + (wrow + min(n0 + tid, a.N - 1)) * nb;
+  } else if (scaled) {
+    const int p = mt.lo + tid - kTileN;
+    ssrc = a.as + static_cast<size_t>(max(p < mt.hi ? source_row(a, p) : 0, 0)) * nb;
+  } else {
+    ssrc = a.ws + wrow * nb;  // loaded like the others, not kept
+  }
+
+  // further ones, with no branch around the load: past the end of the row (and where it has
+  // fewer than 16) something is loaded that is not read
+  const uint8_t* snext = nb < 16 ? a.w : ssrc;
+  const int slast = max(nb - 16, 0);
+  u32x4_t sreg = nb < 16 ? load_short_row(ssrc, nb) : *reinterpret_cast<const loose_u32x4*>(ssrc);
+  if (tid < kTileN)
+    reinterpret_cast<float*>(lds + kBiasOff)[tid] =
+        a.bias ? bf16_to_f32(a.bias[wrow + min(n0 + tid, a.N - 1)]) : 0.0f;
+  if (scaled) *reinterpret_cast<u32x4_t*>(lds + kScaleOff + 16 * tid) = sreg;
+#pragma unroll
+  for (int c = 0; c < kStages; ++c) issue(c);
+
+  f32x16_t acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+
+  const int wrow_l = 32 * NT * wn + r, arow_l = kTileN + 32 * MT * wm + r;
+  const int piece0 = 16 * (half ^ ((r >> 2) & 3));  // of step 0; of step 1: ^ 32
+  u32x4_t wv[2][NT], av[2][MT];
+  uint32_t sw[NT], sa[MT];
+  auto read = [&](int c, int s, u32x4_t(&wo)[NT], u32x4_t(&ao)[MT]) __attribute__((always_inline)) {
+    const uint8_t* stage = lds + (c & (kStages - 1)) * kStageBytes + (piece0 ^ (32 * s));
+#pragma unroll
+    for (int i = 0; i < NT; ++i) wo[i] = *reinterpret_cast<const u32x4_t*>(stage + 64 * wrow_l + 2048 * i);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) ao[j] = *reinterpret_cast<const u32x4_t*>(stage + 64 * arow_l + 2048 * j);
+  };
+  // A lane's byte of step s is block 2 s + half of the chunk's four.
+  auto read_scales = [&](int c) __attribute__((always_inline)) {
+    const uint8_t* at = lds + kScaleOff + ((c >> 2) & 1) * (512 * 16) + 4 * (c & 3);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) sw[i] = *reinterpret_cast<const uint32_t*>(at + 16 * (wrow_l + 32 * i)) >> (8 * half);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sa[j] = *reinterpret_cast<const uint32_t*>(at + 16 * (arow_l + 32 * j)) >> (8 * half);
+  };
+
+  wait_vm<L*(kStages - 1)>();
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  read_scales(0);
+  read(0, 0, wv[0], av[0]);
+
+  int c = 0;
+  auto chunk = [&](auto place) __attribute__((always_inline)) {
+    constexpr int kPlace = decltype(place)::value;  // c % 4
+    read(c, 1, wv[1], av[1]);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(wv[0][i]), mx_operand(av[0][j]), acc[i][j], 4, 4,
+                                                                    0, static_cast<int>(sw[i]), 0, static_cast<int>(sa[j]));
+    if constexpr (kPlace == 3) {
+      const int early = 4 * (c + 1) + 16 - nb;
+      if (early > 0 && early < 16) sreg = shift_bytes(sreg, early);
+      if (scaled) *reinterpret_cast<u32x4_t*>(lds + kScaleOff + (((c >> 2) + 1) & 1) * (512 * 16) + 16 * tid) = sreg;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    wait_vm<L*(kStages - 2)>();          // this wave's loads of chunk c + 1
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // its reads of chunk c
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    uint32_t ow[NT], oa[MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) ow[i] = sw[i];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) oa[j] = sa[j];
+    read_scales(c + 1);
+    read(c + 1, 0, wv[0], av[0]);
+    issue(c + kStages);
+    if constexpr (kPlace == 0) sreg = *reinterpret_cast<const loose_u32x4*>(snext + min(4 * (c + 4), slast));
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(wv[1][i]), mx_operand(av[1][j]), acc[i][j], 4, 4,
+                                                                    2, static_cast<int>(ow[i]), 2, static_cast<int>(oa[j]));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  for (;;) {
+    chunk(std::integral_constant<int, 0>{});
+    if (++c == nch) break;
+    chunk(std::integral_constant<int, 1>{});
+    if (++c == nch) break;
+    chunk(std::integral_constant<int, 2>{});
+    if (++c == nch) break;
+    chunk(std::integral_constant<int, 3>{});
+    if (++c == nch) break;
+  }
+  // the ring becomes the waves' own room, 16 KiB each: no load may still land in it
+  wait_vm<0>();
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  __builtin_amdgcn_s_barrier();
+
+  const float* bias = reinterpret_cast<const float*>(lds + kBiasOff) + 32 * NT * wn;
+  uint8_t* own = lds + 16384 * w;
+  const int cols = a.swiglu ? a.N / 2 : a.N;
+  constexpr int kG = NT < 2 ? NT : 2;  // column tiles that go together
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    const int p = mt.lo + 32 * (MT * wm + j) + r;
+    const bool live = p < mt.hi;
+    const bool zero = live && source_row(a, p) < 0;
+#pragma unroll
+    for (int g = 0; g < NT / kG; ++g) {
+      const int n = n0 + 32 * (NT * wn + kG * g);  // the group's first column
+      float v[kG][16];
+#pragma unroll
+      for (int i = 0; i < kG; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 b = *reinterpret_cast<const float4*>(bias + 32 * (kG * g + i) + 8 * q + 4 * half);
+          const f32x16_t& x = acc[kG * g + i][j];
+          v[i][4 * q + 0] = (zero ? 0.0f : x[4 * q + 0]) + b.x;
+          v[i][4 * q + 1] = (zero ? 0.0f : x[4 * q + 1]) + b.y;
+          v[i][4 * q + 2] = (zero ? 0.0f : x[4 * q + 2]) + b.z;
+          v[i][4 * q + 3] = (zero ? 0.0f : x[4 * q + 3]) + b.w;
+        }
+      if (a.swiglu) {
+#pragma unroll
+        for (int i = 0; i < kG; ++i)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[i][q] = mx_swiglu(v[i][2 * q], v[i][2 * q + 1], a.alpha, a.limit);
+      }
+      if (a.out_packed) {
+        const size_t ob = static_cast<size_t>(p) * (cols / 32);
+        uint32_t code;
+        if (a.swiglu) {
+          if constexpr (kG == 2) {
+            const float x[16] = {v[0][0], v[0][1], v[0][2], v[0][3], v[0][4], v[0][5], v[0][6], v[0][7],
+                                 v[1][0], v[1][1], v[1][2], v[1][3], v[1][4], v[1][5], v[1][6], v[1][7]};
+            const gx_u32x2 d = quantize_block<true>(x, code);
+            if (live && n / 2 < cols) {
+              const size_t at = ob + n / 64;
+              reinterpret_cast<gx_u32x2*>(a.out_packed)[2 * at + half] = d;
+              if (half == 0) a.out_scales[at] = static_cast<uint8_t>(code);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kG; ++i) {
+            const gx_u32x2 d = quantize_block<false>(v[i], code);
+            if (live && n + 32 * i < cols) {
+              const size_t at = ob + n / 32 + i;
+              reinterpret_cast<gx_u32x2*>(a.out_packed)[2 * at + half] = d;
+              if (half == 0) a.out_scales[at] = static_cast<uint8_t>(code);
+            }
+          }
+        }
+        continue;
+      }
+      // through LDS, so that rows are written in whole pieces: 32 rows of `wide` bytes
+      const int size = a.out_fp32 ? 4 : 2, have = 32 * kG >> (a.swiglu ? 1 : 0);
+      const int wide = have * size, pitch = wide + 16;
+#pragma unroll
+      for (int i = 0; i < kG; ++i) {
+        if (a.swiglu) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint8_t* at = own + pitch * r + size * (16 * i + 4 * q + 2 * half);
+            if (a.out_fp32) *reinterpret_cast<float2*>(at) = float2{v[i][2 * q], v[i][2 * q + 1]};
+            else *reinterpret_cast<uint32_t*>(at) = pack_bf16x2(v[i][2 * q], v[i][2 * q + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint8_t* at = own + pitch * r + size * (32 * i + 8 * q + 4 * half);
+            if (a.out_fp32)
+              *reinterpret_cast<float4*>(at) = float4{v[i][4 * q], v[i][4 * q + 1], v[i][4 * q + 2], v[i][4 * q + 3]};
+            else
+              *reinterpret_cast<gx_u32x2*>(at) =
+                  gx_u32x2{pack_bf16x2(v[i][4 * q], v[i][4 * q + 1]), pack_bf16x2(v[i][4 * q + 2], v[i][4 * q + 3])};
+          }
+        }
+      }
+      const int first = a.swiglu ? n / 2 : n;
+      const int per_row = wide / 16, rows_at_once = kWave / per_row;
+      const int row0 = lane / per_row, off = 16 * (lane % per_row);
+      const bool whole = a.vec && first + have <= cols;
+      for (int k = 0; k < 32; k += rows_at_once) {
+        const int rr = k + row0, pp = mt.lo + 32 * (MT * wm + j) + rr;
+        const u32x4_t d = *reinterpret_cast<const u32x4_t*>(own + pitch * rr + off);
+        if (pp >= mt.hi) continue;
+        const int col = first + off / size;
+        uint8_t* o = static_cast<uint8_t*>(a.out) + (static_cast<size_t>(pp) * static_cast<size_t>(a.stride) + col) * size;
+        if (whole) {
+          *reinterpret_cast<u32x4_t*>(o) = d;
+        } else if (a.out_fp32) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (col + x < cols) reinterpret_cast<uint32_t*>(o)[x] = d[x];
+        } else {
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            if (col + x < cols) reinterpret_cast<uint16_t*>(o)[x] = static_cast<uint16_t>(d[x / 2] >> (16 * (x & 1)));
+        }
+      }
+    }
+  }
+}
+
+// Tiles are numbered four m-tiles x all n-tiles at a time, and every XCD (one of eight, in
+// turn by work-group) takes a run of them, so that its L2 serves a tile's rows
+// and weights to its neighbours.
+constexpr int kGroupM = 4;
+
+__global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(MxProductArgs a, int m_tiles, int n_tiles) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLdsBytes];
+  const int total = m_tiles * n_tiles, b = blockIdx.x;
+  const int x = b & 7, share = total >> 3, more = total & 7;
+  const int id = x * share + min(x, more) + (b >> 3);
+  const int group = id / (kGroupM * n_tiles), in_group = id - group * (kGroupM * n_tiles);
+  const int height = min(kGroupM, m_tiles - kGroupM * group);
+  const int m = kGroupM * group + in_group % height, nt = in_group / height;
+  const MTile mt = find_m_tile(a, m, 256, threadIdx.x & (kWave - 1));
+  if (mt.e < 0) return;
+  const int rows = mt.hi - mt.lo;
+  if (rows > 128) tile<4, 2, 2, 4>(a, mt, nt * kTileN, lds);
+  else if (rows > 64) tile<2, 2, 4, 2>(a, mt, nt * kTileN, lds);
+  else tile<2, 1, 4, 2>(a, mt, nt * kTileN, lds);
+}
+
+}  // namespace
+
+hipError_t launch_mx_tile(const MxProductArgs& a, hipStream_t s) {
+  const int m_tiles = a.offsets ? a.rows / 256 + (a.E < a.rows ? a.E : a.rows) : (a.rows + 255) / 256;
+  const int n_tiles = (a.N + kTileN - 1) / kTileN;
+  hipLaunchKernelGGL(tile_kernel, dim3(static_cast<uint32_t>(m_tiles) * static_cast<uint32_t>(n_tiles)), dim3(kTileThreads), 0,
+                     s, a, m_tiles, n_tiles);
+  return hipGetLastError();
+}
+
+}  // namespace gxmoe
