@@ -1,17 +1,17 @@
 // mx_tile.hip -- MXFP4 products of many rows: tiles through LDS.
 //
 // A work-group of eight waves computes TM rows x 256 columns.  K goes in chunks of
-// four blocks: 64 bytes of each of the tile's rows and weight rows reach an LDS ring of
-// four chunks by direct global -> LDS loads, 16 bytes a lane; the 16-byte piece of
-// block b of row r lies at b ^ (r / 4) % 4 of the row's 64 bytes, so that the operand
-// reads (one block of 16 rows at a time) meet all banks.  The scales of 16 blocks of every
-// row come through registers into LDS, one 16-byte load per row and four chunks, since
-// single dwords of the rows would cost the address unit as much as the data.
+// eight blocks: 128 bytes (a line) of each of the tile's rows and weight rows reach one of
+// two LDS stages by direct global -> LDS loads, 16 bytes a lane (the same loads of 64 bytes of a row
+// bring 14.6 TB/s over the chip, of whole lines 25.4); the 16-byte piece of block b of row r lies at
+// b ^ (r / 2) % 8 of the row's 128 bytes, so that the operand reads (one block of 16 rows
+// at a time) meet all banks.  The scales come through registers into LDS, 32 blocks of
+// a row at a time, since dwords of single rows would cost the address unit as much as the data.
 //
-// Per chunk a wave runs two steps of NT x MT products on operands that it read during
-// the step before; between the steps of a chunk it waits for its loads of the next one
-// and meets the others once, after which the chunk's stage is free for the loads of
-// the chunk four ahead.
+// Per chunk a wave runs four steps of NT x MT products on operands that it read
+// during the step before.  Before the last step, whose operands are in registers by then, it waits for
+// its loads of the next chunk and meets the others, after which the chunk's
+// stage is free for the loads of the chunk after the next.
 #include <type_traits>
 
 #include "mx_product.h"
@@ -24,12 +24,11 @@ typedef __attribute__((address_space(3))) void lds_void_t;
 
 constexpr int kTileWaves = 8;
 constexpr int kTileThreads = kTileWaves * kWave;
-constexpr int kStages = 4;
-constexpr int kStageBytes = 512 * 64;                      // up to 512 rows of four blocks
-constexpr int kScaleOff = kStages * kStageBytes;           // [2][512 rows][16]
-constexpr int kBiasOff = kScaleOff + 2 * 512 * 16;         // [256] floats
-constexpr int kLdsBytes = kBiasOff + 1024;
 constexpr int kTileN = 256;
+constexpr int kBlocks = 8;                                 // of a chunk
+constexpr int kStageBytes = 512 * 16 * kBlocks;            // up to 512 rows
+constexpr int kScaleOff = 2 * kStageBytes;                 // [2][4 chunks][512 rows][8]
+constexpr int kLdsBytes = kScaleOff + 2 * 4 * 512 * 8;     // all 160 KiB
 
 template <int N>
 __device__ __forceinline__ void wait_vm() {  // vmcnt(N), the other counters as they are
@@ -66,12 +65,12 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
   static_assert(WN * WM == kTileWaves && 32 * NT * WN == kTileN, "");
   constexpr int kTM = 32 * MT * WM;
   constexpr int kRows = kTileN + kTM;               // the weights', then a's
-  constexpr int kPieces = kRows / 16;               // of 1 KiB
+  constexpr int kPieces = kRows / 8;                // of 1 KiB
   constexpr int L = (kPieces + kTileWaves - 1) / kTileWaves;  // loads per wave and chunk
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = w % WN, wm = w / WN;
   const int r = lane & 31, half = lane >> 5;
-  const int nb = a.K / 32, nch = (nb + 3) / 4;
+  const int nb = a.K / 32, nch = (nb + kBlocks - 1) / kBlocks;
   const size_t row_bytes = static_cast<size_t>(a.K) / 2;
   const size_t wrow = static_cast<size_t>(mt.e) * a.N;
 
@@ -82,7 +81,7 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
 #pragma unroll
   for (int i = 0; i < L; ++i) {
     piece[i] = w + kTileWaves * i < kPieces ? w + kTileWaves * i : w;
-    const int row = 16 * piece[i] + (lane >> 2);
+    const int row = 8 * piece[i] + (lane >> 3);
     if (row < kTileN) {
       src[i] = a.w + (wrow + min(n0 + row, a.N - 1)) * row_bytes;
     } else {
@@ -90,38 +89,59 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
       src[i] = a.a + static_cast<size_t>(max(p < mt.hi ? source_row(a, p) : 0, 0)) * row_bytes;
     }
   }
-  const int blk = (lane & 3) ^ ((lane >> 4) & 3);
+  // (row / 2) % 8 of the lane's rows: all of its pieces are odd or all are even
+  const int blk = (lane & 7) ^ (4 * (w & 1) + (lane >> 4));
   auto issue = [&](int c) __attribute__((always_inline)) {
     // blocks past the end: the last one again (its scale there is 0)
-    const int b = min(4 * c + blk, nb - 1);
-    uint8_t* stage = lds + (c & (kStages - 1)) * kStageBytes;
+    const int b = min(kBlocks * c + blk, nb - 1);
+    uint8_t* stage = lds + (c & 1) * kStageBytes;
 #pragma unroll
     for (int i = 0; i < L; ++i)
       __builtin_amdgcn_global_load_lds(src[i] + 16 * static_cast<size_t>(b), (lds_void_t*)(stage + 1024 * piece[i]), 16, 0, 0);
   };
   // The thread's row of the scales.
-  const bool scaled = tid < kRows;
   const uint8_t* ssrc;
   if (tid < kTileN) {
     ssrc = a.ws + (wrow + min(n0 + tid, a.N - 1)) * nb;
-  } else if (scaled) {
+  } else if (tid < kRows) {
     const int p = mt.lo + tid - kTileN;
     ssrc = a.as + static_cast<size_t>(max(p < mt.hi ? source_row(a, p) : 0, 0)) * nb;
   } else {
     ssrc = a.ws + wrow * nb;  // loaded like the others, not kept
   }
 
-  // further ones, with no branch around the load: past the end of the row (and where it has
-  // fewer than 16) something is loaded that is not read
-  const uint8_t* snext = nb < 16 ? a.w : ssrc;
+  // Loads of 16 bytes with no branch around them: they end within the row, and where it has
+  // fewer than 16 something is loaded that is not read.
+  const uint8_t* sfrom = nb < 16 ? a.w : ssrc;
   const int slast = max(nb - 16, 0);
-  u32x4_t sreg = nb < 16 ? load_short_row(ssrc, nb) : *reinterpret_cast<const loose_u32x4*>(ssrc);
-  if (tid < kTileN)
-    reinterpret_cast<float*>(lds + kBiasOff)[tid] =
-        a.bias ? bf16_to_f32(a.bias[wrow + min(n0 + tid, a.N - 1)]) : 0.0f;
-  if (scaled) *reinterpret_cast<u32x4_t*>(lds + kScaleOff + 16 * tid) = sreg;
+  u32x4_t sreg[2];
+  auto load_scales = [&](int c) __attribute__((always_inline)) {  // of chunks c to c + 3
 #pragma unroll
-  for (int c = 0; c < kStages; ++c) issue(c);
+    for (int i = 0; i < 2; ++i) sreg[i] = *reinterpret_cast<const loose_u32x4*>(sfrom + min(kBlocks * c + 16 * i, slast));
+  };
+  auto put_scales = [&](int c) __attribute__((always_inline)) {
+    // (threads past the last row store what nobody reads: a branch here would cost a wait for all loads)
+    gx_u32x2* to = reinterpret_cast<gx_u32x2*>(lds + kScaleOff) + ((c >> 2) & 1) * 2048 + tid;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int early = kBlocks * c + 16 * i + 16 - nb;
+      if (early > 0) sreg[i] = early < 16 ? shift_bytes(sreg[i], early) : u32x4_t{0u, 0u, 0u, 0u};
+      to[1024 * i] = gx_u32x2{sreg[i][0], sreg[i][1]};
+      to[1024 * i + 512] = gx_u32x2{sreg[i][2], sreg[i][3]};
+    }
+  };
+  issue(0);
+  issue(1);
+  if (nb < 16) {
+    sreg[0] = load_short_row(ssrc, nb);
+    sreg[1] = u32x4_t{0u, 0u, 0u, 0u};
+    gx_u32x2* to = reinterpret_cast<gx_u32x2*>(lds + kScaleOff) + tid;
+    to[0] = gx_u32x2{sreg[0][0], sreg[0][1]};
+    to[512] = gx_u32x2{sreg[0][2], sreg[0][3]};
+  } else {
+    load_scales(0);
+    put_scales(0);
+  }
 
   f32x16_t acc[NT][MT];
 #pragma unroll
@@ -132,84 +152,123 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
       for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
 
   const int wrow_l = 32 * NT * wn + r, arow_l = kTileN + 32 * MT * wm + r;
-  const int piece0 = 16 * (half ^ ((r >> 2) & 3));  // of step 0; of step 1: ^ 32
+  const int piece0 = half ^ ((r >> 1) & 7);  // of step 0; of step s: ^ 2 s
   u32x4_t wv[2][NT], av[2][MT];
-  uint32_t sw[NT], sa[MT];
+  gx_u32x2 sw[NT], sa[MT];
   auto read = [&](int c, int s, u32x4_t(&wo)[NT], u32x4_t(&ao)[MT]) __attribute__((always_inline)) {
-    const uint8_t* stage = lds + (c & (kStages - 1)) * kStageBytes + (piece0 ^ (32 * s));
+    const uint8_t* stage = lds + (c & 1) * kStageBytes + 16 * (piece0 ^ (2 * s));
 #pragma unroll
-    for (int i = 0; i < NT; ++i) wo[i] = *reinterpret_cast<const u32x4_t*>(stage + 64 * wrow_l + 2048 * i);
+    for (int i = 0; i < NT; ++i) wo[i] = *reinterpret_cast<const u32x4_t*>(stage + 128 * wrow_l + 4096 * i);
 #pragma unroll
-    for (int j = 0; j < MT; ++j) ao[j] = *reinterpret_cast<const u32x4_t*>(stage + 64 * arow_l + 2048 * j);
+    for (int j = 0; j < MT; ++j) ao[j] = *reinterpret_cast<const u32x4_t*>(stage + 128 * arow_l + 4096 * j);
   };
-  // A lane's byte of step s is block 2 s + half of the chunk's four.
   auto read_scales = [&](int c) __attribute__((always_inline)) {
-    const uint8_t* at = lds + kScaleOff + ((c >> 2) & 1) * (512 * 16) + 4 * (c & 3);
+    const gx_u32x2* at = reinterpret_cast<const gx_u32x2*>(lds + kScaleOff) + 512 * (c & 7);
 #pragma unroll
-    for (int i = 0; i < NT; ++i) sw[i] = *reinterpret_cast<const uint32_t*>(at + 16 * (wrow_l + 32 * i)) >> (8 * half);
+    for (int i = 0; i < NT; ++i) sw[i] = at[wrow_l + 32 * i];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) sa[j] = *reinterpret_cast<const uint32_t*>(at + 16 * (arow_l + 32 * j)) >> (8 * half);
+    for (int j = 0; j < MT; ++j) sa[j] = at[arow_l + 32 * j];
   };
 
-  wait_vm<L*(kStages - 1)>();
+  wait_vm<0>();
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   read_scales(0);
   read(0, 0, wv[0], av[0]);
 
+  // The products above stay above: without this the compiler gathers those of several
+  // chunks behind the last one's barrier, and keeps all their operands.
+  auto pin = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) asm volatile("" : "+v"(acc[i][j]));
+  };
   int c = 0;
+  // Step s's products; the scale of block 2 s + half is byte 0 or 2 of what is left of the
+  // row's dword s / 2 after a shift by the lane's half.
+  uint32_t ow[NT], oa[MT];
+  auto shift = [&](int d) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) ow[i] = sw[i][d] >> (8 * half);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) oa[j] = sa[j][d] >> (8 * half);
+  };
+  auto products = [&](auto odd) __attribute__((always_inline)) {
+    constexpr int kOdd = decltype(odd)::value;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(wv[kOdd][i]), mx_operand(av[kOdd][j]), acc[i][j],
+                                                                    4, 4, 2 * kOdd, static_cast<int>(ow[i]), 2 * kOdd,
+                                                                    static_cast<int>(oa[j]));
+    pin();
+  };
+  // The next step's reads go out behind the first products of this one.
+  auto order = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < (NT + MT + 1) / 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+  };
+  const std::integral_constant<int, 0> p0{};
+  const std::integral_constant<int, 1> p1{};
+  const std::integral_constant<int, 2> p2{};
+  const std::integral_constant<int, 3> p3{};
   auto chunk = [&](auto place) __attribute__((always_inline)) {
     constexpr int kPlace = decltype(place)::value;  // c % 4
     read(c, 1, wv[1], av[1]);
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < MT; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(wv[0][i]), mx_operand(av[0][j]), acc[i][j], 4, 4,
-                                                                    0, static_cast<int>(sw[i]), 0, static_cast<int>(sa[j]));
-    if constexpr (kPlace == 3) {
-      const int early = 4 * (c + 1) + 16 - nb;
-      if (early > 0 && early < 16) sreg = shift_bytes(sreg, early);
-      if (scaled) *reinterpret_cast<u32x4_t*>(lds + kScaleOff + (((c >> 2) + 1) & 1) * (512 * 16) + 16 * tid) = sreg;
-    }
+    shift(0);
+    products(p0);
+    order();
     __builtin_amdgcn_sched_barrier(0);
-    wait_vm<L*(kStages - 2)>();          // this wave's loads of chunk c + 1
+    read(c, 2, wv[0], av[0]);
+    products(p1);
+    order();
+    __builtin_amdgcn_sched_barrier(0);
+    read(c, 3, wv[1], av[1]);
+    shift(1);
+    products(p0);
+    if constexpr (kPlace == 3) put_scales(c + 1);
+    order();
+    __builtin_amdgcn_sched_barrier(0);
+    wait_vm<0>();                        // this wave's loads of chunk c + 1
     __builtin_amdgcn_s_waitcnt(0xc07f);  // its reads of chunk c
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    uint32_t ow[NT], oa[MT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) ow[i] = sw[i];
-#pragma unroll
-    for (int j = 0; j < MT; ++j) oa[j] = sa[j];
     read_scales(c + 1);
     read(c + 1, 0, wv[0], av[0]);
-    issue(c + kStages);
-    if constexpr (kPlace == 0) sreg = *reinterpret_cast<const loose_u32x4*>(snext + min(4 * (c + 4), slast));
+    issue(c + 2);
+    if constexpr (kPlace == 0) load_scales(c + 4);
+    products(p1);
+    order();
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < MT; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(wv[1][i]), mx_operand(av[1][j]), acc[i][j], 4, 4,
-                                                                    2, static_cast<int>(ow[i]), 2, static_cast<int>(oa[j]));
+    for (int i = 0; i < NT * MT; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, 3, 0);
+    }
     __builtin_amdgcn_sched_barrier(0);
   };
-  for (;;) {
-    chunk(std::integral_constant<int, 0>{});
-    if (++c == nch) break;
-    chunk(std::integral_constant<int, 1>{});
-    if (++c == nch) break;
-    chunk(std::integral_constant<int, 2>{});
-    if (++c == nch) break;
-    chunk(std::integral_constant<int, 3>{});
-    if (++c == nch) break;
+  // (no way out between the chunks of four: it would cost a wait for all loads at the top)
+  for (int left = nch >> 2; left > 0; --left) {
+    chunk(p0), ++c;
+    chunk(p1), ++c;
+    chunk(p2), ++c;
+    chunk(p3), ++c;
   }
+  for (; c < nch; ++c) chunk(p1);  // up to three, whose scales are there
   // the ring becomes the waves' own room, 16 KiB each: no load may still land in it
   wait_vm<0>();
   __builtin_amdgcn_s_waitcnt(0xc07f);
   __builtin_amdgcn_s_barrier();
 
-  const float* bias = reinterpret_cast<const float*>(lds + kBiasOff) + 32 * NT * wn;
+  float* bias_all = reinterpret_cast<float*>(lds + kScaleOff);
+  if (tid < kTileN) bias_all[tid] = a.bias ? bf16_to_f32(a.bias[wrow + min(n0 + tid, a.N - 1)]) : 0.0f;
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  __builtin_amdgcn_s_barrier();
+  const float* bias = bias_all + 32 * NT * wn;
   uint8_t* own = lds + 16384 * w;
   const int cols = a.swiglu ? a.N / 2 : a.N;
   constexpr int kG = NT < 2 ? NT : 2;  // column tiles that go together
