@@ -59,6 +59,8 @@ struct MxProductArgs {
   bool vec;  // out's rows and their pieces of 16 bytes are on 16 bytes
 };
 hipError_t launch_mx_tile(const MxProductArgs& a, hipStream_t s);
+// nt x 16 columns and mt x 16 rows of a wave, ks waves along K
+hipError_t launch_mx_stream(const MxProductArgs& a, int nt, int mt, int ks, hipStream_t s);
 hipError_t launch_mx_product(const MxProductArgs& a, hipStream_t s);
 
 }  // namespace gxmoe

@@ -7,6 +7,8 @@
 // bits, across blocks of any scales and with the accumulator.  The weights are its
 // first operand, so a lane ends with 16 results of one row (token) l % 32: columns
 // 8 (i / 4) + 4 (l / 32) + i % 4 of the tile's 32.
+#include <cstdio>
+#include <cstdlib>
 #include "mx_device.h"
 #include "mx_kernels.h"
 
@@ -191,6 +193,12 @@ __global__ __launch_bounds__(kWaves * kWave) void product_kernel(MxProductArgs a
 }  // namespace
 
 hipError_t launch_mx_product(const MxProductArgs& a, hipStream_t s) {
+  const char* f = getenv("MX_FORCE");
+  if (f) {
+    int nt, mt, ks;
+    if (f[0] == 't') return launch_mx_tile(a, s);
+    if (sscanf(f, "%d,%d,%d", &nt, &mt, &ks) == 3) return launch_mx_stream(a, a.out_packed ? (a.swiglu ? 4 : (nt < 2 ? 2 : nt)) : nt, mt, ks, s);
+  }
   if (a.rows > 64) return launch_mx_tile(a, s);
   const int tiles = a.offsets ? a.rows / kTileM + (a.E < a.rows ? a.E : a.rows) : (a.rows + kTileM - 1) / kTileM;
   const int n_groups = (a.N + kWaves * kTileN - 1) / (kWaves * kTileN);
