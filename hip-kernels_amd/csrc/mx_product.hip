@@ -197,7 +197,7 @@ hipError_t launch_mx_product(const MxProductArgs& a, hipStream_t s) {
   if (f) {
     int nt, mt, ks;
     if (f[0] == 't') return launch_mx_tile(a, s);
-    if (sscanf(f, "%d,%d,%d", &nt, &mt, &ks) == 3 && a.K >= 512) return launch_mx_stream(a, a.out_packed ? (a.swiglu ? 4 : (nt < 2 ? 2 : nt)) : nt, mt, ks, s);
+    if (sscanf(f, "%d,%d,%d", &nt, &mt, &ks) == 3 && a.K >= 512) return launch_mx_stream(a, a.out_packed ? 2 : nt, mt, ks, s);
   }
   if (a.rows > 64) return launch_mx_tile(a, s);
   const int tiles = a.offsets ? a.rows / kTileM + (a.E < a.rows ? a.E : a.rows) : (a.rows + kTileM - 1) / kTileM;
