@@ -1214,18 +1214,28 @@ def select_experts(logits, top_k: int, score: str = "softmax", bias=None, num_gr
     neighbours only the top_groups stay whose group_rank (1 or 2) best choices sum highest.  renormalize: weights over
     their sum; scale: a factor of them.  Ties go to the lower index; a logit or bias of -inf switches an expert off (it
     has weight 0 and comes after the others).  out: preallocated (indices, weights)."""
-    T, E, stride = _strided_rows("logits", logits, (torch.bfloat16, torch.float32))
+    if isinstance(logits, torch.Tensor) and logits.dim() == 2 and logits.is_contiguous() \
+            and (logits.dtype is torch.bfloat16 or logits.dtype is torch.float32):
+        T, E = logits.shape
+        stride = E
+    else:
+        T, E, stride = _strided_rows("logits", logits, (torch.bfloat16, torch.float32))
     dev = logits.device
     _, cfg = _routing_config(score, top_k, num_groups, top_groups, group_rank, bool(renormalize), float(scale))
     if bias is not None:
         _vector("bias", bias, dev, E, torch.float32)
         bias = bias.data_ptr()
     if out is None:
-        _gpu("logits", dev)
+        if dev.type != "cuda":
+            _gpu("logits", dev)
         if top_k > E:
             _bad(f"top_k={top_k} of {E} experts")
-        idx = _empty((T, top_k), torch.int32, dev, stream)
-        w = _empty((T, top_k), torch.float32, dev, stream)
+        if stream is None:
+            idx = logits.new_empty((T, top_k), dtype=torch.int32)
+            w = logits.new_empty((T, top_k), dtype=torch.float32)
+        else:
+            idx = _empty((T, top_k), torch.int32, dev, stream)
+            w = _empty((T, top_k), torch.float32, dev, stream)
     else:
         idx, w = out
         for name, t, dtype in (("indices", idx, torch.int32), ("weights", w, torch.float32)):
@@ -1246,7 +1256,7 @@ class MXFP4Matrix:
     [.., rows, K / 2] (low nibble = even k) and scales uint8 [.., rows, K / 32], both contiguous.  Value = e2m1 *
     2^(scale - 127).  Fixed once made."""
 
-    __slots__ = ("packed", "scales", "device", "experts", "rows", "K", "_packed", "_scales")
+    __slots__ = ("_held", "_tensors", "_device", "_experts", "_rows", "_K", "_packed", "_scales")
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor):
         for name, t in (("packed", packed), ("scales", scales)):
@@ -1261,33 +1271,45 @@ class MXFP4Matrix:
             _bad("K must be positive")
         if packed.device != scales.device:
             _bad(f"packed is on {packed.device}, scales are on {scales.device}")
-        self._set(packed, scales, packed.shape[0] if packed.dim() == 3 else None, packed.shape[-2], 2 * packed.shape[-1])
-
-    def _set(self, packed, scales, experts, rows, K):
-        put = object.__setattr__
-        put(self, "packed", packed)
-        put(self, "scales", scales)
-        put(self, "device", packed.device)
-        put(self, "experts", experts)
-        put(self, "rows", rows)
-        put(self, "K", K)
-        put(self, "_packed", packed.data_ptr())
-        put(self, "_scales", scales.data_ptr())
-        return self
+        self._held, self._tensors, self._device = None, (packed, scales), packed.device
+        self._experts = packed.shape[0] if packed.dim() == 3 else None
+        self._rows, self._K = packed.shape[-2], 2 * packed.shape[-1]
+        self._packed, self._scales = packed.data_ptr(), scales.data_ptr()
 
     @classmethod
-    def _empty(cls, rows, K, device, stream):
-        return cls.__new__(cls)._set(_empty((rows, K // 2), torch.uint8, device, stream),
-                                     _empty((rows, K // 32), torch.uint8, device, stream), None, rows, K)
+    def _empty(cls, rows, K, like, device, stream):
+        """A new [rows, K]: one allocation, whose tensors are made when they are asked for."""
+        n = rows * K
+        self = cls.__new__(cls)
+        if stream is None and like is not None:
+            self._held = like.new_empty((n // 32 * 17,), dtype=torch.uint8)
+        else:
+            self._held = _empty((n // 32 * 17,), torch.uint8, device, stream)
+        self._tensors, self._device, self._experts, self._rows, self._K = None, device, None, rows, K
+        self._packed = where = self._held.data_ptr()
+        self._scales = where + n // 2
+        return self
+
+    def _both(self):
+        if self._tensors is None:
+            n = self._rows * self._K
+            self._tensors = (self._held[:n // 2].view(self._rows, self._K // 2),
+                             self._held[n // 2:].view(self._rows, self._K // 32))
+        return self._tensors
+
+    def _fixed(self, *_):
+        raise AttributeError("an MXFP4Matrix is fixed: calls use the tensors it was made with")
+
+    packed = property(lambda self: self._both()[0], _fixed, _fixed)
+    scales = property(lambda self: self._both()[1], _fixed, _fixed)
+    device = property(lambda self: self._device, _fixed, _fixed)
+    experts = property(lambda self: self._experts, _fixed, _fixed, "of a stack; None of a single matrix")
+    rows = property(lambda self: self._rows, _fixed, _fixed)
+    K = property(lambda self: self._K, _fixed, _fixed)
 
     @property
     def shape(self):
-        return (self.rows, self.K) if self.experts is None else (self.experts, self.rows, self.K)
-
-    def __setattr__(self, name, value):
-        raise AttributeError(f"MXFP4Matrix.{name} is fixed: calls use the tensors it was made with")
-
-    __delattr__ = lambda self, name: self.__setattr__(name, None)  # noqa: E731
+        return (self._rows, self._K) if self._experts is None else (self._experts, self._rows, self._K)
 
     def __repr__(self):
         return f"<gptoss_moe.MXFP4Matrix {'x'.join(str(n) for n in self.shape)} on {self.device}>"
@@ -1296,8 +1318,8 @@ class MXFP4Matrix:
 def _matrix(name: str, m, device=None) -> "MXFP4Matrix":
     if not isinstance(m, MXFP4Matrix):
         _bad(f"{name} must be an MXFP4Matrix, got {type(m).__name__}")
-    if device is not None and m.device != device:
-        _bad(f"{name} is on {m.device}, expected {device}")
+    if device is not None and m._device != device:
+        _bad(f"{name} is on {m._device}, expected {device}")
     return m
 
 
@@ -1305,19 +1327,26 @@ def mxfp4_quantize(x, out: MXFP4Matrix | None = None, stream=None) -> MXFP4Matri
     """x [rows, K] (bfloat16 or float32, rows a multiple of 16 bytes apart, K a multiple of 32) as MXFP4: each 32 values
     share the power of two 2^(floor(log2(largest)) - 2) and are rounded to the nearest e2m1 value, at most 6 of it.  A
     block with an infinity or NaN becomes NaN.  out: a matrix of that shape to write to."""
-    rows, K, stride = _strided_rows("x", x, (torch.bfloat16, torch.float32))
+    if isinstance(x, torch.Tensor) and x.dim() == 2 and x.is_contiguous() \
+            and (x.dtype is torch.bfloat16 or x.dtype is torch.float32):
+        rows, K = x.shape
+        stride = K
+    else:
+        rows, K, stride = _strided_rows("x", x, (torch.bfloat16, torch.float32))
+        stride = stride or K
     dev = x.device
-    if K % 32 or not K:
+    if K & 31 or not K:
         _bad(f"x has {K} columns, a positive multiple of 32 is needed")
     if out is None:
-        _gpu("x", dev)
-        out = MXFP4Matrix._empty(rows, K, dev, stream)
+        if dev.type != "cuda":
+            _gpu("x", dev)
+        out = MXFP4Matrix._empty(rows, K, x, dev, stream)
     else:
         _matrix("out", out, dev)
         if out.shape != (rows, K):
             _bad(f"out has shape {out.shape}, expected {(rows, K)}")
         _gpu("x", dev)
-    _launch(dev, stream, _lib.gptoss_mxfp4_quantize, x.data_ptr(), stride or K, 1 if x.dtype is torch.float32 else 0, rows, K,
+    _launch(dev, stream, _lib.gptoss_mxfp4_quantize, x.data_ptr(), stride, 1 if x.dtype is torch.float32 else 0, rows, K,
             out._packed, out._scales)
     return out
 
@@ -1326,46 +1355,50 @@ def mxfp4_dequantize(m: MXFP4Matrix, dtype=torch.bfloat16, out=None, stream=None
     """The values of m, [rows, K] ([experts, rows, K] of a stack), bfloat16 or float32 (exact in both).  out: a 2-D
     tensor [experts * rows, K], rows a multiple of 16 bytes apart."""
     _matrix("m", m)
-    rows, K = (m.experts or 1) * m.rows if m.experts is None or m.experts else 0, m.K
+    dev, K = m._device, m._K
+    rows = m._rows if m._experts is None else m._experts * m._rows
     if out is None:
         if dtype is not torch.bfloat16 and dtype is not torch.float32:
             _bad(f"dtype must be torch.bfloat16 or torch.float32, got {dtype}")
-        _gpu("m", m.device)
-        out, stride = _empty(m.shape, dtype, m.device, stream), K
+        if dev.type != "cuda":
+            _gpu("m", dev)
+        out, stride = _empty(m.shape, dtype, dev, stream), K
     else:
-        have, cols, stride = _strided_rows("out", out, (torch.bfloat16, torch.float32), m.device)
+        have, cols, stride = _strided_rows("out", out, (torch.bfloat16, torch.float32), dev)
         if (have, cols) != (rows, K):
             _bad(f"out has shape {tuple(out.shape)}, expected {(rows, K)}")
         stride, dtype = stride or K, out.dtype
-        _gpu("m", m.device)
-    _launch(m.device, stream, _lib.gptoss_mxfp4_dequantize, m._packed, m._scales, rows, K, out.data_ptr(), stride,
+        _gpu("m", dev)
+    _launch(dev, stream, _lib.gptoss_mxfp4_dequantize, m._packed, m._scales, rows, K, out.data_ptr(), stride,
             1 if dtype is torch.float32 else 0)
     return out
 
 
 def _product(a, w, rows, offsets, row_index, bias, swiglu, alpha, limit, dtype, quantize, out, stream):
-    _matrix("a", a)
-    dev = a.device
-    _matrix("w", w, dev)
-    if a.experts is not None:
+    dev = a._device
+    if w._device != dev:
+        _bad(f"w is on {w._device}, expected {dev}")
+    if a._experts is not None:
         _bad(f"a must be one matrix, got a stack of shape {a.shape}")
-    if a.K != w.K:
-        _bad(f"a has K={a.K}, w has K={w.K}")
-    N = w.rows
+    K = a._K
+    if K != w._K:
+        _bad(f"a has K={K}, w has K={w._K}")
+    N, E = w._rows, w._experts
     cols = N // 2 if swiglu else N
     if bias is not None:
-        want = (N,) if w.experts is None else (w.experts, N)
+        want = (N,) if E is None else (E, N)
         if not (isinstance(bias, torch.Tensor) and bias.dtype is torch.bfloat16 and bias.shape == want
                 and bias.is_contiguous() and bias.device == dev):
             _on_device("bias", bias, dev, torch.bfloat16)
             _bad(f"bias must be contiguous of shape {want}, got {tuple(bias.shape)}")
         bias = bias.data_ptr()
     if quantize:
-        if cols % 32 or not cols:
+        if cols & 31 or not cols:
             _bad(f"MXFP4 results of {cols} columns, a positive multiple of 32 is needed")
         if out is None:
-            _gpu("a", dev)
-            out = MXFP4Matrix._empty(rows, cols, dev, stream)
+            if dev.type != "cuda":
+                _gpu("a", dev)
+            out = MXFP4Matrix._empty(rows, cols, a._held, dev, stream)
         else:
             _matrix("out", out, dev)
             if out.shape != (rows, cols):
@@ -1376,22 +1409,27 @@ def _product(a, w, rows, offsets, row_index, bias, swiglu, alpha, limit, dtype, 
         if out is None:
             if dtype is not torch.bfloat16 and dtype is not torch.float32:
                 _bad(f"dtype must be torch.bfloat16 or torch.float32, got {dtype}")
-            _gpu("a", dev)
-            out, stride = _empty((rows, cols), dtype, dev, stream), cols
+            if dev.type != "cuda":
+                _gpu("a", dev)
+            like = a._held
+            if stream is None and like is not None:
+                out = like.new_empty((rows, cols), dtype=dtype)
+            else:
+                out = _empty((rows, cols), dtype, dev, stream)
+            stride = cols
         else:
             have, wide, stride = _strided_rows("out", out, (torch.bfloat16, torch.float32), dev)
             if (have, wide) != (rows, cols):
                 _bad(f"out has shape {tuple(out.shape)}, expected {(rows, cols)}")
             stride, dtype = stride or cols, out.dtype
             _gpu("a", dev)
-        res = Mxfp4Result(1 if swiglu else 0, alpha, limit, 1 if dtype is torch.float32 else 0, out.data_ptr(), stride, None,
-                          None)
+        res = Mxfp4Result(1 if swiglu else 0, alpha, limit, 1 if dtype is torch.float32 else 0, out.data_ptr(), stride)
     where = ctypes.addressof(res)
     if offsets is None:
-        _launch(dev, stream, _lib.gptoss_mxfp4_matmul, a._packed, a._scales, rows, w._packed, w._scales, bias, N, a.K, where)
+        _launch(dev, stream, _lib.gptoss_mxfp4_matmul, a._packed, a._scales, rows, w._packed, w._scales, bias, N, K, where)
     else:
-        _launch(dev, stream, _lib.gptoss_moe_grouped_mxfp4_matmul, a._packed, a._scales, a.rows, row_index,
-                offsets.data_ptr(), w.experts, rows, w._packed, w._scales, bias, N, a.K, where)
+        _launch(dev, stream, _lib.gptoss_moe_grouped_mxfp4_matmul, a._packed, a._scales, a._rows, row_index,
+                offsets.data_ptr(), E, rows, w._packed, w._scales, bias, N, K, where)
     return out
 
 
@@ -1400,9 +1438,9 @@ def mxfp4_matmul(a: MXFP4Matrix, w: MXFP4Matrix, bias=None, swiglu: bool = False
     """a [M, K] times w [N, K] transposed, plus bias (bfloat16 [N]): [M, N], summed in fp32.  swiglu: column pairs (gate,
     up) through the clamped SwiGLU, [M, N / 2].  The result is of dtype (bfloat16 or float32), or with quantize an
     MXFP4Matrix.  out: a tensor (rows any distance apart; its dtype counts) or an MXFP4Matrix."""
-    if _matrix("w", w).experts is not None:
+    if _matrix("w", w)._experts is not None:
         _bad(f"w is a stack of shape {w.shape}: grouped_mxfp4_matmul takes these")
-    return _product(a, w, _matrix("a", a).rows, None, None, bias, swiglu, alpha, limit, dtype, quantize, out, stream)
+    return _product(a, w, _matrix("a", a)._rows, None, None, bias, swiglu, alpha, limit, dtype, quantize, out, stream)
 
 
 def grouped_mxfp4_matmul(a: MXFP4Matrix, w: MXFP4Matrix, offsets, rows: int, row_index=None, bias=None,
@@ -1412,12 +1450,12 @@ def grouped_mxfp4_matmul(a: MXFP4Matrix, w: MXFP4Matrix, offsets, rows: int, row
     row p of [rows, N], offsets[e] <= p < offsets[e + 1] (int32 [E + 1], permute_plan's), that of row row_index[p] (int32
     [rows], its perm_token; None: p) of a.  Rows of no expert are left as they were (unset where out is allocated
     here)."""
-    if _matrix("w", w).experts is None:
+    if _matrix("w", w)._experts is None:
         _bad(f"w must be a stack [experts, N, K], got shape {w.shape}")
-    dev = _matrix("a", a).device
+    dev = _matrix("a", a)._device
     if not 0 <= rows <= _INT_MAX:
         _bad(f"rows={rows} must not be negative and below 2^31")
-    _vector("offsets", offsets, dev, w.experts + 1, torch.int32)
+    _vector("offsets", offsets, dev, w._experts + 1, torch.int32)
     if row_index is not None:
         _vector("row_index", row_index, dev, rows, torch.int32)
         row_index = row_index.data_ptr()
