@@ -58,9 +58,19 @@ struct MxProductArgs {
   uint8_t* out_scales;
   bool vec;  // out's rows and their pieces of 16 bytes are on 16 bytes
 };
-hipError_t launch_mx_tile(const MxProductArgs& a, hipStream_t s);
-// nt x 16 columns and mt x 16 rows of a wave, ks waves along K
-hipError_t launch_mx_stream(const MxProductArgs& a, int nt, int mt, int ks, hipStream_t s);
+constexpr int kMxCus = 256;  // of the card
+
+// m-tiles of `rows` rows that the call can have: each expert's last one may be a part.
+inline int64_t most_m_tiles(const MxProductArgs& a, int rows) {
+  return a.offsets ? a.rows / rows + (a.E < a.rows ? a.E : a.rows) : (static_cast<int64_t>(a.rows) + rows - 1) / rows;
+}
+
+// Tiles of 256 x 256, of 128 x 128 (rows x columns) or of 32 x 128.
+enum class MxTile { large, middle, low };
+hipError_t launch_mx_tile(const MxProductArgs& a, MxTile kind, hipStream_t s);
+// 16 rows x 16 columns of a wave, 32 if `wide` (so for MXFP4 results); four waves along K if `split`.
+constexpr int kStreamRows = 16;
+hipError_t launch_mx_stream(const MxProductArgs& a, bool wide, bool split, hipStream_t s);
 hipError_t launch_mx_product(const MxProductArgs& a, hipStream_t s);
 
 }  // namespace gxmoe

@@ -1,7 +1,7 @@
 // mx_stream.hip -- MXFP4 products of few rows: the weights stream through LDS, wave by
 // wave.
 //
-// A wave computes up to 16 MT rows x 16 NT columns over its share of K with
+// A wave computes up to 16 rows x 16 NT columns over its share of K with
 // v_mfma_scale_f32_16x16x128_f8f6f4 (lane l gives row l % 16 of each operand and block l / 16 of
 // four; it ends with columns 4 (l / 16) + {0 .. 3} of row l % 16).  Its weight rows come line by
 // line (128 bytes, eight blocks) into a ring of four lines each, by direct global -> LDS loads, and out
@@ -42,9 +42,9 @@ __host__ __device__ constexpr int scale_pitch(int nb) {
 }
 
 // LDS of a wave: its ring, its scales and, of several, its sums.
-template <int NT, int MT, int KS>
+template <int NT, int KS>
 __host__ __device__ constexpr int wave_bytes(int nb) {
-  return kRing * NT * 2048 + 16 * NT * scale_pitch(nb) + (KS > 1 ? NT * MT * 1024 : 0);
+  return kRing * NT * 2048 + 16 * NT * scale_pitch(nb) + (KS > 1 ? NT * 1024 : 0);
 }
 
 // Neighbouring results of a row from column n on: rounded to bf16 unless fp32, as one store
@@ -158,10 +158,10 @@ __device__ __forceinline__ void write_rows(const MxProductArgs& a, const f32x4_t
   }
 }
 
-template <int NT, int MT, int KS>
+template <int NT, int KS>
 __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles, uint8_t* lds) {
-  constexpr int kM = 16 * MT, kN = 16 * NT, kLine = NT * 2048;
-  constexpr int kLoads = 2 * NT + 4 * MT;  // of a line of the rows, and a chunk of a's
+  constexpr int kN = 16 * NT, kLine = NT * 2048;
+  constexpr int kLoads = 2 * NT + 4;  // of a line of the rows, and a chunk of a's
   constexpr int kLanes = kWave / kN;       // per weight row, for its scales
   constexpr int kPieces = (kSpan / 16 + kLanes - 1) / kLanes;
   static_assert((kRing - 2) * kLoads < 64, "vmcnt range");
@@ -169,7 +169,7 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles
   // This work-group's run of tiles, the columns of an m-tile in turn; XCD b % 8 has neighbouring runs.  Tiles whose
   // results make one block go together.
   const int together = a.swiglu && a.out_packed ? 2 : 1;
-  const int64_t total = static_cast<int64_t>(count_m_tiles(a, kM, lane)) * (n_tiles / together);
+  const int64_t total = static_cast<int64_t>(count_m_tiles(a, kStreamRows, lane)) * (n_tiles / together);
   const int b = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
   int id = static_cast<int>(total * b / gridDim.x) * together;
   const int id_end = static_cast<int>(total * (b + 1) / gridDim.x) * together;
@@ -181,7 +181,7 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles
   const int begin = 8 * first, end = min(8 * last, nb);        // its blocks
   const size_t row_bytes = 16 * static_cast<size_t>(nb);
   const int pitch = scale_pitch(nb);
-  uint8_t* const ring = lds + k * wave_bytes<NT, MT, KS>(nb);
+  uint8_t* const ring = lds + k * wave_bytes<NT, KS>(nb);
   uint8_t* const scales = ring + kRing * kLine;
 
   while (id < id_end) {
@@ -189,24 +189,11 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles
     int n0 = (id - m * n_tiles) * kN;
     int left = min(id_end, (m + 1) * n_tiles) - id;  // tiles of these rows
     id += left;
-    const MTile mt = find_m_tile(a, m, kM, lane);
-    const uint8_t *ap[MT], *asp[MT];
-    bool zero[MT];
-    {
-      int src[MT];
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const int p = min(mt.lo + 16 * j + r, mt.hi - 1);  // past the last row: that one
-        src[j] = a.row_index ? a.row_index[p] : p;
-      }
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        zero[j] = src[j] < 0 || src[j] >= a.a_rows;  // not a row of a: its result is replaced
-        src[j] = zero[j] ? 0 : src[j];
-        ap[j] = a.a + static_cast<size_t>(src[j]) * row_bytes;
-        asp[j] = a.as + static_cast<size_t>(src[j]) * nb;
-      }
-    }
+    const MTile mt = find_m_tile(a, m, kStreamRows, lane);
+    const int p = min(mt.lo + r, mt.hi - 1);  // past the last row: that one
+    const int src = source_row(a, p);         // < 0: its result is replaced
+    const uint8_t* const ap = a.a + static_cast<size_t>(max(src, 0)) * row_bytes;
+    const uint8_t* const asp = a.as + static_cast<size_t>(max(src, 0)) * nb;
     const uint8_t* const w = a.w + static_cast<size_t>(mt.e) * a.N * row_bytes;
     const uint8_t* const ws = a.ws + static_cast<size_t>(mt.e) * a.N * nb;
     // Where a row begins in its first line, in blocks, and how many lines the wave's blocks can take; the ring goes
@@ -217,19 +204,16 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles
     const int furthest = 8 - unit + static_cast<int>(w16 % unit);
     const int turns = ((end - 1 - begin + furthest) / 8 + kRing) / kRing;
 
-    u32x4_t av[kRing][2][MT];
-    uint32_t sa[kRing][2][MT];
+    u32x4_t av[kRing][2];
+    uint32_t sa[kRing][2];
     // Loads of line `line` of the columns from n on, and of a's chunk of that number.  Blocks past the end are the last one
     // again: there are no branches around loads, which would cost waits for all of them.
     auto issue = [&](int slot, int n, int line) __attribute__((always_inline)) {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const uint32_t at = min(begin + 8 * line + 4 * q + g, end - 1);
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          av[slot][q][j] = *reinterpret_cast<const u32x4_t*>(ap[j] + 16 * static_cast<size_t>(at));
-          sa[slot][q][j] = asp[j][at];
-        }
+        av[slot][q] = *reinterpret_cast<const u32x4_t*>(ap + 16 * static_cast<size_t>(at));
+        sa[slot][q] = asp[at];
       }
       // Row 8 i + lane / 8: place lane % 8 of its 128 bytes in LDS holds block (lane % 8) ^ (row / 2) % 8 of the line, so
       // that 16 rows meet all banks.
@@ -259,18 +243,15 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles
       }
     };
 
-    f32x4_t acc[NT][MT], held[MT];
+    f32x4_t acc[NT], held = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     int from[NT];  // where the lane's rows begin
     auto open = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         from[i] = offset(min(n0 + 16 * i + r, a.N - 1));
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
       }
     };
-#pragma unroll
-    for (int j = 0; j < MT; ++j) held[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     open();
     int turn = 0;
     if (begin < end) {
@@ -305,7 +286,7 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles
               const bool in = begin + rel < upto;                      // past the end they are zeros of a
               const int at = min(begin + rel, upto - 1), piece = (at - span) >> 4;
               const int place = max(0, 16 * piece + at - min(span + 16 * piece, nb - 16));
-              u32x4_t wv[NT], x[MT];
+              u32x4_t wv[NT], x;
               uint32_t sw[NT];
 #pragma unroll
               for (int i = 0; i < NT; ++i) {
@@ -315,16 +296,12 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles
                 sw[i] = scales[(16 * i + r) * pitch + place];
               }
 #pragma unroll
-              for (int j = 0; j < MT; ++j)
-#pragma unroll
-                for (int d = 0; d < 4; ++d) x[j][d] = in ? av[slot][q][j][d] : 0u;
+              for (int d = 0; d < 4; ++d) x[d] = in ? av[slot][q][d] : 0u;
 #pragma unroll
               for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int j = 0; j < MT; ++j)
-                  acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(wv[i]), mx_operand(x[j]), acc[i][j],
-                                                                               4, 4, 0, static_cast<int>(sw[i]), 0,
-                                                                               static_cast<int>(sa[slot][q][j]));
+                acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(wv[i]), mx_operand(x), acc[i], 4, 4, 0,
+                                                                          static_cast<int>(sw[i]), 0,
+                                                                          static_cast<int>(sa[slot][q]));
             }
             __builtin_amdgcn_s_waitcnt(0xc07f);  // the line has been read
             __builtin_amdgcn_sched_barrier(0);
@@ -335,40 +312,24 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles
         put_scales();
       }
       if (!ends) continue;
+      const bool live = mt.lo + r < mt.hi;
       if constexpr (KS > 1) {
-        // Wave k sums row tile k of all waves, in turn.
-        const int stride = wave_bytes<NT, MT, KS>(nb) / 16;  // between two waves' sums
+        // The first wave sums those of all, in turn.
+        const int stride = wave_bytes<NT, KS>(nb) / 16;  // between two waves' sums
         f32x4_t* const sums = reinterpret_cast<f32x4_t*>(lds + kRing * kLine + kN * pitch);
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int j = 0; j < MT; ++j) sums[k * stride + (i * MT + j) * kWave + lane] = acc[i][j];
+        for (int i = 0; i < NT; ++i) sums[k * stride + i * kWave + lane] = acc[i];
         lds_barrier();
-        constexpr int kOwn = (MT + KS - 1) / KS;  // (of KS = 2 a wave has two of four row tiles)
+        if (k == 0) {
 #pragma unroll
-        for (int o = 0; o < kOwn; ++o) {
-          const int j = k + KS * o;
-          if (j >= MT) break;
-          f32x4_t v[NT];
+          for (int i = 0; i < NT; ++i)
 #pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            v[i] = sums[(i * MT + j) * kWave + lane];
-#pragma unroll
-            for (int q = 1; q < KS; ++q) v[i] += sums[q * stride + (i * MT + j) * kWave + lane];
-          }
-          const int p = mt.lo + 16 * j + r;
-          write_rows<NT>(a, v, mt.e, n0, p, p < mt.hi, p < mt.hi && source_row(a, p) < 0, lane, held[o]);
+            for (int q = 1; q < KS; ++q) acc[i] += sums[q * stride + i * kWave + lane];
+          write_rows<NT>(a, acc, mt.e, n0, mt.lo + r, live, src < 0, lane, held);
         }
         lds_barrier();  // before the next tile's sums
       } else {
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          const int p = mt.lo + 16 * j + r;
-          f32x4_t v[NT];
-#pragma unroll
-          for (int i = 0; i < NT; ++i) v[i] = acc[i][j];
-          write_rows<NT>(a, v, mt.e, n0, p, p < mt.hi, zero[j], lane, held[j]);
-        }
+        write_rows<NT>(a, acc, mt.e, n0, mt.lo + r, live, src < 0, lane, held);
       }
       n0 += kN;
       if (--left == 0) break;
@@ -379,51 +340,33 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles
   }
 }
 
-template <int NT, int MT, int KS>
+template <int NT, int KS>
 __global__ __launch_bounds__(KS * kWave) void stream_kernel(MxProductArgs a, int n_tiles) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-  stream_tiles<NT, MT, KS>(a, n_tiles, lds);
+  stream_tiles<NT, KS>(a, n_tiles, lds);
 }
 
-template <int NT, int MT, int KS>
-hipError_t launch(const MxProductArgs& a, int cus, hipStream_t s) {
-  constexpr int kM = 16 * MT, kN = 16 * NT;
-  const int64_t m_tiles = a.offsets ? a.rows / kM + (a.E < a.rows ? a.E : a.rows) : (a.rows + kM - 1) / kM;
+template <int NT, int KS>
+hipError_t launch(const MxProductArgs& a, hipStream_t s) {
+  constexpr int kN = 16 * NT;
   int n_tiles = (a.N + kN - 1) / kN;
   const int together = a.swiglu && a.out_packed ? 2 : 1;
   n_tiles = (n_tiles + together - 1) / together * together;
-  const size_t bytes = static_cast<size_t>(KS) * wave_bytes<NT, MT, KS>(a.K / 32);
+  const size_t bytes = static_cast<size_t>(KS) * wave_bytes<NT, KS>(a.K / 32);
   // as many as fit at once (two waves per SIMD with their registers), each with a run of tiles
-  const int64_t by_lds = 160 * 1024 / bytes, by_waves = 8 / KS, fit = cus * (by_lds < by_waves ? by_lds : by_waves);
-  int64_t grid = m_tiles * (n_tiles / together);
+  const int64_t by_lds = 160 * 1024 / bytes, by_waves = 8 / KS, fit = kMxCus * (by_lds < by_waves ? by_lds : by_waves);
+  int64_t grid = most_m_tiles(a, kStreamRows) * (n_tiles / together);
   if (grid > fit) grid = fit;
   grid = (grid + 7) & ~int64_t(7);  // every XCD has as many work-groups
-  hipLaunchKernelGGL((stream_kernel<NT, MT, KS>), dim3(static_cast<uint32_t>(grid)), dim3(KS * kWave), bytes, s, a, n_tiles);
+  hipLaunchKernelGGL((stream_kernel<NT, KS>), dim3(static_cast<uint32_t>(grid)), dim3(KS * kWave), bytes, s, a, n_tiles);
   return hipGetLastError();
-}
-
-template <int NT, int MT>
-hipError_t launch_split(const MxProductArgs& a, int ks, hipStream_t s) {
-  int dev = 0, cus = 0;
-  hipError_t e = hipGetDevice(&dev);
-  if (e == hipSuccess) e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
-  if (e != hipSuccess) return e;
-  if (ks >= 4) return launch<NT, MT, 4>(a, cus, s);
-  if (ks >= 2) return launch<NT, MT, 2>(a, cus, s);
-  return launch<NT, MT, 1>(a, cus, s);
 }
 
 }  // namespace
 
-hipError_t launch_mx_stream(const MxProductArgs& a, int nt, int mt, int ks, hipStream_t s) {
-  if (nt >= 2) {
-    if (mt >= 4) return launch_split<2, 4>(a, ks, s);
-    if (mt >= 2) return launch_split<2, 2>(a, ks, s);
-    return launch_split<2, 1>(a, ks, s);
-  }
-  if (mt >= 4) return launch_split<1, 4>(a, ks, s);
-  if (mt >= 2) return launch_split<1, 2>(a, ks, s);
-  return launch_split<1, 1>(a, ks, s);
+hipError_t launch_mx_stream(const MxProductArgs& a, bool wide, bool split, hipStream_t s) {
+  if (wide) return split ? launch<2, 4>(a, s) : launch<2, 1>(a, s);
+  return split ? launch<1, 4>(a, s) : launch<1, 1>(a, s);
 }
 
 }  // namespace gxmoe

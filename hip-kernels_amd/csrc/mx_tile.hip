@@ -1,17 +1,24 @@
 // mx_tile.hip -- MXFP4 products of many rows: tiles through LDS.
 //
-// A work-group of eight waves computes TM rows x 256 columns.  K goes in chunks of
-// eight blocks: 128 bytes (a line) of each of the tile's rows and weight rows reach one of
-// two LDS stages by direct global -> LDS loads, 16 bytes a lane (the same loads of 64 bytes of a row
-// bring 14.6 TB/s over the chip, of whole lines 25.4); the 16-byte piece of block b of row r lies at
-// b ^ (r / 2) % 8 of the row's 128 bytes, so that the operand reads (one block of 16 rows
-// at a time) meet all banks.  The scales come through registers into LDS, 32 blocks of
-// a row at a time, since dwords of single rows would cost the address unit as much as the data.
+// A work-group computes 256 rows x 256 columns (fewer rows where an expert has no
+// more), 128 x 128 or 32 x 128.  K goes in chunks of eight blocks: 128 bytes (a line) of each of
+// the tile's rows and weight rows reach one of two LDS stages by direct global -> LDS loads, 16
+// bytes a lane (such loads of 64 bytes of a row bring 14.6 TB/s over the chip, of whole
+// lines 25.4); the 16-byte piece of block b of row r lies at b ^ (r / 2) % 8 of the row's 128
+// bytes, so that the operand reads (one block of 16 rows at a time) meet all banks.  The scales
+// come through registers into LDS, 32 blocks of a row at a time, since dwords of single
+// rows would cost the address unit as much as the data.
 //
 // Per chunk a wave runs four steps of NT x MT products on operands that it read
 // during the step before.  Before the last step, whose operands are in registers by then, it waits for
 // its loads of the next chunk and meets the others, after which the chunk's
 // stage is free for the loads of the chunk after the next.
+//
+// Large tiles are bound by the requests for their operands and by the matrix cores' power: 8192 x 8192 x
+// 8192 takes 279 us (3.9 PFLOP/s; products alone reach 6.2 to 6.7 with random operands),
+// each round of tiles 10 us beyond its chunks.  Smaller ones stand two or three on a CU, so
+// that one's first loads and last stores overlap another's chunks; their weights come at 4.2 TB/s
+// with rows of 1440 bytes that straddle lines, at 5.3 where rows begin on them (128 experts of 16 rows each).
 #include <type_traits>
 
 #include "mx_product.h"
@@ -22,13 +29,22 @@ namespace {
 
 typedef __attribute__((address_space(3))) void lds_void_t;
 
-constexpr int kTileWaves = 8;
-constexpr int kTileThreads = kTileWaves * kWave;
-constexpr int kTileN = 256;
-constexpr int kBlocks = 8;                                 // of a chunk
-constexpr int kStageBytes = 512 * 16 * kBlocks;            // up to 512 rows
-constexpr int kScaleOff = 2 * kStageBytes;                 // [2][4 chunks][512 rows][8]
-constexpr int kLdsBytes = kScaleOff + 2 * 4 * 512 * 8;     // all 160 KiB
+constexpr int kBlocks = 8;  // of a chunk
+
+// WN x WM waves, each NT x MT products of 32 columns x 32 rows, with S stages, in a work-group of W
+// waves: those that are left over load, and do another's products to no end.
+template <int NT, int MT, int WN, int WM, int S, int W = WN * WM>
+struct Shape {
+  static constexpr int kWaves = W, kThreads = kWaves * kWave;
+  static constexpr int kTN = 32 * NT * WN, kTM = 32 * MT * WM;
+  static constexpr int kRows = kTN + kTM;                         // the weights', then a's
+  static constexpr int kPieces = kRows / 8;                       // of 1 KiB
+  static constexpr int kLoads = (kPieces + kWaves - 1) / kWaves;  // per wave and chunk
+  static constexpr int kStage = kRows * 16 * kBlocks;
+  static constexpr int kScaleOff = S * kStage;                    // [2][4 chunks][kRows][8]
+  static constexpr int kBytes = kScaleOff + 2 * 4 * kRows * 8;
+  static_assert(kRows <= kThreads && kRows >= kThreads / 2 && kBytes <= 160 * 1024 && (S & (S - 1)) == 0, "");
+};
 
 template <int N>
 __device__ __forceinline__ void wait_vm() {  // vmcnt(N), the other counters as they are
@@ -59,16 +75,13 @@ __device__ __forceinline__ u32x4_t load_short_row(const uint8_t* row, int nb) { 
   return v;
 }
 
-// WN x WM waves, each NT x MT products of 32 columns x 32 rows.
-template <int NT, int MT, int WN, int WM>
+template <int NT, int MT, int WN, int WM, int S, int W = WN * WM>
 __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, int n0, uint8_t* lds) {
-  static_assert(WN * WM == kTileWaves && 32 * NT * WN == kTileN, "");
-  constexpr int kTM = 32 * MT * WM;
-  constexpr int kRows = kTileN + kTM;               // the weights', then a's
-  constexpr int kPieces = kRows / 8;                // of 1 KiB
-  constexpr int L = (kPieces + kTileWaves - 1) / kTileWaves;  // loads per wave and chunk
+  typedef Shape<NT, MT, WN, WM, S, W> Sh;
+  constexpr int kTileWaves = Sh::kWaves, kTileN = Sh::kTN, kRows = Sh::kRows;
+  constexpr int kPieces = Sh::kPieces, L = Sh::kLoads, kStageBytes = Sh::kStage, kScaleOff = Sh::kScaleOff;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wn = w % WN, wm = w / WN;
+  const int wn = w % WN, wm = w / WN % WM;
   const int r = lane & 31, half = lane >> 5;
   const int nb = a.K / 32, nch = (nb + kBlocks - 1) / kBlocks;
   const size_t row_bytes = static_cast<size_t>(a.K) / 2;
@@ -94,20 +107,20 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
   auto issue = [&](int c) __attribute__((always_inline)) {
     // blocks past the end: the last one again (its scale there is 0)
     const int b = min(kBlocks * c + blk, nb - 1);
-    uint8_t* stage = lds + (c & 1) * kStageBytes;
+    uint8_t* stage = lds + (c & (S - 1)) * kStageBytes;
 #pragma unroll
     for (int i = 0; i < L; ++i)
       __builtin_amdgcn_global_load_lds(src[i] + 16 * static_cast<size_t>(b), (lds_void_t*)(stage + 1024 * piece[i]), 16, 0, 0);
   };
-  // The thread's row of the scales.
+  // The thread's row of the scales.  Threads that are left over do as the first ones: the same
+  // bytes to the same place, where a branch would cost a wait for all loads.
+  const int srow = tid < kRows ? tid : tid - kRows;
   const uint8_t* ssrc;
-  if (tid < kTileN) {
-    ssrc = a.ws + (wrow + min(n0 + tid, a.N - 1)) * nb;
-  } else if (tid < kRows) {
-    const int p = mt.lo + tid - kTileN;
-    ssrc = a.as + static_cast<size_t>(max(p < mt.hi ? source_row(a, p) : 0, 0)) * nb;
+  if (srow < kTileN) {
+    ssrc = a.ws + (wrow + min(n0 + srow, a.N - 1)) * nb;
   } else {
-    ssrc = a.ws + wrow * nb;  // loaded like the others, not kept
+    const int p = mt.lo + srow - kTileN;
+    ssrc = a.as + static_cast<size_t>(max(p < mt.hi ? source_row(a, p) : 0, 0)) * nb;
   }
 
   // Loads of 16 bytes with no branch around them: they end within the row, and where it has
@@ -120,26 +133,25 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
     for (int i = 0; i < 2; ++i) sreg[i] = *reinterpret_cast<const loose_u32x4*>(sfrom + min(kBlocks * c + 16 * i, slast));
   };
   auto put_scales = [&](int c) __attribute__((always_inline)) {
-    // (threads past the last row store what nobody reads: a branch here would cost a wait for all loads)
-    gx_u32x2* to = reinterpret_cast<gx_u32x2*>(lds + kScaleOff) + ((c >> 2) & 1) * 2048 + tid;
+    gx_u32x2* to = reinterpret_cast<gx_u32x2*>(lds + kScaleOff) + ((c >> 2) & 1) * (4 * kRows) + srow;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int early = kBlocks * c + 16 * i + 16 - nb;
       if (early > 0) sreg[i] = early < 16 ? shift_bytes(sreg[i], early) : u32x4_t{0u, 0u, 0u, 0u};
-      to[1024 * i] = gx_u32x2{sreg[i][0], sreg[i][1]};
-      to[1024 * i + 512] = gx_u32x2{sreg[i][2], sreg[i][3]};
+      to[2 * kRows * i] = gx_u32x2{sreg[i][0], sreg[i][1]};
+      to[2 * kRows * i + kRows] = gx_u32x2{sreg[i][2], sreg[i][3]};
     }
   };
-  issue(0);
-  issue(1);
+  load_scales(0);
+#pragma unroll
+  for (int c = 0; c < S; ++c) issue(c);
   if (nb < 16) {
     sreg[0] = load_short_row(ssrc, nb);
     sreg[1] = u32x4_t{0u, 0u, 0u, 0u};
-    gx_u32x2* to = reinterpret_cast<gx_u32x2*>(lds + kScaleOff) + tid;
+    gx_u32x2* to = reinterpret_cast<gx_u32x2*>(lds + kScaleOff) + srow;
     to[0] = gx_u32x2{sreg[0][0], sreg[0][1]};
-    to[512] = gx_u32x2{sreg[0][2], sreg[0][3]};
+    to[kRows] = gx_u32x2{sreg[0][2], sreg[0][3]};
   } else {
-    load_scales(0);
     put_scales(0);
   }
 
@@ -156,21 +168,21 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
   u32x4_t wv[2][NT], av[2][MT];
   gx_u32x2 sw[NT], sa[MT];
   auto read = [&](int c, int s, u32x4_t(&wo)[NT], u32x4_t(&ao)[MT]) __attribute__((always_inline)) {
-    const uint8_t* stage = lds + (c & 1) * kStageBytes + 16 * (piece0 ^ (2 * s));
+    const uint8_t* stage = lds + (c & (S - 1)) * kStageBytes + 16 * (piece0 ^ (2 * s));
 #pragma unroll
     for (int i = 0; i < NT; ++i) wo[i] = *reinterpret_cast<const u32x4_t*>(stage + 128 * wrow_l + 4096 * i);
 #pragma unroll
     for (int j = 0; j < MT; ++j) ao[j] = *reinterpret_cast<const u32x4_t*>(stage + 128 * arow_l + 4096 * j);
   };
   auto read_scales = [&](int c) __attribute__((always_inline)) {
-    const gx_u32x2* at = reinterpret_cast<const gx_u32x2*>(lds + kScaleOff) + 512 * (c & 7);
+    const gx_u32x2* at = reinterpret_cast<const gx_u32x2*>(lds + kScaleOff) + kRows * (c & 7);
 #pragma unroll
     for (int i = 0; i < NT; ++i) sw[i] = at[wrow_l + 32 * i];
 #pragma unroll
     for (int j = 0; j < MT; ++j) sa[j] = at[arow_l + 32 * j];
   };
 
-  wait_vm<0>();
+  wait_vm<(S - 1) * L>();
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   read_scales(0);
@@ -234,13 +246,13 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
     if constexpr (kPlace == 3) put_scales(c + 1);
     order();
     __builtin_amdgcn_sched_barrier(0);
-    wait_vm<0>();                        // this wave's loads of chunk c + 1
+    wait_vm<(S - 2) * L>();              // this wave's loads of chunk c + 1
     __builtin_amdgcn_s_waitcnt(0xc07f);  // its reads of chunk c
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     read_scales(c + 1);
     read(c + 1, 0, wv[0], av[0]);
-    issue(c + 2);
+    issue(c + S);
     if constexpr (kPlace == 0) load_scales(c + 4);
     products(p1);
     order();
@@ -259,7 +271,7 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
     chunk(p3), ++c;
   }
   for (; c < nch; ++c) chunk(p1);  // up to three, whose scales are there
-  // the ring becomes the waves' own room, 16 KiB each: no load may still land in it
+  // the ring becomes the waves' own room: no load may still land in it
   wait_vm<0>();
   __builtin_amdgcn_s_waitcnt(0xc07f);
   __builtin_amdgcn_s_barrier();
@@ -268,8 +280,9 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
   if (tid < kTileN) bias_all[tid] = a.bias ? bf16_to_f32(a.bias[wrow + min(n0 + tid, a.N - 1)]) : 0.0f;
   __builtin_amdgcn_s_waitcnt(0xc07f);
   __builtin_amdgcn_s_barrier();
+  if (w >= WN * WM) return;
   const float* bias = bias_all + 32 * NT * wn;
-  uint8_t* own = lds + 16384 * w;
+  uint8_t* own = lds + S * kStageBytes / kTileWaves * w;
   const int cols = a.swiglu ? a.N / 2 : a.N;
   constexpr int kG = NT < 2 ? NT : 2;  // column tiles that go together
 #pragma unroll
@@ -377,35 +390,67 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
 
 // Tiles are numbered four m-tiles x all n-tiles at a time, and every XCD (one of eight, in
 // turn by work-group) takes a run of them, so that its L2 serves a tile's rows
-// and weights to its neighbours.
+// and weights to its neighbours.  The grid has room for every expert's last tile; how many there
+// are is known here.
 constexpr int kGroupM = 4;
 
-// The grid has room for every expert's last tile; how many there are is known here.
-__global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(MxProductArgs a, int n_tiles) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLdsBytes];
-  const int m_tiles = count_m_tiles(a, 256, threadIdx.x & (kWave - 1));
+struct Place {
+  MTile m;
+  int nt;
+};
+
+__device__ __forceinline__ bool find_place(const MxProductArgs& a, int rows, int n_tiles, Place* p) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int m_tiles = count_m_tiles(a, rows, lane);
   const int total = m_tiles * n_tiles, b = blockIdx.x;
   const int x = b & 7, share = total >> 3, more = total & 7;
-  if ((b >> 3) >= share + (x < more ? 1 : 0)) return;
+  if ((b >> 3) >= share + (x < more ? 1 : 0)) return false;
   const int id = x * share + min(x, more) + (b >> 3);
   const int group = id / (kGroupM * n_tiles), in_group = id - group * (kGroupM * n_tiles);
   const int height = min(kGroupM, m_tiles - kGroupM * group);
-  const int m = kGroupM * group + in_group % height, nt = in_group / height;
-  const MTile mt = find_m_tile(a, m, 256, threadIdx.x & (kWave - 1));
-  const int rows = mt.hi - mt.lo;
-  if (rows > 128) tile<4, 2, 2, 4>(a, mt, nt * kTileN, lds);
-  else if (rows > 64) tile<2, 2, 4, 2>(a, mt, nt * kTileN, lds);
-  else tile<2, 1, 4, 2>(a, mt, nt * kTileN, lds);
+  p->m = find_m_tile(a, kGroupM * group + in_group % height, rows, lane);
+  p->nt = in_group / height;
+  return true;
+}
+
+// 256 columns x 256 rows, fewer where an expert has no more.
+__global__ __launch_bounds__(512, 2) void large_tile_kernel(MxProductArgs a, int n_tiles) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<4, 2, 2, 4, 2>::kBytes];
+  Place p;
+  if (!find_place(a, 256, n_tiles, &p)) return;
+  const int rows = p.m.hi - p.m.lo;
+  if (rows > 128) tile<4, 2, 2, 4, 2>(a, p.m, p.nt * 256, lds);
+  else if (rows > 64) tile<2, 2, 4, 2, 2>(a, p.m, p.nt * 256, lds);
+  else tile<2, 1, 4, 2, 2>(a, p.m, p.nt * 256, lds);
+}
+
+// 128 columns x 128 or 64 rows, two work-groups on a CU.
+__global__ __launch_bounds__(256, 2) void middle_tile_kernel(MxProductArgs a, int n_tiles) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<2, 2, 2, 2, 2>::kBytes];
+  Place p;
+  if (!find_place(a, 128, n_tiles, &p)) return;
+  const int rows = p.m.hi - p.m.lo;
+  if (rows > 64) tile<2, 2, 2, 2, 2>(a, p.m, p.nt * 128, lds);
+  else tile<2, 1, 2, 2, 2>(a, p.m, p.nt * 128, lds);
+}
+
+// 128 columns x 32 rows, three work-groups on a CU.
+__global__ __launch_bounds__(256, 3) void low_tile_kernel(MxProductArgs a, int n_tiles) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<2, 1, 2, 1, 2, 4>::kBytes];
+  Place p;
+  if (find_place(a, 32, n_tiles, &p)) tile<2, 1, 2, 1, 2, 4>(a, p.m, p.nt * 128, lds);
 }
 
 }  // namespace
 
-hipError_t launch_mx_tile(const MxProductArgs& a, hipStream_t s) {
-  const int m_tiles = a.offsets ? a.rows / 256 + (a.E < a.rows ? a.E : a.rows) : (a.rows + 255) / 256;
-  const int n_tiles = (a.N + kTileN - 1) / kTileN;
+hipError_t launch_mx_tile(const MxProductArgs& a, MxTile kind, hipStream_t s) {
+  const int rows = kind == MxTile::large ? 256 : kind == MxTile::middle ? 128 : 32;
+  const int cols = kind == MxTile::large ? 256 : 128, n_tiles = (a.N + cols - 1) / cols;
   // a multiple of eight, so that every XCD has work-groups enough for its share
-  const uint32_t grid = (static_cast<uint32_t>(m_tiles) * static_cast<uint32_t>(n_tiles) + 7u) & ~7u;
-  hipLaunchKernelGGL(tile_kernel, dim3(grid), dim3(kTileThreads), 0, s, a, n_tiles);
+  const dim3 grid(static_cast<uint32_t>((most_m_tiles(a, rows) * n_tiles + 7) & ~int64_t(7)));
+  if (kind == MxTile::large) hipLaunchKernelGGL(large_tile_kernel, grid, dim3(512), 0, s, a, n_tiles);
+  else if (kind == MxTile::middle) hipLaunchKernelGGL(middle_tile_kernel, grid, dim3(256), 0, s, a, n_tiles);
+  else hipLaunchKernelGGL(low_tile_kernel, grid, dim3(256), 0, s, a, n_tiles);
   return hipGetLastError();
 }
 

@@ -77,6 +77,45 @@ def test_grouped(gpu, counts, N, K):
             c.check(swiglu=True, bias=gather)
 
 
+@pytest.mark.parametrize("counts, N, K", [([300, 100, 40, 129, 64, 65], 8192, 96), ([700, 0, 3], 9026, 64)])
+def test_many_tiles(gpu, counts, N, K):
+    """Tiles of 256 rows and their smaller ones."""
+    c = Case(gpu, counts, N, K, before=2, after=3)
+    c.check(dtype=F32)
+    c.check(swiglu=True)
+
+
+@pytest.mark.parametrize("N, K", [(256, 512), (258, 608)])
+def test_few_rows_of_many_experts(gpu, N, K):
+    E, used = 1024, {0: 3, 7: 17, 8: 1, 500: 40, 1023: 2}
+    counts = [used.get(e, 0) for e in range(E)]
+    offsets = torch.tensor([sum(counts[:e]) for e in range(E + 1)], dtype=torch.int32, device="cuda")
+    rows = E  # as the call says; those behind the last offset stay as they are
+    gen = gen_of(N)
+    a = ref.random_matrix(gpu, gen, rows, K, low=119, high=124)
+    w = ref.random_matrix(gpu, gen, E, N, K, low=119, high=124)
+    bias = torch.randn((E, N), device="cuda", generator=gen).to(BF16)
+    want, tol = [], []
+    for e, n in used.items():
+        lo = sum(counts[:e])
+        y, t = ref.product(ref.of_matrix(gpu.MXFP4Matrix(a.packed[lo:lo + n], a.scales[lo:lo + n])),
+                           ref.of_matrix(gpu.MXFP4Matrix(w.packed[e], w.scales[e])), bias[e])
+        want.append(y), tol.append(t)
+    want, tol, live = torch.cat(want), torch.cat(tol), sum(counts)
+    out = torch.full((rows, N), 9.0, device="cuda", dtype=BF16)
+    gpu.grouped_mxfp4_matmul(a, w, offsets, rows, bias=bias, out=out)
+    ref.assert_values(out[:live], want, tol)
+    assert bool((out[live:] == 9).all())
+    want, tol = ref.swiglu(want, tol)
+    out = torch.full((rows, N // 2), 9.0, device="cuda", dtype=F32)
+    gpu.grouped_mxfp4_matmul(a, w, offsets, rows, bias=bias, swiglu=True, out=out)
+    ref.assert_values(out[:live], want, tol)
+    assert bool((out[live:] == 9).all())
+    if N % 64 == 0:
+        m = gpu.grouped_mxfp4_matmul(a, w, offsets, rows, bias=bias, swiglu=True, quantize=True)
+        ref.assert_quantized(gpu.MXFP4Matrix(m.packed[:live], m.scales[:live]), want, tol)
+
+
 def test_many_experts(gpu):
     """1024 experts, some of them with tokens."""
     g = torch.Generator().manual_seed(1)

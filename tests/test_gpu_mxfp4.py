@@ -170,6 +170,23 @@ def test_product_swiglu(gpu, M, N, K, with_bias):
         ref.assert_values(gpu.mxfp4_matmul(a, w, bias=bias, swiglu=True, dtype=dtype), want, tol, (M, N, K))
 
 
+@pytest.mark.parametrize("M, N, K", [(1, 96, 4096), (5, 2880, 4128), (17, 130, 4640), (40, 992, 512), (1100, 1920, 64),
+                                     (1031, 1985, 288), (2950, 2944, 96), (2817, 2946, 320)])
+def test_product_of_many_tiles(gpu, M, N, K):
+    """Long rows that several waves share, and calls with tiles enough for the larger ones."""
+    a, w, bias = operands(gpu, M, N, K, M + N, low=119, high=124)
+    want, tol = ref.product(ref.of_matrix(a), ref.of_matrix(w), bias)
+    for dtype in (BF16, F32):
+        ref.assert_values(gpu.mxfp4_matmul(a, w, bias=bias, dtype=dtype), want, tol)
+    if N % 32 == 0:
+        ref.assert_quantized(gpu.mxfp4_matmul(a, w, bias=bias, quantize=True), want, tol)
+    if N % 2 == 0:
+        want, tol = ref.swiglu(want, tol)
+        ref.assert_values(gpu.mxfp4_matmul(a, w, bias=bias, swiglu=True), want, tol)
+        if N % 64 == 0:
+            ref.assert_quantized(gpu.mxfp4_matmul(a, w, bias=bias, swiglu=True, quantize=True), want, tol)
+
+
 @pytest.mark.parametrize("M, N", [(5, 6), (40, 2), (200, 130), (70, 1002)])
 def test_product_swiglu_of_few_columns(gpu, M, N):
     a, w, bias = operands(gpu, M, N, 96, M, low=119, high=124)
