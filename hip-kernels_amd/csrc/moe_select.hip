@@ -28,155 +28,228 @@ __device__ __forceinline__ uint64_t choice_key(double c) {
   return (u >> 63) ? ~u : u | 0x8000000000000000ull;
 }
 
-__device__ __forceinline__ double wave_max(double v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v = __builtin_fmax(v, __shfl_xor(v, m, kWave));
-  return v;
+__device__ __forceinline__ double choice_of(uint64_t key) {  // key > 1
+  return __builtin_bit_cast(double, (key >> 63) ? key & 0x7fffffffffffffffull : ~key);
+}
+
+// A lane's value with those of the lanes before it in its row of 16, then with the rows
+// before: lane 63 ends with the wave's.  `none` stands for lanes that are not there.
+template <int Ctrl, int Rows>
+__device__ __forceinline__ uint32_t from_before(uint32_t v, uint32_t none) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(static_cast<int>(none), static_cast<int>(v), Ctrl, Rows, 0xf, false));
+}
+
+template <typename F>
+__device__ __forceinline__ uint32_t wave_fold(uint32_t v, uint32_t none, F fold) {
+  v = fold(v, from_before<0x111, 0xf>(v, none));  // row_shr 1, 2, 4, 8
+  v = fold(v, from_before<0x112, 0xf>(v, none));
+  v = fold(v, from_before<0x114, 0xf>(v, none));
+  v = fold(v, from_before<0x118, 0xf>(v, none));
+  v = fold(v, from_before<0x142, 0xa>(v, none));  // row_bcast 15 and 31
+  v = fold(v, from_before<0x143, 0xc>(v, none));
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), kWave - 1));
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  return wave_fold(v, 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+  return __uint_as_float(wave_fold(__float_as_uint(v), 0xff800000u, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__builtin_fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+
+template <int Ctrl, int Rows>
+__device__ __forceinline__ double add_before(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = from_before<Ctrl, Rows>(static_cast<uint32_t>(u), 0u);
+  const uint32_t hi = from_before<Ctrl, Rows>(static_cast<uint32_t>(u >> 32), 0u);
+  return v + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), lane);
+  return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
-  return v;
+  v = add_before<0x111, 0xf>(v);
+  v = add_before<0x112, 0xf>(v);
+  v = add_before<0x114, 0xf>(v);
+  v = add_before<0x118, 0xf>(v);
+  v = add_before<0x142, 0xa>(v);
+  v = add_before<0x143, 0xc>(v);
+  return __builtin_bit_cast(double, read_lane(__builtin_bit_cast(uint64_t, v), kWave - 1));
 }
 
-// The largest key of the wave and the lowest expert that has it.
-__device__ __forceinline__ void wave_best(uint64_t& key, int& e) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    const uint64_t k2 = __shfl_xor(key, m, kWave);
-    const int e2 = __shfl_xor(e, m, kWave);
-    if (k2 > key || (k2 == key && e2 < e)) {
-      key = k2;
-      e = e2;
-    }
+// The lowest lane that has the wave's largest key: the upper halves mostly tell.
+__device__ __forceinline__ int best_lane(uint64_t key) {
+  const uint32_t hi = static_cast<uint32_t>(key >> 32), top = wave_max(hi);
+  uint64_t have = __ballot(hi == top);
+  if (have & (have - 1)) {
+    const uint32_t lo = hi == top ? static_cast<uint32_t>(key) : 0u, low = wave_max(lo);
+    have &= __ballot(lo == low);
   }
+  return __builtin_ctzll(have);
 }
 
-// A wave per token, expert lane + 64 j in value j of a lane; everything in 64
-// bits, so that the order is that of the exact values but for gaps of 1e-15.
+// A wave per token, experts NV lane to NV lane + NV - 1 a lane's own, so that of equal choices the
+// lowest lane's first one counts.  Scores and choices are in 64 bits: the order is that of
+// the exact values but for gaps of 1e-15, and a weight is rounded once.  The largest choice of a wave
+// is found on the upper 32 bits of keys of the same order, by six DPP steps.
 template <int NV>
 __global__ __launch_bounds__(kSelectWaves * kWave) void select_kernel(SelectArgs a) {
+  __shared__ double scores[kSelectWaves][NV * kWave];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   const int t = blockIdx.x * kSelectWaves + wave;
   if (t >= a.T) return;  // no barrier below
   const size_t row = static_cast<size_t>(t) * static_cast<size_t>(a.stride);
   const double inf = __builtin_inf();
 
-  double score[NV];
-  uint64_t key[NV];
-  double x[NV], top = -inf;
+  float x[NV], bias[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int e = lane + kWave * j;
-    x[j] = -inf;
-    if (e < a.E)
-      x[j] = a.fp32 ? static_cast<const float*>(a.logits)[row + e]
-                    : bf16_to_f32(static_cast<const uint16_t*>(a.logits)[row + e]);
-    top = __builtin_fmax(top, x[j]);
+    const int e = min(NV * lane + j, a.E - 1);
+    x[j] = a.fp32 ? static_cast<const float*>(a.logits)[row + e]
+                  : bf16_to_f32(static_cast<const uint16_t*>(a.logits)[row + e]);
+    bias[j] = a.bias ? a.bias[e] : 0.0f;
   }
+  double score[NV];
+  uint64_t key[NV];
   if (!a.sigmoid) {
-    top = wave_max(top);
+    float most = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < NV; ++j) most = __builtin_fmaxf(most, x[j]);
+    const float top = wave_max(most);
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      score[j] = x[j] == top ? (top == -inf ? 0.0 : 1.0) : exp(x[j] - top);  // (inf - inf, and a row of -inf)
-      sum += score[j];
+      // (inf - inf, and a row of -inf)
+      score[j] = x[j] == top ? (top == -__builtin_inff() ? 0.0 : 1.0) : exp(static_cast<double>(x[j]) - top);
+      sum += NV * lane + j < a.E ? score[j] : 0.0;
     }
     sum = wave_sum(sum);
 #pragma unroll
     for (int j = 0; j < NV; ++j) score[j] = sum == 0.0 ? 0.0 : score[j] / sum;
   } else {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) score[j] = 1.0 / (1.0 + exp(-x[j]));
+    for (int j = 0; j < NV; ++j) score[j] = 1.0 / (1.0 + exp(-static_cast<double>(x[j])));
   }
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int e = lane + kWave * j;
-    double c = -inf;
-    if (e < a.E) c = score[j] + (a.bias ? static_cast<double>(a.bias[e]) : 0.0);
-    if (x[j] == -inf) c = -inf;
+    double c = score[j] + static_cast<double>(bias[j]);
+    if (x[j] == -__builtin_inff()) c = -inf;
     if (c == -inf) score[j] = 0.0;
-    key[j] = choice_key(c);
-    x[j] = c;
+    key[j] = NV * lane + j < a.E ? choice_key(c) : 0u;
+    scores[wave][NV * lane + j] = score[j];
   }
+
+  __builtin_amdgcn_wave_barrier();
 
   if (a.groups > 1) {
-    // group after group: its members of this lane's values, then the wave's best two
-    const int size = a.E / a.groups;
-    uint64_t mine = 0;  // lane g: the key of group g
-    for (int g = 0; g < a.groups; ++g) {
-      const int lo = g * size, hi = lo + size;
-      double total = 0.0;
-      bool any = false;
-      int taken = -1;
-      for (int r = 0; r < a.group_rank; ++r) {
-        uint64_t best = 0;
-        int at = 0x7fffffff;
+    const int size = a.E / a.groups, lanes = size / NV;
+    if (a.group_rank <= 2 && size % NV == 0 && (lanes & (lanes - 1)) == 0) {
+      // A group is lanes of its own, a power of two: its best two by exchanges among them.
+      uint64_t first = key[0], second = 0;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int e = lane + kWave * j;
-          if (e >= lo && e < hi && e != taken && key[j] > best) {
-            best = key[j];
-            at = e;
+      for (int j = 1; j < NV; ++j) {
+        second = max(second, min(first, key[j]));
+        first = max(first, key[j]);
+      }
+      for (int m = 1; m < lanes; m <<= 1) {
+        const uint64_t f = __shfl_xor(first, m, kWave), s = __shfl_xor(second, m, kWave);
+        second = max(max(second, s), min(first, f));
+        first = max(first, f);
+      }
+      if (first > 1u) {  // (a group of switched off experts stays 1)
+        double total = choice_of(first);
+        if (a.group_rank == 2 && second > 1u) total += choice_of(second);
+        first = choice_key(total);
+      }
+      // its place among the groups, those of equal sums in turn
+      const int mine = lane / lanes;
+      int before = 0;
+      for (int g = 0; g < a.groups; ++g) {
+        const uint64_t other = read_lane(first, g * lanes);
+        before += other > first || (other == first && g < mine) ? 1 : 0;
+      }
+      if (before >= a.top_groups) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) key[j] = 0;
+      }
+    } else {
+      // group after group
+      uint64_t mine = 0;  // lane g: the key of group g
+      for (int g = 0; g < a.groups; ++g) {
+        const int lo = g * size, hi = lo + size;
+        double total = 0.0;
+        bool any = false;
+        uint32_t taken = 0;  // of the lane's experts
+        for (int r = 0; r < a.group_rank; ++r) {
+          uint64_t best = 0;
+          int at = 0;
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            const int e = NV * lane + j;
+            if (e >= lo && e < hi && !((taken >> j) & 1u) && key[j] > best) {
+              best = key[j];
+              at = j;
+            }
           }
+          const int l = best_lane(best);
+          const uint64_t k = read_lane(best, l);
+          if (k <= 1u) break;  // switched off, as all that follow
+          if (lane == l) taken |= 1u << at;
+          any = true;
+          total += choice_of(k);
         }
-        wave_best(best, at);
-        if (best <= 1u) break;  // switched off, as all that follow
-        taken = at;
-        any = true;
-        double c = 0.0;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-          if (lane + kWave * j == at) c = x[j];
-        total += __shfl(c, at & (kWave - 1), kWave);
+        if (lane == g) mine = any ? choice_key(total) : 1u;
       }
-      const uint64_t gk = any ? choice_key(total) : 1u;
-      if (lane == g) mine = gk;
-    }
-    uint64_t kept = 0;
-    for (int r = 0; r < a.top_groups; ++r) {
-      uint64_t best = mine;
-      int at = lane;
-      wave_best(best, at);
-      kept |= 1ull << at;
-      if (lane == at) mine = 0;
-    }
+      uint64_t kept = 0;
+      for (int r = 0; r < a.top_groups; ++r) {
+        const int g = best_lane(mine);
+        kept |= 1ull << g;
+        if (lane == g) mine = 0;
+      }
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int e = lane + kWave * j;
-      if (e < a.E && !((kept >> (e / size)) & 1u)) key[j] = 0;
+      for (int j = 0; j < NV; ++j) {
+        const int e = NV * lane + j;
+        if (e < a.E && !((kept >> (e / size)) & 1u)) key[j] = 0;
+      }
     }
   }
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-    if (lane + kWave * j >= a.E) key[j] = 0;
 
-  int chosen = 0;     // lane s: the s-th choice
-  double weight = 0.0;
+  uint64_t best = key[0];  // the lane's first of its largest
+  int at = 0;
+#pragma unroll
+  for (int j = 1; j < NV; ++j)
+    if (key[j] > best) {
+      best = key[j];
+      at = j;
+    }
+  int chosen = 0;  // lane s: the s-th choice
   for (int s = 0; s < a.k; ++s) {
-    uint64_t best = 0;
-    int at = 0x7fffffff;
+    const int l = best_lane(best);
+    const int e = NV * l + __builtin_amdgcn_readlane(at, l);
+    chosen = lane == s ? e : chosen;
+    if (lane == l) {
+      best = 0;
+      int next = 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (key[j] > best) {
-        best = key[j];
-        at = lane + kWave * j;
+      for (int j = 0; j < NV; ++j) {
+        if (j == at) key[j] = 0;
+        if (key[j] > best) {
+          best = key[j];
+          next = j;
+        }
       }
-    wave_best(best, at);
-    double w = 0.0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (lane + kWave * j == at) {
-        w = score[j];
-        key[j] = 0;
-      }
-    w = __shfl(w, at & (kWave - 1), kWave);
-    if (lane == s) {
-      chosen = at;
-      weight = w;
+      at = next;
     }
   }
+  double weight = lane < a.k ? scores[wave][chosen] : 0.0;
   if (a.renormalize) {
     const double sum = wave_sum(weight);
     weight = sum == 0.0 ? 0.0 : weight / sum;
