@@ -166,13 +166,17 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles
   constexpr int kPieces = (kSpan / 16 + kLanes - 1) / kLanes;
   static_assert((kRing - 2) * kLoads < 64, "vmcnt range");
   const int lane = threadIdx.x & (kWave - 1), k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // This work-group's run of tiles, the columns of an m-tile in turn; XCD b % 8 has neighbouring runs.  Tiles whose
-  // results make one block go together.
+  // This work-group's run of tiles, the columns of an m-tile in turn: as long as all others' but the last, so that none
+  // is left with a longer one (fewer waves hold the bandwidth too).  XCD b % 8 has neighbouring runs.  Tiles whose results
+  // make one block go together.
   const int together = a.swiglu && a.out_packed ? 2 : 1;
   const int64_t total = static_cast<int64_t>(count_m_tiles(a, kStreamRows, lane)) * (n_tiles / together);
-  const int b = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-  int id = static_cast<int>(total * b / gridDim.x) * together;
-  const int id_end = static_cast<int>(total * (b + 1) / gridDim.x) * together;
+  const int64_t run = (total + gridDim.x - 1) / gridDim.x, runs = run ? (total + run - 1) / run : 0;
+  const int xcd = blockIdx.x & 7, share = static_cast<int>(runs >> 3), more = static_cast<int>(runs & 7);
+  if (static_cast<int>(blockIdx.x >> 3) >= share + (xcd < more ? 1 : 0)) return;
+  const int64_t b = xcd * share + min(xcd, more) + static_cast<int>(blockIdx.x >> 3);
+  int id = static_cast<int>(run * b) * together;
+  const int id_end = static_cast<int>(min(run * (b + 1), total)) * together;
 
   const int r = lane & 15, g = lane >> 4;
   const int nb = a.K / 32, chunks = (nb + 7) / 8;
