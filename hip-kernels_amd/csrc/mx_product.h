@@ -85,6 +85,17 @@ __device__ __forceinline__ int source_row(const MxProductArgs& a, int p) {
   return src >= 0 && src < a.a_rows ? src : -1;
 }
 
+// The same of several: their loads go out together.
+template <int N>
+__device__ __forceinline__ void source_rows(const MxProductArgs& a, int (&p)[N]) {
+  if (a.row_index) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = a.row_index[p[i]];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = p[i] >= 0 && p[i] < a.a_rows ? p[i] : -1;
+}
+
 // The lane's 16 results of a block of 32 columns (as both halves of the wave hold them)
 // to MXFP4: eight of its 16 bytes each, and the scale byte.  kPairs: the lane's values
 // are columns 4 q + 2 half + {0, 1} (after SwiGLU), otherwise 8 q + 4 half + {0 .. 3}.

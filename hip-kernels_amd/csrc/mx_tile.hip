@@ -90,18 +90,25 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
   // The lane's row of each piece that its wave loads.  A wave without a piece of its own
   // left loads its first one once more, so that all waves have as many loads in flight.
   const uint8_t* src[L];
-  int piece[L];
+  int piece[L], from[L + 1];
 #pragma unroll
   for (int i = 0; i < L; ++i) {
     piece[i] = w + kTileWaves * i < kPieces ? w + kTileWaves * i : w;
-    const int row = 8 * piece[i] + (lane >> 3);
-    if (row < kTileN) {
-      src[i] = a.w + (wrow + min(n0 + row, a.N - 1)) * row_bytes;
-    } else {
-      const int p = mt.lo + row - kTileN;
-      src[i] = a.a + static_cast<size_t>(max(p < mt.hi ? source_row(a, p) : 0, 0)) * row_bytes;
-    }
+    from[i] = max(mt.lo, min(mt.lo + 8 * piece[i] + (lane >> 3) - kTileN, mt.hi - 1));
   }
+  // The thread's row of the scales.  Threads that are left over do as the first ones: the same
+  // bytes to the same place, where a branch would cost a wait for all loads.
+  const int srow = tid < kRows ? tid : tid - kRows;
+  from[L] = max(mt.lo, min(mt.lo + srow - kTileN, mt.hi - 1));
+  source_rows(a, from);
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    const int row = 8 * piece[i] + (lane >> 3);
+    src[i] = row < kTileN ? a.w + (wrow + min(n0 + row, a.N - 1)) * row_bytes
+                          : a.a + static_cast<size_t>(max(from[i], 0)) * row_bytes;
+  }
+  const uint8_t* const ssrc = srow < kTileN ? a.ws + (wrow + min(n0 + srow, a.N - 1)) * nb
+                                            : a.as + static_cast<size_t>(max(from[L], 0)) * nb;
   // (row / 2) % 8 of the lane's rows: all of its pieces are odd or all are even
   const int blk = (lane & 7) ^ (4 * (w & 1) + (lane >> 4));
   auto issue = [&](int c) __attribute__((always_inline)) {
@@ -112,17 +119,6 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
     for (int i = 0; i < L; ++i)
       __builtin_amdgcn_global_load_lds(src[i] + 16 * static_cast<size_t>(b), (lds_void_t*)(stage + 1024 * piece[i]), 16, 0, 0);
   };
-  // The thread's row of the scales.  Threads that are left over do as the first ones: the same
-  // bytes to the same place, where a branch would cost a wait for all loads.
-  const int srow = tid < kRows ? tid : tid - kRows;
-  const uint8_t* ssrc;
-  if (srow < kTileN) {
-    ssrc = a.ws + (wrow + min(n0 + srow, a.N - 1)) * nb;
-  } else {
-    const int p = mt.lo + srow - kTileN;
-    ssrc = a.as + static_cast<size_t>(max(p < mt.hi ? source_row(a, p) : 0, 0)) * nb;
-  }
-
   // Loads of 16 bytes with no branch around them: they end within the row, and where it has
   // fewer than 16 something is loaded that is not read.
   const uint8_t* sfrom = nb < 16 ? a.w : ssrc;
@@ -285,11 +281,15 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
   uint8_t* own = lds + S * kStageBytes / kTileWaves * w;
   const int cols = a.swiglu ? a.N / 2 : a.N;
   constexpr int kG = NT < 2 ? NT : 2;  // column tiles that go together
+  int reads[MT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j) reads[j] = min(mt.lo + 32 * (MT * wm + j) + r, mt.hi - 1);
+  source_rows(a, reads);
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
     const int p = mt.lo + 32 * (MT * wm + j) + r;
     const bool live = p < mt.hi;
-    const bool zero = live && source_row(a, p) < 0;
+    const bool zero = reads[j] < 0;
 #pragma unroll
     for (int g = 0; g < NT / kG; ++g) {
       const int n = n0 + 32 * (NT * wn + kG * g);  // the group's first column
