@@ -31,9 +31,8 @@ typedef __attribute__((address_space(3))) void lds_void_t;
 
 constexpr int kBlocks = 8;  // of a chunk
 
-// WN x WM waves, each NT x MT products of 32 columns x 32 rows, with S stages, in a work-group of W
-// waves: those that are left over load, and do another's products to no end.
-template <int NT, int MT, int WN, int WM, int S, int W = WN * WM>
+// WN x WM waves, each NT x MT products of 32 columns x 32 rows, in a work-group of W waves: those that are left over load, and do another's products to no end.
+template <int NT, int MT, int WN, int WM, int W = WN * WM>
 struct Shape {
   static constexpr int kWaves = W, kThreads = kWaves * kWave;
   static constexpr int kTN = 32 * NT * WN, kTM = 32 * MT * WM;
@@ -41,9 +40,9 @@ struct Shape {
   static constexpr int kPieces = kRows / 8;                       // of 1 KiB
   static constexpr int kLoads = (kPieces + kWaves - 1) / kWaves;  // per wave and chunk
   static constexpr int kStage = kRows * 16 * kBlocks;
-  static constexpr int kScaleOff = S * kStage;                    // [2][4 chunks][kRows][8]
+  static constexpr int kScaleOff = 2 * kStage;                    // [2][4 chunks][kRows][8]
   static constexpr int kBytes = kScaleOff + 2 * 4 * kRows * 8;
-  static_assert(kRows <= kThreads && kRows >= kThreads / 2 && kBytes <= 160 * 1024 && (S & (S - 1)) == 0, "");
+  static_assert(kRows <= kThreads && kRows >= kThreads / 2 && kBytes <= 160 * 1024, "");
 };
 
 template <int N>
@@ -75,9 +74,9 @@ __device__ __forceinline__ u32x4_t load_short_row(const uint8_t* row, int nb) { 
   return v;
 }
 
-template <int NT, int MT, int WN, int WM, int S, int W = WN * WM>
+template <int NT, int MT, int WN, int WM, int W = WN * WM>
 __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, int n0, uint8_t* lds) {
-  typedef Shape<NT, MT, WN, WM, S, W> Sh;
+  typedef Shape<NT, MT, WN, WM, W> Sh;
   constexpr int kTileWaves = Sh::kWaves, kTileN = Sh::kTN, kRows = Sh::kRows;
   constexpr int kPieces = Sh::kPieces, L = Sh::kLoads, kStageBytes = Sh::kStage, kScaleOff = Sh::kScaleOff;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -111,14 +110,20 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
                                             : a.as + static_cast<size_t>(max(from[L], 0)) * nb;
   // (row / 2) % 8 of the lane's rows: all of its pieces are odd or all are even
   const int blk = (lane & 7) ^ (4 * (w & 1) + (lane >> 4));
-  auto issue = [&](int c) __attribute__((always_inline)) {
+  auto issue = [&](int c, auto from_piece, auto to_piece) __attribute__((always_inline)) {
     // blocks past the end: the last one again (its scale there is 0)
     const int b = min(kBlocks * c + blk, nb - 1);
-    uint8_t* stage = lds + (c & (S - 1)) * kStageBytes;
+    uint8_t* stage = lds + (c & 1) * kStageBytes;
 #pragma unroll
-    for (int i = 0; i < L; ++i)
+    for (int i = decltype(from_piece)::value; i < decltype(to_piece)::value; ++i)
       __builtin_amdgcn_global_load_lds(src[i] + 16 * static_cast<size_t>(b), (lds_void_t*)(stage + 1024 * piece[i]), 16, 0, 0);
   };
+  // A chunk's loads in three parts: the address unit takes one of a wave's in 16 cycles, and a
+  // wave that waits for it gives no products meanwhile.
+  const std::integral_constant<int, 0> part0{};
+  const std::integral_constant<int, (3 * L + 7) / 8> part1{};
+  const std::integral_constant<int, (6 * L + 7) / 8> part2{};
+  const std::integral_constant<int, L> part3{};
   // Loads of 16 bytes with no branch around them: they end within the row, and where it has
   // fewer than 16 something is loaded that is not read.
   const uint8_t* sfrom = nb < 16 ? a.w : ssrc;
@@ -139,8 +144,8 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
     }
   };
   load_scales(0);
-#pragma unroll
-  for (int c = 0; c < S; ++c) issue(c);
+  issue(0, part0, part3);
+  issue(1, part0, part1);
   if (nb < 16) {
     sreg[0] = load_short_row(ssrc, nb);
     sreg[1] = u32x4_t{0u, 0u, 0u, 0u};
@@ -164,7 +169,7 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
   u32x4_t wv[2][NT], av[2][MT];
   gx_u32x2 sw[NT], sa[MT];
   auto read = [&](int c, int s, u32x4_t(&wo)[NT], u32x4_t(&ao)[MT]) __attribute__((always_inline)) {
-    const uint8_t* stage = lds + (c & (S - 1)) * kStageBytes + 16 * (piece0 ^ (2 * s));
+    const uint8_t* stage = lds + (c & 1) * kStageBytes + 16 * (piece0 ^ (2 * s));
 #pragma unroll
     for (int i = 0; i < NT; ++i) wo[i] = *reinterpret_cast<const u32x4_t*>(stage + 128 * wrow_l + 4096 * i);
 #pragma unroll
@@ -178,7 +183,7 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
     for (int j = 0; j < MT; ++j) sa[j] = at[arow_l + 32 * j];
   };
 
-  wait_vm<(S - 1) * L>();
+  wait_vm<decltype(part1)::value>();
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   read_scales(0);
@@ -213,13 +218,19 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
                                                                     static_cast<int>(oa[j]));
     pin();
   };
-  // The next step's reads go out behind the first products of this one.
-  auto order = [&]() __attribute__((always_inline)) {
+  // The next step's reads go out behind the first products of this one, then its loads.
+  auto order = [&](auto from_piece, auto to_piece, auto more) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < (NT + MT + 1) / 2; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
+#pragma unroll
+    for (int i = 0; i < decltype(to_piece)::value - decltype(from_piece)::value + decltype(more)::value; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   };
   const std::integral_constant<int, 0> p0{};
   const std::integral_constant<int, 1> p1{};
@@ -228,36 +239,29 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
   auto chunk = [&](auto place) __attribute__((always_inline)) {
     constexpr int kPlace = decltype(place)::value;  // c % 4
     read(c, 1, wv[1], av[1]);
+    issue(c + 1, part1, part2);
     shift(0);
     products(p0);
-    order();
-    __builtin_amdgcn_sched_barrier(0);
+    order(part1, part2, p0);
     read(c, 2, wv[0], av[0]);
+    issue(c + 1, part2, part3);
     products(p1);
-    order();
-    __builtin_amdgcn_sched_barrier(0);
+    order(part2, part3, p0);
     read(c, 3, wv[1], av[1]);
+    if constexpr (kPlace == 1) load_scales(c + 3);
     shift(1);
     products(p0);
     if constexpr (kPlace == 3) put_scales(c + 1);
-    order();
-    __builtin_amdgcn_sched_barrier(0);
-    wait_vm<(S - 2) * L>();              // this wave's loads of chunk c + 1
+    order(p0, p0, std::integral_constant<int, kPlace == 1 ? 2 : 0>{});
+    wait_vm<kPlace == 1 ? 2 : 0>();      // this wave's loads of chunk c + 1
     __builtin_amdgcn_s_waitcnt(0xc07f);  // its reads of chunk c
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     read_scales(c + 1);
     read(c + 1, 0, wv[0], av[0]);
-    issue(c + S);
-    if constexpr (kPlace == 0) load_scales(c + 4);
+    issue(c + 2, part0, part1);
     products(p1);
-    order();
-#pragma unroll
-    for (int i = 0; i < NT * MT; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x020, 3, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
+    order(part0, part1, p0);
   };
   // (no way out between the chunks of four: it would cost a wait for all loads at the top)
   for (int left = nch >> 2; left > 0; --left) {
@@ -266,7 +270,7 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
     chunk(p2), ++c;
     chunk(p3), ++c;
   }
-  for (; c < nch; ++c) chunk(p1);  // up to three, whose scales are there
+  for (; c < nch; ++c) chunk(p2);  // up to three, whose scales are there
   // the ring becomes the waves' own room: no load may still land in it
   wait_vm<0>();
   __builtin_amdgcn_s_waitcnt(0xc07f);
@@ -278,7 +282,7 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
   __builtin_amdgcn_s_barrier();
   if (w >= WN * WM) return;
   const float* bias = bias_all + 32 * NT * wn;
-  uint8_t* own = lds + S * kStageBytes / kTileWaves * w;
+  uint8_t* own = lds + 2 * kStageBytes / kTileWaves * w;
   const int cols = a.swiglu ? a.N / 2 : a.N;
   constexpr int kG = NT < 2 ? NT : 2;  // column tiles that go together
   int reads[MT];
@@ -415,30 +419,30 @@ __device__ __forceinline__ bool find_place(const MxProductArgs& a, int rows, int
 
 // 256 columns x 256 rows, fewer where an expert has no more.
 __global__ __launch_bounds__(512, 2) void large_tile_kernel(MxProductArgs a, int n_tiles) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<4, 2, 2, 4, 2>::kBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<4, 2, 2, 4>::kBytes];
   Place p;
   if (!find_place(a, 256, n_tiles, &p)) return;
   const int rows = p.m.hi - p.m.lo;
-  if (rows > 128) tile<4, 2, 2, 4, 2>(a, p.m, p.nt * 256, lds);
-  else if (rows > 64) tile<2, 2, 4, 2, 2>(a, p.m, p.nt * 256, lds);
-  else tile<2, 1, 4, 2, 2>(a, p.m, p.nt * 256, lds);
+  if (rows > 128) tile<4, 2, 2, 4>(a, p.m, p.nt * 256, lds);
+  else if (rows > 64) tile<2, 2, 4, 2>(a, p.m, p.nt * 256, lds);
+  else tile<2, 1, 4, 2>(a, p.m, p.nt * 256, lds);
 }
 
 // 128 columns x 128 or 64 rows, two work-groups on a CU.
 __global__ __launch_bounds__(256, 2) void middle_tile_kernel(MxProductArgs a, int n_tiles) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<2, 2, 2, 2, 2>::kBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<2, 2, 2, 2>::kBytes];
   Place p;
   if (!find_place(a, 128, n_tiles, &p)) return;
   const int rows = p.m.hi - p.m.lo;
-  if (rows > 64) tile<2, 2, 2, 2, 2>(a, p.m, p.nt * 128, lds);
-  else tile<2, 1, 2, 2, 2>(a, p.m, p.nt * 128, lds);
+  if (rows > 64) tile<2, 2, 2, 2>(a, p.m, p.nt * 128, lds);
+  else tile<2, 1, 2, 2>(a, p.m, p.nt * 128, lds);
 }
 
 // 128 columns x 32 rows, three work-groups on a CU.
 __global__ __launch_bounds__(256, 3) void low_tile_kernel(MxProductArgs a, int n_tiles) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<2, 1, 2, 1, 2, 4>::kBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<2, 1, 2, 1, 4>::kBytes];
   Place p;
-  if (find_place(a, 32, n_tiles, &p)) tile<2, 1, 2, 1, 2, 4>(a, p.m, p.nt * 128, lds);
+  if (find_place(a, 32, n_tiles, &p)) tile<2, 1, 2, 1, 4>(a, p.m, p.nt * 128, lds);
 }
 
 }  // namespace
