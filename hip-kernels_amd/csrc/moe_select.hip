@@ -109,13 +109,29 @@ __global__ __launch_bounds__(kSelectWaves * kWave) void select_kernel(SelectArgs
   const size_t row = static_cast<size_t>(t) * static_cast<size_t>(a.stride);
   const double inf = __builtin_inf();
 
+  // (branches around all loads of a kind, so that these go out together)
   float x[NV], bias[NV];
+  int at_e[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int e = min(NV * lane + j, a.E - 1);
-    x[j] = a.fp32 ? static_cast<const float*>(a.logits)[row + e]
-                  : bf16_to_f32(static_cast<const uint16_t*>(a.logits)[row + e]);
-    bias[j] = a.bias ? a.bias[e] : 0.0f;
+    at_e[j] = min(NV * lane + j, a.E - 1);
+    bias[j] = 0.0f;
+  }
+  if (a.bias) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) bias[j] = a.bias[at_e[j]];
+  }
+  if (a.fp32) {
+    const float* l = static_cast<const float*>(a.logits) + row;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) x[j] = l[at_e[j]];
+  } else {
+    const uint16_t* l = static_cast<const uint16_t*>(a.logits) + row;
+    uint32_t h[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) h[j] = l[at_e[j]];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) x[j] = __uint_as_float(h[j] << 16);
   }
   double score[NV];
   uint64_t key[NV];
