@@ -167,18 +167,30 @@ __global__ __launch_bounds__(kSelectWaves * kWave) void select_kernel(SelectArgs
 
   if (a.groups > 1) {
     const int size = a.E / a.groups, lanes = size / NV;
-    if (a.group_rank <= 2 && size % NV == 0 && (lanes & (lanes - 1)) == 0) {
-      // A group is lanes of its own, a power of two: its best two by exchanges among them.
+    const bool pow2 = (lanes & (lanes - 1)) == 0;
+    if (a.group_rank <= 2 && size % NV == 0 && (pow2 || lanes <= 16)) {
+      // A group is lanes of its own: its best two by exchanges among them, or from one after the other (8192 tokens, 8
+      // groups of 20: 16 us; group after group, as below, 27).
       uint64_t first = key[0], second = 0;
 #pragma unroll
       for (int j = 1; j < NV; ++j) {
         second = max(second, min(first, key[j]));
         first = max(first, key[j]);
       }
-      for (int m = 1; m < lanes; m <<= 1) {
-        const uint64_t f = __shfl_xor(first, m, kWave), s = __shfl_xor(second, m, kWave);
+      const int mine = lane / lanes;
+      const auto join = [&](uint64_t f, uint64_t s) {
         second = max(max(second, s), min(first, f));
         first = max(first, f);
+      };
+      if (pow2) {
+        for (int m = 1; m < lanes; m <<= 1) join(__shfl_xor(first, m, kWave), __shfl_xor(second, m, kWave));
+      } else {
+        const uint64_t own1 = first, own2 = second;
+        int from = lane;
+        for (int m = 1; m < lanes; ++m) {
+          from = from + 1 < (mine + 1) * lanes ? from + 1 : mine * lanes;
+          join(__shfl(own1, from, kWave), __shfl(own2, from, kWave));
+        }
       }
       if (first > 1u) {  // (a group of switched off experts stays 1)
         double total = choice_of(first);
@@ -186,7 +198,6 @@ __global__ __launch_bounds__(kSelectWaves * kWave) void select_kernel(SelectArgs
         first = choice_key(total);
       }
       // its place among the groups, those of equal sums in turn
-      const int mine = lane / lanes;
       int before = 0;
       for (int g = 0; g < a.groups; ++g) {
         const uint64_t other = read_lane(first, g * lanes);
