@@ -66,17 +66,19 @@ __device__ __forceinline__ MTile find_m_tile(const MxProductArgs& a, int tile, i
   return MTile{-1, 0, 0};
 }
 
-// How many there are.
+// How many there are; whatever the offsets hold, not more than most_m_tiles().
 __device__ __forceinline__ int count_m_tiles(const MxProductArgs& a, int rows, int lane) {
   if (!a.offsets) return (a.rows + rows - 1) / rows;
+  const int most = a.rows / rows + min(a.E, a.rows);
   int n = 0;
   for (int e = lane; e < a.E; e += kWave) {
     const int lo = min(max(a.offsets[e], 0), a.rows), hi = min(max(a.offsets[e + 1], lo), a.rows);
     n += (hi - lo + rows - 1) / rows;
   }
+  n = min(n, most);
 #pragma unroll
   for (int m = 1; m < kWave; m <<= 1) n += __shfl_xor(n, m, kWave);
-  return __builtin_amdgcn_readfirstlane(n);
+  return min(__builtin_amdgcn_readfirstlane(n), most);
 }
 
 // Row of a that result row p reads, -1 for one of zeros.

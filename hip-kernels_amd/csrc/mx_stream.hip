@@ -17,6 +17,9 @@
 // blocks, whose weights' scales are loaded during the span before and put into LDS between
 // the two.  Where tiles are few, KS waves share a tile's K, and their sums meet in LDS in
 // a fixed order.
+//
+// Bound by the weights' bandwidth: one or two rows each of 111 experts, 5760 x 2880, 162 us (5.8 TB/s); 29
+// experts 53 us (4.8); by latency where they are few: 1 x 5120 x 2880, weights in no cache, 7.5 us.
 #include "mx_product.h"
 
 namespace gxmoe {

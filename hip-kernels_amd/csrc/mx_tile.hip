@@ -12,11 +12,13 @@
 // Per chunk a wave runs four steps of NT x MT products on operands that it read
 // during the step before.  Before the last step, whose operands are in registers by then, it waits for
 // its loads of the next chunk and meets the others, after which the chunk's
-// stage is free for the loads of the chunk after the next.
+// stage is free for the loads of the chunk after the next.  These go out in three parts, in
+// that step and the first two of the next chunk (8192^3: 274 us; all at once 279).
 //
-// Large tiles are bound by the requests for their operands and by the matrix cores' power: 8192 x 8192 x
-// 8192 takes 279 us (3.9 PFLOP/s; products alone reach 6.2 to 6.7 with random operands),
-// each round of tiles 10 us beyond its chunks.  Smaller ones stand two or three on a CU, so
+// Large tiles are bound by power: 8192 x 8192 x 8192 takes 274 us (4.0 PFLOP/s; the clock is
+// 1.8 GHz), with operands of zeros 224; products alone, from registers, reach 6.2 to 6.7 PFLOP/s with random
+// operands.  Each round of tiles takes 10 us beyond its chunks.  (Four waves of 128 x 128 each read a third less from
+// LDS, but one wave a SIMD leaves gaps: 329 us.)  Smaller tiles stand two or three on a CU, so
 // that one's first loads and last stores overlap another's chunks; their weights come at 4.2 TB/s
 // with rows of 1440 bytes that straddle lines, at 5.3 where rows begin on them (128 experts of 16 rows each).
 #include <type_traits>
@@ -31,7 +33,8 @@ typedef __attribute__((address_space(3))) void lds_void_t;
 
 constexpr int kBlocks = 8;  // of a chunk
 
-// WN x WM waves, each NT x MT products of 32 columns x 32 rows, in a work-group of W waves: those that are left over load, and do another's products to no end.
+// WN x WM waves, each NT x MT products of 32 columns x 32 rows, in a work-group of W waves:
+// those that are left over load, and do another's products to no end.
 template <int NT, int MT, int WN, int WM, int W = WN * WM>
 struct Shape {
   static constexpr int kWaves = W, kThreads = kWaves * kWave;
@@ -451,7 +454,9 @@ hipError_t launch_mx_tile(const MxProductArgs& a, MxTile kind, hipStream_t s) {
   const int rows = kind == MxTile::large ? 256 : kind == MxTile::middle ? 128 : 32;
   const int cols = kind == MxTile::large ? 256 : 128, n_tiles = (a.N + cols - 1) / cols;
   // a multiple of eight, so that every XCD has work-groups enough for its share
-  const dim3 grid(static_cast<uint32_t>((most_m_tiles(a, rows) * n_tiles + 7) & ~int64_t(7)));
+  const int64_t tiles = (most_m_tiles(a, rows) * n_tiles + 7) & ~int64_t(7);
+  if (tiles * 512 > UINT32_MAX) return hipErrorInvalidConfiguration;  // a launch's threads
+  const dim3 grid(static_cast<uint32_t>(tiles));
   if (kind == MxTile::large) hipLaunchKernelGGL(large_tile_kernel, grid, dim3(512), 0, s, a, n_tiles);
   else if (kind == MxTile::middle) hipLaunchKernelGGL(middle_tile_kernel, grid, dim3(256), 0, s, a, n_tiles);
   else hipLaunchKernelGGL(low_tile_kernel, grid, dim3(256), 0, s, a, n_tiles);
