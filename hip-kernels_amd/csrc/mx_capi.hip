@@ -139,10 +139,9 @@ int product(const uint8_t* a, const uint8_t* as, int a_rows, const int32_t* row_
   p.swiglu = r->swiglu != 0;
   p.alpha = r->alpha;
   p.limit = r->limit;
-  p.out = r->out;
+  p.out = quantized ? r->out_packed : r->out;
   p.stride = r->out_stride;
   p.out_fp32 = r->out_fp32 != 0;
-  p.out_packed = r->out_packed;
   p.out_scales = r->out_scales;
   p.vec = aligned(r->out, 16) && r->out_stride % (r->out_fp32 ? 4 : 8) == 0;
   HIP_TRY(launch_mx_product(p, static_cast<hipStream_t>(stream)), "MXFP4 product launch");

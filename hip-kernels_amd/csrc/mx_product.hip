@@ -25,7 +25,7 @@ hipError_t launch_mx_product(const MxProductArgs& a, hipStream_t s) {
     // Waves of 32 columns read a's rows half as often, and are half as many: 2 each of 128 at N = 2880 take 87 (16 columns:
     // 95), 1 x 5120 x 2880 8.4 (7.5).  Four waves share a long K while there are CUs for it: 1 x 2048 x 8192 7.6
     // (one wave 11.9), 1 x 8192 x 8192 11.1 (13.8); 1 x 10240 x 4096 7.8 (6.9), 32 x 2880 x 4096 11.3 (9.7).
-    return launch_mx_stream(a, a.out_packed || waves > 64 * kMxCus,
+    return launch_mx_stream(a, a.quantized() || waves > 64 * kMxCus,
                             a.K >= 4096 && a.rows <= kStreamRows && waves <= 2 * kMxCus, s);
   }
   //                        32 x 128  128 x 128                        32 x 128  128 x 128

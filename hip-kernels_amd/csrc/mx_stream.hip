@@ -115,7 +115,7 @@ __device__ __forceinline__ void write_rows(const MxProductArgs& a, const f32x4_t
 #pragma unroll
       for (int q = 0; q < 2; ++q) v[i][q] = mx_swiglu(v[i][2 * q], v[i][2 * q + 1], a.alpha, a.limit);
   }
-  if (a.out_packed) {
+  if (a.quantized()) {
     if constexpr (NT == 2) {
       const size_t row = static_cast<size_t>(p) * (cols / 32);
       if (a.swiglu) {
@@ -132,14 +132,14 @@ __device__ __forceinline__ void write_rows(const MxProductArgs& a, const f32x4_t
           d |= ((static_cast<uint32_t>(__shfl(static_cast<int>(mine), r + 16 * q, kWave)) >> (8 * g)) & 0xffu) << (8 * q);
         const int block = (n0 - 32) / 64;
         if (live && 32 * block < cols) {
-          reinterpret_cast<uint32_t*>(a.out_packed)[4 * (row + block) + g] = d;
+          static_cast<uint32_t*>(a.out)[4 * (row + block) + g] = d;
           if (g == 0) a.out_scales[row + block] = static_cast<uint8_t>(code);
         }
       } else {  // columns 4 g + {0 .. 3} and 16 further on
         const float x[8] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
         const uint32_t code = block_scale(x), d = mx_pack8(x, code);
         if (live && n0 < cols) {
-          uint16_t* o = reinterpret_cast<uint16_t*>(a.out_packed + 16 * (row + n0 / 32));
+          uint16_t* o = static_cast<uint16_t*>(a.out) + 8 * (row + n0 / 32);
           o[g] = static_cast<uint16_t>(d);
           o[4 + g] = static_cast<uint16_t>(d >> 16);
           if (g == 0) a.out_scales[row + n0 / 32] = static_cast<uint8_t>(code);
@@ -162,7 +162,7 @@ __device__ __forceinline__ void write_rows(const MxProductArgs& a, const f32x4_t
 }
 
 template <int NT, int KS>
-__device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles, uint8_t* lds) {
+__device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int grid, uint8_t* lds) {
   constexpr int kN = 16 * NT, kLine = NT * 2048;
   constexpr int kLoads = 2 * NT + 4;  // of a line of the rows, and a chunk of a's
   constexpr int kLanes = kWave / kN;       // per weight row, for its scales
@@ -172,9 +172,10 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles
   // This work-group's run of tiles, the columns of an m-tile in turn: as long as all others' but the last, so that none
   // is left with a longer one (fewer waves hold the bandwidth too).  XCD b % 8 has neighbouring runs.  Tiles whose results
   // make one block go together.
-  const int together = a.swiglu && a.out_packed ? 2 : 1;
+  const int together = a.swiglu && a.quantized() ? 2 : 1;
+  const int n_tiles = (a.N + kN * together - 1) / (kN * together) * together;
   const int64_t total = static_cast<int64_t>(count_m_tiles(a, kStreamRows, lane)) * (n_tiles / together);
-  const int64_t run = (total + gridDim.x - 1) / gridDim.x, runs = run ? (total + run - 1) / run : 0;
+  const int64_t run = (total + grid - 1) / grid, runs = run ? (total + run - 1) / run : 0;
   const int xcd = blockIdx.x & 7, share = static_cast<int>(runs >> 3), more = static_cast<int>(runs & 7);
   if (static_cast<int>(blockIdx.x >> 3) >= share + (xcd < more ? 1 : 0)) return;
   const int64_t b = xcd * share + min(xcd, more) + static_cast<int>(blockIdx.x >> 3);
@@ -348,24 +349,23 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int n_tiles
 }
 
 template <int NT, int KS>
-__global__ __launch_bounds__(KS * kWave) void stream_kernel(MxProductArgs a, int n_tiles) {
+__global__ __launch_bounds__(KS * kWave) void stream_kernel(MxProductArgs a, int grid) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-  stream_tiles<NT, KS>(a, n_tiles, lds);
+  stream_tiles<NT, KS>(a, grid, lds);
 }
 
 template <int NT, int KS>
 hipError_t launch(const MxProductArgs& a, hipStream_t s) {
   constexpr int kN = 16 * NT;
-  int n_tiles = (a.N + kN - 1) / kN;
-  const int together = a.swiglu && a.out_packed ? 2 : 1;
-  n_tiles = (n_tiles + together - 1) / together * together;
+  const int pieces = a.swiglu && a.quantized() ? 2 * kN : kN;  // columns that go together
   const size_t bytes = static_cast<size_t>(KS) * wave_bytes<NT, KS>(a.K / 32);
   // as many as fit at once (two waves per SIMD with their registers), each with a run of tiles
   const int64_t by_lds = 160 * 1024 / bytes, by_waves = 8 / KS, fit = kMxCus * (by_lds < by_waves ? by_lds : by_waves);
-  int64_t grid = most_m_tiles(a, kStreamRows) * (n_tiles / together);
+  int64_t grid = most_m_tiles(a, kStreamRows) * ((a.N + pieces - 1) / pieces);
   if (grid > fit) grid = fit;
   grid = (grid + 7) & ~int64_t(7);  // every XCD has as many work-groups
-  hipLaunchKernelGGL((stream_kernel<NT, KS>), dim3(static_cast<uint32_t>(grid)), dim3(KS * kWave), bytes, s, a, n_tiles);
+  hipLaunchKernelGGL((stream_kernel<NT, KS>), dim3(static_cast<uint32_t>(grid)), dim3(KS * kWave), bytes, s, a,
+                     static_cast<int>(grid));
   return hipGetLastError();
 }
 

@@ -318,7 +318,7 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
 #pragma unroll
           for (int q = 0; q < 8; ++q) v[i][q] = mx_swiglu(v[i][2 * q], v[i][2 * q + 1], a.alpha, a.limit);
       }
-      if (a.out_packed) {
+      if (a.quantized()) {
         const size_t ob = static_cast<size_t>(p) * (cols / 32);
         uint32_t code;
         if (a.swiglu) {
@@ -328,7 +328,7 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
             const gx_u32x2 d = quantize_block<true>(x, code);
             if (live && n / 2 < cols) {
               const size_t at = ob + n / 64;
-              reinterpret_cast<gx_u32x2*>(a.out_packed)[2 * at + half] = d;
+              static_cast<gx_u32x2*>(a.out)[2 * at + half] = d;
               if (half == 0) a.out_scales[at] = static_cast<uint8_t>(code);
             }
           }
@@ -338,7 +338,7 @@ __device__ __forceinline__ void tile(const MxProductArgs& a, const MTile& mt, in
             const gx_u32x2 d = quantize_block<false>(v[i], code);
             if (live && n + 32 * i < cols) {
               const size_t at = ob + n / 32 + i;
-              reinterpret_cast<gx_u32x2*>(a.out_packed)[2 * at + half] = d;
+              static_cast<gx_u32x2*>(a.out)[2 * at + half] = d;
               if (half == 0) a.out_scales[at] = static_cast<uint8_t>(code);
             }
           }

@@ -1226,13 +1226,13 @@ def select_experts(logits, top_k: int, score: str = "softmax", bias=None, num_gr
         _vector("bias", bias, dev, E, torch.float32)
         bias = bias.data_ptr()
     if out is None:
-        if dev.type != "cuda":
+        if not logits.is_cuda:
             _gpu("logits", dev)
         if top_k > E:
             _bad(f"top_k={top_k} of {E} experts")
         if stream is None:
-            idx = logits.new_empty((T, top_k), dtype=torch.int32)
-            w = logits.new_empty((T, top_k), dtype=torch.float32)
+            idx = logits.new_empty(T, top_k, dtype=torch.int32)
+            w = logits.new_empty(T, top_k, dtype=torch.float32)
         else:
             idx = _empty((T, top_k), torch.int32, dev, stream)
             w = _empty((T, top_k), torch.float32, dev, stream)
@@ -1282,7 +1282,7 @@ class MXFP4Matrix:
         n = rows * K
         self = cls.__new__(cls)
         if stream is None and like is not None:
-            self._held = like.new_empty((n // 32 * 17,), dtype=torch.uint8)
+            self._held = like.new_empty(n // 32 * 17, dtype=torch.uint8)
         else:
             self._held = _empty((n // 32 * 17,), torch.uint8, device, stream)
         self._tensors, self._device, self._experts, self._rows, self._K = None, device, None, rows, K
@@ -1338,7 +1338,7 @@ def mxfp4_quantize(x, out: MXFP4Matrix | None = None, stream=None) -> MXFP4Matri
     if K & 31 or not K:
         _bad(f"x has {K} columns, a positive multiple of 32 is needed")
     if out is None:
-        if dev.type != "cuda":
+        if not x.is_cuda:
             _gpu("x", dev)
         out = MXFP4Matrix._empty(rows, K, x, dev, stream)
     else:
@@ -1413,7 +1413,7 @@ def _product(a, w, rows, offsets, row_index, bias, swiglu, alpha, limit, dtype, 
                 _gpu("a", dev)
             like = a._held
             if stream is None and like is not None:
-                out = like.new_empty((rows, cols), dtype=dtype)
+                out = like.new_empty(rows, cols, dtype=dtype)
             else:
                 out = _empty((rows, cols), dtype, dev, stream)
             stride = cols
