@@ -170,6 +170,21 @@ def test_product_swiglu(gpu, M, N, K, with_bias):
         ref.assert_values(gpu.mxfp4_matmul(a, w, bias=bias, swiglu=True, dtype=dtype), want, tol, (M, N, K))
 
 
+def test_product_refusals(gpu):
+    a, w, _ = operands(gpu, 3, 64, 64)
+    for kw, text in ((dict(alpha=1e300), "alpha"), (dict(alpha=math.inf), "alpha"), (dict(alpha=math.nan), "alpha"),
+                     (dict(alpha="1"), "alpha"), (dict(limit=-1.0), "limit"), (dict(limit=-1e300), "limit"),
+                     (dict(limit=math.nan), "limit"), (dict(dtype=torch.float16), "dtype"),
+                     (dict(out=torch.empty((3, 33), device="cuda")), "shape"),
+                     (dict(out=torch.empty((3, 32), device="cuda", dtype=torch.float16)), "dtype")):
+        for quantize in (False, True):
+            if not quantize or "dtype" not in kw and "out" not in kw:
+                with pytest.raises(ValueError, match=text):
+                    gpu.mxfp4_matmul(a, w, swiglu=True, quantize=quantize, **kw)
+    with pytest.raises(ValueError, match="K="):
+        gpu.mxfp4_matmul(a, operands(gpu, 3, 64, 96)[1])
+
+
 @pytest.mark.parametrize("M, N, K", [(1, 96, 4096), (5, 2880, 4128), (17, 130, 4640), (40, 992, 512), (1100, 1920, 64),
                                      (1031, 1985, 288), (2950, 2944, 96), (2817, 2946, 320)])
 def test_product_of_many_tiles(gpu, M, N, K):
