@@ -1366,7 +1366,9 @@ def mxfp4_dequantize(m: MXFP4Matrix, dtype=torch.bfloat16, out=None, stream=None
             _bad(f"dtype must be torch.bfloat16 or torch.float32, got {dtype}")
         if dev.type != "cuda":
             _gpu("m", dev)
-        out, stride = _empty(m.shape, dtype, dev, stream), K
+        like, stride = m._held, K
+        out = like.new_empty(rows, K, dtype=dtype) if stream is None and like is not None \
+            else _empty(m.shape, dtype, dev, stream)
     else:
         have, cols, stride = _strided_rows("out", out, (torch.bfloat16, torch.float32), dev)
         if (have, cols) != (rows, K):
