@@ -15,16 +15,16 @@ hipError_t launch_mx_product(const MxProductArgs& a, hipStream_t s) {
 
   // The stream holds the whole of the weights' bandwidth with few rows, and with few tiles its short chain counts:
   //                  stream    32 x 128                          stream    32 x 128
-  //   1 x 5120 x 2880   7.5      12.0        2 each of 128       165       208
-  //   32 x 5120 x 2880  9.6      12.1        4 each of 128       200       240
-  //   64 x 2880 x 4096 12.3      13.8        8 each of 128       242       253
+  //   1 x 5120 x 2880   7.3      12.0        2 each of 128       162       208
+  //   32 x 5120 x 2880  8.3      12.1        4 each of 128       200       240
+  //   64 x 2880 x 4096 11.1      13.8        8 each of 128       242       253
   //   96 x 5120 x 2880 17.4      12.1        8 each of 32         73        63
   //   32 x 32768 x 4096  37      20.8        4 each of 32         66        62
   const int64_t waves = tiles(kStreamRows, 16);
   if (a.K >= 512 && (each <= 4 || waves <= 4 * kMxCus)) {
     // Waves of 32 columns read a's rows half as often, and are half as many: 2 each of 128 at N = 2880 take 87 (16 columns:
     // 95), 1 x 5120 x 2880 8.4 (7.5).  Four waves share a long K while there are CUs for it: 1 x 2048 x 8192 7.6
-    // (one wave 11.9), 1 x 8192 x 8192 11.1 (13.8); 1 x 10240 x 4096 7.8 (6.9), 32 x 2880 x 4096 11.3 (9.7).
+    // (one wave 11.9), 1 x 8192 x 8192 11.1 (13.8); 1 x 10240 x 4096 7.8 (6.9), 32 x 2880 x 4096 11.3 (9.1).
     return launch_mx_stream(a, a.quantized() || waves > 64 * kMxCus,
                             a.K >= 4096 && a.rows <= kStreamRows && waves <= 2 * kMxCus, s);
   }

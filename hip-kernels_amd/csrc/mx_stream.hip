@@ -35,7 +35,7 @@ __device__ __forceinline__ void wait_vm() {  // vmcnt(N), the other counters as 
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0f70);
 }
 
-constexpr int kRing = 4;    // lines
+constexpr int kRing = 4;    // lines (eight: 1 x 5120 x 2880 8.4 us for 7.3, whose 12 lines take two whole turns)
 constexpr int kSpan = 128;  // blocks whose scales are in LDS at a time: whole turns of the ring
 
 // Bytes between the scales of two rows: an odd number of 16, so that 16 rows meet all banks.
@@ -174,13 +174,19 @@ __device__ __forceinline__ void stream_tiles(const MxProductArgs& a, int grid, u
   // make one block go together.
   const int together = a.swiglu && a.quantized() ? 2 : 1;
   const int n_tiles = (a.N + kN * together - 1) / (kN * together) * together;
-  const int64_t total = static_cast<int64_t>(count_m_tiles(a, kStreamRows, lane)) * (n_tiles / together);
+  const int m_tiles = count_m_tiles(a, kStreamRows, lane);
+  const int64_t total = static_cast<int64_t>(m_tiles) * (n_tiles / together);
   const int64_t run = (total + grid - 1) / grid, runs = run ? (total + run - 1) / run : 0;
   const int xcd = blockIdx.x & 7, share = static_cast<int>(runs >> 3), more = static_cast<int>(runs & 7);
   if (static_cast<int>(blockIdx.x >> 3) >= share + (xcd < more ? 1 : 0)) return;
   const int64_t b = xcd * share + min(xcd, more) + static_cast<int>(blockIdx.x >> 3);
-  int id = static_cast<int>(run * b) * together;
-  const int id_end = static_cast<int>(min(run * (b + 1), total)) * together;
+  int id = static_cast<int>(run * b) * together, id_end = static_cast<int>(min(run * (b + 1), total)) * together;
+  if (run == 1) {
+    // Without runs the m-tiles of the same columns are neighbours, whose weights come once to their L2.
+    const int i = static_cast<int>(b);
+    id = i % m_tiles * n_tiles + i / m_tiles * together;
+    id_end = id + together;
+  }
 
   const int r = lane & 15, g = lane >> 4;
   const int nb = a.K / 32, chunks = (nb + 7) / 8;
