@@ -294,6 +294,19 @@ __global__ __launch_bounds__(kSelectWaves * kWave) void select_kernel(SelectArgs
 }  // namespace
 
 hipError_t launch_select_experts(const SelectArgs& a, hipStream_t s) {
+  constexpr int kMost = 1 << 25;  // tokens of a launch, whose threads are below 2^32
+  if (a.T > kMost) {
+    SelectArgs part = a;
+    part.T = kMost;
+    const hipError_t e = launch_select_experts(part, s);
+    if (e != hipSuccess) return e;
+    const size_t row = static_cast<size_t>(a.stride) * (a.fp32 ? 4 : 2), slots = static_cast<size_t>(kMost) * a.k;
+    part.logits = static_cast<const uint8_t*>(a.logits) + row * kMost;
+    part.idx = a.idx + slots;
+    part.w = a.w + slots;
+    part.T = a.T - kMost;
+    return launch_select_experts(part, s);
+  }
   const dim3 grid((a.T + kSelectWaves - 1) / kSelectWaves), block(kSelectWaves * kWave);
   if (a.E <= 64) hipLaunchKernelGGL(select_kernel<1>, grid, block, 0, s, a);
   else if (a.E <= 128) hipLaunchKernelGGL(select_kernel<2>, grid, block, 0, s, a);

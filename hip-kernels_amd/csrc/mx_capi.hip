@@ -77,7 +77,7 @@ int product(const uint8_t* a, const uint8_t* as, int a_rows, const int32_t* row_
   if (rc != GPTOSS_OK) return rc;
   if (N <= 0 || N > kMaxColumns) return set_error(GPTOSS_ERR_INVALID, "N=%d (1 to 2^24)", N);
   if (rows < 0 || rows > kMaxRows) return set_error(GPTOSS_ERR_INVALID, "rows=%d (0 to 2^26)", rows);
-  // a launch's work-groups stay within 32 bits
+  // the kernels count tiles in 32 bits
   if ((static_cast<int64_t>(rows) / 32 + E + 1) * (N / 64 + 1) > INT32_MAX)
     return set_error(GPTOSS_ERR_UNSUPPORTED, "%d rows of %d columns in one call (2^42 results)", rows, N);
   if (r == nullptr) return set_error(GPTOSS_ERR_INVALID, "result is NULL");
@@ -144,7 +144,10 @@ int product(const uint8_t* a, const uint8_t* as, int a_rows, const int32_t* row_
   p.out_fp32 = r->out_fp32 != 0;
   p.out_scales = r->out_scales;
   p.vec = aligned(r->out, 16) && r->out_stride % (r->out_fp32 ? 4 : 8) == 0;
-  HIP_TRY(launch_mx_product(p, static_cast<hipStream_t>(stream)), "MXFP4 product launch");
+  const hipError_t e = launch_mx_product(p, static_cast<hipStream_t>(stream));
+  if (e == hipErrorInvalidConfiguration)
+    return set_error(GPTOSS_ERR_UNSUPPORTED, "%d rows of %d columns in one call: more tiles than a launch holds", rows, N);
+  HIP_TRY(e, "MXFP4 product launch");
   return ok();
 }
 

@@ -1221,6 +1221,8 @@ def select_experts(logits, top_k: int, score: str = "softmax", bias=None, num_gr
     if isinstance(logits, torch.Tensor) and logits.dim() == 2 and logits.is_contiguous() \
             and (logits.dtype is torch.bfloat16 or logits.dtype is torch.float32):
         T, E = logits.shape
+        if T >> 31 or E >> 31:
+            _bad(f"logits of shape {tuple(logits.shape)} is too large")
         stride = E
     else:
         T, E, stride = _strided_rows("logits", logits, (torch.bfloat16, torch.float32))
@@ -1273,6 +1275,8 @@ class MXFP4Matrix:
                  f"{tuple(scales.shape)}")
         if packed.shape[-1] == 0:
             _bad("K must be positive")
+        if any(n > _INT_MAX for n in (*packed.shape[:-1], 2 * packed.shape[-1])):
+            _bad(f"packed of shape {tuple(packed.shape)} is too large")
         if packed.device != scales.device:
             _bad(f"packed is on {packed.device}, scales are on {scales.device}")
         self._held, self._tensors, self._device = None, (packed, scales), packed.device
@@ -1334,6 +1338,8 @@ def mxfp4_quantize(x, out: MXFP4Matrix | None = None, stream=None) -> MXFP4Matri
     if isinstance(x, torch.Tensor) and x.dim() == 2 and x.is_contiguous() \
             and (x.dtype is torch.bfloat16 or x.dtype is torch.float32):
         rows, K = x.shape
+        if rows >> 31 or K >> 31:
+            _bad(f"x of shape {tuple(x.shape)} is too large")
         stride = K
     else:
         rows, K, stride = _strided_rows("x", x, (torch.bfloat16, torch.float32))
@@ -1361,6 +1367,8 @@ def mxfp4_dequantize(m: MXFP4Matrix, dtype=torch.bfloat16, out=None, stream=None
     _matrix("m", m)
     dev, K = m._device, m._K
     rows = m._rows if m._experts is None else m._experts * m._rows
+    if rows > _INT_MAX:
+        _bad(f"a stack of shape {m.shape} is too large")
     if out is None:
         if dtype is not torch.bfloat16 and dtype is not torch.float32:
             _bad(f"dtype must be torch.bfloat16 or torch.float32, got {dtype}")

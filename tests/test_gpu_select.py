@@ -190,6 +190,20 @@ def test_strided_logits_and_given_results(gpu):
     assert gpu.select_experts(wide[:0], 4)[0].shape == (0, 4)
 
 
+def test_the_largest_call(gpu):
+    """2^26 tokens: more threads than one launch holds."""
+    T = 1 << 26
+    logits = torch.zeros((T, 2), device="cuda", dtype=BF16)
+    for t in (0, 12345, (1 << 25) - 1, 1 << 25, T - 2):
+        logits[t, 1] = 1.0 + t % 7
+    idx, w = gpu.select_experts(logits, 1, renormalize=False)
+    torch.cuda.synchronize()
+    assert torch.equal(idx[:, 0].long(), (logits[:, 1] > 0).long())
+    for t in (0, 1, 12345, (1 << 25) - 1, 1 << 25, (1 << 25) + 1, T - 2, T - 1):
+        want = 1 / (1 + math.exp(-float(logits[t, 1])))
+        assert abs(float(w[t]) - want) < 2.0 ** -23 * want
+
+
 def test_a_prefix_gives_the_same(gpu):
     """A token's choice is its own: the same bits in a smaller call, and in another place of it."""
     logits = (2 * torch.randn((3000, 256), device="cuda", generator=gen_of(14))).to(BF16)

@@ -188,6 +188,12 @@ def test_grouped_refusals(g, kw, status, text):
     refused(g, product(g, True, **kw), status, text)
 
 
+def test_product_of_more_tiles_than_a_launch_holds(g):
+    far = {n: (i + 1) << 44 for i, n in enumerate(("a", "asc", "w", "ws", "bias"))}
+    refused(g, product(g, False, dict(out=8 << 44, stride=1 << 16), a_rows=1 << 23, N=1 << 16, K=32, **far), "UNSUPPORTED",
+            b"columns in one call")
+
+
 def test_products_of_nothing(g):
     assert product(g, False, a_rows=0, a=None, asc=None, w=None, ws=None) == g.GPTOSS_OK
     assert product(g, True, a_rows=0, rows=0, a=None, asc=None, off=None) == g.GPTOSS_OK
@@ -212,6 +218,22 @@ def u8(*shape):
 def test_matrix_refusals(g, packed, scales, text):
     with pytest.raises(ValueError, match=text):
         g.MXFP4Matrix(packed, scales)
+
+
+def test_sizes_past_32_bits(g):
+    """Of matrices without memory: a size that the C calls cannot hold is refused and not cut short."""
+    meta = dict(dtype=torch.uint8, device="meta")
+    for shape in ((1 << 31, 32), (1 << 33, 32), (1, 1 << 32), (1 << 32, 1, 32)):
+        with pytest.raises(ValueError, match="too large"):
+            g.MXFP4Matrix(torch.empty((*shape[:-1], shape[-1] // 2), **meta), torch.empty((*shape[:-1], shape[-1] // 32), **meta))
+    for shape in (((1 << 32) + 8, 32), (8, 1 << 32)):
+        with pytest.raises(ValueError, match="too large"):
+            g.mxfp4_quantize(torch.empty(shape, dtype=BF, device="meta"))
+        with pytest.raises(ValueError, match="too large"):
+            g.select_experts(torch.empty(shape, dtype=BF, device="meta"), 4)
+    m = g.MXFP4Matrix(torch.empty((1 << 20, 1 << 12, 16), **meta), torch.empty((1 << 20, 1 << 12, 1), **meta))
+    with pytest.raises(ValueError, match="too large"):
+        g.mxfp4_dequantize(m)
 
 
 def test_matrix_is_fixed(g):
