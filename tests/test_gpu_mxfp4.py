@@ -323,3 +323,55 @@ def test_bf16_patterns_survive_the_trip(gpu):
     again = gpu.mxfp4_quantize(v)
     assert torch.equal(again.scales, m.scales) and torch.equal(gpu.mxfp4_dequantize(again), v)
     assert np.isfinite(v.float().cpu().numpy()).all()
+
+
+def rows_of(gpu, m, at):
+    return gpu.MXFP4Matrix(m.packed[at].contiguous(), m.scales[at].contiguous())
+
+
+def test_quantize_past_32_bits(gpu):
+    """Values, packed bytes and results at offsets beyond 2^32."""
+    rows, K = (1 << 21) + 5, 4128
+    x = torch.empty((rows, K), device="cuda", dtype=BF16)
+    x.view(torch.int16).random_(-17000, 17000)  # with NaN among the negative ones
+    m = gpu.mxfp4_quantize(x)
+    back = gpu.mxfp4_dequantize(m)
+    assert m.packed.numel() > 1 << 32
+    at = torch.tensor([0, 1, 520287, 1040575, 2080895, rows - 2, rows - 1], device="cuda")
+    few = x[at]
+    want = ref.quantize(few)
+    got = rows_of(gpu, m, at)
+    assert torch.equal(ref.unpack(got.packed), want[0]) and torch.equal(got.scales.cpu(), want[1])
+    assert torch.equal(back[at].cpu().double().nan_to_num(-7.25), ref.of_matrix(got).to(BF16).double().nan_to_num(-7.25))
+
+
+def test_products_past_32_bits(gpu):
+    """Weights, and results, at offsets beyond 2^32."""
+    E, N, K = 290, 4096, 8192
+    w = ref.random_matrix(gpu, gen_of(1), E, N, K, low=119, high=124)
+    a = ref.random_matrix(gpu, gen_of(2), 200, K, low=119, high=124)
+    W = ref.of_matrix(gpu.MXFP4Matrix(w.packed[E - 2], w.scales[E - 2]))
+    for n in (3, 40, 200):
+        offsets = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+        offsets[E - 1:] = n
+        want, tol = ref.product(ref.of_matrix(gpu.MXFP4Matrix(a.packed[:n], a.scales[:n])), W)
+        ref.assert_values(gpu.grouped_mxfp4_matmul(a, w, offsets, n), want, tol)
+        all_rows = torch.tensor([0] * E + [n], dtype=torch.int32, device="cuda")
+        last = gpu.grouped_mxfp4_matmul(a, w, all_rows, n)
+        want, tol = ref.product(ref.of_matrix(gpu.MXFP4Matrix(a.packed[:n], a.scales[:n])),
+                                ref.of_matrix(gpu.MXFP4Matrix(w.packed[E - 1], w.scales[E - 1])))
+        ref.assert_values(last, want, tol)
+    flat = gpu.MXFP4Matrix(w.packed.view(E * N, -1), w.scales.view(E * N, -1))  # tiles, by its many columns
+    for n in (2, 8, 40, 200):
+        few = gpu.MXFP4Matrix(a.packed[:n], a.scales[:n])
+        want, tol = ref.product(ref.of_matrix(few), W)
+        ref.assert_values(gpu.mxfp4_matmul(few, flat)[:, (E - 2) * N:(E - 1) * N], want, tol)
+    del w, flat
+    M, N, K = 70001, 32768, 64
+    a, w, _ = operands(gpu, M, N, K, 3, low=119, high=124)
+    got = gpu.mxfp4_matmul(a, w, dtype=F32)
+    packed = gpu.mxfp4_matmul(a, w, quantize=True)
+    at = torch.tensor([0, 16383, 32768, 65535, 65536, M - 2, M - 1], device="cuda")
+    want, tol = ref.product(ref.of_matrix(rows_of(gpu, a, at)), ref.of_matrix(w))
+    ref.assert_values(got[at], want, tol)
+    ref.assert_quantized(rows_of(gpu, packed, at), want, tol)
