@@ -9,7 +9,8 @@
 // do not begin on one (K = 2880: 1440 bytes), a row's blocks lie a few places further on, and a chunk of
 // eight blocks needs two lines.  (Streaming alone, 5 to 8 waves on a CU: 128 bytes of each of 8 rows
 // per load 6.9 TB/s where they are lines, 5.4 where they straddle two.  Loads straight to the
-// operands' registers take 64 bytes of a row at a time: the whole kernel 3.1 TB/s.)  The rows of a, few
+// operands' registers take 64 bytes of a row at a time: the whole kernel 3.1 TB/s.  Lines that no
+// cache keeps, 6 to 8 % faster: 32 experts of a row each that were not read before, 54 us, without 59.)  The rows of a, few
 // and read by all, go to registers four chunks ahead.
 //
 // A wave goes through a run of neighbouring tiles of the same rows, and the loads of the next
