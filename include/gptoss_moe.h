@@ -625,7 +625,8 @@ typedef struct gptoss_routing_config {
  * logits_stride elements apart, as gptoss_moe_route writes them.  bias: device fp32
  * [num_experts] or NULL.  expert_indices and expert_weights ([num_tokens][top_k])
  * are what gptoss_moe_permute_plan, gptoss_moe_layer_forward_routed and
- * gptoss_moe_combine_forward take. */
+ * gptoss_moe_combine_forward take, within their limits (256 experts and 8 of a token for
+ * the plan). */
 int gptoss_moe_select_experts(const void* logits, int64_t logits_stride, int logits_fp32, const float* bias,
                               int num_tokens, int num_experts, const gptoss_routing_config* cfg,
                               int32_t* expert_indices, float* expert_weights, void* stream);
