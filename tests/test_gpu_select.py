@@ -105,6 +105,30 @@ def test_choices_that_32_bits_do_not_tell_apart(gpu, score, groups):
     check(gpu, logits, 8, score=score, bias=bias, groups=groups, top_groups=(groups + 1) // 2)
 
 
+@pytest.mark.parametrize("E, groups", [(129, 1), (256, 1), (256, 8), (300, 3), (1000, 1), (1024, 16)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_many_chosen_of_many(gpu, E, groups, score):
+    """Ties on the border of what is chosen and within it, choices of all sizes and signs, few left, infinite and NaN ones."""
+    gen = gen_of(E)
+    kw = dict(score=score, groups=groups, top_groups=(groups + 1) // 2)
+    few = torch.randint(0, 3, (12, E), device="cuda", generator=gen).float()
+    some = torch.randint(0, 60, (12, E), device="cuda", generator=gen).float() / 16
+    plain = torch.randn((12, E), device="cuda", generator=gen)
+    size = torch.exp2(torch.randint(-100, 100, (E,), device="cuda", generator=gen).float())
+    wide = torch.randn(E, device="cuda", generator=gen) * size
+    two = torch.where(torch.rand(E, device="cuda", generator=gen) < 0.02, 1e30, -1e-30)
+    left = torch.full((E,), -math.inf, device="cuda")
+    left[::E // 9] = 0.25
+    odd = wide.clone()
+    odd[3], odd[E // 2], odd[E - 1] = math.inf, math.nan, -math.inf
+    for k in (6, 8, 32):
+        for logits in (few, some, some.to(BF16), plain):
+            check(gpu, logits, k, **kw)
+            check(gpu, logits, k, bias=torch.full((E,), 0.5, device="cuda"), **kw)
+        for bias in (wide, -wide.abs(), two, left, odd):
+            check(gpu, plain, k, bias=bias, renormalize=False, **kw)
+
+
 def test_close_choices_among_others(gpu):
     """Pairs of nearly equal choices here and there in ordinary rows."""
     E, T = 256, 64
