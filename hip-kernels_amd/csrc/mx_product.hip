@@ -15,27 +15,27 @@ hipError_t launch_mx_product(const MxProductArgs& a, hipStream_t s) {
 
   // The stream holds the whole of the weights' bandwidth with few rows, and with few tiles its short chain counts:
   //                  stream    32 x 128                          stream    32 x 128
-  //   1 x 5120 x 2880   7.3      12.0        2 each of 128       162       208
-  //   32 x 5120 x 2880  8.3      12.1        4 each of 128       200       240
-  //   64 x 2880 x 4096 11.1      13.8        8 each of 128       242       253
-  //   96 x 5120 x 2880 17.4      12.1        8 each of 32         73        63
-  //   32 x 32768 x 4096  37      20.8        4 each of 32         66        62
+  //   1 x 5120 x 2880   7.4      14.5        2 each of 128       164       207
+  //   32 x 5120 x 2880  8.5      15.0        4 each of 128       210       238
+  //   64 x 2880 x 4096 11.3      16.2        8 each of 128       244       251
+  //   96 x 5120 x 2880 16.6      14.0        4 each of 32         56        62
+  //   32 x 32768 x 4096  42      19.9        8 each of 32         66        62
   const int64_t waves = tiles(kStreamRows, 16);
   if (a.K >= 512 && (each <= 4 || waves <= 4 * kMxCus)) {
     // Waves of 32 columns read a's rows half as often, and are half as many: 2 each of 128 at N = 2880 take 87 (16 columns:
-    // 95), 1 x 5120 x 2880 8.4 (7.5).  Four waves share a long K while there are CUs for it: 1 x 2048 x 8192 7.6
+    // 96), 1 x 5120 x 2880 8.4 (7.5).  Four waves share a long K while there are CUs for it: 1 x 2048 x 8192 7.6
     // (one wave 11.9), 1 x 8192 x 8192 11.1 (13.8); 1 x 10240 x 4096 7.8 (6.9), 32 x 2880 x 4096 11.3 (9.1).
     return launch_mx_stream(a, a.quantized() || waves > 64 * kMxCus,
                             a.K >= 4096 && a.rows <= kStreamRows && waves <= 2 * kMxCus, s);
   }
   //                        32 x 128  128 x 128                        32 x 128  128 x 128
-  //   256 x 5120 x 2880      15.1      15.9        16 each of 128       270       293
-  //   512 x 5120 x 2880      21.5      16.3        32 each of 128       349       311
-  //   777 x 1001 x 2016      11.8      16.8        32 each of 32         88        70
+  //   256 x 5120 x 2880      18.4      17.6        16 each of 128       266       296
+  //   512 x 5120 x 2880      24.3      17.6        32 each of 128       349       310
+  //   777 x 1001 x 2016      10.6      13.6        32 each of 32         89        72
   if (each <= 24 || tiles(32, 128) < 2 * kMxCus) return launch_mx_tile(a, MxTile::low, s);
   //                       128 x 128 256 x 256                       128 x 128 256 x 256
-  //   1500 x 5120 x 2880     25.4      30.7        96 each of 32         88        95
-  //   2048 x 5120 x 2880     38.0      31.1       128 each of 32        131       110
+  //   1500 x 5120 x 2880     26.9      33.1        96 each of 32         94        92
+  //   2048 x 5120 x 2880     40.6      32.0        128 each of 32       132       105
   if (each <= 96 || tiles(128, 128) <= 2 * kMxCus) return launch_mx_tile(a, MxTile::middle, s);
   return launch_mx_tile(a, MxTile::large, s);
 }
