@@ -7,10 +7,10 @@
 //   k       highest choices of these, descending, ties to the lower index
 //   weight  the score; over the sum of the chosen ones if renormalize; times scale
 //
-// An expert whose logit or choice is -inf or whose choice is NaN is switched off:
+// An expert whose logit or bias is -inf, or whose choice is NaN, is switched off:
 // it comes behind the others of the kept groups (lower index first), counts 0 in
-// its group's sum and has weight 0.  (A NaN choice keeps its score as weight, so
-// that NaN logits show.)
+// its group's sum and has weight 0.  (A NaN choice without such a logit or bias keeps its
+// score as weight, so that NaN logits show.)
 //
 // Bound by latency for few tokens (64 of 256 experts in 8 groups, 8 chosen: 5.7 us; one of 128, 4 chosen: 2.7) and
 // by vector instructions for many (8192 of the same: 13 us, where reading the logits takes 1.6).
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(kSelectWaves * kWave) void select_kernel(SelectArgs
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     double c = score[j] + static_cast<double>(bias[j]);
-    if (x[j] == -__builtin_inff()) c = -inf;
+    if (x[j] == -__builtin_inff() || bias[j] == -__builtin_inff()) c = -inf;  // (the sum of NaN and -inf is NaN)
     if (c == -inf) score[j] = 0.0;
     key[j] = NV * lane + j < a.E ? choice_key(c) : 0u;
     scores[wave][NV * lane + j] = score[j];

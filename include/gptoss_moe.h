@@ -608,9 +608,10 @@ enum { GPTOSS_SCORE_SOFTMAX = 0, GPTOSS_SCORE_SIGMOID = 1 };
  * than that may come in either order), weights rounded once.
  * An expert whose logit or bias is -inf is switched off: it counts 0 in
  * its group's sum (a group of these alone comes last), is chosen only where the
- * kept groups have no other left, lower index first, and has weight 0, so
- * indices are distinct and valid in any case.  A choice of NaN is last too, with its
- * score as the weight; a NaN logit makes a softmax row's weights NaN. */
+ * kept groups have no other left, lower index first, and has weight 0 (whatever
+ * its score is), so indices are distinct and valid in any case.  A choice of NaN is last
+ * too, with its score as the weight; a NaN logit makes a softmax row's weights NaN.
+ * Over a sum that is NaN all of a token's weights are. */
 typedef struct gptoss_routing_config {
   int score;        /* GPTOSS_SCORE_SOFTMAX or GPTOSS_SCORE_SIGMOID */
   int top_k;        /* 1 to 32, at most the experts of top_groups groups */

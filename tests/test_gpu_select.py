@@ -272,3 +272,45 @@ def test_streams_and_graphs(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_a_bias_that_switches_off_a_nan(gpu, groups, dtype):
+    """A bias of -inf switches its expert off whatever the score is: weight 0 beside NaN, and nothing in the sum."""
+    E, off = 8, (2, 5)
+    bias = torch.zeros(E, device="cuda")
+    bias[list(off)] = -math.inf
+    logits = torch.linspace(-2, 2, 3 * E, device="cuda").view(3, E).to(dtype)
+    logits[0, 2] = math.nan  # of an expert that is off
+    logits[1, 2], logits[1, 6] = math.nan, math.nan  # and of one that is not
+    logits[2, 6] = math.nan
+    kw = dict(bias=bias, num_groups=groups, top_groups=groups)
+    x = logits.double().cpu()
+
+    def order(nan):  # finite choices, the larger first, then the others by index
+        last = sorted(set(off) | set(nan))
+        return sorted(set(range(E)) - set(last), reverse=True) + last
+
+    # sigmoid: each score is its own
+    idx, w = gpu.select_experts(logits, E, score="sigmoid", renormalize=False, **kw)
+    for t, nan in enumerate(((), (6,), (6,))):
+        assert idx[t].tolist() == order(nan)
+        for e, got in zip(idx[t].tolist(), w[t].tolist()):
+            if e in off:
+                assert got == 0.0, (t, e, got)
+            elif e in nan:
+                assert math.isnan(got)
+            else:
+                assert abs(got - float(torch.sigmoid(x[t, e]))) <= (2.0 ** -24 + 2.0 ** -48) * got  # rounded once from 64 bits
+    idx, w = gpu.select_experts(logits, E, score="sigmoid", **kw)
+    s = torch.sigmoid(x[0])
+    s[list(off)] = 0
+    want = (s / s.sum())[idx[0].cpu().long()]
+    assert bool(((w[0].cpu().double() - want).abs() <= (2.0 ** -24 + 2.0 ** -48) * want).all())
+    # softmax over a row with a NaN: the scores are NaN, but of experts that are off
+    idx, w = gpu.select_experts(logits, E, renormalize=False, **kw)
+    for t in range(3):
+        assert idx[t].tolist() == list(range(E))
+        assert [e for e in range(E) if not math.isnan(float(w[t, e]))] == list(off)
+        assert not w[t, list(off)].any()
