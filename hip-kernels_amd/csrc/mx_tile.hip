@@ -81,10 +81,12 @@ __device__ __forceinline__ u32x4_t load_short_row(const uint8_t* row, int nb) { 
 
 // Up to 32 rows from LDS, `pitch` bytes apart, to rows `step` bytes apart: a T a lane, `across` lanes (a power of two) to a row, kBatch
 // rows' reads ahead of their stores.  (A loop and not its copies: small calls would wait for their
-// instructions.)
+// instructions.)  LDS is read through a type that may alias: the results were put there as others, two bf16 of SwiGLU
+// as a dword, and nothing else holds the reads behind those stores.
 template <typename T, int kBatch>
 __device__ __forceinline__ void store_rows(const uint8_t* own, int pitch, int across, uint8_t* out, int64_t step, int rows, bool in,
                                            int lane) {
+  typedef T __attribute__((may_alias)) any_t;
   const int log = __builtin_ctz(across), at_once = kWave >> log, row0 = lane >> log, off = sizeof(T) * (lane & (across - 1));
   const uint8_t* from = own + pitch * row0 + off;
   uint8_t* to = out + row0 * step + off;
@@ -94,7 +96,7 @@ __device__ __forceinline__ void store_rows(const uint8_t* own, int pitch, int ac
   for (int k = 0; k < 32; k += kBatch * at_once) {
     T d[kBatch];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) d[u] = *reinterpret_cast<const T*>(from + pitch * at_once * u);
+    for (int u = 0; u < kBatch; ++u) d[u] = *reinterpret_cast<const any_t*>(from + pitch * at_once * u);
     from += kBatch * pitch * at_once;
     if (left > (kBatch - 1) * at_once) {
 #pragma unroll

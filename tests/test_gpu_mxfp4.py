@@ -375,3 +375,18 @@ def test_products_past_32_bits(gpu):
     want, tol = ref.product(ref.of_matrix(rows_of(gpu, a, at)), ref.of_matrix(w))
     ref.assert_values(got[at], want, tol)
     ref.assert_quantized(rows_of(gpu, packed, at), want, tol)
+
+
+@pytest.mark.parametrize("M, N", [(5, 6), (40, 2), (200, 130), (70, 1002), (650, 3206), (2900, 2946)])
+def test_swiglu_of_few_columns_in_bf16(gpu, M, N):
+    """In rows that begin on no more than an element: the same as the fp32 results, rounded."""
+    a, w, bias = operands(gpu, M, N, 96, M, low=119, high=124)
+    want = gpu.mxfp4_matmul(a, w, bias=bias, swiglu=True, dtype=F32).to(BF16)
+    y, tol = ref.product(ref.of_matrix(a), ref.of_matrix(w), bias)
+    ref.assert_values(want, *ref.swiglu(y, tol))
+    for before, after in ((0, 0), (1, 0), (3, 4), (2, 1)):
+        buf = torch.full((M, before + N // 2 + after), 7.0, device="cuda", dtype=BF16)
+        out = buf[:, before:before + N // 2]
+        gpu.mxfp4_matmul(a, w, bias=bias, swiglu=True, out=out)
+        assert torch.equal(out, want), (before, after)
+        assert bool((buf[:, :before] == 7).all()) and bool((buf[:, before + N // 2:] == 7).all())
