@@ -83,8 +83,9 @@ int product(const uint8_t* a, const uint8_t* as, int a_rows, const int32_t* row_
   if (r == nullptr) return set_error(GPTOSS_ERR_INVALID, "result is NULL");
   const bool quantized = r->out_packed != nullptr || r->out_scales != nullptr;
   if (r->swiglu && N % 2 != 0) return set_error(GPTOSS_ERR_INVALID, "swiglu needs pairs of columns, N=%d", N);
-  if (r->swiglu && (std::isnan(r->alpha) || std::isinf(r->alpha) || !(r->limit >= 0.0f)))
-    return set_error(GPTOSS_ERR_INVALID, "swiglu: alpha=%g must be finite, limit=%g not negative",
+  // (the kernels hold alpha / ln 2: an infinite one would make NaN of a gate of zero)
+  if (r->swiglu && (!(std::fabs(r->alpha) <= 0x1p127f) || !(r->limit >= 0.0f)))
+    return set_error(GPTOSS_ERR_INVALID, "swiglu: alpha=%g must be within 2^127, limit=%g not negative",
                      static_cast<double>(r->alpha), static_cast<double>(r->limit));
   const int cols = r->swiglu ? N / 2 : N;
   if (quantized && cols % 32 != 0)

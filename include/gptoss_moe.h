@@ -652,7 +652,8 @@ int gptoss_mxfp4_dequantize(const uint8_t* packed, const uint8_t* scales, int ro
 
 /* Where a product's results go.  swiglu: columns 2i (gate) and 2i + 1 (up) give
  * column i, (clamp(up, -limit, limit) + 1) * g * sigmoid(alpha * g),
- * g = min(gate, limit); NaN is kept.  Then either values, bf16 or fp32 in rows out_stride
+ * g = min(gate, limit); NaN is kept; alpha is finite and at most 2^127 in magnitude, limit
+ * is not negative.  Then either values, bf16 or fp32 in rows out_stride
  * elements apart, or (out NULL) MXFP4 as gptoss_mxfp4_quantize makes it of the
  * fp32 results, a multiple of 32 columns, out_packed 16-byte aligned.  Nothing is rounded in between. */
 typedef struct gptoss_mxfp4_result {

@@ -390,3 +390,18 @@ def test_swiglu_of_few_columns_in_bf16(gpu, M, N):
         gpu.mxfp4_matmul(a, w, bias=bias, swiglu=True, out=out)
         assert torch.equal(out, want), (before, after)
         assert bool((buf[:, :before] == 7).all()) and bool((buf[:, before + N // 2:] == 7).all())
+
+
+@pytest.mark.parametrize("M, N, K", [(1, 64, 512), (3, 64, 4096), (40, 64, 32), (650, 3200, 32), (2900, 2944, 32)])
+def test_swiglu_of_the_steepest_alpha(gpu, M, N, K):
+    """alpha of 2^127: the sigmoid is 0 or 1, and 1/2 of a gate of zero; gates and ups are the biases."""
+    a, w, _ = operands(gpu, M, N, K)
+    a.packed.zero_()
+    gate = torch.tensor([0.0, 1.0, -1.0, 0.5, -8.0, 8.0, -0.0, 2.0], device="cuda").repeat(N // 16)
+    up = torch.linspace(-8, 8, N // 2, device="cuda").to(BF16).float()
+    bias = torch.stack((gate, up), 1).flatten().to(BF16)
+    g, u = gate.clamp(max=7), up.clamp(-7, 7)
+    for alpha in (2.0 ** 127, -2.0 ** 127):
+        on = (g * alpha) > 0
+        got = gpu.mxfp4_matmul(a, w, bias=bias, swiglu=True, alpha=alpha, dtype=F32)
+        assert torch.equal(got, torch.where(on, (u + 1) * g, torch.zeros_like(g)).expand(M, -1))

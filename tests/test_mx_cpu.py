@@ -194,6 +194,17 @@ def test_product_of_more_tiles_than_a_launch_holds(g):
             b"columns in one call")
 
 
+@pytest.mark.parametrize("grouped", [False, True])
+def test_alpha(g, grouped):
+    """Over ln 2 it has to be finite in 32 bits; without swiglu it does not count."""
+    none = dict(a_rows=0, rows=0)
+    for alpha in (3e38, -3e38, 1.8e38, float("inf"), -float("inf")):
+        refused(g, product(g, grouped, dict(swiglu=1, alpha=alpha), **none), "INVALID", b"alpha")
+        assert product(g, grouped, dict(alpha=alpha), **none) == g.GPTOSS_OK
+    for alpha in (2.0 ** 127, -2.0 ** 127, 0.0, 1e-40):
+        assert product(g, grouped, dict(swiglu=1, alpha=alpha), **none) == g.GPTOSS_OK
+
+
 def test_products_of_nothing(g):
     assert product(g, False, a_rows=0, a=None, asc=None, w=None, ws=None) == g.GPTOSS_OK
     assert product(g, True, a_rows=0, rows=0, a=None, asc=None, off=None) == g.GPTOSS_OK
