@@ -314,3 +314,30 @@ def test_a_bias_that_switches_off_a_nan(gpu, groups, dtype):
         assert idx[t].tolist() == list(range(E))
         assert [e for e in range(E) if not math.isnan(float(w[t, e]))] == list(off)
         assert not w[t, list(off)].any()
+
+
+def weights_of_64_bits(logits, k, score="softmax", **kw):
+    """mx_ref's selection, and how far 64-bit arithmetic with one rounding at the end may be from it.  The exponential's
+    argument is a difference of fp32 values, off by 2^-53 of its size, the exponential by two units of 2^-52; sums of up to
+    1024 terms by lanes and then across them, two divisions and the scale have fewer than 40 roundings of 2^-53; the
+    oracle's own arithmetic has no more.  Then half a unit of fp32, 2^-24 of a normal number and 2^-150 below."""
+    idx, w, _ = ref.select(logits, k, score, **kw)
+    x = logits.detach().cpu().double()
+    far = (x - x.amax(1, keepdim=True) if score == "softmax" else x).abs().amax(1, keepdim=True)
+    return idx, w, w.abs() * (2.0 ** -24 + (far + 64) * 2.0 ** -51) + 2.0 ** -150
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E, k, groups", [(8, 2, 1), (32, 4, 1), (64, 8, 4), (128, 4, 1), (128, 8, 8), (256, 8, 8), (384, 6, 1),
+                                          (1000, 32, 1), (1024, 32, 16)])
+@pytest.mark.parametrize("spread", [0.01, 2.0, 60.0])
+def test_weights_are_rounded_once(gpu, E, k, groups, score, dtype, spread):
+    gen = gen_of(E + k)
+    logits = (spread * torch.randn((50, E), device="cuda", generator=gen)).to(dtype)
+    bias = 0.1 * torch.randn(E, device="cuda", generator=gen) if groups > 1 else None
+    for renormalize, scale in ((True, 1.0), (True, 2.5), (False, 0.75)):
+        kw = dict(score=score, bias=bias, renormalize=renormalize, scale=scale)
+        got = gpu.select_experts(logits, k, num_groups=groups, top_groups=(groups + 1) // 2, **kw)
+        ref.assert_selected(got, weights_of_64_bits(logits, k, groups=groups, top_groups=(groups + 1) // 2, **kw),
+                            (renormalize, scale))
