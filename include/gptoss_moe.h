@@ -655,7 +655,8 @@ int gptoss_mxfp4_dequantize(const uint8_t* packed, const uint8_t* scales, int ro
  * g = min(gate, limit); NaN is kept; alpha is finite and at most 2^127 in magnitude, limit
  * is not negative.  Then either values, bf16 or fp32 in rows out_stride
  * elements apart, or (out NULL) MXFP4 as gptoss_mxfp4_quantize makes it of the
- * fp32 results, a multiple of 32 columns, out_packed 16-byte aligned.  Nothing is rounded in between. */
+ * fp32 results, a multiple of 32 columns, out_packed 16-byte aligned.  Nothing is rounded in between; a sigmoid
+ * below 2^-126 counts as 0. */
 typedef struct gptoss_mxfp4_result {
   int swiglu;
   float alpha, limit;
@@ -679,7 +680,8 @@ int gptoss_mxfp4_matmul(const uint8_t* a_packed, const uint8_t* a_scales, int M,
  * a (perm_token; NULL: row p) with w_e and bias_e, w [num_experts][N][K],
  * bias [num_experts][N].  expert_offsets (device, [num_experts + 1], at most 1024
  * experts) is nondecreasing within [0, rows]; result rows outside of it are left as they
- * were.  A row number outside [0, a_rows) stands for a row of zeros. */
+ * were.  A row number outside [0, a_rows) stands for a row of zeros: its sums are 0, also with
+ * weights that are NaN, and its results those of the bias alone. */
 int gptoss_moe_grouped_mxfp4_matmul(const uint8_t* a_packed, const uint8_t* a_scales, int a_rows, const int32_t* row_index,
                                     const int32_t* expert_offsets, int num_experts, int rows, const uint8_t* w_packed,
                                     const uint8_t* w_scales, const uint16_t* bias, int N, int K,

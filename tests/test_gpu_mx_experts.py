@@ -244,3 +244,21 @@ def test_two_streams_at_once(gpu):
         torch.cuda.synchronize()
         for a, w in zip(got, want):
             assert torch.equal(a, w)
+
+
+@pytest.mark.parametrize("counts, N, K", [([3, 0, 5], 96, 512), ([2, 3], 64, 4096), ([40, 3, 100], 96, 160),
+                                          ([40] * 12, 1472, 64), ([300, 100, 40, 129, 64, 65], 8192, 96)])
+def test_rows_of_zeros_and_weights_of_nan(gpu, counts, N, K):
+    """A row number outside of a gives the bias alone, whatever the weights hold; other rows are NaN in such columns."""
+    c = Case(gpu, counts, N, K, seed=3, before=1, after=1)
+    c.w.scales[:, ::3, 0] = 255
+    c.index[::2] = -1
+    c.index[1::4] = c.a.rows
+    expert = torch.cat([torch.full((n,), e) for e, n in enumerate(counts)])
+    got = gpu.grouped_mxfp4_matmul(c.a, c.w, c.offsets, c.rows, row_index=c.index, bias=c.bias, dtype=F32)[c.lo:c.hi].cpu()
+    index, bias = c.index[c.lo:c.hi].cpu(), c.bias.float().cpu()[expert]
+    zero = (index < 0) | (index >= c.a.rows)
+    assert bool(zero.any()) and bool((~zero).any())
+    assert torch.equal(got[zero], bias[zero])
+    nan = torch.isnan(got[~zero])
+    assert bool(nan[:, ::3].all()) and not nan[:, 1::3].any() and not nan[:, 2::3].any()
