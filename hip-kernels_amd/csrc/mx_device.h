@@ -32,7 +32,7 @@ __device__ __forceinline__ uint32_t mx_magnitude(float v) { return __float_as_ui
 
 // Clamped SwiGLU of one (gate, up) pair, NaN kept (a minimum would drop it):
 // (up + 1) * gate * sigmoid(alpha * gate), with the hardware's exponential and
-// reciprocal, each within one unit of fp32's last place.  The IEEE division and the polynomial exponential
+// reciprocal, each within one unit of fp32's last place; a sigmoid below 2^-126 is 0, as that reciprocal of it is.  The IEEE division and the polynomial exponential
 // of gx_swiglu are five times the instructions, 16 us of a tile of 256 x 256.
 __device__ __forceinline__ float mx_swiglu(float g, float u, float alpha, float limit) {
   g = g > limit ? limit : g;

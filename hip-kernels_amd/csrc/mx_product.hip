@@ -4,7 +4,8 @@
 // tiles of 32 x 128, 128 x 128 and 256 x 256.  The rule is on the rows that an expert has on
 // average and on how many tiles the call has for 256 CUs; the figures are us on both
 // sides of each border, one expert unless said (rows x N x K, or rows of each of E experts at N = 5760, K = 2880
-// with SwiGLU and MXFP4 results).
+// with SwiGLU and MXFP4 results).  Experts have equally many rows there; how uneven they are is known on the device
+// only, and calls whose rows go to a few of many experts were not measured on both sides.
 #include "mx_kernels.h"
 
 namespace gxmoe {

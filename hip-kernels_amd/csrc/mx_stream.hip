@@ -19,7 +19,7 @@
 // the two.  Where tiles are few, KS waves share a tile's K, and their sums meet in LDS in
 // a fixed order.
 //
-// Bound by the weights' bandwidth: one or two rows each of 111 experts, 5760 x 2880, 162 us (5.8 TB/s); 29
+// Bound by the weights' bandwidth: one to six rows each of 107 experts, 5760 x 2880, 163 us (5.8 TB/s); one or two of 29
 // experts 53 us (4.8); by latency where they are few: 1 x 5120 x 2880, weights in no cache, 7.5 us.
 #include "mx_product.h"
 
@@ -366,7 +366,8 @@ hipError_t launch(const MxProductArgs& a, hipStream_t s) {
   constexpr int kN = 16 * NT;
   const int pieces = a.swiglu && a.quantized() ? 2 * kN : kN;  // columns that go together
   const size_t bytes = static_cast<size_t>(KS) * wave_bytes<NT, KS>(a.K / 32);
-  // as many as fit at once (two waves per SIMD with their registers), each with a run of tiles
+  // As many as fit at once, each with a run of tiles: eight waves on a CU, the two a SIMD that 32 columns' 203 and more
+  // registers leave.  (16 columns' 143 and 146 would leave three; that was not measured.)
   const int64_t by_lds = 160 * 1024 / bytes, by_waves = 8 / KS, fit = kMxCus * (by_lds < by_waves ? by_lds : by_waves);
   int64_t grid = most_m_tiles(a, kStreamRows) * ((a.N + pieces - 1) / pieces);
   if (grid > fit) grid = fit;

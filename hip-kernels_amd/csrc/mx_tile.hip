@@ -15,8 +15,8 @@
 // stage is free for the loads of the chunk after the next.  These go out in three parts, in
 // that step and the first two of the next chunk (8192^3: 274 us; all at once 279).
 //
-// Large tiles are bound by power: 8192 x 8192 x 8192 takes 274 us (4.0 PFLOP/s; the clock is
-// 1.8 GHz), with operands of zeros 224; products alone, from registers, reach 6.2 to 6.7 PFLOP/s with random
+// Large tiles are bound by power: 8192 x 8192 x 8192 takes 270 us (4.1 PFLOP/s; the clock is
+// 1.8 GHz), with operands of zeros 197; products alone, from registers, reach 6.2 to 6.7 PFLOP/s with random
 // operands.  Each round of tiles takes 10 us beyond its chunks.  (Four waves of 128 x 128 each read a third less from
 // LDS, but one wave a SIMD leaves gaps: 329 us.)  Smaller tiles stand two or three on a CU, so
 // that one's first loads and last stores overlap another's chunks; their weights come at 4.2 TB/s
